@@ -50,9 +50,19 @@ _SIGS = {
                           _P, _P],
     "dg_pkm_backward": [_I, _I, _I, _I, _I, _I64, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P,
                         _P, _P],
+    "dg_gated_scan_forward": [_I, _I, _I, _I, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P,
+                              _P],
+    "dg_gated_scan_backward": [_I, _I, _I, _I, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I64,
+                               _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P],
+    "dg_gated_scan_step": [_I, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P],
+    "dg_gated_ffn_forward": [_I, _I64, _I, _I, _I, _P, _I64, _P, _P, _P, _P, _P],
+    "dg_gated_ffn_backward_workspace_size": [_I, _I64, _I, _I],
+    "dg_gated_ffn_backward": [_I, _I64, _I, _I, _I, _P, _I64, _P, _P, _P, _I64, _P, _P, _P, _P, _SZ, _P, _P],
+    "dg_sample": [_I, _I, _I, _P, _I64, _P, _P, ctypes.c_float, _P, ctypes.c_int32, _P, ctypes.c_float, _P,
+                  ctypes.c_float, _P, _P, _P],
 }
 _RESTYPE = {"dg_status_string": ctypes.c_char_p, "dg_set_wait_limit": ctypes.c_uint, "dg_pkm_forward_workspace_size": ctypes.c_size_t,
-            "dg_dense_backward_workspace_size": ctypes.c_size_t}
+            "dg_dense_backward_workspace_size": ctypes.c_size_t, "dg_gated_ffn_backward_workspace_size": ctypes.c_size_t}
 
 _lib = None
 _lock = threading.Lock()

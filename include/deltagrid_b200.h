@@ -304,6 +304,101 @@ int dg_pkm_route(int dtype, int B, int H, int T, int dh, int g0, int g1, int top
                  void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Language-model operators next to the memory layer: the gated linear recurrence,
+ * the gated feed-forward block and token sampling.  f32, f16 and bf16 storage
+ * (f64: DG_ERR_UNSUPPORTED); sums, states and statistics are fp32 or wider.
+ * ------------------------------------------------------------------------- */
+
+/* Steps between the states that dg_gated_scan_forward leaves for the backward pass. */
+#define DG_SCAN_MARK_STEPS 128
+
+/*
+ * Gated linear recurrence over a sequence, per batch row b and channel d:
+ *   a_t = sigmoid(gate_t)        h_t = c_t h_{t-1} + (1 - a_t) x_t        y_t = h_t silu(out_gate_t)
+ * with c_t = a_t, or 0 where resets[b,t] is not 0 (a new document starts there), and
+ * y_t = h_t when out_gate is NULL.
+ *   x, gate, out_gate [B,T,D]: element strides (batch, step) each, last dimension contiguous
+ *   h0 [B,D] fp32 or NULL (zeros);  lengths [B] int32 or NULL (all T);  resets [B,T] bytes or NULL
+ *   y [B,T,D] contiguous;  h_last [B,D] fp32 or NULL
+ *   marks [B, ceil(T / DG_SCAN_MARK_STEPS), D] fp32 or NULL: the state before each block of
+ *   DG_SCAN_MARK_STEPS steps, which the backward pass needs
+ * Steps t >= lengths[b] leave the state as it is, give y = 0, and their inputs are not used
+ * (they may hold anything); lengths are clamped to [0, T].
+ */
+int dg_gated_scan_forward(int dtype, int B, int T, int D, const void* x, int64_t x_sb, int64_t x_st,
+                          const void* gate, int64_t gate_sb, int64_t gate_st, const void* out_gate,
+                          int64_t out_gate_sb, int64_t out_gate_st, const float* h0, const int32_t* lengths,
+                          const uint8_t* resets, void* y, float* h_last, float* marks, void* stream);
+
+/*
+ * Backward of dg_gated_scan_forward, from the same inputs and its marks:
+ *   e_t = dy_t silu(out_gate_t) + c_{t+1} e_{t+1}  (dh_last enters after the last valid step)
+ *   dx = e (1 - a)   dgate = e (c_t != reset ? h_{t-1} - x : -x) a (1 - a)   dout_gate = dy h silu'   dh0 = c_0 e_0
+ * dy, dx, dgate, dout_gate [B,T,D] with (batch, step) strides; dh_last, dh0 [B,D] fp32 or NULL.
+ * out_gate and dout_gate are both given or both NULL.  No atomics: results repeat bit for bit.
+ */
+int dg_gated_scan_backward(int dtype, int B, int T, int D, const void* x, int64_t x_sb, int64_t x_st,
+                           const void* gate, int64_t gate_sb, int64_t gate_st, const void* out_gate,
+                           int64_t out_gate_sb, int64_t out_gate_st, const int32_t* lengths, const uint8_t* resets,
+                           const float* marks, const void* dy, int64_t dy_sb, int64_t dy_st, const float* dh_last,
+                           void* dx, int64_t dx_sb, int64_t dx_st, void* dgate, int64_t dgate_sb, int64_t dgate_st,
+                           void* dout_gate, int64_t dout_gate_sb, int64_t dout_gate_st, float* dh0, void* stream);
+
+/* One step of the recurrence: x, gate, out_gate (or NULL) [B,D] with a row stride each; the
+ * state h [B,D] fp32 contiguous is updated in place; y [B,D] contiguous. */
+int dg_gated_scan_step(int dtype, int B, int D, const void* x, int64_t x_sb, const void* gate, int64_t gate_sb,
+                       const void* out_gate, int64_t out_gate_sb, float* h, void* y, void* stream);
+
+typedef enum dg_activation {
+    DG_ACT_SILU = 0, /* z / (1 + exp(-z)) */
+    DG_ACT_GELU = 1  /* z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+} dg_activation;
+
+/*
+ * Gated feed-forward: both projections, the activation and the product,
+ *   G = x Wg^T + bg     U = x Wu^T + bu     h = act(G) * U
+ *   x [M,D] (row stride ldx >= D)   weight [2F,D] contiguous: the F gate rows Wg, then the F value
+ *   rows Wu   bias [2F] (storage dtype) or NULL   h [M,F] contiguous
+ * The products accumulate in fp32 and h is rounded once.  M may be 0.  dev_status (or NULL)
+ * gets DG_DEVCHK_TIMEOUT if a bounded wait inside a kernel gave up.
+ */
+int dg_gated_ffn_forward(int dtype, int64_t M, int D, int F, int activation, const void* x, int64_t ldx,
+                         const void* weight, const void* bias, void* h, int32_t* dev_status, void* stream);
+
+/* Bytes of device workspace (16-byte aligned) dg_gated_ffn_backward needs for this shape. */
+size_t dg_gated_ffn_backward_workspace_size(int dtype, int64_t M, int D, int F);
+
+/*
+ * Backward of dg_gated_ffn_forward; G and U are formed again from x and the weights.
+ *   dU = dh act(G)   dG = dh U act'(G)   dx = dG Wg + dU Wu   dweight = [dG^T x; dU^T x]
+ *   dbias = column sums of [dG, dU] (summed in fp32 before any rounding)
+ *   dh [M,F] (row stride ld_dh)   dx [M,D], dweight [2F,D], dbias [2F] contiguous, NULL where not wanted
+ * dG and dU pass through the workspace in the storage dtype.  No atomics.
+ */
+int dg_gated_ffn_backward(int dtype, int64_t M, int D, int F, int activation, const void* x, int64_t ldx,
+                          const void* weight, const void* bias, const void* dh, int64_t ld_dh, void* dx,
+                          void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                          int32_t* dev_status, void* stream);
+
+/*
+ * Draws one token per row from given uniform numbers.
+ *   logits [B,V] (row stride in elements, last dimension contiguous)   u [B] fp32 in [0, 1)
+ * With m the row's largest logit, token i has the mass w_i = floor(2^40 exp((l_i - m) / temperature)),
+ * a 64-bit integer, so that sums do not depend on the order they are taken in.  In descending order of
+ * logits (equal logits: lower index first) top_k keeps the first k (k <= 0 or k > V: all); top_p keeps
+ * those of them with less than top_p times their mass before them, at least one (steps of 2^-24);
+ * min_p keeps those with w_i >= min_p 2^40.  The token is the first kept index whose running mass, in
+ * index order, exceeds floor(u * kept mass).  temperature <= 0: the largest logit, lowest index.
+ * A NaN logit counts as -inf, an infinite one takes all the mass; a row of -inf gives token -1.
+ * Each parameter is a device array of B values or, where the pointer is NULL, the scalar beside it.
+ *   token [B] int64   logprob [B] fp32 or NULL: log(w_token / kept mass), -inf for token -1
+ */
+int dg_sample(int dtype, int B, int V, const void* logits, int64_t row_stride, const float* u,
+              const float* temperature, float temperature_value, const int32_t* top_k, int32_t top_k_value,
+              const float* top_p, float top_p_value, const float* min_p, float min_p_value, int64_t* token,
+              float* logprob, void* stream);
+
+/* ---------------------------------------------------------------------------
  * The reference C++ engine's files (src/cpp/engine), read and written on the
  * host so that its weights and recurrent state can drive the GPU recurrence
  * (dg_fxp_* for Q16.16 files, dg_dense_forward / dg_pkm_forward for fp32 ones).
