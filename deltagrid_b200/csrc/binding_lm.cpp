@@ -240,6 +240,16 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& h, con
 // gated feed-forward
 // ---------------------------------------------------------------------------
 
+// a matrix as TMA can read it: rows of 16-bit values start on 16-byte boundaries.  One that is laid
+// out otherwise is copied, where its row length allows: the copy costs less than the kernel for
+// any alignment.
+Tensor matrix(const Tensor& t) {
+    Tensor r = rows(t);
+    if (r.size(0) > 1 && r.stride(0) < r.size(1)) r = r.contiguous();
+    const bool off = (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15) || (r.size(0) > 1 && r.stride(0) % 8);
+    return off && r.element_size() == 2 && r.size(1) % 8 == 0 ? r.clone(at::MemoryFormat::Contiguous) : r;
+}
+
 struct FfnArgs {
     Tensor x, w, b;             // x [M,D] rows
     int code = 0, D = 0, F = 0, act = 0;
@@ -257,17 +267,15 @@ FfnArgs ffn_args(const Tensor& x, const Tensor& w, const Tensor& b, int64_t act)
     same_device(x, op, "weight", w);
     same_dtype(x, op, "weight", w);
     a.D = to_int(w.size(1), op), a.F = to_int(w.size(0) / 2, op), a.act = (int)act;
-    a.w = contig(w);
+    a.w = matrix(contig(w));
     if (b.defined()) {
         same_device(x, op, "bias", b);
         same_dtype(x, op, "bias", b);
         TORCH_CHECK(b.dim() == 1 && b.size(0) == w.size(0), op, ": expected bias [2F], got ", b.sizes());
-        a.b = contig(b);
+        a.b = matrix(contig(b).view({1, -1}));
     }
-    a.x = x.dim() == 2 ? rows(x) : x.contiguous().view({-1, a.D});
+    a.x = matrix(x.dim() == 2 ? x : x.contiguous().view({-1, a.D}));
     a.M = a.x.size(0);
-    // a row stride below D (an expanded or overlapping tensor) is laid out first
-    if (a.M > 1 && a.x.stride(0) < a.D) a.x = a.x.contiguous();
     return a;
 }
 
@@ -306,8 +314,7 @@ struct GatedFfn : public torch::autograd::Function<GatedFfn> {
         const auto s = ctx->get_saved_variables();
         const FfnArgs a = ffn_args(s[0], s[1], s[2], ctx->saved_data["act"].toInt());
         const int64_t want = ctx->saved_data["want"].toInt();
-        Tensor dh = grads[0].dim() == 2 ? rows(grads[0]) : grads[0].contiguous().view({-1, a.F});
-        if (a.M > 1 && dh.stride(0) < a.F) dh = dh.contiguous();
+        const Tensor dh = matrix(grads[0].dim() == 2 ? grads[0] : grads[0].contiguous().view({-1, a.F}));
         Tensor dx, dw, db;
         if (want & 1) dx = at::empty(s[0].sizes(), s[0].options());
         if (want & 2) dw = at::empty(s[1].sizes(), s[1].options());

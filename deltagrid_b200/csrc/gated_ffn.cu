@@ -1,8 +1,21 @@
 // gated_ffn.cu -- the gated feed-forward block h = act(x Wg^T + bg) * (x Wu^T + bu) and its
 // backward pass on CUDA cores: 64 x 64 output tiles, 16 of the contracted axis at a time
-// through shared memory, 4 x 4 outputs per thread.  It takes any storage type, size and
-// alignment.
+// through shared memory, 4 x 4 outputs per thread.  These kernels take any storage type, size
+// and alignment; 16-bit calls with D and F multiples of 8 and 16-byte aligned rows go to the
+// tcgen05 kernel of gated_ffn_tc.cu.
 #include "lm_common.cuh"
+
+namespace dg_host {
+bool ffn_tc_supports(int dtype, int64_t M, int D, int F);
+bool ffn_tc_aligned(const void* a, int64_t lda, const void* b, const void* c, const void* d, int64_t ldd,
+                    const void* e, const void* f);
+int ffn_tc_forward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
+                   const void* bias, void* h, int32_t* status, cudaStream_t s);
+size_t ffn_tc_workspace(int64_t M, int D, int F);
+int ffn_tc_backward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
+                    const void* bias, const void* dh, int64_t ld_dh, void* dx, void* dw, void* db, void* workspace,
+                    int32_t* status, cudaStream_t s);
+}  // namespace dg_host
 
 namespace {
 
@@ -147,7 +160,8 @@ int dg_gated_ffn_forward(int dtype, int64_t M, int D, int F, int activation, con
     if (M == 0) return DG_OK;
     if (!x || !weight || !h || ldx < D) return DG_ERR_INVALID_ARGUMENT;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    (void)dev_status;
+    if (dg_host::ffn_tc_supports(dtype, M, D, F) && dg_host::ffn_tc_aligned(x, ldx, weight, bias, h, 0, h, h))
+        return dg_host::ffn_tc_forward(dtype, M, D, F, activation, x, ldx, weight, bias, h, dev_status, s);
     const dim3 grid((F + TN - 1) / TN, (unsigned)((M + TM - 1) / TM));
     DG_DISPATCH_LM(dtype, S, {
         auto k = activation == DG_ACT_SILU ? ffn_gate_kernel<S, DG_ACT_SILU> : ffn_gate_kernel<S, DG_ACT_GELU>;
@@ -159,7 +173,10 @@ int dg_gated_ffn_forward(int dtype, int64_t M, int D, int F, int activation, con
 
 size_t dg_gated_ffn_backward_workspace_size(int dtype, int64_t M, int D, int F) {
     if (check_args(dtype, M, D, F, DG_ACT_SILU) != DG_OK) return 0;
-    return round16((size_t)M * 2 * F * dg_host::dtype_size(dtype)) + round16((size_t)((M + TM - 1) / TM) * 2 * F * 4);
+    const size_t simple =
+        round16((size_t)M * 2 * F * dg_host::dtype_size(dtype)) + round16((size_t)((M + TM - 1) / TM) * 2 * F * 4);
+    const size_t tc = dg_host::ffn_tc_supports(dtype, M, D, F) ? dg_host::ffn_tc_workspace(M, D, F) : 0;
+    return simple > tc ? simple : tc;
 }
 
 int dg_gated_ffn_backward(int dtype, int64_t M, int D, int F, int activation, const void* x, int64_t ldx,
@@ -173,7 +190,10 @@ int dg_gated_ffn_backward(int dtype, int64_t M, int D, int F, int activation, co
                   (reinterpret_cast<uintptr_t>(workspace) & 15)))
         return DG_ERR_WORKSPACE;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    (void)dev_status;
+    if (M > 0 && dg_host::ffn_tc_supports(dtype, M, D, F) &&
+        dg_host::ffn_tc_aligned(x, ldx, weight, bias, dh, ld_dh, dx, dweight))
+        return dg_host::ffn_tc_backward(dtype, M, D, F, activation, x, ldx, weight, bias, dh, ld_dh, dx, dweight,
+                                        dbias, workspace, dev_status, s);
     const unsigned mt = (unsigned)((M + TM - 1) / TM);
     DG_DISPATCH_LM(dtype, S, {
         S* dz = static_cast<S*>(workspace);

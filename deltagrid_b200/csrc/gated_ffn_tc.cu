@@ -1,0 +1,687 @@
+// gated_ffn_tc.cu -- the products of the gated feed-forward block on tcgen05 (f16 / bf16),
+// one persistent kernel in three roles:
+//   GATE    G = x Wg^T, U = x Wu^T of one tile side by side in TMEM; epilogue
+//           h = act(G + bg) * (U + bu)
+//   DGATE   the same products again; epilogue dG = dh U act'(G), dU = dh act(G) and, where
+//           the bias gradient is wanted, their sums over 32 rows in fp32
+//   PLAIN   C = A B for dx = [dG dU] W and dW = [dG dU]^T x (operands of either major),
+//           optionally split along the contracted axis into fp32 partial products
+//
+// A pair of CTAs (cta_group::2) shares one tile of 256 rows x 256 columns: each CTA holds
+// its 128 rows of A and half of B's columns (GATE: the even CTA the 128 gate rows of the
+// weights, the odd one the 128 value rows), so each operand byte that enters shared memory
+// feeds twice the products it would in a tile of one CTA.  One thread of the even CTA issues
+// the MMAs of the pair (M = 256, N = 256, K = 16) into one of two accumulators of 256 TMEM
+// columns, so that the epilogue of a tile runs under the products of the next.
+//
+// Roles per CTA (384 threads): warp 0 loads operand stages by TMA, warp 1 issues the MMAs
+// (even CTA only), warp 2 loads DGATE's dh tiles, warps 4-7 and 8-11 are two epilogue groups
+// (thread = TMEM lane = row) that take alternate slices of 64 columns.
+//
+// Every wait is bounded by the library's wait limit; a role that gives up flags
+// DG_DEVCHK_TIMEOUT, the others run into their own limits, and the CTA lets what it has in
+// flight land before it frees its TMEM.
+#include <cuda.h>
+
+#include "chunk_common.cuh"
+#include "lm_common.cuh"
+
+namespace {
+
+enum Role { GATE = 0, DGATE = 1, PLAIN = 2 };
+
+constexpr int BM = 128;                    // rows per CTA (256 per pair)
+constexpr int BN = 256;                    // accumulator columns of a tile
+constexpr int BK = 64;                     // contracted elements per stage: 128 bytes
+constexpr int THREADS = 384;
+constexpr uint32_t TILE = BM * BK * 2;     // 16 KB: one operand tile, one staging buffer
+constexpr int GROUP_M = 8;                 // tile rows walked together, for L2
+
+template <int ROLE> struct Cfg {
+    static constexpr int STAGES = ROLE == DGATE ? 5 : 6;
+    static constexpr uint32_t DH = STAGES * 2 * TILE;              // DGATE: dh, then dG (one slice per group)
+    static constexpr uint32_t OUT = DH + (ROLE == DGATE ? 2 * TILE : 0);
+    static constexpr uint32_t BAR = OUT + 2 * TILE;
+    static constexpr uint32_t BYTES = BAR + 256;
+};
+
+struct FfnParams {
+    int64_t M;                 // output rows
+    int N;                     // output columns (GATE, DGATE: features F)
+    int K;                     // contracted elements
+    int m_tiles, n_tiles, splits, kb_per_split;
+    const void* bias;          // GATE, DGATE: [2F] or null
+    float* colsum;             // DGATE: [4 x row tiles of 128][2F] or null
+    int32_t* status;
+    uint32_t wait_limit;
+};
+
+// ---- cluster and cta_group::2 forms -------------------------------------------
+__device__ __forceinline__ uint32_t cta_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// address of the same shared-memory location in the even CTA of the pair
+__device__ __forceinline__ uint32_t in_leader(const void* p) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(tc::smem_u32(p)));
+    return a;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3}], [%4];" ::"r"(tc::smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// arrive on this barrier in both CTAs once the MMAs issued so far have completed
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            tc::smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t n) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(dst)), "r"(n)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t t, uint32_t n) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(n) : "memory");
+}
+
+// work item -> tile row, tile column and split; GROUP_M tile rows at a time, so that the tiles
+// in flight share both operands in L2
+struct Work {
+    int mt, nt, split;
+};
+__device__ __forceinline__ Work work_of(const FfnParams& p, int64_t i) {
+    const int tiles = p.m_tiles * p.n_tiles;
+    const int s = (int)(i / tiles), t = (int)(i - (int64_t)s * tiles);
+    const int per = GROUP_M * p.n_tiles, g = t / per, r = t - g * per;
+    const int rows = min(GROUP_M, p.m_tiles - g * GROUP_M);
+    return {g * GROUP_M + r % rows, r / rows, s};
+}
+
+__device__ __forceinline__ void load_bias8(const void* bias, int64_t at, bool bf16, float (&b)[8]) {
+    const uint4 v = dg::ldg16(static_cast<const uint16_t*>(bias) + at);
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = bf16 ? dgc::Io<__nv_bfloat16>::unpack2(u[i]) : dgc::Io<__half>::unpack2(u[i]);
+        b[2 * i] = f.x;
+        b[2 * i + 1] = f.y;
+    }
+}
+
+// sums of v[c] over the warp's 32 lanes for c = 0..31: lane c gets column c's
+__device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const float send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+            v[i] = keep + __shfl_xor_sync(DG_FULL_MASK, send, o);
+        }
+    }
+    return v[0];
+}
+
+template <typename T, int ROLE, int ACT, bool A_MN, bool B_MN, bool F32_OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    ffn_tc_kernel(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmb,
+                  const __grid_constant__ CUtensorMap tmd, const __grid_constant__ CUtensorMap tmo, FfnParams p) {
+    using C = Cfg<ROLE>;
+    constexpr bool BF16 = !std::is_same<T, __half>::value;
+    constexpr int ST = C::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::BAR);      // [ST], counted in the even CTA
+    uint64_t* empty = full + ST;                                    // [ST]
+    uint64_t* acc_full = empty + ST;                                // [2]
+    uint64_t* acc_empty = acc_full + 2;                             // [2], counted in the even CTA
+    uint64_t* dh_full = acc_empty + 2;                              // [2] one per epilogue group
+    uint64_t* dh_empty = dh_full + 2;                               // [2]
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dh_empty + 2);
+    int* aborted = reinterpret_cast<int*>(tmem_holder + 1);
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const uint32_t rank = cta_rank();
+    const int64_t items = (int64_t)p.m_tiles * p.n_tiles * p.splits;
+    const int64_t first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+    const int nkb_all = (p.K + BK - 1) / BK;
+
+    if (warp == 0) tmem_alloc_pair(tmem_holder, 512);
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            tc::mbar_init(full + i, 1);
+            tc::mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(acc_full + i, 1);
+            tc::mbar_init(acc_empty + i, 4);
+            tc::mbar_init(dh_full + i, 1);
+            tc::mbar_init(dh_empty + i, 1);
+        }
+        *aborted = 0;
+        tc::fence_barrier_init();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    bool bad = false;
+
+    if (warp == 0 && (tid & 31) == 0) {
+        // ============================ operand loads ============================
+        tc::prefetch_tmap(&tma);
+        tc::prefetch_tmap(&tmb);
+        int s = 0;
+        uint32_t ph = 1;                       // the empty barriers' first phase counts as passed
+        for (int64_t it = first; it < items && !bad; it += stride) {
+            const Work w = work_of(p, it);
+            const int row = w.mt * 2 * BM + (int)rank * BM;
+            // B's half of this CTA: GATE / DGATE the gate or the value rows, PLAIN columns
+            const int col = ROLE == PLAIN ? w.nt * BN + (int)rank * BM : (int)rank * p.N + w.nt * BM;
+            const int kb0 = w.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, nkb_all);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!tc::mbar_wait(empty + s, ph, p.wait_limit)) { bad = true; break; }
+                if (rank == 0) tc::mbar_expect_tx(full + s, 4 * TILE);
+                const uint32_t bar = in_leader(full + s);
+                uint8_t* a = sm + s * 2 * TILE;
+                uint8_t* b = a + TILE;
+                const int k = kb * BK;
+                if (A_MN) {
+                    tma_load_pair(a, &tma, bar, row, k);
+                    tma_load_pair(a + TILE / 2, &tma, bar, row + 64, k);
+                } else {
+                    tma_load_pair(a, &tma, bar, k, row);
+                }
+                if (B_MN) {
+                    tma_load_pair(b, &tmb, bar, col, k);
+                    tma_load_pair(b + TILE / 2, &tmb, bar, col + 64, k);
+                } else {
+                    tma_load_pair(b, &tmb, bar, k, col);
+                }
+                if (++s == ST) { s = 0; ph ^= 1; }
+            }
+        }
+    } else if (warp == 1 && rank == 0 && (tid & 31) == 0) {
+        // ================================= MMAs =================================
+        constexpr uint32_t idesc = tc::make_idesc(2 * BM, BN, BF16 ? 1 : 0, A_MN ? 1 : 0, B_MN ? 1 : 0);
+        int s = 0, acc = 0;
+        uint32_t ph = 0, acc_ph = 1;
+        for (int64_t it = first; it < items && !bad; it += stride) {
+            const Work w = work_of(p, it);
+            const int kb0 = w.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, nkb_all);
+            if (!tc::mbar_wait(acc_empty + acc, acc_ph, p.wait_limit)) { bad = true; break; }
+            tc::tc_fence_after();
+            const uint32_t d = tmem + acc * BN;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!tc::mbar_wait(full + s, ph, p.wait_limit)) { bad = true; break; }
+                tc::tc_fence_after();
+                const uint32_t a = tc::smem_u32(sm + s * 2 * TILE), b = a + TILE;
+#pragma unroll
+                for (int kk = 0; kk < BK / 16; ++kk) {
+                    // K-major: 16 elements are 32 bytes of each 128-byte row, 8 rows 1024 bytes apart.
+                    // MN-major: 16 k-rows of 128 bytes; the two blocks of 64 are TILE / 2 apart.
+                    const uint64_t ad = A_MN ? tc::make_desc(a + kk * 2048, TILE / 2, 1024)
+                                             : tc::make_desc(a + kk * 32, 16, 1024);
+                    const uint64_t bd = B_MN ? tc::make_desc(b + kk * 2048, TILE / 2, 1024)
+                                             : tc::make_desc(b + kk * 32, 16, 1024);
+                    mma_pair(d, ad, bd, idesc, kb != kb0 || kk != 0);
+                }
+                commit_pair(empty + s);
+                if (++s == ST) { s = 0; ph ^= 1; }
+            }
+            if (bad) break;
+            commit_pair(acc_full + acc);
+            if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+        }
+    } else if (ROLE == DGATE && warp == 2 && (tid & 31) == 0) {
+        // ============================ dh tiles ============================
+        uint32_t ph = 1;
+        for (int64_t it = first; it < items && !bad; it += stride, ph ^= 1) {
+            const Work w = work_of(p, it);
+            for (int g = 0; g < 2; ++g) {
+                if (!tc::mbar_wait(dh_empty + g, ph, p.wait_limit)) { bad = true; break; }
+                tc::mbar_expect_tx(dh_full + g, TILE);
+                tc::tma_load_2d(sm + C::DH + g * TILE, &tmd, dh_full + g, w.nt * BM + 64 * g,
+                                w.mt * 2 * BM + (int)rank * BM);
+            }
+        }
+    } else if (warp >= 4) {
+        // =============================== epilogue ===============================
+        const int g = (warp - 4) >> 2, t = tid - 128 - 128 * g, lane = tid & 31;
+        const uint32_t bar_id = 1 + g;
+        const uint32_t trow = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        uint8_t* out = sm + C::OUT + g * TILE;
+        uint8_t* dh = sm + C::DH + g * TILE;
+        int acc = 0;
+        uint32_t acc_ph = 0, dh_ph = 0;
+        // the buffer's last TMA store has read it
+        auto buffer_free = [&]() {
+            if (t == 0) tc::bulk_wait_read0();
+            tc::group_sync(bar_id);
+        };
+        auto release_acc = [&]() {
+            tc::tc_fence_before();
+            tc::group_sync(bar_id);
+            if (t == 0) arrive_at(in_leader(acc_empty + acc));
+        };
+        for (int64_t it = first; it < items; it += stride) {
+            const Work w = work_of(p, it);
+            const int row0 = w.mt * 2 * BM + (int)rank * BM;
+            bad = !tc::mbar_wait(acc_full + acc, acc_ph, p.wait_limit);
+            if (ROLE == DGATE && !bad) bad = !tc::mbar_wait(dh_full + g, dh_ph, p.wait_limit);
+            if (tc::group_sync_or(bar_id, bad)) { bad = true; break; }
+            tc::tc_fence_after();
+            const uint32_t d = trow + acc * BN;
+            if (ROLE != PLAIN) {
+                const int f0 = w.nt * BM + 64 * g;             // this group's 64 features
+                buffer_free();
+                float sums[4];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t gr[32], ur[32];
+                    tc::tmem_ld32(d + 64 * g + 32 * half, gr);
+                    tc::tmem_ld32(d + BM + 64 * g + 32 * half, ur);
+                    tc::tmem_wait_ld();
+                    if (half == 1 && ROLE == GATE) release_acc();
+                    float zg[32], zu[32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float bg[8] = {}, bu[8] = {};
+                        const int f = f0 + 32 * half + 8 * c;
+                        if (p.bias && f < p.N) {
+                            load_bias8(p.bias, f, BF16, bg);
+                            load_bias8(p.bias, (int64_t)p.N + f, BF16, bu);
+                        }
+                        const uint32_t at = tc::sw128((uint32_t)t, (uint32_t)(4 * half + c));
+                        uint32_t o[4], o2[4], q[4];
+                        if (ROLE == DGATE) *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(dh + at);
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            const int i = 8 * c + e;
+                            const float g0 = __uint_as_float(gr[i]) + bg[e], g1 = __uint_as_float(gr[i + 1]) + bg[e + 1];
+                            const float u0 = __uint_as_float(ur[i]) + bu[e], u1 = __uint_as_float(ur[i + 1]) + bu[e + 1];
+                            if (ROLE == GATE) {
+                                o[e / 2] = dgc::Io<T>::pack2(dg::act_fn<ACT>(g0) * u0, dg::act_fn<ACT>(g1) * u1);
+                            } else {
+                                const float2 dv = dgc::Io<T>::unpack2(q[e / 2]);
+                                float a0, a1, s0, s1;
+                                dg::act_grad<ACT>(g0, a0, s0);
+                                dg::act_grad<ACT>(g1, a1, s1);
+                                zg[i] = dv.x * u0 * s0;
+                                zg[i + 1] = dv.y * u1 * s1;
+                                zu[i] = dv.x * a0;
+                                zu[i + 1] = dv.y * a1;
+                                o[e / 2] = dgc::Io<T>::pack2(zg[i], zg[i + 1]);
+                                o2[e / 2] = dgc::Io<T>::pack2(zu[i], zu[i + 1]);
+                            }
+                        }
+                        if (ROLE == GATE) {
+                            *reinterpret_cast<uint4*>(out + at) = *reinterpret_cast<const uint4*>(o);
+                        } else {      // dG takes dh's place
+                            *reinterpret_cast<uint4*>(dh + at) = *reinterpret_cast<const uint4*>(o);
+                            *reinterpret_cast<uint4*>(out + at) = *reinterpret_cast<const uint4*>(o2);
+                        }
+                    }
+                    if (ROLE == DGATE && p.colsum) {
+                        sums[2 * half] = column_sums(zg, lane);
+                        sums[2 * half + 1] = column_sums(zu, lane);
+                    }
+                }
+                if (ROLE == DGATE) {
+                    release_acc();
+                    if (p.colsum) {
+                        float* dst = p.colsum + ((int64_t)(w.mt * 2 + (int)rank) * 4 + (warp & 3)) * 2 * p.N;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int f = f0 + 32 * half + lane;
+                            if (f < p.N) {
+                                dst[f] = sums[2 * half];
+                                dst[p.N + f] = sums[2 * half + 1];
+                            }
+                        }
+                    }
+                }
+                tc::fence_proxy_async();
+                tc::group_sync(bar_id);
+                if (t == 0) {
+                    if (f0 < p.N && row0 < p.M) {
+                        if (ROLE == GATE) {
+                            tc::tma_store_2d(&tmo, out, f0, row0);
+                        } else {
+                            tc::tma_store_3d(&tmo, dh, f0, 0, row0);
+                            tc::tma_store_3d(&tmo, out, f0, 1, row0);
+                        }
+                    }
+                    tc::bulk_commit_group();
+                    if (ROLE == DGATE) {               // dG has been read: the next dh may land there
+                        tc::bulk_wait_read0();
+                        tc::mbar_arrive(dh_empty + g);
+                    }
+                }
+            } else {
+                constexpr int W = F32_OUT ? 32 : 64;   // columns of a slice of 128 bytes
+#pragma unroll 1
+                for (int j = g; j < BN / W; j += 2) {
+                    const int col = w.nt * BN + W * j;
+                    uint32_t ra[32], rb[32];
+                    tc::tmem_ld32(d + W * j, ra);
+                    if (!F32_OUT) tc::tmem_ld32(d + W * j + 32, rb);
+                    tc::tmem_wait_ld();
+                    if (j + 2 >= BN / W) release_acc();
+                    buffer_free();
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (F32_OUT) {
+                                o[e] = ra[4 * c + e];
+                            } else {
+                                const int i = (8 * c + 2 * e) & 31;
+                                o[e] = c < 4 ? dgc::Io<T>::pack2(__uint_as_float(ra[i]), __uint_as_float(ra[i + 1]))
+                                             : dgc::Io<T>::pack2(__uint_as_float(rb[i]), __uint_as_float(rb[i + 1]));
+                            }
+                        }
+                        *reinterpret_cast<uint4*>(out + tc::sw128((uint32_t)t, (uint32_t)c)) =
+                            *reinterpret_cast<const uint4*>(o);
+                    }
+                    tc::fence_proxy_async();
+                    tc::group_sync(bar_id);
+                    if (t == 0) {
+                        if (col < p.N && row0 < p.M) tc::tma_store_3d(&tmo, out, col, row0, w.split);
+                        tc::bulk_commit_group();
+                    }
+                }
+            }
+            if (++acc == 2) { acc = 0; acc_ph ^= 1; }
+            dh_ph ^= 1;
+        }
+        if (t == 0) tc::bulk_wait0();
+    }
+    if (bad) {
+        dg::flag_status(p.status, DG_DEVCHK_TIMEOUT);
+        *aborted = 1;
+    }
+    __syncwarp();
+    tc::tc_fence_before();
+    __syncthreads();
+    if (*aborted) {              // loads and products in flight land within microseconds
+        const uint64_t t0 = tc::globaltimer_ns();
+        for (int i = 0; i < (1 << 20) && tc::globaltimer_ns() - t0 < 2000000; ++i) __nanosleep(1000);
+    }
+    __syncwarp();
+    cluster_sync();
+    if (warp == 0) {
+        tc::tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+// dbias[c] = sum over the 32-row sums, in a fixed order: warp w of the block takes rows w, w + 8, ...
+template <typename T>
+__global__ void __launch_bounds__(256) colsum_kernel(int rows, int cols, const float* part, T* out) {
+    __shared__ float s[8][32];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+    float a = 0.f;
+    if (c < cols)
+        for (int r = w; r < rows; r += 8) a += part[(int64_t)r * cols + c];
+    s[w][threadIdx.x & 31] = a;
+    __syncthreads();
+    if (w == 0 && c < cols) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v += s[i][threadIdx.x];
+        out[c] = dg::from_f<T>(v);
+    }
+}
+
+// out = sum of the fp32 partial products, in order of the splits
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(int64_t n8, int splits, const float4* part, uint4* out) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n8) return;
+    float4 a = part[2 * i], b = part[2 * i + 1];
+    for (int s = 1; s < splits; ++s) {
+        const float4 c = part[2 * (n8 * s + i)], d = part[2 * (n8 * s + i) + 1];
+        a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+        b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
+    }
+    uint4 v;
+    v.x = dgc::Io<T>::pack2(a.x, a.y);
+    v.y = dgc::Io<T>::pack2(a.z, a.w);
+    v.z = dgc::Io<T>::pack2(b.x, b.y);
+    v.w = dgc::Io<T>::pack2(b.z, b.w);
+    out[i] = v;
+}
+
+CUtensorMapDataType map_type(bool bf16) {
+    return bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// rank-2 or rank-3 map with 128-byte rows in the box, 128B swizzle; strides in bytes
+bool make_tmap(CUtensorMap* m, CUtensorMapDataType type, const void* base, int rank, const cuuint64_t* dims,
+               const cuuint64_t* strides, const cuuint32_t* box) {
+    dgc::EncodeTiledFn fn = dgc::encode_fn();
+    if (!fn) return false;
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(m, type, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// 16-bit [rows][cols] matrix, box of 64 columns x box_rows
+bool map_matrix(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, bool bf16) {
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    return make_tmap(m, map_type(bf16), base, 2, dims, strides, box);
+}
+
+}  // namespace
+
+namespace dg_host {
+
+uint32_t wait_limit();
+int sm_count(int device, int* out);
+
+namespace {
+
+int pairs(int* out) {
+    int dev = 0, nsm = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    const int rc = sm_count(dev, &nsm);
+    *out = nsm / 2;
+    return rc;
+}
+
+template <typename K>
+int launch(K kern, uint32_t smem, int64_t items, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d,
+           const CUtensorMap& o, const FfnParams& p, cudaStream_t s) {
+    int np = 0;
+    const int rc = pairs(&np);
+    if (rc != DG_OK) return rc;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem + 1024);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    kern<<<(unsigned)(2 * (items < np ? items : np)), THREADS, smem + 1024, s>>>(a, b, d, o, p);
+    return check_launch();
+}
+
+FfnParams tiles_of(int64_t M, int N, int K, int tile_n, int32_t* status) {
+    FfnParams p{};
+    p.M = M, p.N = N, p.K = K;
+    p.m_tiles = (int)((M + 2 * BM - 1) / (2 * BM));
+    p.n_tiles = (N + tile_n - 1) / tile_n;
+    p.splits = 1;
+    p.kb_per_split = (K + BK - 1) / BK;
+    p.status = status;
+    p.wait_limit = wait_limit();
+    return p;
+}
+
+// splits of a PLAIN product whose tiles would not fill the pairs: as many as fit one wave, each
+// with at least 8 stages of the contracted axis (below that the pipeline hardly fills)
+int splits_of(int64_t M, int N, int64_t K, int np) {
+    const int64_t tiles = ((M + 2 * BM - 1) / (2 * BM)) * ((N + BN - 1) / BN);
+    const int64_t nkb = (K + BK - 1) / BK;
+    int64_t s = np / (tiles > 0 ? tiles : 1);
+    if (s > nkb / 8) s = nkb / 8;
+    return (int)(s < 1 ? 1 : s);
+}
+
+// C [M,N] = A B, contracted length K; A as [M,K] (a_mn: [K,M]), B as [N,K] (b_mn: [K,N])
+template <typename T, bool A_MN, bool B_MN>
+int product(int64_t M, int N, int64_t K, const void* a, int64_t lda, const void* b, int64_t ldb, void* c, float* part,
+            int splits, int32_t* status, cudaStream_t s) {
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    FfnParams p = tiles_of(M, N, (int)K, BN, status);
+    const int nkb = p.kb_per_split;
+    p.kb_per_split = (nkb + splits - 1) / splits;
+    p.splits = splits = (nkb + p.kb_per_split - 1) / p.kb_per_split;       // none empty
+    CUtensorMap ma, mb, mo;
+    bool ok = A_MN ? map_matrix(&ma, a, K, M, lda, BK, bf16) : map_matrix(&ma, a, M, K, lda, BM, bf16);
+    ok = ok && (B_MN ? map_matrix(&mb, b, K, N, ldb, BK, bf16) : map_matrix(&mb, b, N, K, ldb, BM, bf16));
+    const int e = splits > 1 ? 4 : 2;
+    cuuint64_t dims[3] = {(cuuint64_t)N, (cuuint64_t)M, (cuuint64_t)splits};
+    cuuint64_t strides[2] = {(cuuint64_t)N * e, (cuuint64_t)N * e * (cuuint64_t)M};
+    cuuint32_t box[3] = {(cuuint32_t)(128 / e), BM, 1};
+    ok = ok && make_tmap(&mo, splits > 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : map_type(bf16),
+                         splits > 1 ? static_cast<void*>(part) : c, 3, dims, strides, box);
+    if (!ok) return DG_ERR_UNSUPPORTED;
+    const int64_t items = (int64_t)p.m_tiles * p.n_tiles * p.splits;
+    if (splits == 1)
+        return launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, false>, Cfg<PLAIN>::BYTES, items, ma, mb, ma, mo, p, s);
+    const int rc = launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, true>, Cfg<PLAIN>::BYTES, items, ma, mb, ma, mo, p, s);
+    if (rc != DG_OK) return rc;
+    const int64_t n8 = M * N / 8;
+    join_kernel<T><<<(unsigned)((n8 + 255) / 256), 256, 0, s>>>(n8, splits, reinterpret_cast<const float4*>(part),
+                                                               static_cast<uint4*>(c));
+    return check_launch();
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+struct Spaces {
+    size_t dz, colsum, part, total;
+    int splits_dx, splits_dw;
+};
+Spaces spaces(int64_t M, int D, int F) {
+    int np = 74;
+    if (pairs(&np) != DG_OK) np = 74;          // no device here: the size for a whole B200
+    Spaces w;
+    w.splits_dx = splits_of(M, D, 2 * (int64_t)F, np);
+    w.splits_dw = splits_of(2 * (int64_t)F, D, M, np);
+    w.dz = round256((size_t)M * 2 * F * 2);
+    w.colsum = round256((size_t)((M + 2 * BM - 1) / (2 * BM)) * 8 * 2 * F * 4);
+    const size_t dx = w.splits_dx > 1 ? (size_t)w.splits_dx * M * D * 4 : 0;
+    const size_t dw = w.splits_dw > 1 ? (size_t)w.splits_dw * 2 * F * D * 4 : 0;
+    w.part = round256(dx > dw ? dx : dw);
+    w.total = w.dz + w.colsum + w.part;
+    return w;
+}
+
+}  // namespace
+
+// 16-bit types whose rows TMA can address: D and F multiples of 8, 16-byte aligned tensors
+bool ffn_tc_supports(int dtype, int64_t M, int D, int F) {
+    return (dtype == DG_DTYPE_F16 || dtype == DG_DTYPE_BF16) && D % 8 == 0 && F % 8 == 0 && M <= (int64_t)1 << 30;
+}
+bool ffn_tc_aligned(const void* a, int64_t lda, const void* b, const void* c, const void* d, int64_t ldd,
+                    const void* e, const void* f) {
+    return aligned(a) && aligned(b) && aligned(c) && aligned(d) && aligned(e) && aligned(f) && lda % 8 == 0 &&
+           ldd % 8 == 0;
+}
+
+template <typename T>
+static int forward_t(int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w, const void* bias,
+                     void* h, int32_t* status, cudaStream_t s) {
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    FfnParams p = tiles_of(M, F, D, BM, status);
+    p.bias = bias;
+    CUtensorMap mx, mw, mh;
+    if (!map_matrix(&mx, x, M, D, ldx, BM, bf16) || !map_matrix(&mw, w, 2 * (int64_t)F, D, D, BM, bf16) ||
+        !map_matrix(&mh, h, M, F, F, BM, bf16))
+        return DG_ERR_UNSUPPORTED;
+    const int64_t items = (int64_t)p.m_tiles * p.n_tiles;
+    return act == DG_ACT_SILU
+               ? launch(ffn_tc_kernel<T, GATE, DG_ACT_SILU, false, false, false>, Cfg<GATE>::BYTES, items, mx, mw, mx,
+                        mh, p, s)
+               : launch(ffn_tc_kernel<T, GATE, DG_ACT_GELU, false, false, false>, Cfg<GATE>::BYTES, items, mx, mw, mx,
+                        mh, p, s);
+}
+
+int ffn_tc_forward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
+                   const void* bias, void* h, int32_t* status, cudaStream_t s) {
+    return dtype == DG_DTYPE_F16 ? forward_t<__half>(M, D, F, act, x, ldx, w, bias, h, status, s)
+                                 : forward_t<__nv_bfloat16>(M, D, F, act, x, ldx, w, bias, h, status, s);
+}
+
+size_t ffn_tc_workspace(int64_t M, int D, int F) { return spaces(M, D, F).total; }
+
+template <typename T>
+static int backward_t(int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w, const void* bias,
+                      const void* dh, int64_t ld_dh, void* dx, void* dw, void* db, void* workspace, int32_t* status,
+                      cudaStream_t s) {
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    const Spaces sp = spaces(M, D, F);
+    char* ws = static_cast<char*>(workspace);
+    void* dz = ws;
+    float* colsum = reinterpret_cast<float*>(ws + sp.dz);
+    float* part = reinterpret_cast<float*>(ws + sp.dz + sp.colsum);
+    FfnParams p = tiles_of(M, F, D, BM, status);
+    p.bias = bias;
+    p.colsum = db ? colsum : nullptr;
+    CUtensorMap mx, mw, md, mz;
+    cuuint64_t dims[3] = {(cuuint64_t)F, 2, (cuuint64_t)M};
+    cuuint64_t strides[2] = {(cuuint64_t)F * 2, (cuuint64_t)F * 4};
+    cuuint32_t box[3] = {64, 1, BM};
+    if (!map_matrix(&mx, x, M, D, ldx, BM, bf16) || !map_matrix(&mw, w, 2 * (int64_t)F, D, D, BM, bf16) ||
+        !map_matrix(&md, dh, M, F, ld_dh, BM, bf16) || !make_tmap(&mz, map_type(bf16), dz, 3, dims, strides, box))
+        return DG_ERR_UNSUPPORTED;
+    const int64_t items = (int64_t)p.m_tiles * p.n_tiles;
+    int rc = act == DG_ACT_SILU
+                 ? launch(ffn_tc_kernel<T, DGATE, DG_ACT_SILU, false, false, false>, Cfg<DGATE>::BYTES, items, mx, mw,
+                          md, mz, p, s)
+                 : launch(ffn_tc_kernel<T, DGATE, DG_ACT_GELU, false, false, false>, Cfg<DGATE>::BYTES, items, mx, mw,
+                          md, mz, p, s);
+    if (rc == DG_OK && dx)
+        rc = product<T, false, true>(M, D, 2 * (int64_t)F, dz, 2 * (int64_t)F, w, D, dx, part, sp.splits_dx, status, s);
+    if (rc == DG_OK && dw)
+        rc = product<T, true, true>(2 * (int64_t)F, D, M, dz, 2 * (int64_t)F, x, ldx, dw, part, sp.splits_dw, status, s);
+    if (rc == DG_OK && db) {
+        colsum_kernel<T><<<(2 * F + 31) / 32, 256, 0, s>>>(p.m_tiles * 8, 2 * F, colsum, static_cast<T*>(db));
+        rc = check_launch();
+    }
+    return rc;
+}
+
+int ffn_tc_backward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
+                    const void* bias, const void* dh, int64_t ld_dh, void* dx, void* dw, void* db, void* workspace,
+                    int32_t* status, cudaStream_t s) {
+    return dtype == DG_DTYPE_F16
+               ? backward_t<__half>(M, D, F, act, x, ldx, w, bias, dh, ld_dh, dx, dw, db, workspace, status, s)
+               : backward_t<__nv_bfloat16>(M, D, F, act, x, ldx, w, bias, dh, ld_dh, dx, dw, db, workspace, status, s);
+}
+
+}  // namespace dg_host
