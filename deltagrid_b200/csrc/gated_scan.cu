@@ -3,34 +3,41 @@
 //
 // A run of steps acts on the state as h -> P h + H (P the product of its c, H its end state
 // from zero), and such maps compose, so the sequence splits along time:
-//   - a thread takes R = 8 consecutive steps of VEC channels; its maps are composed with its
-//     neighbours' by shuffles and, through shared memory, with the other warps';
-//   - a CTA (256 threads) takes a tile of 256 / LPR x 8 steps by LPR x VEC channels and
-//     walks the sequence tile by tile with the state in registers;
+//   - a thread takes R consecutive steps of VEC channels and composes its map with its
+//     neighbours' by shuffles;
+//   - a CTA (256 threads) takes a tile of 256 / LPR x R steps by LPR x VEC channels: each warp
+//     leaves its map in shared memory, one thread per channel carries the state through them,
+//     and every thread applies its steps to the state it starts from.  The CTA walks the
+//     sequence tile by tile;
 //   - where rows and channels give too few CTAs, a cluster of up to 16 takes consecutive
 //     tiles and exchanges their maps through distributed shared memory, one cluster barrier
 //     per tile.
 // Each input is read and each output written once.  The order of every composition is fixed
 // by the sizes alone, so results repeat bit for bit.
 //
-// Inputs come by cp.async into shared memory that only the copying thread reads, one tile
-// ahead: no registers are held for data in flight and no barrier waits for it.
+// Inputs come one tile ahead by cp.async into shared memory that only the copying warp (or
+// thread) reads: no registers are held for data in flight and no CTA barrier waits for it.
 //
 // The backward pass carries r_t = c_t (d_t + r_{t+1}) (d the gradient that enters at step t)
 // the same way in reverse, and forms the states again from the marks that the forward pass
 // leaves every DG_SCAN_MARK_STEPS steps: fp32 states, so nothing is lost to the rounding of
 // y, for 4 / 64 bytes a step.
+//
+// What bounds it: HBM at 4 (forward, 16-bit) to 14 bytes (backward) an element, with the
+// special-function unit close behind (two operations for each sigmoid); pairs of channels use
+// the two-wide fp32 instructions to keep the issue slots free.
 #include <type_traits>
 
 #include "lm_common.cuh"
 
 namespace {
 
-constexpr int R = 8;                       // consecutive steps per thread
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int STAGES = 2;                  // tiles of input in shared memory
-static_assert(DG_SCAN_MARK_STEPS % R == 0, "a mark falls on a thread's first step");
+// steps per thread: forward as many as registers and shared memory allow
+template <typename T> constexpr int kForwardSteps = sizeof(T) == 4 ? 8 : 16;
+constexpr int kBackwardSteps = 8;
 
 struct ScanIn {
     const void *x, *g, *o;
@@ -50,15 +57,16 @@ struct ScanGrad {
     float* dh0;
 };
 
-// ---- cp.async ------------------------------------------------------------------
-// copies BYTES (4 or 8), or zeros where !on
+// ---- cp.async and clusters -------------------------------------------------------
+// copies BYTES (4, 8 or 16), or zeros where !on
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* dst, const void* src, bool on) {
     const int n = on ? BYTES : 0;
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(
-                     (uint32_t)__cvta_generic_to_shared(dst)),
-                 "l"(src), "n"(BYTES), "r"(n)
-                 : "memory");
+    const uint32_t a = (uint32_t)__cvta_generic_to_shared(dst);
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(a), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(a), "l"(src), "n"(BYTES), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -77,410 +85,517 @@ __device__ __forceinline__ void store_remote(float2* p, uint32_t rank, float2 v)
     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(v.x), "f"(v.y) : "memory");
 }
 
+// ---- one or two channels at a time ------------------------------------------------
+template <int VEC> struct alignas(4 * VEC) Fv {
+    float v[VEC];
+};
+template <int VEC> __device__ __forceinline__ Fv<VEC> all(float x) {
+    Fv<VEC> r;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r.v[i] = x;
+    return r;
+}
+__device__ __forceinline__ Fv<1> vfma(Fv<1> a, Fv<1> b, Fv<1> c) { return {fmaf(a.v[0], b.v[0], c.v[0])}; }
+__device__ __forceinline__ Fv<1> vmul(Fv<1> a, Fv<1> b) { return {a.v[0] * b.v[0]}; }
+__device__ __forceinline__ Fv<1> vadd(Fv<1> a, Fv<1> b) { return {a.v[0] + b.v[0]}; }
+__device__ __forceinline__ uint64_t bits(Fv<2> a) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v[0]), "f"(a.v[1]));
+    return r;
+}
+__device__ __forceinline__ Fv<2> unbits(uint64_t a) {
+    Fv<2> r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.v[0]), "=f"(r.v[1]) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ Fv<2> vfma(Fv<2> a, Fv<2> b, Fv<2> c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return unbits(r);
+}
+__device__ __forceinline__ Fv<2> vmul(Fv<2> a, Fv<2> b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return unbits(r);
+}
+__device__ __forceinline__ Fv<2> vadd(Fv<2> a, Fv<2> b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return unbits(r);
+}
+
 // VEC storage elements
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack {
     T v[VEC];
 };
-
-// maps of a tile, per channel: one per warp, and one per CTA of the cluster
-template <int CH> struct Maps {
-    float2 warp[2][WARPS][CH];             // (P, H)
-    float2 cta[2][16][CH];
-};
-
-template <typename T, int VEC, int LPR, int ARRAYS> struct Tile {
-    static constexpr int GROUPS = THREADS / LPR, STEPS = GROUPS * R, CH = LPR * VEC;
-    typedef Pack<T, VEC> P;
-    static constexpr size_t STAGE = (size_t)ARRAYS * R * THREADS * sizeof(P);
-};
-
-// one thread's 8 steps of one input into its own column of the stage
-template <typename T, int VEC>
-__device__ __forceinline__ void fetch(Pack<T, VEC>* st, const T* p, int64_t step, int n, bool on) {
+template <typename T, int VEC> __device__ __forceinline__ Fv<VEC> widen(const Pack<T, VEC>& p) {
+    Fv<VEC> r;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value && VEC == 2) {
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(&p);
+        r.v[0] = __uint_as_float(u << 16);
+        r.v[1] = __uint_as_float(u & 0xffff0000u);
+    } else {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const bool live = on && r < n;
-        if constexpr (sizeof(T) * VEC >= 4) {
-            copy_async<sizeof(T) * VEC>(st + r * THREADS, live ? p + r * step : p, live);
-        } else {                           // 2 bytes: below what cp.async copies
-            T z = dg::from_f<T>(0.f);
-            if (live) z = p[r * step];
-            st[r * THREADS].v[0] = z;
+        for (int i = 0; i < VEC; ++i) r.v[i] = dg::to_f(p.v[i]);
+    }
+    return r;
+}
+template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> narrow(Fv<VEC> a) {
+    Pack<T, VEC> p;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value && VEC == 2) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a.v[0], a.v[1]);
+        p = *reinterpret_cast<const Pack<T, VEC>*>(&h);
+    } else if constexpr (std::is_same<T, __half>::value && VEC == 2) {
+        const __half2 h = __floats2half2_rn(a.v[0], a.v[1]);
+        p = *reinterpret_cast<const Pack<T, VEC>*>(&h);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) p.v[i] = dg::from_f<T>(a.v[i]);
+    }
+    return p;
+}
+
+// a = sigmoid(z) and na = 1 - a = exp(-z) a, each to fp32's relative precision for z > -80
+template <int VEC> __device__ __forceinline__ void gates(Fv<VEC> z, Fv<VEC>& a, Fv<VEC>& na) {
+    Fv<VEC> e = vmul(z, all<VEC>(-1.4426950408889634f));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e.v[i] = dg::exp2_ftz(fminf(e.v[i], 115.f));
+    a = vadd(e, all<VEC>(1.f));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) a.v[i] = dg::rcp_ftz(a.v[i]);
+    na = vmul(e, a);
+}
+template <int VEC> __device__ __forceinline__ Fv<VEC> silu(Fv<VEC> z) {
+    Fv<VEC> a, na;
+    gates(z, a, na);
+    return vmul(z, a);
+}
+
+// What a CTA keeps of its tile, per channel; the maps of the cluster's CTAs (two tiles' worth of
+// [cluster][CH]) lie behind the input stages
+template <int CH> struct Maps {
+    float2 warp[WARPS][CH];                // each warp's (P, H)
+    float carry[WARPS][CH];                // the state each warp starts from
+};
+template <int CH> struct MapsBack : Maps<CH> {
+    float back[WARPS][CH];                 // each warp's Q of the reverse map
+    float carry_back[WARPS][CH];
+};
+
+template <typename T, int VEC, int LPR, int R, int ARRAYS> struct Tile {
+    static constexpr int STEPS = THREADS / LPR * R, CH = LPR * VEC;
+    static constexpr int WARP_STEPS = 32 / LPR * R;
+    typedef Pack<T, VEC> P;
+    // one input's tile: [warp][step of the warp][channel]
+    static constexpr int ARRAY = THREADS * R;                     // packs
+    static constexpr size_t STAGE = (size_t)ARRAYS * ARRAY * sizeof(P);
+    static constexpr size_t bytes(int cluster) {
+        return STAGES * STAGE + (cluster > 1 ? 2 * cluster * CH * sizeof(float2) : 0);
+    }
+};
+
+// A warp's steps of one input into its part of a stage.  WIDE: 16 bytes a lane, any lane any
+// step of the warp.  Otherwise each thread copies the steps it reads itself.
+template <typename T, int VEC, int LPR, int R, bool WIDE>
+__device__ __forceinline__ void fetch(Pack<T, VEC>* warp_part, const T* row, int64_t step, int t_warp, int len, int d0,
+                                      int D, int lane) {
+    constexpr int PPS = LPR;                                      // packs per step
+    if constexpr (WIDE) {
+        constexpr int E = 16 / sizeof(T), CPS = LPR * VEC / E, N = 32 / LPR * R * CPS / 32;
+        const int col = lane % CPS * E;
+        const bool on = d0 + col < D;
+        const T* p = row + (int64_t)(t_warp + lane / CPS) * step + d0 + col;
+        T* dst = reinterpret_cast<T*>(warp_part) + lane * E;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int s = lane / CPS + i * (32 / CPS);
+            const bool live = on && t_warp + s < len;
+            copy_async<16>(dst + i * 32 * E, live ? p : row, live);
+            p += (32 / CPS) * step;
+        }
+    } else {
+        const int lc = lane % LPR, s0 = lane / LPR * R, d = d0 + lc * VEC;
+        const T* p = row + (int64_t)(t_warp + s0) * step + d;
+        Pack<T, VEC>* dst = warp_part + s0 * PPS + lc;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const bool live = d < D && t_warp + s0 + r < len;
+            if constexpr (sizeof(T) * VEC >= 4) {
+                copy_async<sizeof(T) * VEC>(dst + r * PPS, live ? p : row, live);
+            } else {                       // 2 bytes: below what cp.async copies
+                T z = dg::from_f<T>(0.f);
+                if (live) z = *p;
+                dst[r * PPS].v[0] = z;
+            }
+            p += step;
         }
     }
 }
 
-// composes (P, H) maps over the row groups of a warp: in: the thread's own map, out: the map of
-// the groups before it; returns the whole warp's map in the last group
-template <int LPR>
-__device__ __forceinline__ void warp_before(float P, float H, float& Pb, float& Hb, float& Pw, float& Hw, int lane) {
+// composes (P, H) maps over the row groups of a warp.  In: the thread's own map; out: the map of
+// the groups before it (FORWARD) or after it, and the whole warp's, which the last (first) group has
+template <int LPR, int VEC, bool FORWARD>
+__device__ __forceinline__ void warp_maps(Fv<VEC> P, Fv<VEC> H, Fv<VEC>& Pb, Fv<VEC>& Hb, Fv<VEC>& Pw, Fv<VEC>& Hw,
+                                          int lane) {
+    auto from = [&](float x, int o) {
+        return FORWARD ? __shfl_up_sync(DG_FULL_MASK, x, o) : __shfl_down_sync(DG_FULL_MASK, x, o);
+    };
 #pragma unroll
-    for (int o = LPR; o < 32; o <<= 1) {
-        const float p = __shfl_up_sync(DG_FULL_MASK, P, o), h = __shfl_up_sync(DG_FULL_MASK, H, o);
-        if (lane >= o) {
-            H = fmaf(P, h, H);
-            P *= p;
+    for (int v = 0; v < VEC; ++v) {
+#pragma unroll
+        for (int o = LPR; o < 32; o <<= 1) {
+            const float p = from(P.v[v], o), h = from(H.v[v], o);
+            if (FORWARD ? lane >= o : lane + o < 32) {
+                H.v[v] = fmaf(P.v[v], h, H.v[v]);
+                P.v[v] *= p;
+            }
+        }
+        Pb.v[v] = 1.f;
+        Hb.v[v] = 0.f;
+        if (LPR < 32) {
+            const float p = from(P.v[v], LPR & 31), h = from(H.v[v], LPR & 31);
+            if (FORWARD ? lane >= LPR : lane + LPR < 32) {
+                Pb.v[v] = p;
+                Hb.v[v] = h;
+            }
         }
     }
     Pw = P;
     Hw = H;
-    Pb = 1.f;
-    Hb = 0.f;
-    if (LPR < 32) {
-        const float p = __shfl_up_sync(DG_FULL_MASK, P, LPR & 31), h = __shfl_up_sync(DG_FULL_MASK, H, LPR & 31);
-        if (lane >= LPR) {
-            Pb = p;
-            Hb = h;
-        }
-    }
 }
-// the same from the other end of the warp; the whole warp's map is in the first group
-template <int LPR>
-__device__ __forceinline__ void warp_after(float P, float Q, float& Pb, float& Qb, float& Pw, float& Qw, int lane) {
+
+// where a thread stands: shared by both passes
+template <int LPR, int VEC, int R> struct Place {
+    int warp, lane, lc, rank, b, d0, d, len, span, ntiles;
+    bool on;
+    __device__ __forceinline__ Place(const ScanIn& in) {
+        constexpr int CH = LPR * VEC, STEPS = THREADS / LPR * R;
+        warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lc = lane % LPR;
+        rank = in.cluster > 1 ? (int)cluster_rank() : 0;
+        const int blocks = (in.D + CH - 1) / CH, unit = blockIdx.x / in.cluster;
+        b = unit / blocks;
+        d0 = unit % blocks * CH;
+        d = d0 + lc * VEC;
+        on = d < in.D;
+        len = in.lengths ? min(max(in.lengths[b], 0), in.T) : in.T;
+        span = in.cluster * STEPS;
+        ntiles = (in.T + span - 1) / span;
+    }
+    // the first step of this warp in tile `it`, and of this thread
+    __device__ __forceinline__ int warp_step(int it) const {
+        return it * span + rank * (THREADS / LPR * R) + warp * (32 / LPR * R);
+    }
+    __device__ __forceinline__ int step(int it) const { return warp_step(it) + lane / LPR * R; }
+};
+
+// bit r: a document starts at step r of this thread.  The loads were made a tile earlier: lane lc
+// of a group holds steps lc and, for R > LPR, lc + LPR.
+template <int LPR, int R> struct Resets {
+    uint8_t next[(R + LPR - 1) / LPR];
+    __device__ __forceinline__ void load(const uint8_t* rs, int t, int lc, int len) {
 #pragma unroll
-    for (int o = LPR; o < 32; o <<= 1) {
-        const float p = __shfl_down_sync(DG_FULL_MASK, P, o), q = __shfl_down_sync(DG_FULL_MASK, Q, o);
-        if (lane + o < 32) {
-            Q = fmaf(P, q, Q);
-            P *= p;
+        for (int i = 0; i < (R + LPR - 1) / LPR; ++i) {
+            const int r = lc + i * LPR;
+            next[i] = (r < R && t + r < len) ? rs[t + r] : 0;
         }
     }
-    Pw = P;
-    Qw = Q;
-    Pb = 1.f;
-    Qb = 0.f;
-    if (LPR < 32) {
-        const float p = __shfl_down_sync(DG_FULL_MASK, P, LPR & 31), q = __shfl_down_sync(DG_FULL_MASK, Q, LPR & 31);
-        if (lane + LPR < 32) {
-            Pb = p;
-            Qb = q;
+    __device__ __forceinline__ unsigned bits(int lane) const {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < (R + LPR - 1) / LPR; ++i) {
+            const unsigned all = __ballot_sync(DG_FULL_MASK, next[i] != 0) >> (lane & ~(LPR - 1));
+            m |= (LPR < 32 ? all & ((1u << (LPR & 31)) - 1) : all) << (i * LPR);
         }
+        return m;
     }
-}
+};
 
-template <typename T, int VEC, int LPR, bool OG>
-__global__ void __launch_bounds__(THREADS, 3)
+template <typename T, int VEC, int LPR, bool WIDE, bool OG>
+__global__ void __launch_bounds__(THREADS, 2)
     scan_forward_kernel(ScanIn in, const float* h0, T* y, float* h_last, float* marks) {
-    typedef Tile<T, VEC, LPR, OG ? 3 : 2> Tl;
+    constexpr int R = kForwardSteps<T>;
+    static_assert(DG_SCAN_MARK_STEPS % R == 0, "a mark falls on a thread's first step");
+    typedef Tile<T, VEC, LPR, R, OG ? 3 : 2> Tl;
     typedef Pack<T, VEC> Pk;
+    typedef Fv<VEC> V;
     extern __shared__ __align__(16) uint8_t smem[];
+    float2* cta_maps = reinterpret_cast<float2*>(smem + STAGES * Tl::STAGE);
     __shared__ Maps<Tl::CH> maps;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int S = in.cluster, rank = S > 1 ? (int)cluster_rank() : 0;
-    const int blocks = (in.D + Tl::CH - 1) / Tl::CH;
-    const int unit = blockIdx.x / S, b = unit / blocks;
-    const int lc = tid % LPR, d = (unit % blocks) * Tl::CH + lc * VEC;
-    const bool on = d < in.D;
-    const int len = in.lengths ? min(max(in.lengths[b], 0), in.T) : in.T;
-    const T* x = (const T*)in.x + b * in.x_sb + d;
-    const T* g = (const T*)in.g + b * in.g_sb + d;
-    const T* o = OG ? (const T*)in.o + b * in.o_sb + d : nullptr;
-    const uint8_t* rs = in.resets ? in.resets + (int64_t)b * in.T : nullptr;
+    const Place<LPR, VEC, R> at(in);
+    const int tid = threadIdx.x, S = in.cluster, d = at.d, len = at.len;
+    const T* x = (const T*)in.x + at.b * in.x_sb;
+    const T* g = (const T*)in.g + at.b * in.g_sb;
+    const T* o = OG ? (const T*)in.o + at.b * in.o_sb : nullptr;
+    const uint8_t* rs = in.resets ? in.resets + (int64_t)at.b * in.T : nullptr;
     const int nblk = (in.T + DG_SCAN_MARK_STEPS - 1) / DG_SCAN_MARK_STEPS;
-    Pk* mine = reinterpret_cast<Pk*>(smem) + tid;
-    constexpr int ARR = R * THREADS, STG = (OG ? 3 : 2) * ARR;
-    const int span = S * Tl::STEPS, ntiles = (in.T + span - 1) / span;
-    const int t_first = rank * Tl::STEPS + (tid / LPR) * R;
+    constexpr int ARR = Tl::ARRAY, STG = (OG ? 3 : 2) * ARR;
+    Pk* warp_part = reinterpret_cast<Pk*>(smem) + at.warp * Tl::WARP_STEPS * LPR;
+    const int own = at.lane / LPR * R * LPR + at.lc;              // this thread's first pack in it
 
-    uint8_t next_reset = 0;                // of step lc of this thread's group, for lc < R
+    Resets<LPR, R> rst;
     auto prefetch = [&](int it) {
-        const int t = it * span + t_first;
-        Pk* st = mine + (it & 1) * STG;
-        fetch<T, VEC>(st, x + t * in.x_st, in.x_st, len - t, on);
-        fetch<T, VEC>(st + ARR, g + t * in.g_st, in.g_st, len - t, on);
-        if (OG) fetch<T, VEC>(st + 2 * ARR, o + t * in.o_st, in.o_st, len - t, on);
+        const int t = at.warp_step(it);
+        Pk* st = warp_part + (it & 1) * STG;
+        fetch<T, VEC, LPR, R, WIDE>(st, x, in.x_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, R, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
+        if (OG) fetch<T, VEC, LPR, R, WIDE>(st + 2 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
         copy_commit();
-        if (rs) next_reset = (lc < R && t + lc < len) ? rs[t + lc] : 0;
+        if (rs) rst.load(rs, at.step(it), at.lc, len);
     };
 
-    float state[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) state[v] = (h0 && on) ? h0[(int64_t)b * in.D + d + v] : 0.f;
-    if (ntiles > 0) prefetch(0);
-    for (int it = 0; it < ntiles; ++it) {
-        const int t = it * span + t_first;
-        unsigned resets = 0;
-        if (rs) resets = __ballot_sync(DG_FULL_MASK, next_reset != 0) >> (lane & ~(LPR - 1));
-        if (it + 1 < ntiles) prefetch(it + 1);
+    // thread c < CH carries channel d0 + c from tile to tile
+    float state = 0.f;
+    if (tid < Tl::CH && h0 && at.d0 + tid < in.D) state = h0[(int64_t)at.b * in.D + at.d0 + tid];
+    if (at.ntiles > 0) prefetch(0);
+    for (int it = 0; it < at.ntiles; ++it) {
+        const int t = at.step(it);
+        const unsigned resets = rs ? rst.bits(at.lane) : 0;
+        __syncwarp();                      // the other stage has been read
+        if (it + 1 < at.ntiles) prefetch(it + 1);
         else copy_commit();
         copy_wait<1>();
-        const Pk* st = mine + (it & 1) * STG;
-        float c[R][VEC], u[R][VEC], P[VEC], H[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) P[v] = 1.f, H[v] = 0.f;
+        __syncwarp();
+        const Pk* st = warp_part + (it & 1) * STG + own;
+        V c[R], u[R], P = all<VEC>(1.f), H = all<VEC>(0.f);
+        const bool whole = t + R <= len && resets == 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const Pk xv = st[r * THREADS], gv = st[ARR + r * THREADS];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float a, na;
-                dg::sigmoid_pair(dg::to_f(gv.v[v]), a, na);
-                c[r][v] = t + r < len ? ((resets >> r) & 1 ? 0.f : a) : 1.f;
-                u[r][v] = t + r < len ? na * dg::to_f(xv.v[v]) : 0.f;
-                H[v] = fmaf(c[r][v], H[v], u[r][v]);
-                P[v] *= c[r][v];
+            V na;
+            gates(widen(st[ARR + r * LPR]), c[r], na);
+            u[r] = vmul(na, widen(st[r * LPR]));
+            if (!whole) {
+                if (t + r >= len) c[r] = all<VEC>(1.f), u[r] = all<VEC>(0.f);
+                else if ((resets >> r) & 1) c[r] = all<VEC>(0.f);
             }
+            H = vfma(c[r], H, u[r]);
+            P = vmul(P, c[r]);
         }
-        float Pb[VEC], Hb[VEC];
+        V Pb, Hb, Pw, Hw;
+        warp_maps<LPR, VEC, true>(P, H, Pb, Hb, Pw, Hw, at.lane);
+        if (at.lane >= 32 - LPR)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            float Pw, Hw;
-            warp_before<LPR>(P[v], H[v], Pb[v], Hb[v], Pw, Hw, lane);
-            if (lane >= 32 - LPR) maps.warp[it & 1][warp][lc * VEC + v] = make_float2(Pw, Hw);
-        }
+            for (int v = 0; v < VEC; ++v) maps.warp[at.warp][at.lc * VEC + v] = make_float2(Pw.v[v], Hw.v[v]);
         __syncthreads();
-        float h[VEC];
-        if (S > 1) {
-            for (int i = tid; i < S * Tl::CH; i += THREADS) {       // this CTA's map to every CTA
-                const int ch = i % Tl::CH;
-                float2 m = maps.warp[it & 1][0][ch];
+        float2 m[WARPS];
+        if (tid < Tl::CH) {
 #pragma unroll
-                for (int w = 1; w < WARPS; ++w) {
-                    const float2 n = maps.warp[it & 1][w][ch];
-                    m.y = fmaf(n.x, m.y, n.y);
-                    m.x *= n.x;
-                }
-                store_remote(&maps.cta[it & 1][rank][ch], i / Tl::CH, m);
+            for (int w = 0; w < WARPS; ++w) m[w] = maps.warp[w][tid];
+            if (S > 1) {
+                float2 a = m[0];
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) a = make_float2(a.x * m[w].x, fmaf(m[w].x, a.y, m[w].y));
+                for (int k = 0; k < S; ++k) store_remote(cta_maps + ((it & 1) * S + at.rank) * Tl::CH + tid, k, a);
             }
+        }
+        if (S > 1) {
             __syncwarp();
             cluster_barrier();
         }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const int ch = lc * VEC + v;
-            float s = state[v], mine_s = s;
+        if (tid < Tl::CH) {
+            float s = state;
             if (S > 1) {
+                float mine = s;
                 for (int k = 0; k < S; ++k) {
-                    if (k == rank) mine_s = s;
-                    const float2 m = maps.cta[it & 1][k][ch];
-                    s = fmaf(m.x, s, m.y);
+                    if (k == at.rank) mine = s;
+                    const float2 a = cta_maps[((it & 1) * S + k) * Tl::CH + tid];
+                    s = fmaf(a.x, s, a.y);
                 }
-                state[v] = s;
-                s = mine_s;
+                state = s;
+                s = mine;
             }
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                if (w == warp) mine_s = s;
-                const float2 m = maps.warp[it & 1][w][ch];
-                s = fmaf(m.x, s, m.y);
+                maps.carry[w][tid] = s;
+                s = fmaf(m[w].x, s, m[w].y);
             }
-            if (S == 1) state[v] = s;
-            h[v] = fmaf(Pb[v], mine_s, Hb[v]);
+            if (S == 1) state = s;
         }
-        if (!on) continue;
-        if (marks && t < in.T && t % DG_SCAN_MARK_STEPS == 0)
+        __syncthreads();
+        V h = *reinterpret_cast<const V*>(&maps.carry[at.warp][at.lc * VEC]);
+        h = vfma(Pb, h, Hb);
+        if (at.on) {
+            if (marks && t < in.T && t % DG_SCAN_MARK_STEPS == 0)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) marks[((int64_t)b * nblk + t / DG_SCAN_MARK_STEPS) * in.D + d + v] = h[v];
-        T* yp = y + ((int64_t)b * in.T + t) * in.D + d;
+                for (int v = 0; v < VEC; ++v)
+                    marks[((int64_t)at.b * nblk + t / DG_SCAN_MARK_STEPS) * in.D + d + v] = h.v[v];
+            T* yp = y + ((int64_t)at.b * in.T + t) * in.D + d;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (t + r >= in.T) break;
-            Pk out;
-            Pk ov;
-            if (OG) ov = st[2 * ARR + r * THREADS];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                h[v] = fmaf(c[r][v], h[v], u[r][v]);
-                float w = h[v];
-                if (OG) {
-                    const float z = dg::to_f(ov.v[v]);
-                    w *= z * dg::sigmoid(z);
-                }
-                out.v[v] = dg::from_f<T>(t + r < len ? w : 0.f);
+            for (int r = 0; r < R; ++r) {
+                h = vfma(c[r], h, u[r]);
+                V w = h;
+                if (OG) w = vmul(w, silu(widen(st[2 * ARR + r * LPR])));
+                if (!whole && t + r >= len) w = all<VEC>(0.f);
+                if (whole || t + r < in.T) *reinterpret_cast<Pk*>(yp) = narrow<T>(w);
+                yp += in.D;
             }
-            *reinterpret_cast<Pk*>(yp + (int64_t)r * in.D) = out;
         }
     }
-    if (h_last && on && rank == 0 && tid < LPR)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) h_last[(int64_t)b * in.D + d + v] = state[v];
+    if (h_last && at.rank == 0 && tid < Tl::CH && at.d0 + tid < in.D)
+        h_last[(int64_t)at.b * in.D + at.d0 + tid] = state;
 }
 
-template <typename T, int VEC, int LPR, bool OG>
+template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, ScanGrad q) {
-    typedef Tile<T, VEC, LPR, OG ? 4 : 3> Tl;
+    constexpr int R = kBackwardSteps;
+    typedef Tile<T, VEC, LPR, R, OG ? 4 : 3> Tl;
+    static_assert(Tl::STEPS % DG_SCAN_MARK_STEPS == 0 && DG_SCAN_MARK_STEPS % R == 0, "tiles start at marks");
     typedef Pack<T, VEC> Pk;
+    typedef Fv<VEC> V;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ Maps<Tl::CH> maps;          // warp: (P, H) forward; cta: (P, Q) reverse
-    __shared__ float back[2][WARPS][Tl::CH];        // Q per warp, reverse (its P is the forward one)
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int S = in.cluster, rank = S > 1 ? (int)cluster_rank() : 0;
-    const int blocks = (in.D + Tl::CH - 1) / Tl::CH;
-    const int unit = blockIdx.x / S, b = unit / blocks;
-    const int lc = tid % LPR, d = (unit % blocks) * Tl::CH + lc * VEC;
-    const bool on = d < in.D;
-    const int len = in.lengths ? min(max(in.lengths[b], 0), in.T) : in.T;
-    const T* x = (const T*)in.x + b * in.x_sb + d;
-    const T* g = (const T*)in.g + b * in.g_sb + d;
-    const T* o = OG ? (const T*)in.o + b * in.o_sb + d : nullptr;
-    const T* dy = (const T*)q.dy + b * q.dy_sb + d;
-    const uint8_t* rs = in.resets ? in.resets + (int64_t)b * in.T : nullptr;
+    float2* cta_maps = reinterpret_cast<float2*>(smem + STAGES * Tl::STAGE);
+    __shared__ MapsBack<Tl::CH> maps;
+    const Place<LPR, VEC, R> at(in);
+    const int tid = threadIdx.x, S = in.cluster, d = at.d, len = at.len;
+    const T* x = (const T*)in.x + at.b * in.x_sb;
+    const T* g = (const T*)in.g + at.b * in.g_sb;
+    const T* o = OG ? (const T*)in.o + at.b * in.o_sb : nullptr;
+    const T* dy = (const T*)q.dy + at.b * q.dy_sb;
+    const uint8_t* rs = in.resets ? in.resets + (int64_t)at.b * in.T : nullptr;
     const int nblk = (in.T + DG_SCAN_MARK_STEPS - 1) / DG_SCAN_MARK_STEPS;
-    Pk* mine = reinterpret_cast<Pk*>(smem) + tid;
-    constexpr int ARR = R * THREADS, STG = (OG ? 4 : 3) * ARR;
-    const int span = S * Tl::STEPS, ntiles = (in.T + span - 1) / span;
-    const int t_first = rank * Tl::STEPS + (tid / LPR) * R;
+    constexpr int ARR = Tl::ARRAY, STG = (OG ? 4 : 3) * ARR;
+    Pk* warp_part = reinterpret_cast<Pk*>(smem) + at.warp * Tl::WARP_STEPS * LPR;
+    const int own = at.lane / LPR * R * LPR + at.lc;
+    const bool carries = tid < Tl::CH && at.d0 + tid < in.D;      // thread c carries channel d0 + c
 
-    uint8_t next_reset = 0;
-    float next_mark[VEC];                  // the state before the CTA's tile
+    Resets<LPR, R> rst;
+    float next_mark = 0.f;                 // the state before the CTA's tile
     auto prefetch = [&](int it) {
-        const int t = it * span + t_first, t0 = it * span + rank * Tl::STEPS;
-        Pk* st = mine + (it & 1) * STG;
-        fetch<T, VEC>(st, x + t * in.x_st, in.x_st, len - t, on);
-        fetch<T, VEC>(st + ARR, g + t * in.g_st, in.g_st, len - t, on);
-        fetch<T, VEC>(st + 2 * ARR, dy + t * q.dy_st, q.dy_st, len - t, on);
-        if (OG) fetch<T, VEC>(st + 3 * ARR, o + t * in.o_st, in.o_st, len - t, on);
+        const int t = at.warp_step(it), t0 = it * at.span + at.rank * Tl::STEPS;
+        Pk* st = warp_part + (it & 1) * STG;
+        fetch<T, VEC, LPR, R, WIDE>(st, x, in.x_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, R, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, R, WIDE>(st + 2 * ARR, dy, q.dy_st, t, len, at.d0, in.D, at.lane);
+        if (OG) fetch<T, VEC, LPR, R, WIDE>(st + 3 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
         copy_commit();
-        if (rs) next_reset = (lc < R && t + lc < len) ? rs[t + lc] : 0;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-            next_mark[v] = (on && t0 < in.T) ? q.marks[((int64_t)b * nblk + t0 / DG_SCAN_MARK_STEPS) * in.D + d + v] : 0.f;
+        if (rs) rst.load(rs, at.step(it), at.lc, len);
+        if (carries && t0 < in.T)
+            next_mark = q.marks[((int64_t)at.b * nblk + t0 / DG_SCAN_MARK_STEPS) * in.D + at.d0 + tid];
     };
 
-    float state[VEC];                      // r of the step after the tiles done so far
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) state[v] = (q.dh_last && on) ? q.dh_last[(int64_t)b * in.D + d + v] : 0.f;
-    if (ntiles > 0) prefetch(ntiles - 1);
-    for (int it = ntiles - 1; it >= 0; --it) {
-        const int t = it * span + t_first;
-        unsigned resets = 0;
-        if (rs) resets = __ballot_sync(DG_FULL_MASK, next_reset != 0) >> (lane & ~(LPR - 1));
-        float mark[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) mark[v] = next_mark[v];
+    float state = 0.f;                     // r of the step after the tiles done so far
+    if (carries && q.dh_last) state = q.dh_last[(int64_t)at.b * in.D + at.d0 + tid];
+    if (at.ntiles > 0) prefetch(at.ntiles - 1);
+    for (int it = at.ntiles - 1; it >= 0; --it) {
+        const int t = at.step(it);
+        const unsigned resets = rs ? rst.bits(at.lane) : 0;
+        const float mark = next_mark;
+        __syncwarp();
         if (it > 0) prefetch(it - 1);
         else copy_commit();
         copy_wait<1>();
-        const Pk* st = mine + (it & 1) * STG;
-        // c, u of the forward map and the gradient that enters at each step
-        float c[R][VEC], u[R][VEC], na[R][VEC], e[R][VEC], P[VEC], H[VEC], Q[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) P[v] = 1.f, H[v] = 0.f, Q[v] = 0.f;
+        __syncwarp();
+        const Pk* st = warp_part + (it & 1) * STG + own;
+        const bool whole = t + R <= len && resets == 0;
+        // c and u of the forward map, and the gradient that enters at each step
+        V c[R], u[R], na[R], e[R], P = all<VEC>(1.f), H = all<VEC>(0.f), Q = all<VEC>(0.f);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const Pk xv = st[r * THREADS], gv = st[ARR + r * THREADS], dv = st[2 * ARR + r * THREADS];
-            Pk ov;
-            if (OG) ov = st[3 * ARR + r * THREADS];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float a;
-                dg::sigmoid_pair(dg::to_f(gv.v[v]), a, na[r][v]);
-                c[r][v] = t + r < len ? ((resets >> r) & 1 ? 0.f : a) : 1.f;
-                u[r][v] = t + r < len ? na[r][v] * dg::to_f(xv.v[v]) : 0.f;
-                float w = dg::to_f(dv.v[v]);
-                if (OG) {
-                    const float z = dg::to_f(ov.v[v]);
-                    w *= z * dg::sigmoid(z);
-                }
-                e[r][v] = t + r < len ? w : 0.f;
-                H[v] = fmaf(c[r][v], H[v], u[r][v]);
-                P[v] *= c[r][v];
+            gates(widen(st[ARR + r * LPR]), c[r], na[r]);
+            u[r] = vmul(na[r], widen(st[r * LPR]));
+            e[r] = widen(st[2 * ARR + r * LPR]);
+            if (OG) e[r] = vmul(e[r], silu(widen(st[3 * ARR + r * LPR])));
+            if (!whole) {
+                if (t + r >= len) c[r] = all<VEC>(1.f), u[r] = e[r] = all<VEC>(0.f);
+                else if ((resets >> r) & 1) c[r] = all<VEC>(0.f);
             }
+            H = vfma(c[r], H, u[r]);
+            P = vmul(P, c[r]);
         }
 #pragma unroll
-        for (int r = R - 1; r >= 0; --r)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) Q[v] = c[r][v] * (Q[v] + e[r][v]);
-        float Pb[VEC], Hb[VEC], Pa[VEC], Qa[VEC];
+        for (int r = R - 1; r >= 0; --r) Q = vmul(c[r], vadd(Q, e[r]));
+        V Pb, Hb, Pa, Qa, Pw, Hw, Pv, Qw;
+        warp_maps<LPR, VEC, true>(P, H, Pb, Hb, Pw, Hw, at.lane);
+        warp_maps<LPR, VEC, false>(P, Q, Pa, Qa, Pv, Qw, at.lane);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            float Pw, Hw, Pv, Qw;
-            warp_before<LPR>(P[v], H[v], Pb[v], Hb[v], Pw, Hw, lane);
-            warp_after<LPR>(P[v], Q[v], Pa[v], Qa[v], Pv, Qw, lane);
-            if (lane >= 32 - LPR) maps.warp[it & 1][warp][lc * VEC + v] = make_float2(Pw, Hw);
-            if (lane < LPR) back[it & 1][warp][lc * VEC + v] = Qw;
+            if (at.lane >= 32 - LPR) maps.warp[at.warp][at.lc * VEC + v] = make_float2(Pw.v[v], Hw.v[v]);
+            if (at.lane < LPR) maps.back[at.warp][at.lc * VEC + v] = Qw.v[v];
         }
         __syncthreads();
-        if (S > 1) {
-            for (int i = tid; i < S * Tl::CH; i += THREADS) {
-                const int ch = i % Tl::CH;
-                float2 m = make_float2(1.f, 0.f);
+        float2 m[WARPS];
+        float bk[WARPS];
+        if (tid < Tl::CH) {
 #pragma unroll
-                for (int w = WARPS - 1; w >= 0; --w) {
-                    const float p = maps.warp[it & 1][w][ch].x;
-                    m.y = fmaf(p, m.y, back[it & 1][w][ch]);
-                    m.x *= p;
-                }
-                store_remote(&maps.cta[it & 1][rank][ch], i / Tl::CH, m);
+            for (int w = 0; w < WARPS; ++w) m[w] = maps.warp[w][tid], bk[w] = maps.back[w][tid];
+            if (S > 1) {
+                float2 a = make_float2(m[WARPS - 1].x, bk[WARPS - 1]);
+#pragma unroll
+                for (int w = WARPS - 2; w >= 0; --w) a = make_float2(a.x * m[w].x, fmaf(m[w].x, a.y, bk[w]));
+                for (int k = 0; k < S; ++k) store_remote(cta_maps + ((it & 1) * S + at.rank) * Tl::CH + tid, k, a);
             }
+            float f = mark;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                maps.carry[w][tid] = f;
+                f = fmaf(m[w].x, f, m[w].y);
+            }
+        }
+        if (S > 1) {
             __syncwarp();
             cluster_barrier();
         }
-        float rr[VEC], h[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const int ch = lc * VEC + v;
-            float s = state[v], mine_s = s;
+        if (tid < Tl::CH) {
+            float s = state;
             if (S > 1) {
+                float mine = s;
                 for (int k = S - 1; k >= 0; --k) {
-                    if (k == rank) mine_s = s;
-                    const float2 m = maps.cta[it & 1][k][ch];
-                    s = fmaf(m.x, s, m.y);
+                    if (k == at.rank) mine = s;
+                    const float2 a = cta_maps[((it & 1) * S + k) * Tl::CH + tid];
+                    s = fmaf(a.x, s, a.y);
                 }
-                state[v] = s;
-                s = mine_s;
+                state = s;
+                s = mine;
             }
-            float f = mark[v], mine_f = f;
 #pragma unroll
             for (int w = WARPS - 1; w >= 0; --w) {
-                if (w == warp) mine_s = s;
-                s = fmaf(maps.warp[it & 1][w][ch].x, s, back[it & 1][w][ch]);
+                maps.carry_back[w][tid] = s;
+                s = fmaf(m[w].x, s, bk[w]);
             }
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                if (w == warp) mine_f = f;
-                const float2 m = maps.warp[it & 1][w][ch];
-                f = fmaf(m.x, f, m.y);
-            }
-            if (S == 1) state[v] = s;
-            rr[v] = fmaf(Pa[v], mine_s, Qa[v]);
-            h[v] = fmaf(Pb[v], mine_f, Hb[v]);
+            if (S == 1) state = s;
         }
-        if (!on) continue;
-        // forward: u becomes the state before each step; then back through the steps
+        __syncthreads();
+        V h = *reinterpret_cast<const V*>(&maps.carry[at.warp][at.lc * VEC]);
+        V rr = *reinterpret_cast<const V*>(&maps.carry_back[at.warp][at.lc * VEC]);
+        h = vfma(Pb, h, Hb);
+        rr = vfma(Pa, rr, Qa);
+        if (!at.on) continue;
+        // forward: u becomes the state before each step (0 at a reset); then back through the steps
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float before = h[v];
-                h[v] = fmaf(c[r][v], before, u[r][v]);
-                u[r][v] = (resets >> r) & 1 ? 0.f : before;
-            }
+        for (int r = 0; r < R; ++r) {
+            const V before = h;
+            h = vfma(c[r], before, u[r]);
+            u[r] = !whole && ((resets >> r) & 1) ? all<VEC>(0.f) : before;
+        }
+        T* px = (T*)q.dx + at.b * q.dx_sb + (int64_t)(t + R - 1) * q.dx_st + d;
+        T* pg = (T*)q.dg_ + at.b * q.dg_sb + (int64_t)(t + R - 1) * q.dg_st + d;
+        T* po = OG ? (T*)q.do_ + at.b * q.do_sb + (int64_t)(t + R - 1) * q.do_st + d : nullptr;
 #pragma unroll
         for (int r = R - 1; r >= 0; --r) {
-            const Pk xv = st[r * THREADS];
-            Pk ov, dv, px, pg, po;
+            const V xt = widen(st[r * LPR]), et = vadd(e[r], rr), n = na[r];
+            V a = c[r];
+            if (!whole && ((resets >> r) & 1)) a = vfma(n, all<VEC>(-1.f), all<VEC>(1.f));      // c is 0 there
+            const V en = vmul(et, n);
+            V gx = en, gg = vmul(vmul(en, a), vfma(xt, all<VEC>(-1.f), u[r])), go = all<VEC>(0.f);
             if (OG) {
-                dv = st[2 * ARR + r * THREADS];
-                ov = st[3 * ARR + r * THREADS];
+                const V z = widen(st[3 * ARR + r * LPR]);
+                V sg, sn;
+                gates(z, sg, sn);
+                const V ht = vfma(a, u[r], vmul(n, xt));
+                go = vmul(vmul(widen(st[2 * ARR + r * LPR]), ht), vmul(sg, vfma(z, sn, all<VEC>(1.f))));
             }
-            const bool live = t + r < len;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float xt = dg::to_f(xv.v[v]), et = e[r][v] + rr[v], n = na[r][v];
-                float a = c[r][v];
-                if ((resets >> r) & 1) a = 1.f - n;             // c is 0 there
-                px.v[v] = dg::from_f<T>(live ? et * n : 0.f);
-                pg.v[v] = dg::from_f<T>(live ? et * (u[r][v] - xt) * (a * n) : 0.f);
-                if (OG) {
-                    const float z = dg::to_f(ov.v[v]);
-                    float sg, sn;
-                    dg::sigmoid_pair(z, sg, sn);
-                    const float ht = fmaf(a, u[r][v], n * xt);
-                    po.v[v] = dg::from_f<T>(live ? dg::to_f(dv.v[v]) * ht * (sg * fmaf(z, sn, 1.f)) : 0.f);
-                }
-                rr[v] = c[r][v] * et;
+            rr = vmul(c[r], et);
+            if (!whole && t + r >= len) gx = gg = go = all<VEC>(0.f);
+            if (whole || t + r < in.T) {
+                *reinterpret_cast<Pk*>(px) = narrow<T>(gx);
+                *reinterpret_cast<Pk*>(pg) = narrow<T>(gg);
+                if (OG) *reinterpret_cast<Pk*>(po) = narrow<T>(go);
             }
-            if (t + r < in.T) {
-                *reinterpret_cast<Pk*>((T*)q.dx + b * q.dx_sb + (t + r) * q.dx_st + d) = px;
-                *reinterpret_cast<Pk*>((T*)q.dg_ + b * q.dg_sb + (t + r) * q.dg_st + d) = pg;
-                if (OG) *reinterpret_cast<Pk*>((T*)q.do_ + b * q.do_sb + (t + r) * q.do_st + d) = po;
-            }
+            px -= q.dx_st;
+            pg -= q.dg_st;
+            if (OG) po -= q.do_st;
         }
     }
-    if (q.dh0 && on && rank == 0 && tid < LPR)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) q.dh0[(int64_t)b * in.D + d + v] = state[v];
+    if (q.dh0 && at.rank == 0 && carries) q.dh0[(int64_t)at.b * in.D + at.d0 + tid] = state;
 }
 
 template <typename T>
@@ -505,34 +620,44 @@ __global__ void scan_step_kernel(int D, const T* x, int64_t x_sb, const T* g, in
 // launches
 // ---------------------------------------------------------------------------
 
-// whether rows can be read and written VEC elements at a time
+// How rows can be read and written: 0 one element at a time, 1 two, 2 two with inputs read
+// 16 bytes at a time
 struct Row {
     const void* p;
     int64_t sb, st;
 };
-bool pairs_aligned(int D, size_t elem, std::initializer_list<Row> rows) {
-    if (D % 2) return false;
+int width_of(int D, size_t elem, std::initializer_list<Row> rows) {
+    int64_t units = D;                     // every start and stride in elements, as one set of bits
+    uintptr_t bytes = 0;
     for (const Row& r : rows)
-        if (r.p && ((reinterpret_cast<uintptr_t>(r.p) % (2 * elem)) || r.sb % 2 || r.st % 2)) return false;
-    return true;
+        if (r.p) {
+            bytes |= reinterpret_cast<uintptr_t>(r.p);
+            units |= r.sb | r.st;
+        }
+    if (units % 2 || bytes % (2 * elem)) return 0;
+    return units % (int64_t)(16 / elem) || bytes % 16 ? 1 : 2;
 }
 
-// Channels per CTA (lpr x vec) and cluster size.  Each CTA walks ceil(tiles / cluster) tiles, and
-// `occ` of them share an SM, clusters staying inside one of eight groups of about 18 SMs: the
-// least waves x walked steps, taking wide channel blocks (whole 128-byte lines) and small
-// clusters (cheap barriers) where that is a tie.
+// Channels per CTA (lpr x vec) and cluster size: the least work of the busiest SM, ceil(CTAs / SMs)
+// x walked steps x channels.  An SM with a single CTA waits at its barriers (1.5 x its work here),
+// a cluster's barrier costs a little more the larger it is, and clusters stay inside one of eight
+// groups of about 18 SMs, `occ` CTAs each.
 struct Shape {
     int lpr, cluster;
 };
-Shape shape_of(int B, int T, int D, int vec, int occ) {
+Shape shape_of(int B, int T, int D, int vec, int steps_per_thread, int occ, bool narrow) {
     Shape best{32, 1};
-    int64_t least = -1;
+    double least = -1.0;
     for (int lpr = 32; lpr >= 8; lpr /= 2) {
+        if (lpr == 16 && !narrow) continue;
         const int64_t units = (int64_t)B * ((D + lpr * vec - 1) / (lpr * vec));
-        const int steps = THREADS / lpr * R, tiles = (T + steps - 1) / steps;
-        for (int s = 1; s <= 16 && (s == 1 || s <= tiles); ++s) {
-            const int64_t slots = s == 1 ? 148 * occ : 8 * (18 * occ / s) * s;
-            const int64_t cost = (units * s + slots - 1) / slots * ((tiles + s - 1) / s) * steps;
+        const int steps = THREADS / lpr * steps_per_thread, tiles = (T + steps - 1) / steps;
+        const int most = lpr * vec > 32 ? 8 : 16;      // beyond, the cluster's maps take the second CTA's place
+        for (int s = 1; s <= most && (s == 1 || s <= tiles); ++s) {
+            const int64_t n = units * s, slots = s == 1 ? 148 * occ : 8 * (18 * occ / s) * s;
+            const int64_t waves = (n + slots - 1) / slots, per_sm = (n + 147) / 148;
+            double cost = waves > 1 ? (double)waves * occ : per_sm > 1 ? (double)per_sm : 1.5;
+            cost *= (double)((tiles + s - 1) / s) * steps * lpr * (1.0 + 0.01 * s + (lpr < 32 ? 0.04 : 0.0));
             if (least < 0 || cost < least) {
                 least = cost;
                 best = {lpr, s};
@@ -566,32 +691,36 @@ int launch(K kern, unsigned grid, int cluster, size_t smem, cudaStream_t stream,
     return dg_host::check_launch();
 }
 
-template <typename T, int VEC, int LPR, bool OG>
+template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 int run_forward(const ScanIn& in, const float* h0, void* y, float* h_last, float* marks, cudaStream_t s) {
-    typedef Tile<T, VEC, LPR, OG ? 3 : 2> Tl;
+    typedef Tile<T, VEC, LPR, kForwardSteps<T>, OG ? 3 : 2> Tl;
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
-    return launch(scan_forward_kernel<T, VEC, LPR, OG>, (unsigned)grid, in.cluster, STAGES * Tl::STAGE, s, in, h0, (T*)y,
-                  h_last, marks);
+    return launch(scan_forward_kernel<T, VEC, LPR, WIDE, OG>, (unsigned)grid, in.cluster, Tl::bytes(in.cluster), s, in, h0,
+                  (T*)y, h_last, marks);
 }
-template <typename T, int VEC, int LPR, bool OG>
+template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 int run_backward(const ScanIn& in, const ScanGrad& q, cudaStream_t s) {
-    typedef Tile<T, VEC, LPR, OG ? 4 : 3> Tl;
+    typedef Tile<T, VEC, LPR, kBackwardSteps, OG ? 4 : 3> Tl;
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
-    return launch(scan_backward_kernel<T, VEC, LPR, OG>, (unsigned)grid, in.cluster, STAGES * Tl::STAGE, s, in, q);
+    return launch(scan_backward_kernel<T, VEC, LPR, WIDE, OG>, (unsigned)grid, in.cluster, Tl::bytes(in.cluster), s, in, q);
 }
 
-// calls F<T, VEC, LPR, OG>(...) for the sizes at hand
-#define SCAN_LPR(F, T, VEC, OG, lpr, ...)                                          \
-    ((lpr) == 32 ? F<T, VEC, 32, OG>(__VA_ARGS__) : (lpr) == 16 ? F<T, VEC, 16, OG>(__VA_ARGS__) \
-                                                                : F<T, VEC, 8, OG>(__VA_ARGS__))
-#define SCAN_RUN(F, T, two, og, lpr, ...)                                                       \
-    ((two) ? ((og) ? SCAN_LPR(F, T, 2, true, lpr, __VA_ARGS__) : SCAN_LPR(F, T, 2, false, lpr, __VA_ARGS__)) \
-           : ((og) ? SCAN_LPR(F, T, 1, true, lpr, __VA_ARGS__) : SCAN_LPR(F, T, 1, false, lpr, __VA_ARGS__)))
+// calls F<T, VEC, LPR, WIDE, OG>(...) for the shape at hand
+#define SCAN_OG(F, T, VEC, LPR, WIDE, og, ...) \
+    ((og) ? F<T, VEC, LPR, WIDE, true>(__VA_ARGS__) : F<T, VEC, LPR, WIDE, false>(__VA_ARGS__))
+#define SCAN_RUN(F, T, width, lpr, og, ...)                                  \
+    ((width) == 2   ? (lpr) == 32   ? SCAN_OG(F, T, 2, 32, true, og, __VA_ARGS__)  \
+                      : (lpr) == 16 ? SCAN_OG(F, T, 2, 16, true, og, __VA_ARGS__)  \
+                                    : SCAN_OG(F, T, 2, 8, true, og, __VA_ARGS__)   \
+     : (width) == 1 ? (lpr) == 32 ? SCAN_OG(F, T, 2, 32, false, og, __VA_ARGS__)   \
+                                  : SCAN_OG(F, T, 2, 8, false, og, __VA_ARGS__)    \
+     : (lpr) == 32  ? SCAN_OG(F, T, 1, 32, false, og, __VA_ARGS__)                 \
+                    : SCAN_OG(F, T, 1, 8, false, og, __VA_ARGS__))
 
 // CTAs that share an SM, by shared memory and registers
-constexpr int occupancy(bool backward, size_t elem) { return elem == 4 ? 1 : backward ? 2 : 3; }
+constexpr int occupancy(bool backward, size_t elem) { return backward && elem == 4 ? 1 : 2; }
 
 }  // namespace
 
@@ -608,14 +737,15 @@ int dg_gated_scan_forward(int dtype, int B, int T, int D, const void* x, int64_t
     if (T == 0 && !h_last) return DG_OK;
     if (T > (1 << 30)) return DG_ERR_UNSUPPORTED;
     const size_t elem = dg_host::dtype_size(dtype);
-    const bool two = pairs_aligned(D, elem, {{x, x_sb, x_st}, {gate, gate_sb, gate_st}, {out_gate, out_gate_sb, out_gate_st},
-                                             {y, 0, 0}});
-    const Shape sh = shape_of(B, T, D, two ? 2 : 1, occupancy(false, elem));
+    const int width = width_of(D, elem, {{x, x_sb, x_st}, {gate, gate_sb, gate_st}, {out_gate, out_gate_sb, out_gate_st},
+                                         {y, 0, 0}});
+    const Shape sh = shape_of(B, T, D, width ? 2 : 1, elem == 4 ? kForwardSteps<float> : kForwardSteps<__half>,
+                              occupancy(false, elem), width == 2);
     const ScanIn in{x, gate, out_gate, x_sb, x_st, gate_sb, gate_st, out_gate_sb, out_gate_st, lengths, resets, B, T, D,
                     sh.cluster};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     DG_DISPATCH_LM(dtype, S, {
-        return SCAN_RUN(run_forward, S, two, out_gate != nullptr, sh.lpr, in, h0, y, h_last, marks, s);
+        return SCAN_RUN(run_forward, S, width, sh.lpr, out_gate != nullptr, in, h0, y, h_last, marks, s);
     });
     return DG_OK;
 }
@@ -634,16 +764,16 @@ int dg_gated_scan_backward(int dtype, int B, int T, int D, const void* x, int64_
     if (T == 0 && !dh0) return DG_OK;
     if (T > (1 << 30)) return DG_ERR_UNSUPPORTED;
     const size_t elem = dg_host::dtype_size(dtype);
-    const bool two = pairs_aligned(D, elem, {{x, x_sb, x_st}, {gate, gate_sb, gate_st}, {out_gate, out_gate_sb, out_gate_st},
-                                             {dy, dy_sb, dy_st}, {dx, dx_sb, dx_st}, {dgate, dgate_sb, dgate_st},
-                                             {dout_gate, dout_gate_sb, dout_gate_st}});
-    const Shape sh = shape_of(B, T, D, two ? 2 : 1, occupancy(true, elem));
+    const int width = width_of(D, elem, {{x, x_sb, x_st}, {gate, gate_sb, gate_st}, {out_gate, out_gate_sb, out_gate_st},
+                                         {dy, dy_sb, dy_st}, {dx, dx_sb, dx_st}, {dgate, dgate_sb, dgate_st},
+                                         {dout_gate, dout_gate_sb, dout_gate_st}});
+    const Shape sh = shape_of(B, T, D, width ? 2 : 1, kBackwardSteps, occupancy(true, elem), width == 2);
     const ScanIn in{x, gate, out_gate, x_sb, x_st, gate_sb, gate_st, out_gate_sb, out_gate_st, lengths, resets, B, T, D,
                     sh.cluster};
     const ScanGrad q{marks, dy, dy_sb, dy_st, dh_last, dx, dgate, dout_gate, dx_sb, dx_st, dgate_sb, dgate_st,
                      dout_gate_sb, dout_gate_st, dh0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DG_DISPATCH_LM(dtype, S, { return SCAN_RUN(run_backward, S, two, out_gate != nullptr, sh.lpr, in, q, s); });
+    DG_DISPATCH_LM(dtype, S, { return SCAN_RUN(run_backward, S, width, sh.lpr, out_gate != nullptr, in, q, s); });
     return DG_OK;
 }
 

@@ -15,14 +15,28 @@
 
 namespace dg {
 
+// one special-function operation each, results below the normal range flushed to 0
+__device__ __forceinline__ float exp2_ftz(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_ftz(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // a = sigmoid(z) and 1 - a, each to fp32's relative precision: with e = exp(-z),
 // a = 1 / (1 + e) and 1 - a = e a.  z is held above -80, where a is 2e-35 (and e finite).
 __device__ __forceinline__ void sigmoid_pair(float z, float& a, float& one_minus_a) {
-    const float e = __expf(-fmaxf(z, -80.f));
-    a = __fdividef(1.f, 1.f + e);
+    const float e = exp2_ftz(fminf(z * -1.4426950408889634f, 115.f));
+    a = rcp_ftz(1.f + e);
     one_minus_a = e * a;
 }
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-fmaxf(z, -80.f))); }
+__device__ __forceinline__ float sigmoid(float z) {
+    return rcp_ftz(1.f + exp2_ftz(fminf(z * -1.4426950408889634f, 115.f)));
+}
 
 // activations of the feed-forward block and their derivatives
 template <int ACT>
