@@ -51,9 +51,9 @@ _SIGS = {
     "dg_pkm_backward": [_I, _I, _I, _I, _I, _I64, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P,
                         _P, _P],
     "dg_gated_scan_forward": [_I, _I, _I, _I, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P,
-                              _P],
+                              _P, _P],
     "dg_gated_scan_backward": [_I, _I, _I, _I, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I64,
-                               _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P],
+                               _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P],
     "dg_gated_scan_step": [_I, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P],
     "dg_gated_ffn_forward": [_I, _I64, _I, _I, _I, _P, _I64, _P, _P, _P, _P, _P],
     "dg_gated_ffn_backward_workspace_size": [_I, _I64, _I, _I],

@@ -105,7 +105,7 @@ ScanOut scan_forward(const ScanArgs& a, bool save) {
                                 st(a.out_gate, 1), (const float*)ptr_or_null(a.h0),
                                 (const int32_t*)ptr_or_null(a.lengths), (const uint8_t*)ptr_or_null(a.resets),
                                 r.y.data_ptr(), r.h_last.data_ptr<float>(), (float*)ptr_or_null(r.marks),
-                                stream_of(a.x)),
+                                status_word(a.x.device()).data_ptr<int32_t>(), stream_of(a.x)),
           "dg_gated_scan_forward");
     return r;
 }
@@ -125,7 +125,7 @@ Tensor scan_backward(const ScanArgs& a, const Tensor& marks, const Tensor& g_y, 
               (const int32_t*)ptr_or_null(a.lengths), (const uint8_t*)ptr_or_null(a.resets), marks.data_ptr<float>(),
               dy.data_ptr(), st(dy, 0), st(dy, 1), (const float*)ptr_or_null(dh), dx.data_ptr(), st(dx, 0), st(dx, 1),
               dgate.data_ptr(), st(dgate, 0), st(dgate, 1), ptr_or_null(dout), st(dout, 0), st(dout, 1),
-              (float*)ptr_or_null(dh0), stream_of(a.x)),
+              (float*)ptr_or_null(dh0), status_word(a.x.device()).data_ptr<int32_t>(), stream_of(a.x)),
           "dg_gated_scan_backward");
     return dh0;
 }

@@ -10,8 +10,8 @@
 //     and every thread applies its steps to the state it starts from.  The CTA walks the
 //     sequence tile by tile;
 //   - where rows and channels give too few CTAs, a cluster of up to 16 takes consecutive
-//     tiles and exchanges their maps through distributed shared memory, one cluster barrier
-//     per tile.
+//     tiles and exchanges their maps through distributed shared memory: asynchronous stores
+//     that count on the receiver's mbarrier, so that no fence waits for a warp's other stores.
 // Each input is read and each output written once.  The order of every composition is fixed
 // by the sizes alone, so results repeat bit for bit.
 //
@@ -29,15 +29,19 @@
 #include <type_traits>
 
 #include "lm_common.cuh"
+#include "tc_util.cuh"
+
+namespace dg_host {
+uint32_t wait_limit();
+}
 
 namespace {
 
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int STAGES = 2;                  // tiles of input in shared memory
-// steps per thread: forward as many as registers and shared memory allow
-template <typename T> constexpr int kForwardSteps = sizeof(T) == 4 ? 8 : 16;
-constexpr int kBackwardSteps = 8;
+constexpr int R = 8;                       // steps per thread
+static_assert(DG_SCAN_MARK_STEPS % R == 0, "a mark falls on a thread's first step");
 
 struct ScanIn {
     const void *x, *g, *o;
@@ -45,6 +49,8 @@ struct ScanIn {
     const int32_t* lengths;
     const uint8_t* resets;
     int B, T, D, cluster;
+    int32_t* status;
+    uint32_t wait_limit;
 };
 
 struct ScanGrad {
@@ -79,10 +85,14 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void store_remote(float2* p, uint32_t rank, float2 v) {
-    uint32_t a;
+// stores v at p's place in CTA `rank` and counts its 8 bytes on `bar` there
+__device__ __forceinline__ void store_remote(float2* p, uint64_t* bar, uint32_t rank, float2 v) {
+    uint32_t a, m;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(v.x), "f"(v.y) : "memory");
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(m) : "r"((uint32_t)__cvta_generic_to_shared(bar)), "r"(rank));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(a), "f"(v.x),
+                 "f"(v.y), "r"(m)
+                 : "memory");
 }
 
 // ---- one or two channels at a time ------------------------------------------------
@@ -176,13 +186,14 @@ template <int VEC> __device__ __forceinline__ Fv<VEC> silu(Fv<VEC> z) {
 template <int CH> struct Maps {
     float2 warp[WARPS][CH];                // each warp's (P, H)
     float carry[WARPS][CH];                // the state each warp starts from
+    uint64_t received[2];                  // the cluster's maps of even and odd tiles
 };
 template <int CH> struct MapsBack : Maps<CH> {
     float back[WARPS][CH];                 // each warp's Q of the reverse map
     float carry_back[WARPS][CH];
 };
 
-template <typename T, int VEC, int LPR, int R, int ARRAYS> struct Tile {
+template <typename T, int VEC, int LPR, int ARRAYS> struct Tile {
     static constexpr int STEPS = THREADS / LPR * R, CH = LPR * VEC;
     static constexpr int WARP_STEPS = 32 / LPR * R;
     typedef Pack<T, VEC> P;
@@ -196,7 +207,7 @@ template <typename T, int VEC, int LPR, int R, int ARRAYS> struct Tile {
 
 // A warp's steps of one input into its part of a stage.  WIDE: 16 bytes a lane, any lane any
 // step of the warp.  Otherwise each thread copies the steps it reads itself.
-template <typename T, int VEC, int LPR, int R, bool WIDE>
+template <typename T, int VEC, int LPR, bool WIDE>
 __device__ __forceinline__ void fetch(Pack<T, VEC>* warp_part, const T* row, int64_t step, int t_warp, int len, int d0,
                                       int D, int lane) {
     constexpr int PPS = LPR;                                      // packs per step
@@ -265,7 +276,7 @@ __device__ __forceinline__ void warp_maps(Fv<VEC> P, Fv<VEC> H, Fv<VEC>& Pb, Fv<
 }
 
 // where a thread stands: shared by both passes
-template <int LPR, int VEC, int R> struct Place {
+template <int LPR, int VEC> struct Place {
     int warp, lane, lc, rank, b, d0, d, len, span, ntiles;
     bool on;
     __device__ __forceinline__ Place(const ScanIn& in) {
@@ -288,40 +299,104 @@ template <int LPR, int VEC, int R> struct Place {
     __device__ __forceinline__ int step(int it) const { return warp_step(it) + lane / LPR * R; }
 };
 
-// bit r: a document starts at step r of this thread.  The loads were made a tile earlier: lane lc
-// of a group holds steps lc and, for R > LPR, lc + LPR.
-template <int LPR, int R> struct Resets {
-    uint8_t next[(R + LPR - 1) / LPR];
-    __device__ __forceinline__ void load(const uint8_t* rs, int t, int lc, int len) {
+// bit r: a document starts at step r of this thread.  The load was made a tile earlier: lane r of
+// a group holds step r.
+template <int LPR> __device__ __forceinline__ uint8_t load_reset(const uint8_t* rs, int t, int lc, int len) {
+    return lc < R && t + lc < len ? rs[t + lc] : 0;
+}
+template <int LPR> __device__ __forceinline__ unsigned reset_bits(uint8_t mine, int lane) {
+    static_assert(LPR >= R, "one lane per step");
+    return __ballot_sync(DG_FULL_MASK, mine != 0) >> (lane & ~(LPR - 1)) & ((1u << R) - 1);
+}
+
+// the forward map of a thread's steps: c, u and their composition (P, H).  WHOLE: every step is
+// valid and none starts a document.
+template <bool WHOLE, typename T, int VEC, int LPR>
+__device__ __forceinline__ void forward_map(const Pack<T, VEC>* xs, const Pack<T, VEC>* gs, int left, unsigned resets,
+                                            Fv<VEC> (&c)[R], Fv<VEC> (&u)[R], Fv<VEC>* nas, Fv<VEC>& P, Fv<VEC>& H) {
 #pragma unroll
-        for (int i = 0; i < (R + LPR - 1) / LPR; ++i) {
-            const int r = lc + i * LPR;
-            next[i] = (r < R && t + r < len) ? rs[t + r] : 0;
+    for (int r = 0; r < R; ++r) {
+        Fv<VEC> na;
+        gates(widen(gs[r * LPR]), c[r], na);
+        u[r] = vmul(na, widen(xs[r * LPR]));
+        if (!WHOLE) {
+            if (r >= left) c[r] = all<VEC>(1.f), u[r] = all<VEC>(0.f);
+            else if ((resets >> r) & 1) c[r] = all<VEC>(0.f);
         }
+        H = r == 0 ? u[0] : vfma(c[r], H, u[r]);
+        P = r == 0 ? c[0] : vmul(P, c[r]);
+        if (nas) nas[r] = na;
     }
-    __device__ __forceinline__ unsigned bits(int lane) const {
-        unsigned m = 0;
+}
+
+// y of a thread's steps from the state h before them; `left` valid steps, `room` steps inside T
+template <bool WHOLE, typename T, int VEC, int LPR, bool OG>
+__device__ __forceinline__ void forward_apply(Fv<VEC> h, const Fv<VEC> (&c)[R], const Fv<VEC> (&u)[R],
+                                              const Pack<T, VEC>* os, T* y, int D, int left, int room) {
 #pragma unroll
-        for (int i = 0; i < (R + LPR - 1) / LPR; ++i) {
-            const unsigned all = __ballot_sync(DG_FULL_MASK, next[i] != 0) >> (lane & ~(LPR - 1));
-            m |= (LPR < 32 ? all & ((1u << (LPR & 31)) - 1) : all) << (i * LPR);
-        }
-        return m;
+    for (int r = 0; r < R; ++r) {
+        h = vfma(c[r], h, u[r]);
+        Fv<VEC> w = h;
+        if (OG) w = vmul(w, silu(widen(os[r * LPR])));
+        if (!WHOLE && r >= left) w = all<VEC>(0.f);
+        if (WHOLE || r < room) *reinterpret_cast<Pack<T, VEC>*>(y + (int64_t)r * D) = narrow<T>(w);
     }
-};
+}
+
+// The cluster's part of a tile: this CTA's map to all, then the state before this CTA and (returned
+// in `state`) after the whole span.  Called by the threads that carry a channel.
+template <int CH, bool FORWARD>
+__device__ __forceinline__ float through_cluster(float2* maps, uint64_t* received, float2 own, int tid, int rank, int S,
+                                                 int n, float& state, uint32_t limit, bool& bad) {
+    const int buf = n & 1;
+    float2* m = maps + (size_t)buf * S * CH;
+    if (tid == 0) tc::mbar_expect_tx(received + buf, S * CH * (uint32_t)sizeof(float2));
+    for (int k = 0; k < S; ++k) store_remote(m + rank * CH + tid, received + buf, k, own);
+    if (!bad) bad = !tc::mbar_wait(received + buf, (n >> 1) & 1, limit);
+    float s = state, before = s;
+    for (int i = 0; i < S; ++i) {
+        const int k = FORWARD ? i : S - 1 - i;
+        if (k == rank) before = s;
+        const float2 a = m[k * CH + tid];
+        s = fmaf(a.x, s, a.y);
+    }
+    state = s;
+    return before;
+}
+
+// Barriers of the cluster exchange: set up before the first tile; at the end, a CTA whose wait gave
+// up says so and stays until the others' stores have landed.
+__device__ __forceinline__ void open_exchange(uint64_t* received, int S) {
+    if (S == 1) return;
+    if (threadIdx.x == 0) {
+        tc::mbar_init(received, 1);
+        tc::mbar_init(received + 1, 1);
+        tc::fence_barrier_init();
+    }
+    __syncthreads();
+    cluster_barrier();
+}
+__device__ __forceinline__ void close_exchange(int S, bool bad, int32_t* status) {
+    if (S == 1) return;
+    if (bad) dg::flag_status(status, DG_DEVCHK_TIMEOUT);
+    if (__syncthreads_or(bad)) {
+        const uint64_t t0 = tc::globaltimer_ns();
+        for (int i = 0; i < (1 << 20) && tc::globaltimer_ns() - t0 < 2000000; ++i) __nanosleep(1000);
+    }
+    __syncwarp();
+    cluster_barrier();
+}
 
 template <typename T, int VEC, int LPR, bool WIDE, bool OG>
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(THREADS, 3)
     scan_forward_kernel(ScanIn in, const float* h0, T* y, float* h_last, float* marks) {
-    constexpr int R = kForwardSteps<T>;
-    static_assert(DG_SCAN_MARK_STEPS % R == 0, "a mark falls on a thread's first step");
-    typedef Tile<T, VEC, LPR, R, OG ? 3 : 2> Tl;
+    typedef Tile<T, VEC, LPR, OG ? 3 : 2> Tl;
     typedef Pack<T, VEC> Pk;
     typedef Fv<VEC> V;
     extern __shared__ __align__(16) uint8_t smem[];
     float2* cta_maps = reinterpret_cast<float2*>(smem + STAGES * Tl::STAGE);
     __shared__ Maps<Tl::CH> maps;
-    const Place<LPR, VEC, R> at(in);
+    const Place<LPR, VEC> at(in);
     const int tid = threadIdx.x, S = in.cluster, d = at.d, len = at.len;
     const T* x = (const T*)in.x + at.b * in.x_sb;
     const T* g = (const T*)in.g + at.b * in.g_sb;
@@ -331,16 +406,18 @@ __global__ void __launch_bounds__(THREADS, 2)
     constexpr int ARR = Tl::ARRAY, STG = (OG ? 3 : 2) * ARR;
     Pk* warp_part = reinterpret_cast<Pk*>(smem) + at.warp * Tl::WARP_STEPS * LPR;
     const int own = at.lane / LPR * R * LPR + at.lc;              // this thread's first pack in it
+    bool bad = false;
+    open_exchange(maps.received, S);
 
-    Resets<LPR, R> rst;
+    uint8_t next_reset = 0;
     auto prefetch = [&](int it) {
         const int t = at.warp_step(it);
         Pk* st = warp_part + (it & 1) * STG;
-        fetch<T, VEC, LPR, R, WIDE>(st, x, in.x_st, t, len, at.d0, in.D, at.lane);
-        fetch<T, VEC, LPR, R, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
-        if (OG) fetch<T, VEC, LPR, R, WIDE>(st + 2 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, WIDE>(st, x, in.x_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
+        if (OG) fetch<T, VEC, LPR, WIDE>(st + 2 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
         copy_commit();
-        if (rs) rst.load(rs, at.step(it), at.lc, len);
+        if (rs) next_reset = load_reset<LPR>(rs, at.step(it), at.lc, len);
     };
 
     // thread c < CH carries channel d0 + c from tile to tile
@@ -349,59 +426,34 @@ __global__ void __launch_bounds__(THREADS, 2)
     if (at.ntiles > 0) prefetch(0);
     for (int it = 0; it < at.ntiles; ++it) {
         const int t = at.step(it);
-        const unsigned resets = rs ? rst.bits(at.lane) : 0;
+        const unsigned resets = rs ? reset_bits<LPR>(next_reset, at.lane) : 0;
         __syncwarp();                      // the other stage has been read
         if (it + 1 < at.ntiles) prefetch(it + 1);
         else copy_commit();
         copy_wait<1>();
         __syncwarp();
         const Pk* st = warp_part + (it & 1) * STG + own;
-        V c[R], u[R], P = all<VEC>(1.f), H = all<VEC>(0.f);
+        V c[R], u[R], P, H;
         const bool whole = t + R <= len && resets == 0;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            V na;
-            gates(widen(st[ARR + r * LPR]), c[r], na);
-            u[r] = vmul(na, widen(st[r * LPR]));
-            if (!whole) {
-                if (t + r >= len) c[r] = all<VEC>(1.f), u[r] = all<VEC>(0.f);
-                else if ((resets >> r) & 1) c[r] = all<VEC>(0.f);
-            }
-            H = vfma(c[r], H, u[r]);
-            P = vmul(P, c[r]);
-        }
+        if (whole) forward_map<true, T, VEC, LPR>(st, st + ARR, R, 0, c, u, nullptr, P, H);
+        else forward_map<false, T, VEC, LPR>(st, st + ARR, len - t, resets, c, u, nullptr, P, H);
         V Pb, Hb, Pw, Hw;
         warp_maps<LPR, VEC, true>(P, H, Pb, Hb, Pw, Hw, at.lane);
         if (at.lane >= 32 - LPR)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) maps.warp[at.warp][at.lc * VEC + v] = make_float2(Pw.v[v], Hw.v[v]);
         __syncthreads();
-        float2 m[WARPS];
         if (tid < Tl::CH) {
+            float2 m[WARPS];
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) m[w] = maps.warp[w][tid];
+            float s = state;
             if (S > 1) {
                 float2 a = m[0];
 #pragma unroll
                 for (int w = 1; w < WARPS; ++w) a = make_float2(a.x * m[w].x, fmaf(m[w].x, a.y, m[w].y));
-                for (int k = 0; k < S; ++k) store_remote(cta_maps + ((it & 1) * S + at.rank) * Tl::CH + tid, k, a);
-            }
-        }
-        if (S > 1) {
-            __syncwarp();
-            cluster_barrier();
-        }
-        if (tid < Tl::CH) {
-            float s = state;
-            if (S > 1) {
-                float mine = s;
-                for (int k = 0; k < S; ++k) {
-                    if (k == at.rank) mine = s;
-                    const float2 a = cta_maps[((it & 1) * S + k) * Tl::CH + tid];
-                    s = fmaf(a.x, s, a.y);
-                }
-                state = s;
-                s = mine;
+                s = through_cluster<Tl::CH, true>(cta_maps, maps.received, a, tid, at.rank, S, it, state, in.wait_limit,
+                                                  bad);
             }
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
@@ -412,39 +464,63 @@ __global__ void __launch_bounds__(THREADS, 2)
         }
         __syncthreads();
         V h = *reinterpret_cast<const V*>(&maps.carry[at.warp][at.lc * VEC]);
-        h = vfma(Pb, h, Hb);
+        if (LPR < 32) h = vfma(Pb, h, Hb);
         if (at.on) {
             if (marks && t < in.T && t % DG_SCAN_MARK_STEPS == 0)
 #pragma unroll
                 for (int v = 0; v < VEC; ++v)
                     marks[((int64_t)at.b * nblk + t / DG_SCAN_MARK_STEPS) * in.D + d + v] = h.v[v];
             T* yp = y + ((int64_t)at.b * in.T + t) * in.D + d;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                h = vfma(c[r], h, u[r]);
-                V w = h;
-                if (OG) w = vmul(w, silu(widen(st[2 * ARR + r * LPR])));
-                if (!whole && t + r >= len) w = all<VEC>(0.f);
-                if (whole || t + r < in.T) *reinterpret_cast<Pk*>(yp) = narrow<T>(w);
-                yp += in.D;
-            }
+            if (whole) forward_apply<true, T, VEC, LPR, OG>(h, c, u, st + 2 * ARR, yp, in.D, R, R);
+            else forward_apply<false, T, VEC, LPR, OG>(h, c, u, st + 2 * ARR, yp, in.D, len - t, in.T - t);
         }
     }
     if (h_last && at.rank == 0 && tid < Tl::CH && at.d0 + tid < in.D)
         h_last[(int64_t)at.b * in.D + at.d0 + tid] = state;
+    close_exchange(S, bad, in.status);
+}
+
+// the gradients of a thread's steps, last to first: u holds the state before each step (0 at a
+// reset), rr what comes back from the steps after them
+template <bool WHOLE, typename T, int VEC, int LPR, bool OG>
+__device__ __forceinline__ void backward_apply(Fv<VEC> rr, const Fv<VEC> (&c)[R], const Fv<VEC> (&u)[R],
+                                               const Fv<VEC> (&na)[R], const Fv<VEC> (&e)[R], const Pack<T, VEC>* xs,
+                                               const Pack<T, VEC>* dys, const Pack<T, VEC>* os, T* px, int64_t sx, T* pg,
+                                               int64_t sg, T* po, int64_t so, int left, int room, unsigned resets) {
+#pragma unroll
+    for (int r = R - 1; r >= 0; --r) {
+        const Fv<VEC> xt = widen(xs[r * LPR]), et = vadd(e[r], rr), n = na[r];
+        Fv<VEC> a = c[r];
+        if (!WHOLE && ((resets >> r) & 1)) a = vfma(n, all<VEC>(-1.f), all<VEC>(1.f));      // c is 0 there
+        const Fv<VEC> en = vmul(et, n);
+        Fv<VEC> gx = en, gg = vmul(vmul(en, a), vfma(xt, all<VEC>(-1.f), u[r])), go = all<VEC>(0.f);
+        if (OG) {
+            const Fv<VEC> z = widen(os[r * LPR]);
+            Fv<VEC> sg_, sn;
+            gates(z, sg_, sn);
+            const Fv<VEC> ht = vfma(a, u[r], vmul(n, xt));
+            go = vmul(vmul(widen(dys[r * LPR]), ht), vmul(sg_, vfma(z, sn, all<VEC>(1.f))));
+        }
+        rr = vmul(c[r], et);
+        if (!WHOLE && r >= left) gx = gg = go = all<VEC>(0.f);
+        if (WHOLE || r < room) {
+            *reinterpret_cast<Pack<T, VEC>*>(px + r * sx) = narrow<T>(gx);
+            *reinterpret_cast<Pack<T, VEC>*>(pg + r * sg) = narrow<T>(gg);
+            if (OG) *reinterpret_cast<Pack<T, VEC>*>(po + r * so) = narrow<T>(go);
+        }
+    }
 }
 
 template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, ScanGrad q) {
-    constexpr int R = kBackwardSteps;
-    typedef Tile<T, VEC, LPR, R, OG ? 4 : 3> Tl;
-    static_assert(Tl::STEPS % DG_SCAN_MARK_STEPS == 0 && DG_SCAN_MARK_STEPS % R == 0, "tiles start at marks");
+    typedef Tile<T, VEC, LPR, OG ? 4 : 3> Tl;
+    static_assert(Tl::STEPS % DG_SCAN_MARK_STEPS == 0, "tiles start at marks");
     typedef Pack<T, VEC> Pk;
     typedef Fv<VEC> V;
     extern __shared__ __align__(16) uint8_t smem[];
     float2* cta_maps = reinterpret_cast<float2*>(smem + STAGES * Tl::STAGE);
     __shared__ MapsBack<Tl::CH> maps;
-    const Place<LPR, VEC, R> at(in);
+    const Place<LPR, VEC> at(in);
     const int tid = threadIdx.x, S = in.cluster, d = at.d, len = at.len;
     const T* x = (const T*)in.x + at.b * in.x_sb;
     const T* g = (const T*)in.g + at.b * in.g_sb;
@@ -456,18 +532,20 @@ __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, Sc
     Pk* warp_part = reinterpret_cast<Pk*>(smem) + at.warp * Tl::WARP_STEPS * LPR;
     const int own = at.lane / LPR * R * LPR + at.lc;
     const bool carries = tid < Tl::CH && at.d0 + tid < in.D;      // thread c carries channel d0 + c
+    bool bad = false;
+    open_exchange(maps.received, S);
 
-    Resets<LPR, R> rst;
+    uint8_t next_reset = 0;
     float next_mark = 0.f;                 // the state before the CTA's tile
     auto prefetch = [&](int it) {
         const int t = at.warp_step(it), t0 = it * at.span + at.rank * Tl::STEPS;
         Pk* st = warp_part + (it & 1) * STG;
-        fetch<T, VEC, LPR, R, WIDE>(st, x, in.x_st, t, len, at.d0, in.D, at.lane);
-        fetch<T, VEC, LPR, R, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
-        fetch<T, VEC, LPR, R, WIDE>(st + 2 * ARR, dy, q.dy_st, t, len, at.d0, in.D, at.lane);
-        if (OG) fetch<T, VEC, LPR, R, WIDE>(st + 3 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, WIDE>(st, x, in.x_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, WIDE>(st + 2 * ARR, dy, q.dy_st, t, len, at.d0, in.D, at.lane);
+        if (OG) fetch<T, VEC, LPR, WIDE>(st + 3 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
         copy_commit();
-        if (rs) rst.load(rs, at.step(it), at.lc, len);
+        if (rs) next_reset = load_reset<LPR>(rs, at.step(it), at.lc, len);
         if (carries && t0 < in.T)
             next_mark = q.marks[((int64_t)at.b * nblk + t0 / DG_SCAN_MARK_STEPS) * in.D + at.d0 + tid];
     };
@@ -477,7 +555,7 @@ __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, Sc
     if (at.ntiles > 0) prefetch(at.ntiles - 1);
     for (int it = at.ntiles - 1; it >= 0; --it) {
         const int t = at.step(it);
-        const unsigned resets = rs ? rst.bits(at.lane) : 0;
+        const unsigned resets = rs ? reset_bits<LPR>(next_reset, at.lane) : 0;
         const float mark = next_mark;
         __syncwarp();
         if (it > 0) prefetch(it - 1);
@@ -487,22 +565,15 @@ __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, Sc
         const Pk* st = warp_part + (it & 1) * STG + own;
         const bool whole = t + R <= len && resets == 0;
         // c and u of the forward map, and the gradient that enters at each step
-        V c[R], u[R], na[R], e[R], P = all<VEC>(1.f), H = all<VEC>(0.f), Q = all<VEC>(0.f);
+        V c[R], u[R], na[R], e[R], P, H, Q = all<VEC>(0.f);
+        if (whole) forward_map<true, T, VEC, LPR>(st, st + ARR, R, 0, c, u, na, P, H);
+        else forward_map<false, T, VEC, LPR>(st, st + ARR, len - t, resets, c, u, na, P, H);
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            gates(widen(st[ARR + r * LPR]), c[r], na[r]);
-            u[r] = vmul(na[r], widen(st[r * LPR]));
+        for (int r = R - 1; r >= 0; --r) {
             e[r] = widen(st[2 * ARR + r * LPR]);
             if (OG) e[r] = vmul(e[r], silu(widen(st[3 * ARR + r * LPR])));
-            if (!whole) {
-                if (t + r >= len) c[r] = all<VEC>(1.f), u[r] = e[r] = all<VEC>(0.f);
-                else if ((resets >> r) & 1) c[r] = all<VEC>(0.f);
-            }
-            H = vfma(c[r], H, u[r]);
-            P = vmul(P, c[r]);
+            Q = r == R - 1 ? vmul(c[r], e[r]) : vmul(c[r], vadd(Q, e[r]));       // dy is 0 beyond len
         }
-#pragma unroll
-        for (int r = R - 1; r >= 0; --r) Q = vmul(c[r], vadd(Q, e[r]));
         V Pb, Hb, Pa, Qa, Pw, Hw, Pv, Qw;
         warp_maps<LPR, VEC, true>(P, H, Pb, Hb, Pw, Hw, at.lane);
         warp_maps<LPR, VEC, false>(P, Q, Pa, Qa, Pv, Qw, at.lane);
@@ -512,39 +583,23 @@ __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, Sc
             if (at.lane < LPR) maps.back[at.warp][at.lc * VEC + v] = Qw.v[v];
         }
         __syncthreads();
-        float2 m[WARPS];
-        float bk[WARPS];
         if (tid < Tl::CH) {
+            float2 m[WARPS];
+            float bk[WARPS];
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) m[w] = maps.warp[w][tid], bk[w] = maps.back[w][tid];
-            if (S > 1) {
-                float2 a = make_float2(m[WARPS - 1].x, bk[WARPS - 1]);
-#pragma unroll
-                for (int w = WARPS - 2; w >= 0; --w) a = make_float2(a.x * m[w].x, fmaf(m[w].x, a.y, bk[w]));
-                for (int k = 0; k < S; ++k) store_remote(cta_maps + ((it & 1) * S + at.rank) * Tl::CH + tid, k, a);
-            }
-            float f = mark;
+            float f = mark, s = state;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
                 maps.carry[w][tid] = f;
                 f = fmaf(m[w].x, f, m[w].y);
             }
-        }
-        if (S > 1) {
-            __syncwarp();
-            cluster_barrier();
-        }
-        if (tid < Tl::CH) {
-            float s = state;
             if (S > 1) {
-                float mine = s;
-                for (int k = S - 1; k >= 0; --k) {
-                    if (k == at.rank) mine = s;
-                    const float2 a = cta_maps[((it & 1) * S + k) * Tl::CH + tid];
-                    s = fmaf(a.x, s, a.y);
-                }
-                state = s;
-                s = mine;
+                float2 a = make_float2(m[WARPS - 1].x, bk[WARPS - 1]);
+#pragma unroll
+                for (int w = WARPS - 2; w >= 0; --w) a = make_float2(a.x * m[w].x, fmaf(m[w].x, a.y, bk[w]));
+                s = through_cluster<Tl::CH, false>(cta_maps, maps.received, a, tid, at.rank, S, at.ntiles - 1 - it, state,
+                                                   in.wait_limit, bad);
             }
 #pragma unroll
             for (int w = WARPS - 1; w >= 0; --w) {
@@ -556,46 +611,34 @@ __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, Sc
         __syncthreads();
         V h = *reinterpret_cast<const V*>(&maps.carry[at.warp][at.lc * VEC]);
         V rr = *reinterpret_cast<const V*>(&maps.carry_back[at.warp][at.lc * VEC]);
-        h = vfma(Pb, h, Hb);
-        rr = vfma(Pa, rr, Qa);
-        if (!at.on) continue;
-        // forward: u becomes the state before each step (0 at a reset); then back through the steps
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const V before = h;
-            h = vfma(c[r], before, u[r]);
-            u[r] = !whole && ((resets >> r) & 1) ? all<VEC>(0.f) : before;
+        if (LPR < 32) {
+            h = vfma(Pb, h, Hb);
+            rr = vfma(Pa, rr, Qa);
         }
-        T* px = (T*)q.dx + at.b * q.dx_sb + (int64_t)(t + R - 1) * q.dx_st + d;
-        T* pg = (T*)q.dg_ + at.b * q.dg_sb + (int64_t)(t + R - 1) * q.dg_st + d;
-        T* po = OG ? (T*)q.do_ + at.b * q.do_sb + (int64_t)(t + R - 1) * q.do_st + d : nullptr;
+        if (at.on) {
 #pragma unroll
-        for (int r = R - 1; r >= 0; --r) {
-            const V xt = widen(st[r * LPR]), et = vadd(e[r], rr), n = na[r];
-            V a = c[r];
-            if (!whole && ((resets >> r) & 1)) a = vfma(n, all<VEC>(-1.f), all<VEC>(1.f));      // c is 0 there
-            const V en = vmul(et, n);
-            V gx = en, gg = vmul(vmul(en, a), vfma(xt, all<VEC>(-1.f), u[r])), go = all<VEC>(0.f);
-            if (OG) {
-                const V z = widen(st[3 * ARR + r * LPR]);
-                V sg, sn;
-                gates(z, sg, sn);
-                const V ht = vfma(a, u[r], vmul(n, xt));
-                go = vmul(vmul(widen(st[2 * ARR + r * LPR]), ht), vmul(sg, vfma(z, sn, all<VEC>(1.f))));
+            for (int r = 0; r < R; ++r) {  // u becomes the state before each step
+                const V before = h;
+                h = vfma(c[r], before, u[r]);
+                u[r] = before;
             }
-            rr = vmul(c[r], et);
-            if (!whole && t + r >= len) gx = gg = go = all<VEC>(0.f);
-            if (whole || t + r < in.T) {
-                *reinterpret_cast<Pk*>(px) = narrow<T>(gx);
-                *reinterpret_cast<Pk*>(pg) = narrow<T>(gg);
-                if (OG) *reinterpret_cast<Pk*>(po) = narrow<T>(go);
+            T* px = (T*)q.dx + at.b * q.dx_sb + t * q.dx_st + d;
+            T* pg = (T*)q.dg_ + at.b * q.dg_sb + t * q.dg_st + d;
+            T* po = OG ? (T*)q.do_ + at.b * q.do_sb + t * q.do_st + d : nullptr;
+            if (whole) {
+                backward_apply<true, T, VEC, LPR, OG>(rr, c, u, na, e, st, st + 2 * ARR, st + 3 * ARR, px, q.dx_st, pg,
+                                                      q.dg_st, po, q.do_st, R, R, 0);
+            } else {
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if ((resets >> r) & 1) u[r] = all<VEC>(0.f);
+                backward_apply<false, T, VEC, LPR, OG>(rr, c, u, na, e, st, st + 2 * ARR, st + 3 * ARR, px, q.dx_st, pg,
+                                                       q.dg_st, po, q.do_st, len - t, in.T - t, resets);
             }
-            px -= q.dx_st;
-            pg -= q.dg_st;
-            if (OG) po -= q.do_st;
         }
     }
     if (q.dh0 && at.rank == 0 && carries) q.dh0[(int64_t)at.b * in.D + at.d0 + tid] = state;
+    close_exchange(S, bad, in.status);
 }
 
 template <typename T>
@@ -638,24 +681,27 @@ int width_of(int D, size_t elem, std::initializer_list<Row> rows) {
     return units % (int64_t)(16 / elem) || bytes % 16 ? 1 : 2;
 }
 
-// Channels per CTA (lpr x vec) and cluster size: the least work of the busiest SM, ceil(CTAs / SMs)
-// x walked steps x channels.  An SM with a single CTA waits at its barriers (1.5 x its work here),
-// a cluster's barrier costs a little more the larger it is, and clusters stay inside one of eight
-// groups of about 18 SMs, `occ` CTAs each.
+// Channels per CTA (lpr x vec) and cluster size: the least work of the busiest SM, CTAs on it x
+// walked steps x channels.  An SM with a single CTA waits at its barriers (1.5 x its work here);
+// larger clusters and narrower rows cost a little more, which also decides ties.
 struct Shape {
     int lpr, cluster;
 };
-Shape shape_of(int B, int T, int D, int vec, int steps_per_thread, int occ, bool narrow) {
+// Clusters of 1..16 CTAs that are resident at once on a whole B200 with 1, 2 or 3 such CTAs to an SM
+// (cudaOccupancyMaxActiveClusters; a cluster stays inside one group of SMs)
+constexpr int kClusters[3][16] = {{148, 74, 45, 33, 26, 22, 15, 15, 15, 11, 7, 7, 7, 7, 7, 7},
+                                  {296, 148, 93, 71, 56, 45, 37, 33, 30, 26, 21, 21, 17, 14, 14, 14},
+                                  {444, 222, 142, 104, 82, 71, 56, 48, 45, 41, 31, 31, 28, 24, 24, 21}};
+Shape shape_of(int B, int T, int D, int vec, int occ, bool narrow) {
     Shape best{32, 1};
     double least = -1.0;
     for (int lpr = 32; lpr >= 8; lpr /= 2) {
         if (lpr == 16 && !narrow) continue;
         const int64_t units = (int64_t)B * ((D + lpr * vec - 1) / (lpr * vec));
-        const int steps = THREADS / lpr * steps_per_thread, tiles = (T + steps - 1) / steps;
-        const int most = lpr * vec > 32 ? 8 : 16;      // beyond, the cluster's maps take the second CTA's place
-        for (int s = 1; s <= most && (s == 1 || s <= tiles); ++s) {
-            const int64_t n = units * s, slots = s == 1 ? 148 * occ : 8 * (18 * occ / s) * s;
-            const int64_t waves = (n + slots - 1) / slots, per_sm = (n + 147) / 148;
+        const int steps = THREADS / lpr * R, tiles = (T + steps - 1) / steps;
+        for (int s = 1; s <= 16 && (s == 1 || s <= tiles); ++s) {
+            const int64_t waves = (units + kClusters[occ - 1][s - 1] - 1) / kClusters[occ - 1][s - 1];
+            const int64_t per_sm = (units * s + 147) / 148;
             double cost = waves > 1 ? (double)waves * occ : per_sm > 1 ? (double)per_sm : 1.5;
             cost *= (double)((tiles + s - 1) / s) * steps * lpr * (1.0 + 0.01 * s + (lpr < 32 ? 0.04 : 0.0));
             if (least < 0 || cost < least) {
@@ -693,7 +739,7 @@ int launch(K kern, unsigned grid, int cluster, size_t smem, cudaStream_t stream,
 
 template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 int run_forward(const ScanIn& in, const float* h0, void* y, float* h_last, float* marks, cudaStream_t s) {
-    typedef Tile<T, VEC, LPR, kForwardSteps<T>, OG ? 3 : 2> Tl;
+    typedef Tile<T, VEC, LPR, OG ? 3 : 2> Tl;
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
     return launch(scan_forward_kernel<T, VEC, LPR, WIDE, OG>, (unsigned)grid, in.cluster, Tl::bytes(in.cluster), s, in, h0,
@@ -701,7 +747,7 @@ int run_forward(const ScanIn& in, const float* h0, void* y, float* h_last, float
 }
 template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 int run_backward(const ScanIn& in, const ScanGrad& q, cudaStream_t s) {
-    typedef Tile<T, VEC, LPR, kBackwardSteps, OG ? 4 : 3> Tl;
+    typedef Tile<T, VEC, LPR, OG ? 4 : 3> Tl;
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
     return launch(scan_backward_kernel<T, VEC, LPR, WIDE, OG>, (unsigned)grid, in.cluster, Tl::bytes(in.cluster), s, in, q);
@@ -720,7 +766,7 @@ int run_backward(const ScanIn& in, const ScanGrad& q, cudaStream_t s) {
                     : SCAN_OG(F, T, 1, 8, false, og, __VA_ARGS__))
 
 // CTAs that share an SM, by shared memory and registers
-constexpr int occupancy(bool backward, size_t elem) { return backward && elem == 4 ? 1 : 2; }
+constexpr int occupancy(bool backward, size_t elem) { return backward ? (elem == 4 ? 1 : 2) : (elem == 4 ? 2 : 3); }
 
 }  // namespace
 
@@ -729,7 +775,8 @@ extern "C" {
 int dg_gated_scan_forward(int dtype, int B, int T, int D, const void* x, int64_t x_sb, int64_t x_st,
                           const void* gate, int64_t gate_sb, int64_t gate_st, const void* out_gate,
                           int64_t out_gate_sb, int64_t out_gate_st, const float* h0, const int32_t* lengths,
-                          const uint8_t* resets, void* y, float* h_last, float* marks, void* stream) {
+                          const uint8_t* resets, void* y, float* h_last, float* marks, int32_t* dev_status,
+                          void* stream) {
     if (dtype == DG_DTYPE_F64) return DG_ERR_UNSUPPORTED;
     if (dtype < DG_DTYPE_F32 || dtype > DG_DTYPE_BF16 || B < 0 || T < 0 || D < 0) return DG_ERR_INVALID_ARGUMENT;
     if (B == 0 || D == 0) return DG_OK;
@@ -739,10 +786,9 @@ int dg_gated_scan_forward(int dtype, int B, int T, int D, const void* x, int64_t
     const size_t elem = dg_host::dtype_size(dtype);
     const int width = width_of(D, elem, {{x, x_sb, x_st}, {gate, gate_sb, gate_st}, {out_gate, out_gate_sb, out_gate_st},
                                          {y, 0, 0}});
-    const Shape sh = shape_of(B, T, D, width ? 2 : 1, elem == 4 ? kForwardSteps<float> : kForwardSteps<__half>,
-                              occupancy(false, elem), width == 2);
+    const Shape sh = shape_of(B, T, D, width ? 2 : 1, occupancy(false, elem), width == 2);
     const ScanIn in{x, gate, out_gate, x_sb, x_st, gate_sb, gate_st, out_gate_sb, out_gate_st, lengths, resets, B, T, D,
-                    sh.cluster};
+                    sh.cluster, dev_status, dg_host::wait_limit()};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     DG_DISPATCH_LM(dtype, S, {
         return SCAN_RUN(run_forward, S, width, sh.lpr, out_gate != nullptr, in, h0, y, h_last, marks, s);
@@ -755,7 +801,8 @@ int dg_gated_scan_backward(int dtype, int B, int T, int D, const void* x, int64_
                            int64_t out_gate_sb, int64_t out_gate_st, const int32_t* lengths, const uint8_t* resets,
                            const float* marks, const void* dy, int64_t dy_sb, int64_t dy_st, const float* dh_last,
                            void* dx, int64_t dx_sb, int64_t dx_st, void* dgate, int64_t dgate_sb, int64_t dgate_st,
-                           void* dout_gate, int64_t dout_gate_sb, int64_t dout_gate_st, float* dh0, void* stream) {
+                           void* dout_gate, int64_t dout_gate_sb, int64_t dout_gate_st, float* dh0,
+                           int32_t* dev_status, void* stream) {
     if (dtype == DG_DTYPE_F64) return DG_ERR_UNSUPPORTED;
     if (dtype < DG_DTYPE_F32 || dtype > DG_DTYPE_BF16 || B < 0 || T < 0 || D < 0) return DG_ERR_INVALID_ARGUMENT;
     if ((out_gate == nullptr) != (dout_gate == nullptr)) return DG_ERR_INVALID_ARGUMENT;
@@ -767,9 +814,9 @@ int dg_gated_scan_backward(int dtype, int B, int T, int D, const void* x, int64_
     const int width = width_of(D, elem, {{x, x_sb, x_st}, {gate, gate_sb, gate_st}, {out_gate, out_gate_sb, out_gate_st},
                                          {dy, dy_sb, dy_st}, {dx, dx_sb, dx_st}, {dgate, dgate_sb, dgate_st},
                                          {dout_gate, dout_gate_sb, dout_gate_st}});
-    const Shape sh = shape_of(B, T, D, width ? 2 : 1, kBackwardSteps, occupancy(true, elem), width == 2);
+    const Shape sh = shape_of(B, T, D, width ? 2 : 1, occupancy(true, elem), width == 2);
     const ScanIn in{x, gate, out_gate, x_sb, x_st, gate_sb, gate_st, out_gate_sb, out_gate_st, lengths, resets, B, T, D,
-                    sh.cluster};
+                    sh.cluster, dev_status, dg_host::wait_limit()};
     const ScanGrad q{marks, dy, dy_sb, dy_st, dh_last, dx, dgate, dout_gate, dx_sb, dx_st, dgate_sb, dgate_st,
                      dout_gate_sb, dout_gate_st, dh0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);

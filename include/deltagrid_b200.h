@@ -323,12 +323,14 @@ int dg_pkm_route(int dtype, int B, int H, int T, int dh, int g0, int g1, int top
  *   marks [B, ceil(T / DG_SCAN_MARK_STEPS), D] fp32 or NULL: the state before each block of
  *   DG_SCAN_MARK_STEPS steps, which the backward pass needs
  * Steps t >= lengths[b] leave the state as it is, give y = 0, and their inputs are not used
- * (they may hold anything); lengths are clamped to [0, T].
+ * (they may hold anything); lengths are clamped to [0, T].  dev_status (or NULL) gets
+ * DG_DEVCHK_TIMEOUT if a bounded wait inside the kernel gave up (results invalid).
  */
 int dg_gated_scan_forward(int dtype, int B, int T, int D, const void* x, int64_t x_sb, int64_t x_st,
                           const void* gate, int64_t gate_sb, int64_t gate_st, const void* out_gate,
                           int64_t out_gate_sb, int64_t out_gate_st, const float* h0, const int32_t* lengths,
-                          const uint8_t* resets, void* y, float* h_last, float* marks, void* stream);
+                          const uint8_t* resets, void* y, float* h_last, float* marks, int32_t* dev_status,
+                          void* stream);
 
 /*
  * Backward of dg_gated_scan_forward, from the same inputs and its marks:
@@ -342,7 +344,8 @@ int dg_gated_scan_backward(int dtype, int B, int T, int D, const void* x, int64_
                            int64_t out_gate_sb, int64_t out_gate_st, const int32_t* lengths, const uint8_t* resets,
                            const float* marks, const void* dy, int64_t dy_sb, int64_t dy_st, const float* dh_last,
                            void* dx, int64_t dx_sb, int64_t dx_st, void* dgate, int64_t dgate_sb, int64_t dgate_st,
-                           void* dout_gate, int64_t dout_gate_sb, int64_t dout_gate_st, float* dh0, void* stream);
+                           void* dout_gate, int64_t dout_gate_sb, int64_t dout_gate_st, float* dh0,
+                           int32_t* dev_status, void* stream);
 
 /* One step of the recurrence: x, gate, out_gate (or NULL) [B,D] with a row stride each; the
  * state h [B,D] fp32 contiguous is updated in place; y [B,D] contiguous. */

@@ -210,3 +210,22 @@ def test_refusals():
     leaf = w.clone().requires_grad_(True)
     with pytest.raises(RuntimeError, match="not differentiable"):
         torch.autograd.grad(gated_ffn(x, leaf).sum(), leaf, create_graph=True)
+
+
+def test_wait_timeout_flags_status():
+    """Wait budget zero: the kernel's first waits give up, it drains what it issued, flags
+    DG_DEVCHK_TIMEOUT and returns; the next call is right again."""
+    x, w, b, dh = _inputs(600, 256, 384, torch.bfloat16, seed=8)
+    want = gated_ffn(x, w, b)
+    torch.cuda.synchronize()
+    ext.device_status()
+    old = ext.set_wait_limit(0)
+    try:
+        gated_ffn(x, w, b)
+        torch.cuda.synchronize()
+    finally:
+        ext.set_wait_limit(old)
+    assert ext.device_status() & 0x4
+    again = gated_ffn(x, w, b)
+    torch.cuda.synchronize()
+    assert ext.device_status() == 0 and torch.equal(want, again)

@@ -280,3 +280,24 @@ def test_refusals():
     y, _ = gated_scan(leaf, x)
     with pytest.raises(RuntimeError, match="not differentiable"):
         torch.autograd.grad(y.sum(), leaf, create_graph=True)
+
+
+def test_wait_timeout_flags_status():
+    """Wait budget zero: the exchange between the CTAs of a cluster gives up at once, the launch says
+    so and ends; the next call is right again."""
+    from deltagrid_b200 import hsru_delta_cuda as ext
+    parts, h, _, _, _, _ = _inputs(1, 4000, 64, torch.bfloat16, seed=21)       # few channels: clusters
+    want = gated_scan(*parts, h)
+    torch.cuda.synchronize()
+    ext.device_status()
+    old = ext.set_wait_limit(0)
+    try:
+        gated_scan(*parts, h)
+        torch.cuda.synchronize()
+    finally:
+        ext.set_wait_limit(old)
+    assert ext.device_status() & 0x4
+    again = gated_scan(*parts, h)
+    torch.cuda.synchronize()
+    assert ext.device_status() == 0
+    assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])

@@ -9,7 +9,7 @@ F = ctypes.c_float
 
 def test_gated_scan_refusals():
     L = _lib.lib()
-    tail = [None] * 7
+    tail = [None] * 8
     assert L.dg_gated_scan_forward(7, 1, 4, 8, None, 0, 0, None, 0, 0, None, 0, 0, *tail) == -1
     assert L.dg_gated_scan_forward(1, 1, 4, 8, None, 0, 0, None, 0, 0, None, 0, 0, *tail) == -2      # f64
     assert L.dg_gated_scan_forward(0, 1, 4, 8, None, 0, 0, None, 0, 0, None, 0, 0, *tail) == -1      # null x
@@ -18,7 +18,7 @@ def test_gated_scan_refusals():
     one = ctypes.c_float(0)
     p = ctypes.addressof(one)
     args = [0, 1, 4, 8, p, 0, 0, p, 0, 0, p, 0, 0, None, None, p, p, 0, 0, None, p, 0, 0, p, 0, 0]
-    assert L.dg_gated_scan_backward(*args, None, 0, 0, None, None) == -1        # out_gate without its gradient
+    assert L.dg_gated_scan_backward(*args, None, 0, 0, None, None, None) == -1        # out_gate without its gradient
     assert L.dg_gated_scan_step(0, 1, 8, None, 0, None, 0, None, 0, None, None, None) == -1
     assert L.dg_gated_scan_step(1, 1, 8, None, 0, None, 0, None, 0, None, None, None) == -2
 
