@@ -195,10 +195,10 @@ template <int CH> struct MapsBack : Maps<CH> {
 
 template <typename T, int VEC, int LPR, int ARRAYS> struct Tile {
     static constexpr int STEPS = THREADS / LPR * R, CH = LPR * VEC;
-    static constexpr int WARP_STEPS = 32 / LPR * R;
     typedef Pack<T, VEC> P;
-    // one input's tile: [warp][step of the warp][channel]
-    static constexpr int ARRAY = THREADS * R;                     // packs
+    // one input's tile: [warp][row group][step][channel]
+    static constexpr int WARP_PACKS = 32 / LPR * (R * LPR + (LPR < 32 ? LPR : 0));
+    static constexpr int ARRAY = WARPS * WARP_PACKS;              // packs
     static constexpr size_t STAGE = (size_t)ARRAYS * ARRAY * sizeof(P);
     static constexpr size_t bytes(int cluster) {
         return STAGES * STAGE + (cluster > 1 ? 2 * cluster * CH * sizeof(float2) : 0);
@@ -206,37 +206,40 @@ template <typename T, int VEC, int LPR, int ARRAYS> struct Tile {
 };
 
 // A warp's steps of one input into its part of a stage.  WIDE: 16 bytes a lane, any lane any
-// step of the warp.  Otherwise each thread copies the steps it reads itself.
+// step of the warp.  Otherwise each thread copies the steps it reads itself.  Row groups lie kPad
+// packs further apart than their steps need, so that a warp's reads meet 32 different banks.
+template <int LPR> constexpr int kPad = LPR < 32 ? LPR : 0;
 template <typename T, int VEC, int LPR, bool WIDE>
 __device__ __forceinline__ void fetch(Pack<T, VEC>* warp_part, const T* row, int64_t step, int t_warp, int len, int d0,
                                       int D, int lane) {
-    constexpr int PPS = LPR;                                      // packs per step
+    constexpr int GROUP = R * LPR + kPad<LPR>;                    // packs from one row group to the next
     if constexpr (WIDE) {
-        constexpr int E = 16 / sizeof(T), CPS = LPR * VEC / E, N = 32 / LPR * R * CPS / 32;
+        constexpr int E = 16 / sizeof(T), CPS = LPR * VEC / E, SPC = 32 / CPS, N = 32 / LPR * R / SPC;
         const int col = lane % CPS * E;
         const bool on = d0 + col < D;
-        const T* p = row + (int64_t)(t_warp + lane / CPS) * step + d0 + col;
-        T* dst = reinterpret_cast<T*>(warp_part) + lane * E;
+        const T* p = on ? row + (int64_t)(t_warp + lane / CPS) * step + d0 + col : row;
+        const int64_t advance = on ? SPC * step : 0;
+        const int left = on ? len - t_warp - lane / CPS : 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int s = lane / CPS + i * (32 / CPS);
-            const bool live = on && t_warp + s < len;
-            copy_async<16>(dst + i * 32 * E, live ? p : row, live);
-            p += (32 / CPS) * step;
+            const int s = lane / CPS + i * SPC;
+            T* dst = reinterpret_cast<T*>(warp_part) + (s / R * GROUP + s % R * LPR) * VEC + col;
+            copy_async<16>(dst, p, i * SPC < left);                // reads nothing where it is false
+            p += advance;
         }
     } else {
         const int lc = lane % LPR, s0 = lane / LPR * R, d = d0 + lc * VEC;
         const T* p = row + (int64_t)(t_warp + s0) * step + d;
-        Pack<T, VEC>* dst = warp_part + s0 * PPS + lc;
+        Pack<T, VEC>* dst = warp_part + lane / LPR * GROUP + lc;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const bool live = d < D && t_warp + s0 + r < len;
             if constexpr (sizeof(T) * VEC >= 4) {
-                copy_async<sizeof(T) * VEC>(dst + r * PPS, live ? p : row, live);
+                copy_async<sizeof(T) * VEC>(dst + r * LPR, live ? p : row, live);
             } else {                       // 2 bytes: below what cp.async copies
                 T z = dg::from_f<T>(0.f);
                 if (live) z = *p;
-                dst[r * PPS].v[0] = z;
+                dst[r * LPR].v[0] = z;
             }
             p += step;
         }
@@ -404,8 +407,8 @@ __global__ void __launch_bounds__(THREADS, 3)
     const uint8_t* rs = in.resets ? in.resets + (int64_t)at.b * in.T : nullptr;
     const int nblk = (in.T + DG_SCAN_MARK_STEPS - 1) / DG_SCAN_MARK_STEPS;
     constexpr int ARR = Tl::ARRAY, STG = (OG ? 3 : 2) * ARR;
-    Pk* warp_part = reinterpret_cast<Pk*>(smem) + at.warp * Tl::WARP_STEPS * LPR;
-    const int own = at.lane / LPR * R * LPR + at.lc;              // this thread's first pack in it
+    Pk* warp_part = reinterpret_cast<Pk*>(smem) + at.warp * Tl::WARP_PACKS;
+    const int own = at.lane / LPR * (R * LPR + kPad<LPR>) + at.lc;              // this thread's first pack in it
     bool bad = false;
     open_exchange(maps.received, S);
 
@@ -529,8 +532,8 @@ __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, Sc
     const uint8_t* rs = in.resets ? in.resets + (int64_t)at.b * in.T : nullptr;
     const int nblk = (in.T + DG_SCAN_MARK_STEPS - 1) / DG_SCAN_MARK_STEPS;
     constexpr int ARR = Tl::ARRAY, STG = (OG ? 4 : 3) * ARR;
-    Pk* warp_part = reinterpret_cast<Pk*>(smem) + at.warp * Tl::WARP_STEPS * LPR;
-    const int own = at.lane / LPR * R * LPR + at.lc;
+    Pk* warp_part = reinterpret_cast<Pk*>(smem) + at.warp * Tl::WARP_PACKS;
+    const int own = at.lane / LPR * (R * LPR + kPad<LPR>) + at.lc;
     const bool carries = tid < Tl::CH && at.d0 + tid < in.D;      // thread c carries channel d0 + c
     bool bad = false;
     open_exchange(maps.received, S);
@@ -682,8 +685,9 @@ int width_of(int D, size_t elem, std::initializer_list<Row> rows) {
 }
 
 // Channels per CTA (lpr x vec) and cluster size: the least work of the busiest SM, CTAs on it x
-// walked steps x channels.  An SM with a single CTA waits at its barriers (1.5 x its work here);
-// larger clusters and narrower rows cost a little more, which also decides ties.
+// walked steps x channels.  Clusters fill some SMs before others, so the busiest has `occ` of their
+// CTAs.  An SM with a single CTA waits at its barriers (1.5 x its work here); larger clusters and
+// narrower rows cost a little more, which also decides ties.
 struct Shape {
     int lpr, cluster;
 };
@@ -702,7 +706,7 @@ Shape shape_of(int B, int T, int D, int vec, int occ, bool narrow) {
         for (int s = 1; s <= 16 && (s == 1 || s <= tiles); ++s) {
             const int64_t waves = (units + kClusters[occ - 1][s - 1] - 1) / kClusters[occ - 1][s - 1];
             const int64_t per_sm = (units * s + 147) / 148;
-            double cost = waves > 1 ? (double)waves * occ : per_sm > 1 ? (double)per_sm : 1.5;
+            double cost = waves > 1 || (s > 1 && units * s > 148) ? (double)waves * occ : per_sm > 1 ? (double)per_sm : 1.5;
             cost *= (double)((tiles + s - 1) / s) * steps * lpr * (1.0 + 0.01 * s + (lpr < 32 ? 0.04 : 0.0));
             if (least < 0 || cost < least) {
                 least = cost;
