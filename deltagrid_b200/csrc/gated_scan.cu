@@ -21,7 +21,7 @@
 // The backward pass carries r_t = c_t (d_t + r_{t+1}) (d the gradient that enters at step t)
 // the same way in reverse, and forms the states again from the marks that the forward pass
 // leaves every DG_SCAN_MARK_STEPS steps: fp32 states, so nothing is lost to the rounding of
-// y, for 4 / 64 bytes a step.
+// y, for 4 / 32 of a byte a step.
 //
 // What bounds it: HBM at 4 (forward, 16-bit) to 14 bytes (backward) an element, with the
 // special-function unit close behind (two operations for each sigmoid); pairs of channels use
@@ -40,8 +40,7 @@ namespace {
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int STAGES = 2;                  // tiles of input in shared memory
-constexpr int R = 8;                       // steps per thread
-static_assert(DG_SCAN_MARK_STEPS % R == 0, "a mark falls on a thread's first step");
+constexpr int kForwardSteps = 8, kBackwardSteps = 4;      // steps per thread, by the registers of three CTAs to an SM
 
 struct ScanIn {
     const void *x, *g, *o;
@@ -193,7 +192,7 @@ template <int CH> struct MapsBack : Maps<CH> {
     float carry_back[WARPS][CH];
 };
 
-template <typename T, int VEC, int LPR, int ARRAYS> struct Tile {
+template <typename T, int VEC, int LPR, int R, int ARRAYS> struct Tile {
     static constexpr int STEPS = THREADS / LPR * R, CH = LPR * VEC;
     typedef Pack<T, VEC> P;
     // one input's tile: [warp][row group][step][channel]
@@ -209,7 +208,7 @@ template <typename T, int VEC, int LPR, int ARRAYS> struct Tile {
 // step of the warp.  Otherwise each thread copies the steps it reads itself.  Row groups lie kPad
 // packs further apart than their steps need, so that a warp's reads meet 32 different banks.
 template <int LPR> constexpr int kPad = LPR < 32 ? LPR : 0;
-template <typename T, int VEC, int LPR, bool WIDE>
+template <typename T, int VEC, int LPR, int R, bool WIDE>
 __device__ __forceinline__ void fetch(Pack<T, VEC>* warp_part, const T* row, int64_t step, int t_warp, int len, int d0,
                                       int D, int lane) {
     constexpr int GROUP = R * LPR + kPad<LPR>;                    // packs from one row group to the next
@@ -279,7 +278,7 @@ __device__ __forceinline__ void warp_maps(Fv<VEC> P, Fv<VEC> H, Fv<VEC>& Pb, Fv<
 }
 
 // where a thread stands: shared by both passes
-template <int LPR, int VEC> struct Place {
+template <int LPR, int VEC, int R> struct Place {
     int warp, lane, lc, rank, b, d0, d, len, span, ntiles;
     bool on;
     __device__ __forceinline__ Place(const ScanIn& in) {
@@ -304,17 +303,17 @@ template <int LPR, int VEC> struct Place {
 
 // bit r: a document starts at step r of this thread.  The load was made a tile earlier: lane r of
 // a group holds step r.
-template <int LPR> __device__ __forceinline__ uint8_t load_reset(const uint8_t* rs, int t, int lc, int len) {
+template <int LPR, int R> __device__ __forceinline__ uint8_t load_reset(const uint8_t* rs, int t, int lc, int len) {
     return lc < R && t + lc < len ? rs[t + lc] : 0;
 }
-template <int LPR> __device__ __forceinline__ unsigned reset_bits(uint8_t mine, int lane) {
+template <int LPR, int R> __device__ __forceinline__ unsigned reset_bits(uint8_t mine, int lane) {
     static_assert(LPR >= R, "one lane per step");
     return __ballot_sync(DG_FULL_MASK, mine != 0) >> (lane & ~(LPR - 1)) & ((1u << R) - 1);
 }
 
 // the forward map of a thread's steps: c, u and their composition (P, H).  WHOLE: every step is
 // valid and none starts a document.
-template <bool WHOLE, typename T, int VEC, int LPR>
+template <bool WHOLE, typename T, int VEC, int LPR, int R>
 __device__ __forceinline__ void forward_map(const Pack<T, VEC>* xs, const Pack<T, VEC>* gs, int left, unsigned resets,
                                             Fv<VEC> (&c)[R], Fv<VEC> (&u)[R], Fv<VEC>* nas, Fv<VEC>& P, Fv<VEC>& H) {
 #pragma unroll
@@ -333,7 +332,7 @@ __device__ __forceinline__ void forward_map(const Pack<T, VEC>* xs, const Pack<T
 }
 
 // y of a thread's steps from the state h before them; `left` valid steps, `room` steps inside T
-template <bool WHOLE, typename T, int VEC, int LPR, bool OG>
+template <bool WHOLE, typename T, int VEC, int LPR, bool OG, int R>
 __device__ __forceinline__ void forward_apply(Fv<VEC> h, const Fv<VEC> (&c)[R], const Fv<VEC> (&u)[R],
                                               const Pack<T, VEC>* os, T* y, int D, int left, int room) {
 #pragma unroll
@@ -393,13 +392,15 @@ __device__ __forceinline__ void close_exchange(int S, bool bad, int32_t* status)
 template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 __global__ void __launch_bounds__(THREADS, 3)
     scan_forward_kernel(ScanIn in, const float* h0, T* y, float* h_last, float* marks) {
-    typedef Tile<T, VEC, LPR, OG ? 3 : 2> Tl;
+    constexpr int R = kForwardSteps;
+    static_assert(DG_SCAN_MARK_STEPS % R == 0, "a mark falls on a thread's first step");
+    typedef Tile<T, VEC, LPR, R, OG ? 3 : 2> Tl;
     typedef Pack<T, VEC> Pk;
     typedef Fv<VEC> V;
     extern __shared__ __align__(16) uint8_t smem[];
     float2* cta_maps = reinterpret_cast<float2*>(smem + STAGES * Tl::STAGE);
     __shared__ Maps<Tl::CH> maps;
-    const Place<LPR, VEC> at(in);
+    const Place<LPR, VEC, R> at(in);
     const int tid = threadIdx.x, S = in.cluster, d = at.d, len = at.len;
     const T* x = (const T*)in.x + at.b * in.x_sb;
     const T* g = (const T*)in.g + at.b * in.g_sb;
@@ -416,11 +417,11 @@ __global__ void __launch_bounds__(THREADS, 3)
     auto prefetch = [&](int it) {
         const int t = at.warp_step(it);
         Pk* st = warp_part + (it & 1) * STG;
-        fetch<T, VEC, LPR, WIDE>(st, x, in.x_st, t, len, at.d0, in.D, at.lane);
-        fetch<T, VEC, LPR, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
-        if (OG) fetch<T, VEC, LPR, WIDE>(st + 2 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, R, WIDE>(st, x, in.x_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, R, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
+        if (OG) fetch<T, VEC, LPR, R, WIDE>(st + 2 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
         copy_commit();
-        if (rs) next_reset = load_reset<LPR>(rs, at.step(it), at.lc, len);
+        if (rs) next_reset = load_reset<LPR, R>(rs, at.step(it), at.lc, len);
     };
 
     // thread c < CH carries channel d0 + c from tile to tile
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 3)
     if (at.ntiles > 0) prefetch(0);
     for (int it = 0; it < at.ntiles; ++it) {
         const int t = at.step(it);
-        const unsigned resets = rs ? reset_bits<LPR>(next_reset, at.lane) : 0;
+        const unsigned resets = rs ? reset_bits<LPR, R>(next_reset, at.lane) : 0;
         __syncwarp();                      // the other stage has been read
         if (it + 1 < at.ntiles) prefetch(it + 1);
         else copy_commit();
@@ -438,8 +439,8 @@ __global__ void __launch_bounds__(THREADS, 3)
         const Pk* st = warp_part + (it & 1) * STG + own;
         V c[R], u[R], P, H;
         const bool whole = t + R <= len && resets == 0;
-        if (whole) forward_map<true, T, VEC, LPR>(st, st + ARR, R, 0, c, u, nullptr, P, H);
-        else forward_map<false, T, VEC, LPR>(st, st + ARR, len - t, resets, c, u, nullptr, P, H);
+        if (whole) forward_map<true, T, VEC, LPR, R>(st, st + ARR, R, 0, c, u, nullptr, P, H);
+        else forward_map<false, T, VEC, LPR, R>(st, st + ARR, len - t, resets, c, u, nullptr, P, H);
         V Pb, Hb, Pw, Hw;
         warp_maps<LPR, VEC, true>(P, H, Pb, Hb, Pw, Hw, at.lane);
         if (at.lane >= 32 - LPR)
@@ -474,8 +475,8 @@ __global__ void __launch_bounds__(THREADS, 3)
                 for (int v = 0; v < VEC; ++v)
                     marks[((int64_t)at.b * nblk + t / DG_SCAN_MARK_STEPS) * in.D + d + v] = h.v[v];
             T* yp = y + ((int64_t)at.b * in.T + t) * in.D + d;
-            if (whole) forward_apply<true, T, VEC, LPR, OG>(h, c, u, st + 2 * ARR, yp, in.D, R, R);
-            else forward_apply<false, T, VEC, LPR, OG>(h, c, u, st + 2 * ARR, yp, in.D, len - t, in.T - t);
+            if (whole) forward_apply<true, T, VEC, LPR, OG, R>(h, c, u, st + 2 * ARR, yp, in.D, R, R);
+            else forward_apply<false, T, VEC, LPR, OG, R>(h, c, u, st + 2 * ARR, yp, in.D, len - t, in.T - t);
         }
     }
     if (h_last && at.rank == 0 && tid < Tl::CH && at.d0 + tid < in.D)
@@ -485,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, 3)
 
 // the gradients of a thread's steps, last to first: u holds the state before each step (0 at a
 // reset), rr what comes back from the steps after them
-template <bool WHOLE, typename T, int VEC, int LPR, bool OG>
+template <bool WHOLE, typename T, int VEC, int LPR, bool OG, int R>
 __device__ __forceinline__ void backward_apply(Fv<VEC> rr, const Fv<VEC> (&c)[R], const Fv<VEC> (&u)[R],
                                                const Fv<VEC> (&na)[R], const Fv<VEC> (&e)[R], const Pack<T, VEC>* xs,
                                                const Pack<T, VEC>* dys, const Pack<T, VEC>* os, T* px, int64_t sx, T* pg,
@@ -515,15 +516,16 @@ __device__ __forceinline__ void backward_apply(Fv<VEC> rr, const Fv<VEC> (&c)[R]
 }
 
 template <typename T, int VEC, int LPR, bool WIDE, bool OG>
-__global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, ScanGrad q) {
-    typedef Tile<T, VEC, LPR, OG ? 4 : 3> Tl;
+__global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, ScanGrad q) {
+    constexpr int R = kBackwardSteps;
+    typedef Tile<T, VEC, LPR, R, OG ? 4 : 3> Tl;
     static_assert(Tl::STEPS % DG_SCAN_MARK_STEPS == 0, "tiles start at marks");
     typedef Pack<T, VEC> Pk;
     typedef Fv<VEC> V;
     extern __shared__ __align__(16) uint8_t smem[];
     float2* cta_maps = reinterpret_cast<float2*>(smem + STAGES * Tl::STAGE);
     __shared__ MapsBack<Tl::CH> maps;
-    const Place<LPR, VEC> at(in);
+    const Place<LPR, VEC, R> at(in);
     const int tid = threadIdx.x, S = in.cluster, d = at.d, len = at.len;
     const T* x = (const T*)in.x + at.b * in.x_sb;
     const T* g = (const T*)in.g + at.b * in.g_sb;
@@ -543,12 +545,12 @@ __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, Sc
     auto prefetch = [&](int it) {
         const int t = at.warp_step(it), t0 = it * at.span + at.rank * Tl::STEPS;
         Pk* st = warp_part + (it & 1) * STG;
-        fetch<T, VEC, LPR, WIDE>(st, x, in.x_st, t, len, at.d0, in.D, at.lane);
-        fetch<T, VEC, LPR, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
-        fetch<T, VEC, LPR, WIDE>(st + 2 * ARR, dy, q.dy_st, t, len, at.d0, in.D, at.lane);
-        if (OG) fetch<T, VEC, LPR, WIDE>(st + 3 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, R, WIDE>(st, x, in.x_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, R, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
+        fetch<T, VEC, LPR, R, WIDE>(st + 2 * ARR, dy, q.dy_st, t, len, at.d0, in.D, at.lane);
+        if (OG) fetch<T, VEC, LPR, R, WIDE>(st + 3 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
         copy_commit();
-        if (rs) next_reset = load_reset<LPR>(rs, at.step(it), at.lc, len);
+        if (rs) next_reset = load_reset<LPR, R>(rs, at.step(it), at.lc, len);
         if (carries && t0 < in.T)
             next_mark = q.marks[((int64_t)at.b * nblk + t0 / DG_SCAN_MARK_STEPS) * in.D + at.d0 + tid];
     };
@@ -558,7 +560,7 @@ __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, Sc
     if (at.ntiles > 0) prefetch(at.ntiles - 1);
     for (int it = at.ntiles - 1; it >= 0; --it) {
         const int t = at.step(it);
-        const unsigned resets = rs ? reset_bits<LPR>(next_reset, at.lane) : 0;
+        const unsigned resets = rs ? reset_bits<LPR, R>(next_reset, at.lane) : 0;
         const float mark = next_mark;
         __syncwarp();
         if (it > 0) prefetch(it - 1);
@@ -569,8 +571,8 @@ __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, Sc
         const bool whole = t + R <= len && resets == 0;
         // c and u of the forward map, and the gradient that enters at each step
         V c[R], u[R], na[R], e[R], P, H, Q = all<VEC>(0.f);
-        if (whole) forward_map<true, T, VEC, LPR>(st, st + ARR, R, 0, c, u, na, P, H);
-        else forward_map<false, T, VEC, LPR>(st, st + ARR, len - t, resets, c, u, na, P, H);
+        if (whole) forward_map<true, T, VEC, LPR, R>(st, st + ARR, R, 0, c, u, na, P, H);
+        else forward_map<false, T, VEC, LPR, R>(st, st + ARR, len - t, resets, c, u, na, P, H);
 #pragma unroll
         for (int r = R - 1; r >= 0; --r) {
             e[r] = widen(st[2 * ARR + r * LPR]);
@@ -629,13 +631,13 @@ __global__ void __launch_bounds__(THREADS, 2) scan_backward_kernel(ScanIn in, Sc
             T* pg = (T*)q.dg_ + at.b * q.dg_sb + t * q.dg_st + d;
             T* po = OG ? (T*)q.do_ + at.b * q.do_sb + t * q.do_st + d : nullptr;
             if (whole) {
-                backward_apply<true, T, VEC, LPR, OG>(rr, c, u, na, e, st, st + 2 * ARR, st + 3 * ARR, px, q.dx_st, pg,
+                backward_apply<true, T, VEC, LPR, OG, R>(rr, c, u, na, e, st, st + 2 * ARR, st + 3 * ARR, px, q.dx_st, pg,
                                                       q.dg_st, po, q.do_st, R, R, 0);
             } else {
 #pragma unroll
                 for (int r = 0; r < R; ++r)
                     if ((resets >> r) & 1) u[r] = all<VEC>(0.f);
-                backward_apply<false, T, VEC, LPR, OG>(rr, c, u, na, e, st, st + 2 * ARR, st + 3 * ARR, px, q.dx_st, pg,
+                backward_apply<false, T, VEC, LPR, OG, R>(rr, c, u, na, e, st, st + 2 * ARR, st + 3 * ARR, px, q.dx_st, pg,
                                                        q.dg_st, po, q.do_st, len - t, in.T - t, resets);
             }
         }
@@ -696,13 +698,13 @@ struct Shape {
 constexpr int kClusters[3][16] = {{148, 74, 45, 33, 26, 22, 15, 15, 15, 11, 7, 7, 7, 7, 7, 7},
                                   {296, 148, 93, 71, 56, 45, 37, 33, 30, 26, 21, 21, 17, 14, 14, 14},
                                   {444, 222, 142, 104, 82, 71, 56, 48, 45, 41, 31, 31, 28, 24, 24, 21}};
-Shape shape_of(int B, int T, int D, int vec, int occ, bool narrow) {
+Shape shape_of(int B, int T, int D, int vec, int steps_per_thread, int occ, bool narrow) {
     Shape best{32, 1};
     double least = -1.0;
     for (int lpr = 32; lpr >= 8; lpr /= 2) {
         if (lpr == 16 && !narrow) continue;
         const int64_t units = (int64_t)B * ((D + lpr * vec - 1) / (lpr * vec));
-        const int steps = THREADS / lpr * R, tiles = (T + steps - 1) / steps;
+        const int steps = THREADS / lpr * steps_per_thread, tiles = (T + steps - 1) / steps;
         for (int s = 1; s <= 16 && (s == 1 || s <= tiles); ++s) {
             const int64_t waves = (units + kClusters[occ - 1][s - 1] - 1) / kClusters[occ - 1][s - 1];
             const int64_t per_sm = (units * s + 147) / 148;
@@ -743,7 +745,7 @@ int launch(K kern, unsigned grid, int cluster, size_t smem, cudaStream_t stream,
 
 template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 int run_forward(const ScanIn& in, const float* h0, void* y, float* h_last, float* marks, cudaStream_t s) {
-    typedef Tile<T, VEC, LPR, OG ? 3 : 2> Tl;
+    typedef Tile<T, VEC, LPR, kForwardSteps, OG ? 3 : 2> Tl;
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
     return launch(scan_forward_kernel<T, VEC, LPR, WIDE, OG>, (unsigned)grid, in.cluster, Tl::bytes(in.cluster), s, in, h0,
@@ -751,7 +753,7 @@ int run_forward(const ScanIn& in, const float* h0, void* y, float* h_last, float
 }
 template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 int run_backward(const ScanIn& in, const ScanGrad& q, cudaStream_t s) {
-    typedef Tile<T, VEC, LPR, OG ? 4 : 3> Tl;
+    typedef Tile<T, VEC, LPR, kBackwardSteps, OG ? 4 : 3> Tl;
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
     return launch(scan_backward_kernel<T, VEC, LPR, WIDE, OG>, (unsigned)grid, in.cluster, Tl::bytes(in.cluster), s, in, q);
@@ -770,7 +772,7 @@ int run_backward(const ScanIn& in, const ScanGrad& q, cudaStream_t s) {
                     : SCAN_OG(F, T, 1, 8, false, og, __VA_ARGS__))
 
 // CTAs that share an SM, by shared memory and registers
-constexpr int occupancy(bool backward, size_t elem) { return backward ? (elem == 4 ? 1 : 2) : (elem == 4 ? 2 : 3); }
+constexpr int occupancy(bool backward, size_t elem) { return elem == 4 ? 2 : 3; }
 
 }  // namespace
 
@@ -790,7 +792,7 @@ int dg_gated_scan_forward(int dtype, int B, int T, int D, const void* x, int64_t
     const size_t elem = dg_host::dtype_size(dtype);
     const int width = width_of(D, elem, {{x, x_sb, x_st}, {gate, gate_sb, gate_st}, {out_gate, out_gate_sb, out_gate_st},
                                          {y, 0, 0}});
-    const Shape sh = shape_of(B, T, D, width ? 2 : 1, occupancy(false, elem), width == 2);
+    const Shape sh = shape_of(B, T, D, width ? 2 : 1, kForwardSteps, occupancy(false, elem), width == 2);
     const ScanIn in{x, gate, out_gate, x_sb, x_st, gate_sb, gate_st, out_gate_sb, out_gate_st, lengths, resets, B, T, D,
                     sh.cluster, dev_status, dg_host::wait_limit()};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -818,7 +820,7 @@ int dg_gated_scan_backward(int dtype, int B, int T, int D, const void* x, int64_
     const int width = width_of(D, elem, {{x, x_sb, x_st}, {gate, gate_sb, gate_st}, {out_gate, out_gate_sb, out_gate_st},
                                          {dy, dy_sb, dy_st}, {dx, dx_sb, dx_st}, {dgate, dgate_sb, dgate_st},
                                          {dout_gate, dout_gate_sb, dout_gate_st}});
-    const Shape sh = shape_of(B, T, D, width ? 2 : 1, occupancy(true, elem), width == 2);
+    const Shape sh = shape_of(B, T, D, width ? 2 : 1, kBackwardSteps, occupancy(true, elem), width == 2);
     const ScanIn in{x, gate, out_gate, x_sb, x_st, gate_sb, gate_st, out_gate_sb, out_gate_st, lengths, resets, B, T, D,
                     sh.cluster, dev_status, dg_host::wait_limit()};
     const ScanGrad q{marks, dy, dy_sb, dy_st, dh_last, dx, dgate, dout_gate, dx_sb, dx_st, dgate_sb, dgate_st,

@@ -310,7 +310,7 @@ int dg_pkm_route(int dtype, int B, int H, int T, int dh, int g0, int g1, int top
  * ------------------------------------------------------------------------- */
 
 /* Steps between the states that dg_gated_scan_forward leaves for the backward pass. */
-#define DG_SCAN_MARK_STEPS 64
+#define DG_SCAN_MARK_STEPS 32
 
 /*
  * Gated linear recurrence over a sequence, per batch row b and channel d:
