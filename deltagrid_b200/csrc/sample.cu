@@ -45,55 +45,69 @@ struct SampleParams {
 // ---- keys ------------------------------------------------------------------------
 // Unsigned, in the order of the values; NaN counts as -inf, -0 equals +0.  0 is no value's key: it
 // marks places outside the row.
-template <typename T> struct Key {         // 16-bit logits, two at a time
+template <typename T> struct Key {         // 16-bit logits, two to a word
     typedef uint16_t type;
-    static constexpr int BITS = 16;
+    static constexpr int BITS = 16, PER = 2;
     static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-    __device__ static __forceinline__ uint32_t pair(uint32_t x) {
-        const uint32_t inf = BF16 ? 0x7f807f80u : 0x7c007c00u;
-        const uint32_t nan = __vcmpgtu2(x & 0x7fff7fffu, inf);
-        x = (x & ~nan) | ((inf | 0x80008000u) & nan);
-        x &= ~__vcmpeq2(x, 0x80008000u);
-        const uint32_t neg = ((x >> 15) & 0x00010001u) * 0xffffu;
+    // NaN -> -inf (the larger of the two that is a number), -0 -> +0
+    __device__ static __forceinline__ uint32_t clean(uint32_t x) {
+        if constexpr (BF16) {
+            const uint32_t inf = 0xff80ff80u, zero = 0;
+            __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&inf));
+            v = __hadd2(v, *reinterpret_cast<const __nv_bfloat162*>(&zero));
+            return *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+            const uint32_t inf = 0xfc00fc00u, zero = 0;
+            __half2 v = __hmax2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&inf));
+            v = __hadd2(v, *reinterpret_cast<const __half2*>(&zero));
+            return *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
+    __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {        // of cleaned values
+        if constexpr (BF16) {
+            const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+            return *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+            const __half2 v = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+            return *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
+    __device__ static __forceinline__ uint32_t ordered(uint32_t x) {      // cleaned values -> keys
+        uint32_t neg;                                                     // each half's sign in all its bits
+        asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(neg) : "r"(x));
         return x ^ (neg | 0x80008000u);
     }
-    __device__ static __forceinline__ uint4 vec(uint4 v) { return make_uint4(pair(v.x), pair(v.y), pair(v.z), pair(v.w)); }
-    __device__ static __forceinline__ uint32_t one(T l) { return pair(*reinterpret_cast<const uint16_t*>(&l)) & 0xffffu; }
+    static constexpr uint32_t NONE = BF16 ? 0xff80ff80u : 0xfc00fc00u;    // -inf
+    __device__ static __forceinline__ uint32_t one(T l) { return ordered(clean(*reinterpret_cast<const uint16_t*>(&l))) & 0xffffu; }
     __device__ static __forceinline__ float value(uint32_t k) {
         const uint32_t b = (k ^ ((k & 0x8000u) ? 0x8000u : 0xffffu)) & 0xffffu;
         if (BF16) return __uint_as_float(b << 16);
         const uint16_t h = (uint16_t)b;
         return __half2float(*reinterpret_cast<const __half*>(&h));
     }
-    // the largest key of a vector
-    __device__ static __forceinline__ uint32_t most(uint4 v) {
-        const uint32_t m = __vmaxu2(__vmaxu2(v.x, v.y), __vmaxu2(v.z, v.w));
-        return max(m & 0xffffu, m >> 16);
-    }
-    __device__ static __forceinline__ uint32_t at(const uint4& v, int e) {
-        const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
-        return e & 1 ? w >> 16 : w & 0xffffu;
-    }
+    // key `e` of a word, and the larger of its two
+    __device__ static __forceinline__ uint32_t at(uint32_t w, int e) { return e ? w >> 16 : w & 0xffffu; }
+    __device__ static __forceinline__ uint32_t most(uint32_t w) { return max(w >> 16, w & 0xffffu); }
+    __device__ static __forceinline__ uint32_t near(float l) { return one(dg::from_f<T>(l)); }
 };
 template <> struct Key<float> {
     typedef uint32_t type;
-    static constexpr int BITS = 32;
-    __device__ static __forceinline__ uint32_t one(float l) {
-        if (l != l) l = -INFINITY;
-        const uint32_t b = __float_as_uint(l + 0.f);
-        return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+    static constexpr int BITS = 32, PER = 1;
+    static constexpr uint32_t NONE = 0xff800000u;
+    __device__ static __forceinline__ uint32_t clean(uint32_t x) {
+        return __float_as_uint(fmaxf(__uint_as_float(x), -INFINITY) + 0.f);
     }
-    __device__ static __forceinline__ uint4 vec(uint4 v) {
-        return make_uint4(one(__uint_as_float(v.x)), one(__uint_as_float(v.y)), one(__uint_as_float(v.z)),
-                          one(__uint_as_float(v.w)));
+    __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
     }
+    __device__ static __forceinline__ uint32_t ordered(uint32_t b) { return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u); }
+    __device__ static __forceinline__ uint32_t one(float l) { return ordered(clean(__float_as_uint(l))); }
     __device__ static __forceinline__ float value(uint32_t k) {
         return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
     }
-    __device__ static __forceinline__ uint32_t most(uint4 v) { return max(max(v.x, v.y), max(v.z, v.w)); }
-    __device__ static __forceinline__ uint32_t at(const uint4& v, int e) {
-        return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
-    }
+    __device__ static __forceinline__ uint32_t at(uint32_t w, int) { return w; }
+    __device__ static __forceinline__ uint32_t most(uint32_t w) { return w; }
+    __device__ static __forceinline__ uint32_t near(float l) { return one(l); }
 };
 
 // The mass of a token; the row's maximum m is above -inf.  Below -28 (2^40 e^-28 < 1) it is 0, as it
@@ -141,12 +155,11 @@ __device__ __forceinline__ uint32_t remote_add(uint32_t* p, uint32_t rank, uint3
 struct Shared {
     u64 list[CAP];                         // collected tokens: key << 32 | ~index, or index << 32 | key
     uint32_t hist[4][256];                 // counts, and the masses' 13 + 13 + 14 bits
-    u64 bins[256];
+    u64 bins[2][256];                      // what they amount to; this CTA's, read by the cluster
+    uint32_t reach[3 * 16];                // partial maxima that reach a candidate bound
     u64 warp[WARPS];
     u64 post[8];                           // values that the cluster's other CTAs read
     uint32_t collected;
-    uint32_t found_bin;
-    u64 found_above;
     uint32_t flag;
 };
 
@@ -237,65 +250,74 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     typedef Key<T> K;
     typedef typename K::type key_t;
     constexpr int E = 16 / sizeof(T);
+    constexpr int W = K::PER;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Shared s;
     uint4* vecs = reinterpret_cast<uint4*>(smem);
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(smem);
     key_t* keys = reinterpret_cast<key_t*>(smem);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int C = p.cluster, rank = C > 1 ? (int)cluster_rank() : 0, row = blockIdx.x / C;
     const int V = p.V, s0 = min(rank * p.slice, V), n = min(p.slice, V - s0);
     const T* src = static_cast<const T*>(p.logits) + (int64_t)row * p.row_stride + s0;
 
+    // ---- parameters
+    const float temp = p.temperature ? p.temperature[row] : p.temperature_v;
+    int k = p.top_k ? p.top_k[row] : p.top_k_v;
+    const float top_p = p.top_p ? p.top_p[row] : p.top_p_v, min_p = p.min_p ? p.min_p[row] : p.min_p_v, u = p.u[row];
+
     // ---- the slice as keys: element i at keys[off + i], whole 16-byte vectors of the row on whole
     // vectors of the table, zeros around the slice
     const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / (int)sizeof(T), n);
     const int off = (E - head % E) % E, nv = (off + n + E - 1) / E, body = (n - head) / E, v0 = (off + head) / E;
-    uint32_t most0 = 0, most1 = 0;         // largest keys of this thread's even and odd vectors
+    const int nw = nv * 4;                 // words
+    uint32_t top0 = K::NONE, top1 = K::NONE;       // largest values of this thread's even and odd vectors
+    if (tid < 4 * 256) (&s.hist[0][0])[tid] = (&s.hist[0][0])[tid + ST] = 0;
+    if (tid < 48) s.reach[tid] = 0;
+    if (tid == 0) s.collected = 0;
     if (tid < off) keys[tid] = 0;
     if (tid < nv * E - off - n) keys[off + n + tid] = 0;
+    uint32_t most0 = 0, most1 = 0;
     if (tid < head) {
-        const uint32_t k = K::one(src[tid]);
-        keys[off + tid] = (key_t)k;
-        most0 = max(most0, k);
+        most0 = K::one(src[tid]);
+        keys[off + tid] = (key_t)most0;
     }
     if (tid < n - head - body * E) {
-        const uint32_t k = K::one(src[head + body * E + tid]);
-        keys[off + head + body * E + tid] = (key_t)k;
-        most1 = max(most1, k);
+        most1 = K::one(src[head + body * E + tid]);
+        keys[off + head + body * E + tid] = (key_t)most1;
     }
     const uint4* vsrc = reinterpret_cast<const uint4*>(src + head);
     for (int i = tid; i < body; i += 8 * ST) {
         uint4 v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i + j * ST < body) v[j] = dg::ldg16(vsrc + i + j * ST);
+        for (int q = 0; q < 8; ++q)
+            if (i + q * ST < body) v[q] = dg::ldg16(vsrc + i + q * ST);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i + j * ST < body) {
-                v[j] = K::vec(v[j]);
-                vecs[v0 + i + j * ST] = v[j];
-                const uint32_t k = K::most(v[j]);
-                if (j & 1) most1 = max(most1, k);
-                else most0 = max(most0, k);
+        for (int q = 0; q < 8; ++q)
+            if (i + q * ST < body) {
+                v[q] = make_uint4(K::clean(v[q].x), K::clean(v[q].y), K::clean(v[q].z), K::clean(v[q].w));
+                const uint32_t t = K::larger(K::larger(v[q].x, v[q].y), K::larger(v[q].z, v[q].w));
+                if (q & 1) top1 = K::larger(top1, t);
+                else top0 = K::larger(top0, t);
+                vecs[v0 + i + q * ST] =
+                    make_uint4(K::ordered(v[q].x), K::ordered(v[q].y), K::ordered(v[q].z), K::ordered(v[q].w));
             }
     }
-    if (tid == 0) s.collected = 0;
+    if (tid < body) most0 = max(most0, K::most(K::ordered(top0)));
+    if (tid + ST < body) most1 = max(most1, K::most(K::ordered(top1)));
 
-    // ---- parameters
-    const float temp = p.temperature ? p.temperature[row] : p.temperature_v;
     const bool greedy = !(temp > 0.f);
     const float tdiv = greedy ? 1.f : temp;
-    int k = p.top_k ? p.top_k[row] : p.top_k_v;
     if (k <= 0 || k > V) k = V;
     if (greedy) k = 1;
-    const u64 P = (u64)(fminf(fmaxf(p.top_p ? p.top_p[row] : p.top_p_v, 0.f), 1.f) * 16777216.f);
-    const u64 least = (u64)(fminf(fmaxf(p.min_p ? p.min_p[row] : p.min_p_v, 0.f), 1.f) * 1099511627776.f);
-    const u64 U = (u64)(fminf(fmaxf(p.u[row], 0.f), 1.f - 1.f / 16777216.f) * 16777216.f);
+    const u64 P = (u64)(fminf(fmaxf(top_p, 0.f), 1.f) * 16777216.f);
+    const u64 least = (u64)(fminf(fmaxf(min_p, 0.f), 1.f) * 1099511627776.f);
+    const u64 U = (u64)(fminf(fmaxf(u, 0.f), 1.f - 1.f / 16777216.f) * 16777216.f);
     const bool cut_k = k < V, cut_p = P < (1u << 24);
 
     // ---- the row's maximum, and the bound
     const int j_all = cut_k ? k : 256, j = (j_all + C - 1) / C;   // this CTA's share
-    const bool collect = (cut_k || cut_p) && j <= 512;
+    bool collect = (cut_k || cut_p) && j <= 512;
     uint32_t bound = 0;
     u64 mx = __reduce_max_sync(DG_FULL_MASK, max(most0, most1));
     if (lane == 0) s.warp[warp] = mx;
@@ -303,12 +325,21 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) mx = max(mx, s.warp[i]);
     if (collect) {
-        // the largest multiple of 2^low that j partial maxima reach; 20 bits of a 32-bit key are enough
+        // the largest multiple of 2^low that j partial maxima reach, two bits at a time; 20 bits of a
+        // 32-bit key are enough
         constexpr int low = K::BITS == 32 ? 12 : 0;
-        for (int bit = K::BITS - 1; bit >= low; --bit) {
-            const uint32_t c = bound | (1u << bit);
-            const int reach = __syncthreads_count(most0 >= c) + __syncthreads_count(most1 >= c);
-            if (reach >= j) bound = c;
+        int step = 0;
+        for (int bit = K::BITS - 2; bit >= low; bit -= 2, ++step) {
+#pragma unroll
+            for (uint32_t q = 1; q < 4; ++q) {
+                const uint32_t c = bound | (q << bit);
+                const int r = __popc(__ballot_sync(DG_FULL_MASK, most0 >= c)) + __popc(__ballot_sync(DG_FULL_MASK, most1 >= c));
+                if (lane == 0 && r) atomicAdd(&s.reach[3 * step + q - 1], (uint32_t)r);
+            }
+            __syncthreads();
+            uint32_t q = 0;
+            while (q < 3 && s.reach[3 * step + q] >= (uint32_t)j) ++q;
+            bound |= q << bit;
         }
     }
     if (C > 1) {
@@ -318,8 +349,6 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
         });
         mx = both >> 32;
         bound = 0xffffffffu - (uint32_t)both;
-    } else {
-        __syncthreads();                   // the keys are there
     }
     const float m = K::value((uint32_t)mx);
     if (m == -INFINITY) {                  // nothing can be drawn
@@ -331,35 +360,44 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
         return;
     }
     auto mass = [&](uint32_t key) { return mass_of(K::value(key), m, tdiv); };
-    // f(key, place) for the keys of this CTA's vectors, any order
+    // f(key, place) for the keys of this CTA's words, any order
     auto each = [&](auto&& f) {
-        for (int i = tid; i < nv; i += ST) {
-            const uint4 v = vecs[i];
+#pragma unroll 2
+        for (int i = tid; i < nw; i += ST) {
+            const uint32_t w = words[i];
 #pragma unroll
-            for (int e = 0; e < E; ++e) f(K::at(v, e), i * E + e);
+            for (int e = 0; e < W; ++e) f(K::at(w, e), i * W + e);
         }
     };
+    auto add = [](u64 a, u64 b) { return a + b; };
 
-    // ---- the mass of the whole row, where top_k does not fix what top_p is a share of
+    // ---- the mass of the whole row, where top_k does not fix what top_p is a share of, and of what would
+    // be collected: where that is too little, nothing is
     u64 total_k = 0;
     if (!cut_k && cut_p) {
-        u64 w = 0;
-        each([&](uint32_t key, int) { if (key) w += mass(key); });
-        total_k = over_cluster(block_sum(w, s), 1, C, s, [](u64 a, u64 b) { return a + b; });
+        u64 w = 0, in = 0;
+        each([&](uint32_t key, int) {
+            const u64 v = key ? mass(key) : 0;
+            w += v;
+            if (key >= bound) in += v;
+        });
+        total_k = over_cluster(block_sum(w, s), 1, C, s, add);
+        in = over_cluster(block_sum(in, s), 6, C, s, add);
+        collect = collect && in >= fraction_of(P, total_k, true);
     }
 
     // ---- collect, sort and draw
     if (collect) {
-        for (int i = tid; i < nv; i += ST) {
-            const uint4 v = vecs[i];
+        for (int i = tid; i < nw; i += ST) {
+            const uint32_t v = words[i];
             if (K::most(v) < bound) continue;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
+            for (int e = 0; e < W; ++e) {
                 const uint32_t key = K::at(v, e);
                 if (key >= bound && key) {
                     const uint32_t at = C > 1 ? remote_add(&s.collected, 0, 1) : atomicAdd(&s.collected, 1u);
                     if (at < CAP) {
-                        const u64 entry = (u64)key << 32 | (0xffffffffu - (uint32_t)(s0 + i * E + e - off));
+                        const u64 entry = (u64)key << 32 | (0xffffffffu - (uint32_t)(s0 + i * W + e - off));
                         if (C > 1) remote_store64(&s.list[at], 0, entry);
                         else s.list[at] = entry;
                     }
@@ -422,24 +460,25 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     }
 
     // ---- the cut by counting
-    // the largest key K with measure(key >= K) >= target, and *above = measure(key > K)
+    // the largest key K with measure(key >= K) >= target, and *above = measure(key > K).  The counters are
+    // zero before and after a call.
+    int buf = 0;
     auto find_cut = [&](bool by_mass, u64 target, u64* above_out) {
         u64 above = 0;
         uint32_t lo = 1, hi = (uint32_t)mx;
-        const float span = fminf(28.f * tdiv, 3.0e38f);
-        const float scale = 255.f / span;
+        const float scale = 255.f / fminf(28.f * tdiv, 3.0e38f);
         auto far = [&](uint32_t key) {     // bins of the distance below the maximum; monotone in the key
             const float dist = (m - K::value(key)) * scale;
             return dist < 255.f ? (int)dist : dist == dist ? 255 : 0;
         };
-        bool first = true;
-        int shift = 0;
+        int far_bin = -1, shift = 0;
         while (true) {
-            for (int i = tid; i < 4 * 256; i += ST) (&s.hist[0][0])[i] = 0;
-            join(C);
             each([&](uint32_t key, int) {
-                if (key < lo || key > hi || key == 0) return;
-                const int b = first ? far(key) : (int)((hi - key) >> shift);
+                if (key < lo || key > hi) return;
+                int b;
+                if (far_bin < 0) b = far(key);
+                else if (far(key) != far_bin) return;
+                else b = (int)((hi - key) >> shift);
                 atomicAdd(&s.hist[0][b], 1u);
                 if (by_mass) {
                     const u64 w = mass(key);
@@ -450,73 +489,67 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
                     }
                 }
             });
-            join(C);
-            if (tid < 256) {
-                u64 v = 0;
-                for (int r = 0; r < C; ++r) {
-                    auto get = [&](int q) { return (u64)(C > 1 ? remote_load32(&s.hist[q][tid], r) : s.hist[q][tid]); };
-                    v += by_mass ? get(1) + (get(2) << 13) + (get(3) << 26) : get(0);
-                }
-                s.bins[tid] = v;
-            }
-            join(C);                       // the counts may be cleared again
-            if (warp == 0) {               // lane l: bins 8 l to 8 l + 7
-                u64 v[8], sum = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = s.bins[8 * lane + i], sum += v[i];
-                const u64 inc = warp_scan(sum, lane) + above;
-                const unsigned hit = __ballot_sync(DG_FULL_MASK, inc >= target);
-                // (the last bin is taken where rounding could leave none: never, as sums are exact)
-                if (lane == (hit ? __ffs(hit) - 1 : 31)) {
-                    u64 run = inc - sum;
-                    int i = 0;
-                    while (i < 7 && run + v[i] < target) run += v[i++];
-                    s.found_bin = 8 * lane + i;
-                    s.found_above = run;
-                }
-            }
             __syncthreads();
-            const int bin = (int)s.found_bin;
-            above = s.found_above;
-            if (first) {
-                // the keys of the bin
-                u64 least_k = 0xffffffffu, most_k = 0;
-                each([&](uint32_t key, int) {
-                    if (key && far(key) == bin) {
-                        least_k = min(least_k, (u64)key);
-                        most_k = max(most_k, (u64)key);
-                    }
-                });
-                const uint32_t a = __reduce_min_sync(DG_FULL_MASK, (uint32_t)least_k);
-                const uint32_t b = __reduce_max_sync(DG_FULL_MASK, (uint32_t)most_k);
-                __syncthreads();
-                if (lane == 0) s.warp[warp] = (u64)b << 32 | (0xffffffffu - a);
-                __syncthreads();
-                u64 ab = 0;
-                auto both = [](u64 x, u64 y) { return max(x >> 32, y >> 32) << 32 | max(x & 0xffffffffu, y & 0xffffffffu); };
+            if (tid < 256) {
+                s.bins[buf][tid] = by_mass ? (u64)s.hist[1][tid] + ((u64)s.hist[2][tid] << 13) + ((u64)s.hist[3][tid] << 26)
+                                           : (u64)s.hist[0][tid];
 #pragma unroll
-                for (int i = 0; i < WARPS; ++i) ab = both(ab, s.warp[i]);
-                ab = over_cluster(ab, 2, C, s, both);
-                lo = 0xffffffffu - (uint32_t)ab;
-                hi = (uint32_t)(ab >> 32);
-                first = false;
+                for (int q = 0; q < 4; ++q) s.hist[q][tid] = 0;
+            }
+            join(C);
+            // every warp finds the bin for itself; lane l: bins 8 l to 8 l + 7
+            u64 v[8], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = C > 1 ? 0 : s.bins[buf][8 * lane + i];
+            if (C > 1) {                   // the cluster's sums, a part of the bins to each warp
+                const int b = tid >> 1;
+                u64 x = 0;
+                for (int r = tid & 1; r < C; r += 2) x += remote_load64(&s.bins[buf][b], r);
+                x += __shfl_xor_sync(DG_FULL_MASK, x, 1);
+                if (!(tid & 1)) s.list[b] = x;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = s.list[8 * lane + i];
+            }
+            buf ^= 1;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += v[i];
+            const u64 inc = warp_scan(sum, lane) + above;
+            const unsigned hit = __ballot_sync(DG_FULL_MASK, inc >= target);
+            const int at = hit ? __ffs(hit) - 1 : 31;
+            u64 run = inc - sum;
+            int bin = 8 * lane;
+#pragma unroll
+            for (int i = 0; i < 7; ++i)
+                if (run + v[i] < target && bin == 8 * lane + i) run += v[i], ++bin;
+            bin = __shfl_sync(DG_FULL_MASK, bin, at);
+            above = __shfl_sync(DG_FULL_MASK, run, at);
+            if (far_bin < 0) {
+                // keys that surely hold the bin's, rounding errors of m and the distance included; the
+                // digits below only count those in it
+                far_bin = bin;
+                const float edge = (float)(bin + 1) / scale, fuzz = 1e-6f * (edge + fabsf(m));
+                const uint32_t a = K::near(m - edge - fuzz), b = K::near(m - (float)bin / scale + fuzz);
+                lo = bin == 255 || a <= 2 ? 1 : a - 2;
+                hi = bin == 0 ? (uint32_t)mx : min((uint32_t)mx, b + 2);
             } else {
-                const uint32_t top = hi - ((uint32_t)bin << shift);
-                const uint32_t bottom = top - ((1u << shift) - 1);
+                const uint32_t top = hi - ((uint32_t)bin << shift), bottom = top - ((1u << shift) - 1);
                 lo = bottom > lo && bottom <= top ? bottom : lo;
                 hi = top;
             }
             if (lo >= hi) break;
             shift = 0;
             while (((hi - lo) >> shift) > 255) ++shift;
+            if (C > 1) __syncthreads();    // list[] has been read
         }
+        __syncthreads();
         *above_out = above;
         return hi;
     };
     auto mass_above = [&](uint32_t key, int slot) {
         u64 w = 0;
         each([&](uint32_t kk, int) { if (kk > key) w += mass(kk); });
-        return over_cluster(block_sum(w, s), slot, C, s, [](u64 a, u64 b) { return a + b; });
+        return over_cluster(block_sum(w, s), slot, C, s, add);
     };
     uint32_t cut = 0;                      // kept: key > cut, and the first `ties` with key == cut
     u64 ties = 0;
@@ -536,57 +569,57 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
         }
     }
 
-    // ---- the draw in index order: each warp walks a contiguous piece of the vectors
-    const int piece = (nv + WARPS - 1) / WARPS, i0 = min(warp * piece, nv), i1 = min(i0 + piece, nv);
-    u64 seen0 = 0;                         // tokens with the cut key before this warp's piece
+    // ---- the draw in index order: each warp walks a contiguous piece of the words
+    const int piece = (nw + WARPS - 1) / WARPS, i0 = min(warp * piece, nw), i1 = min(i0 + piece, nw);
+    uint32_t seen0 = 0;                    // tokens with the cut key before this warp's piece
     if (cut) {
-        u64 c = 0;
+        uint32_t c = 0;
         for (int i = i0 + lane; i < i1; i += 32) {
-            const uint4 v = vecs[i];
+            const uint32_t w = words[i];
 #pragma unroll
-            for (int e = 0; e < E; ++e) c += K::at(v, e) == cut;
+            for (int e = 0; e < W; ++e) c += K::at(w, e) == cut;
         }
-        c = warp_sum(c);
+        c = __reduce_add_sync(DG_FULL_MASK, c);
         u64 all;
-        seen0 = block_before(lane == 0 ? c : 0, &all, s);
-        seen0 = __shfl_sync(DG_FULL_MASK, seen0, 0);
+        const u64 before = block_before(lane == 0 ? c : 0, &all, s);
+        seen0 = (uint32_t)__shfl_sync(DG_FULL_MASK, before, 0);
         if (C > 1) {
             if (tid == 0) s.post[4] = all;
             join(C);
-            for (int r = 0; r < rank; ++r) seen0 += remote_load64(&s.post[4], r);
+            for (int r = 0; r < rank; ++r) seen0 += (uint32_t)remote_load64(&s.post[4], r);
         }
     }
-    // f(vector index, this lane's masses of it) in index order; returns when f says so
+    // f(word index, the masses of this lane's keys in it) in index order; returns when f says so
     auto walk = [&](auto&& f) {
-        u64 seen = seen0;
+        uint32_t seen = seen0;
         for (int b = i0; b < i1; b += 32) {
             const int i = b + lane;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (i < i1) v = vecs[i];
-            u64 t = 0;
+            const uint32_t word = i < i1 ? words[i] : 0;
+            u64 w[W];
+            uint32_t t = seen;
             if (cut) {
-                u64 c = 0;
+                unsigned is[W];
 #pragma unroll
-                for (int e = 0; e < E; ++e) c += K::at(v, e) == cut;
-                const u64 inc = warp_scan(c, lane);
-                t = seen + inc - c;
-                seen += __shfl_sync(DG_FULL_MASK, inc, 31);
+                for (int e = 0; e < W; ++e) {
+                    is[e] = __ballot_sync(DG_FULL_MASK, K::at(word, e) == cut);
+                    t += __popc(is[e] & ((1u << lane) - 1));
+                    seen += __popc(is[e]);
+                }
             }
-            u64 w[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const uint32_t key = K::at(v, e);
+            for (int e = 0; e < W; ++e) {
+                const uint32_t key = K::at(word, e);
                 w[e] = key > cut || (cut && key == cut && t < ties) ? mass(key) : 0;
-                t += cut && key == cut;
+                t += key == cut;
                 if (w[e] < least) w[e] = 0;
             }
             if (f(i, w)) return;
         }
     };
     u64 mine = 0;
-    walk([&](int, const u64 (&w)[E]) {
+    walk([&](int, const u64 (&w)[W]) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) mine += w[e];
+        for (int e = 0; e < W; ++e) mine += w[e];
         return false;
     });
     mine = warp_sum(mine);
@@ -607,25 +640,19 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     const u64 at = fraction_of(U, total, false);
     if (start <= at && at < start + mine) {
         u64 run = start;
-        walk([&](int i, const u64 (&w)[E]) {
+        walk([&](int i, const u64 (&w)[W]) {
             u64 sum = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum += w[e];
+            for (int e = 0; e < W; ++e) sum += w[e];
             const u64 inc = warp_scan(sum, lane);
             const unsigned hit = __ballot_sync(DG_FULL_MASK, run + inc > at);
             if (hit) {
                 if (lane == __ffs(hit) - 1) {
-                    u64 r = run + inc - sum;
-                    bool open = true;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        if (open && at < r + w[e]) {
-                            open = false;
-                            p.token[row] = (int64_t)s0 + i * E + e - off;
-                            if (p.logprob) p.logprob[row] = logf(__fdiv_rn((float)w[e], (float)total));
-                        }
-                        r += w[e];
-                    }
+                    const u64 r = run + inc - sum;
+                    const int e = W > 1 && at >= r + w[0] ? 1 : 0;
+                    const u64 we = w[e ? W - 1 : 0];
+                    p.token[row] = (int64_t)s0 + i * W + e - off;
+                    if (p.logprob) p.logprob[row] = logf(__fdiv_rn((float)we, (float)total));
                 }
                 return true;
             }
@@ -636,11 +663,11 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
 }
 
 // CTAs per row: rows alone where they fill the SMs; else up to 16, with at least 2048 logits each; and
-// as many as a slice of at most 96 KB (two CTAs to an SM) asks for.
+// as many as a slice of at most 92 KB (two CTAs to an SM) asks for.
 int cluster_of(int B, int V, size_t elem) {
     int c = 1;
     while (c < 16 && ((int64_t)B * c * 2 <= 296 && V / (2 * c) >= 2048)) c *= 2;
-    while (c < 16 && ((size_t)V + c - 1) / c * elem > 96 * 1024) c *= 2;
+    while (c < 16 && ((size_t)V + c - 1) / c * elem > 92 * 1024) c *= 2;
     return c;
 }
 
