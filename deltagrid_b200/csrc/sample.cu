@@ -156,8 +156,7 @@ struct Shared {
     u64 list[CAP];                         // collected tokens: key << 32 | ~index, or index << 32 | key
     uint32_t hist[4][256];                 // counts, and the masses' 13 + 13 + 14 bits
     u64 bins[2][256];                      // what they amount to; this CTA's, read by the cluster
-    uint32_t reach[3 * 16];                // partial maxima that reach a candidate bound
-    u64 warp[WARPS];
+    u64 warp[WARPS], warp2[WARPS];
     u64 post[8];                           // values that the cluster's other CTAs read
     uint32_t collected;
     uint32_t flag;
@@ -197,6 +196,40 @@ __device__ __forceinline__ u64 block_sum(u64 v, Shared& s) {
     for (int i = 0; i < WARPS; ++i) t += s.warp[i];
     return t;
 }
+__device__ __forceinline__ void block_sum2(u64& a, u64& b, Shared& s) {
+    a = warp_sum(a);
+    b = warp_sum(b);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5] = a, s.warp2[threadIdx.x >> 5] = b;
+    __syncthreads();
+    a = b = 0;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) a += s.warp[i], b += s.warp2[i];
+}
+// barrier of the first `threads` threads (whole warps)
+__device__ __forceinline__ void part_sync(int threads) {
+    if (threads == 32) __syncwarp();
+    else asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+}
+// exclusive prefix sum over the first `threads` threads; *total in each of them
+__device__ __forceinline__ u64 part_before(u64 v, u64* total, int threads, Shared& s) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const u64 inc = warp_scan(v, lane);
+    if (threads == 32) {
+        *total = __shfl_sync(DG_FULL_MASK, inc, 31);
+        return inc - v;
+    }
+    part_sync(threads);
+    if (lane == 31) s.warp[warp] = inc;
+    part_sync(threads);
+    u64 before = 0, t = 0;
+    for (int i = 0; i < threads / 32; ++i) {
+        if (i == warp) before = t;
+        t += s.warp[i];
+    }
+    *total = t;
+    return before + inc - v;
+}
 // exclusive prefix sum over the CTA's threads; *total in every thread
 __device__ __forceinline__ u64 block_before(u64 v, u64* total, Shared& s) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -224,25 +257,24 @@ template <typename F> __device__ __forceinline__ u64 over_cluster(u64 v, int slo
     return r;
 }
 
-// sorts list[0, n2) (n2 a power of two, 64 to 1024), one exchange per thread and stage; exchanges inside
-// 64 elements stay within a warp
+// sorts list[0, n2) (n2 a power of two, 64 to 1024) by the first n2 / 2 threads, one exchange per thread
+// and stage; exchanges inside 64 elements stay within a warp
 __device__ __forceinline__ void sort_list(u64* list, int n2, bool descending) {
     const int t = threadIdx.x;
+#pragma unroll 1
     for (int size = 2; size <= n2; size *= 2)
+#pragma unroll 1
         for (int j = size / 2; j; j /= 2) {
-            if (t < n2 / 2) {
-                const int i = 2 * t - (t & (j - 1)), k = i + j;
-                const u64 a = list[i], b = list[k];
-                const bool down = ((i & size) == 0) == descending;
-                if (down ? a < b : a > b) {
-                    list[i] = b;
-                    list[k] = a;
-                }
+            const int i = 2 * t - (t & (j - 1)), k = i + j;
+            const u64 a = list[i], b = list[k];
+            const bool down = ((i & size) == 0) == descending;
+            if (down ? a < b : a > b) {
+                list[i] = b;
+                list[k] = a;
             }
-            if (j > 32 || (j == 1 && size >= 64)) __syncthreads();
+            if (j > 32 || (j == 1 && size >= 64)) part_sync(n2 / 2);
             else __syncwarp();
         }
-    __syncthreads();
 }
 
 template <typename T>
@@ -273,7 +305,6 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     const int nw = nv * 4;                 // words
     uint32_t top0 = K::NONE, top1 = K::NONE;       // largest values of this thread's even and odd vectors
     if (tid < 4 * 256) (&s.hist[0][0])[tid] = (&s.hist[0][0])[tid + ST] = 0;
-    if (tid < 48) s.reach[tid] = 0;
     if (tid == 0) s.collected = 0;
     if (tid < off) keys[tid] = 0;
     if (tid < nv * E - off - n) keys[off + n + tid] = 0;
@@ -325,22 +356,41 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) mx = max(mx, s.warp[i]);
     if (collect) {
-        // the largest multiple of 2^low that j partial maxima reach, two bits at a time; 20 bits of a
-        // 32-bit key are enough
-        constexpr int low = K::BITS == 32 ? 12 : 0;
-        int step = 0;
-        for (int bit = K::BITS - 2; bit >= low; bit -= 2, ++step) {
+        // counts of the partial maxima by their keys' distance below the largest (bf16's resolution
+        // for 32-bit keys); the bound is the first key of the bin in which the j-th lies
+        constexpr int low = K::BITS - 16;
+        auto bin_of = [&](uint32_t key) { return min(((uint32_t)mx - key) >> low, 255u); };
+        if (most0) atomicAdd(&s.hist[0][bin_of(most0)], 1u);
+        if (most1) atomicAdd(&s.hist[0][bin_of(most1)], 1u);
+        __syncthreads();
+        uint32_t v[8], sum = 0;
 #pragma unroll
-            for (uint32_t q = 1; q < 4; ++q) {
-                const uint32_t c = bound | (q << bit);
-                const int r = __popc(__ballot_sync(DG_FULL_MASK, most0 >= c)) + __popc(__ballot_sync(DG_FULL_MASK, most1 >= c));
-                if (lane == 0 && r) atomicAdd(&s.reach[3 * step + q - 1], (uint32_t)r);
-            }
-            __syncthreads();
-            uint32_t q = 0;
-            while (q < 3 && s.reach[3 * step + q] >= (uint32_t)j) ++q;
-            bound |= q << bit;
+        for (int i = 0; i < 8; ++i) v[i] = s.hist[0][8 * lane + i], sum += v[i];
+        uint32_t run = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(DG_FULL_MASK, run, o);
+            if (lane >= o) run += x;
         }
+        const unsigned hit = __ballot_sync(DG_FULL_MASK, run >= (uint32_t)j);
+        run -= sum;
+        uint32_t bin = 8 * lane;
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (run + v[i] < (uint32_t)j && bin == 8 * lane + i) run += v[i], ++bin;
+        bin = __shfl_sync(DG_FULL_MASK, bin, hit ? __ffs(hit) - 1 : 31);
+        if (bin < 255 && (uint64_t)mx >= ((uint64_t)(bin + 1) << low)) {
+            bound = (uint32_t)mx - (((bin + 1) << low) - 1);
+        } else {
+            // further down: bit by bit, to the same resolution
+            for (int bit = K::BITS - 1; bit >= low; --bit) {
+                const uint32_t c = bound | (1u << bit);
+                const int reach = __syncthreads_count(most0 >= c) + __syncthreads_count(most1 >= c);
+                if (reach >= j) bound = c;
+            }
+        }
+        __syncthreads();
+        if (tid < 256) s.hist[0][tid] = 0;
     }
     if (C > 1) {
         // j tokens of each CTA reach its bound, so C j reach the smallest
@@ -381,23 +431,29 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
             w += v;
             if (key >= bound) in += v;
         });
-        total_k = over_cluster(block_sum(w, s), 1, C, s, add);
-        in = over_cluster(block_sum(in, s), 6, C, s, add);
+        block_sum2(w, in, s);
+        total_k = w;
+        if (C > 1) {
+            if (tid == 0) s.post[1] = w, s.post[2] = in;
+            join(C);
+            for (int r = 0; r < C; ++r)
+                if (r != rank) total_k += remote_load64(&s.post[1], r), in += remote_load64(&s.post[2], r);
+        }
         collect = collect && in >= fraction_of(P, total_k, true);
     }
 
     // ---- collect, sort and draw
     if (collect) {
-        for (int i = tid; i < nw; i += ST) {
-            const uint32_t v = words[i];
-            if (K::most(v) < bound) continue;
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                const uint32_t key = K::at(v, e);
+        for (int i = tid; i < nv; i += ST) {
+            const uint4 v = vecs[i];
+            if (max(max(K::most(v.x), K::most(v.y)), max(K::most(v.z), K::most(v.w))) < bound) continue;
+#pragma unroll 1
+            for (int e = 0; e < E; ++e) {
+                const uint32_t key = keys[i * E + e];
                 if (key >= bound && key) {
                     const uint32_t at = C > 1 ? remote_add(&s.collected, 0, 1) : atomicAdd(&s.collected, 1u);
                     if (at < CAP) {
-                        const u64 entry = (u64)key << 32 | (0xffffffffu - (uint32_t)(s0 + i * W + e - off));
+                        const u64 entry = (u64)key << 32 | (0xffffffffu - (uint32_t)(s0 + i * E + e - off));
                         if (C > 1) remote_store64(&s.list[at], 0, entry);
                         else s.list[at] = entry;
                     }
@@ -405,57 +461,55 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
             }
         }
         join(C);
-        bool done = false;
         if (rank == 0) {
             const int nc = (int)min(s.collected, (uint32_t)CAP + 1);
-            if (nc <= CAP) {
-                int n2 = 64;
-                while (n2 < nc) n2 *= 2;
-                for (int i = nc + tid; i < n2; i += ST) s.list[i] = 0;
-                __syncthreads();
+            int n2 = 64;
+            while (n2 < nc) n2 *= 2;
+            if (nc <= CAP && tid < n2 / 2) {
+                // the first n2 / 2 threads: elements 2t and 2t + 1 of the order
+                const int i0 = 2 * tid, lim = min(nc, k);
+                if (i0 >= nc) s.list[i0] = 0;
+                if (i0 + 1 >= nc) s.list[i0 + 1] = 0;
+                part_sync(n2 / 2);
                 sort_list(s.list, n2, true);
-                // thread t: elements 2t and 2t + 1 of the order
-                const int i0 = 2 * tid;
-                const u64 e0 = i0 < n2 ? s.list[i0] : 0, e1 = i0 < n2 ? s.list[i0 + 1] : 0;
-                const int lim = min(nc, k);
+                const u64 e0 = s.list[i0], e1 = s.list[i0 + 1];
                 u64 w0 = i0 < lim ? mass((uint32_t)(e0 >> 32)) : 0, w1 = i0 + 1 < lim ? mass((uint32_t)(e1 >> 32)) : 0;
                 u64 sum;
-                const u64 before = block_before(w0 + w1, &sum, s);
-                if (cut_k) total_k = sum;
-                const u64 tau = max(fraction_of(P, total_k, true), 1ull);
-                done = cut_k || sum >= tau;
+                const u64 before = part_before(w0 + w1, &sum, n2 / 2, s);
+                const u64 tau = max(fraction_of(P, cut_k ? sum : total_k, true), 1ull);
+                const bool done = cut_k || sum >= tau;
                 if (done) {
                     const bool keep0 = i0 < lim && before < tau && w0 >= least;
                     const bool keep1 = i0 + 1 < lim && before + w0 < tau && w1 >= least;
-                    const int kept = __syncthreads_count(keep0) + __syncthreads_count(keep1);     // the first `kept`
+                    u64 kept;              // the first `kept` of the order
+                    part_before((u64)keep0 + keep1, &kept, n2 / 2, s);
+                    s.list[i0] = keep0 ? (u64)(0xffffffffu - (uint32_t)e0) << 32 | e0 >> 32 : ~0ull;
+                    s.list[i0 + 1] = keep1 ? (u64)(0xffffffffu - (uint32_t)e1) << 32 | e1 >> 32 : ~0ull;
+                    part_sync(n2 / 2);
                     n2 = 64;
-                    while (n2 < kept) n2 *= 2;
-                    if (i0 < n2) {
-                        s.list[i0] = keep0 ? (u64)(0xffffffffu - (uint32_t)e0) << 32 | e0 >> 32 : ~0ull;
-                        s.list[i0 + 1] = keep1 ? (u64)(0xffffffffu - (uint32_t)e1) << 32 | e1 >> 32 : ~0ull;
-                    }
-                    __syncthreads();
-                    sort_list(s.list, n2, false);
-                    const u64 d0 = i0 < kept ? s.list[i0] : 0, d1 = i0 + 1 < kept ? s.list[i0 + 1] : 0;
-                    w0 = i0 < kept ? mass((uint32_t)d0) : 0;
-                    w1 = i0 + 1 < kept ? mass((uint32_t)d1) : 0;
-                    u64 total;
-                    const u64 run = block_before(w0 + w1, &total, s), at = fraction_of(U, total, false);
-                    if (run <= at && at < run + w0 + w1) {
-                        const bool second = at >= run + w0;
-                        p.token[row] = (int64_t)((second ? d1 : d0) >> 32);
-                        if (p.logprob)
-                            p.logprob[row] = logf(__fdiv_rn((float)(second ? w1 : w0), (float)total));
+                    while (n2 < (int)kept) n2 *= 2;
+                    if (tid < n2 / 2) {
+                        sort_list(s.list, n2, false);
+                        const u64 d0 = s.list[i0], d1 = s.list[i0 + 1];
+                        w0 = i0 < (int)kept ? mass((uint32_t)d0) : 0;
+                        w1 = i0 + 1 < (int)kept ? mass((uint32_t)d1) : 0;
+                        u64 total;
+                        const u64 run = part_before(w0 + w1, &total, n2 / 2, s), at = fraction_of(U, total, false);
+                        if (run <= at && at < run + w0 + w1) {
+                            const bool second = at >= run + w0;
+                            p.token[row] = (int64_t)((second ? d1 : d0) >> 32);
+                            if (p.logprob) p.logprob[row] = logf(__fdiv_rn((float)(second ? w1 : w0), (float)total));
+                        }
                     }
                 }
+                if (tid == 0) s.flag = done;
+            } else if (nc > CAP && tid == 0) {
+                s.flag = 0;
             }
-            if (tid == 0) s.flag = done;
         }
         join(C);
-        if (C > 1) {
-            done = remote_load32(&s.flag, 0) != 0;
-            join(C);
-        }
+        const bool done = C > 1 ? remote_load32(&s.flag, 0) != 0 : s.flag != 0;
+        if (C > 1) join(C);
         if (done) return;
     }
 
@@ -662,11 +716,12 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     }
 }
 
-// CTAs per row: rows alone where they fill the SMs; else up to 16, with at least 2048 logits each; and
-// as many as a slice of at most 92 KB (two CTAs to an SM) asks for.
+// CTAs per row: as many (up to 16) as give each SM one, with at least 2048 logits each; and as many as a
+// slice of at most 92 KB (two CTAs to an SM) asks for.  A CTA's work beyond its logits is the same
+// whatever it holds, so more CTAs than SMs cost more than they save.
 int cluster_of(int B, int V, size_t elem) {
     int c = 1;
-    while (c < 16 && ((int64_t)B * c * 2 <= 296 && V / (2 * c) >= 2048)) c *= 2;
+    while (c < 16 && ((int64_t)B * c * 2 <= 148 && V / (2 * c) >= 2048)) c *= 2;
     while (c < 16 && ((size_t)V + c - 1) / c * elem > 92 * 1024) c *= 2;
     return c;
 }
