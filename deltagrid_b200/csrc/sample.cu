@@ -7,26 +7,27 @@
 //
 // A row is read once, by one CTA or by a cluster of up to 16 that share its slices, and kept
 // in shared memory as integer keys in the order of the values (16 bits for 16-bit logits).
-//   1. The j-th largest of 1024 partial maxima is a bound that at least j tokens reach: with
-//      j = top_k (or 256 where only top_p cuts) few more than j tokens do.  They are collected
-//      in one CTA and sorted; prefix sums of their masses give the cut, a second sort brings
-//      the kept ones into index order, and prefix sums again give the token.
-//   2. Where more than 1024 tokens reach the bound, or the collected ones do not hold enough
-//      mass, the cut key is found by counting: 256 bins over the distance below the maximum,
-//      then 256 bins over the keys of the bin that holds the cut, until one key is left.  Then
-//      two walks over the keys in index order draw the token.  Without a cut (no top_k, no
-//      top_p) only the walks are needed.
-// In the first way only collected tokens need an exponential, unless top_p alone cuts.
+//   1. top_k: the k-th largest of 1024 partial maxima is a bound that at least k tokens reach
+//      and few more do.  They are collected in one CTA; up to 256 are ranked by comparing
+//      each with all (512 threads share that), more are sorted.  Ranks and the mass before
+//      each give the kept ones, the same comparison by index gives the token.  Only collected
+//      tokens need an exponential.
+//   2. Where that does not do (no top_k, a large one, many equal logits): counts and masses in
+//      256 bins of the distance below the maximum.  If the bins down to the one that holds
+//      the cut have few tokens, these are collected as in 1.  Otherwise the cut's bin is
+//      counted again by keys, until one key is left, and two walks over the keys in index
+//      order draw the token.  Without a cut (no top_k, no top_p) only the walks are needed.
 //
-// What bounds it: reading the row once (64 KB of bf16 logits a row, two rows to an SM), then
-// the latency of some forty barriers; the row's CTAs idle at neither, as two share an SM.
+// What bounds it: not the 64 KB of a bf16 row of 32000 (2.5 us for 256 rows) but the latency
+// of the steps after it, some fifteen barriers of up to 512 threads; two CTAs share an SM.
 #include "lm_common.cuh"
 
 namespace {
 
 constexpr int ST = 512;                    // threads per CTA
 constexpr int WARPS = ST / 32;
-constexpr int CAP = 1024;                  // tokens collected and sorted
+constexpr int CAP = 1024;                  // tokens collected at most
+constexpr int RANKED = 256;                // up to here ranked by comparing all, beyond sorted
 typedef unsigned long long u64;
 
 struct SampleParams {
@@ -88,6 +89,17 @@ template <typename T> struct Key {         // 16-bit logits, two to a word
     // key `e` of a word, and the larger of its two
     __device__ static __forceinline__ uint32_t at(uint32_t w, int e) { return e ? w >> 16 : w & 0xffffu; }
     __device__ static __forceinline__ uint32_t most(uint32_t w) { return max(w >> 16, w & 0xffffu); }
+    __device__ static __forceinline__ uint32_t larger_key(uint32_t a, uint32_t b) {       // of both halves
+        uint32_t r;
+        asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    // whether any key of the vector reaches bound (above 0)
+    __device__ static __forceinline__ bool reaches(const uint4& v, uint32_t bound) {
+        const uint32_t below = (bound - 1) * 0x10001u;
+        const uint32_t m = larger_key(larger_key(v.x, v.y), larger_key(v.z, v.w));
+        return larger_key(m, below) != below;
+    }
     __device__ static __forceinline__ uint32_t near(float l) { return one(dg::from_f<T>(l)); }
 };
 template <> struct Key<float> {
@@ -107,16 +119,27 @@ template <> struct Key<float> {
     }
     __device__ static __forceinline__ uint32_t at(uint32_t w, int) { return w; }
     __device__ static __forceinline__ uint32_t most(uint32_t w) { return w; }
+    __device__ static __forceinline__ bool reaches(const uint4& v, uint32_t bound) {
+        return max(max(v.x, v.y), max(v.z, v.w)) >= bound;
+    }
     __device__ static __forceinline__ uint32_t near(float l) { return one(l); }
 };
 
 // The mass of a token; the row's maximum m is above -inf.  Below -28 (2^40 e^-28 < 1) it is 0, as it
-// is for -inf and for the undefined quotients of infinite operands.
-__device__ __forceinline__ u64 mass_of(float l, float m, float T) {
-    if (l == m) return 1ull << 40;
-    const float z = __fdiv_rn(l - m, T);
-    return z > -28.f ? (u64)__float2ll_rz(expf(z) * 1099511627776.f) : 0ull;
-}
+// is for -inf and for the undefined quotients of infinite operands.  Dividing by a power of two is
+// the same as multiplying by its inverse.
+struct Mass {
+    float m, T, inverse;
+    bool exact;
+    __device__ __forceinline__ Mass(float m_, float T_) : m(m_), T(T_), inverse(1.f / T_) {
+        exact = (__float_as_uint(T_) & 0x7fffffu) == 0 && T_ > 1e-18f && T_ < 1e18f;
+    }
+    __device__ __forceinline__ u64 operator()(float l) const {
+        if (l == m) return 1ull << 40;
+        const float d = l - m, z = exact ? d * inverse : __fdiv_rn(d, T);
+        return z > -28.f ? (u64)__float2ll_rz(expf(z) * 1099511627776.f) : 0ull;
+    }
+};
 // floor (up = 0) or ceiling of n f / 2^24, f <= 2^24, n < 2^58
 __device__ __forceinline__ u64 fraction_of(u64 f, u64 n, bool up) {
     return f * (n >> 24) + ((f * (n & 0xffffff) + (up ? 0xffffff : 0)) >> 24);
@@ -153,10 +176,14 @@ __device__ __forceinline__ uint32_t remote_add(uint32_t* p, uint32_t rank, uint3
 }
 
 struct Shared {
-    u64 list[CAP];                         // collected tokens: key << 32 | ~index, or index << 32 | key
+    u64 list[CAP];                         // collected tokens: key << 32 | ~index
+    u64 masses[RANKED];                    // theirs
     uint32_t hist[4][256];                 // counts, and the masses' 13 + 13 + 14 bits
-    u64 bins[2][256];                      // what they amount to; this CTA's, read by the cluster
-    u64 warp[WARPS], warp2[WARPS];
+    u64 bin_mass[2][256];                  // what they amount to: this CTA's, read by the cluster
+    uint32_t bin_count[2][256];
+    u64 all_mass[256];                     // the cluster's
+    uint32_t all_count[256];
+    u64 warp[WARPS];
     u64 post[8];                           // values that the cluster's other CTAs read
     uint32_t collected;
     uint32_t flag;
@@ -195,16 +222,6 @@ __device__ __forceinline__ u64 block_sum(u64 v, Shared& s) {
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) t += s.warp[i];
     return t;
-}
-__device__ __forceinline__ void block_sum2(u64& a, u64& b, Shared& s) {
-    a = warp_sum(a);
-    b = warp_sum(b);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5] = a, s.warp2[threadIdx.x >> 5] = b;
-    __syncthreads();
-    a = b = 0;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) a += s.warp[i], b += s.warp2[i];
 }
 // barrier of the first `threads` threads (whole warps)
 __device__ __forceinline__ void part_sync(int threads) {
@@ -347,8 +364,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     const bool cut_k = k < V, cut_p = P < (1u << 24);
 
     // ---- the row's maximum, and the bound
-    const int j_all = cut_k ? k : 256, j = (j_all + C - 1) / C;   // this CTA's share
-    bool collect = (cut_k || cut_p) && j <= 512;
+    const int j = (k + C - 1) / C;         // this CTA's share
+    const bool collect = cut_k && j <= 512;
     uint32_t bound = 0;
     u64 mx = __reduce_max_sync(DG_FULL_MASK, max(most0, most1));
     if (lane == 0) s.warp[warp] = mx;
@@ -409,48 +426,27 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
         if (C > 1) join(C);                // the others may still read this CTA's slot
         return;
     }
-    auto mass = [&](uint32_t key) { return mass_of(K::value(key), m, tdiv); };
-    // f(key, place) for the keys of this CTA's words, any order
+    const Mass mass_of(m, tdiv);
+    auto mass = [&](uint32_t key) { return mass_of(K::value(key)); };
+    // f(key) for the keys of this CTA's words, any order
     auto each = [&](auto&& f) {
-#pragma unroll 2
+#pragma unroll 4
         for (int i = tid; i < nw; i += ST) {
             const uint32_t w = words[i];
 #pragma unroll
-            for (int e = 0; e < W; ++e) f(K::at(w, e), i * W + e);
+            for (int e = 0; e < W; ++e) f(K::at(w, e));
         }
     };
-    auto add = [](u64 a, u64 b) { return a + b; };
 
-    // ---- the mass of the whole row, where top_k does not fix what top_p is a share of, and of what would
-    // be collected: where that is too little, nothing is
-    u64 total_k = 0;
-    if (!cut_k && cut_p) {
-        u64 w = 0, in = 0;
-        each([&](uint32_t key, int) {
-            const u64 v = key ? mass(key) : 0;
-            w += v;
-            if (key >= bound) in += v;
-        });
-        block_sum2(w, in, s);
-        total_k = w;
-        if (C > 1) {
-            if (tid == 0) s.post[1] = w, s.post[2] = in;
-            join(C);
-            for (int r = 0; r < C; ++r)
-                if (r != rank) total_k += remote_load64(&s.post[1], r), in += remote_load64(&s.post[2], r);
-        }
-        collect = collect && in >= fraction_of(P, total_k, true);
-    }
-
-    // ---- collect, sort and draw
-    if (collect) {
+    // ---- collect the tokens that reach `bound`, and draw from them: thread t of the CTA that holds the
+    // list.  Returns whether they were few enough; uniform over the cluster.
+    auto collect_and_draw = [&](uint32_t bound, u64 total_k) {
         for (int i = tid; i < nv; i += ST) {
-            const uint4 v = vecs[i];
-            if (max(max(K::most(v.x), K::most(v.y)), max(K::most(v.z), K::most(v.w))) < bound) continue;
+            if (!K::reaches(vecs[i], bound)) continue;
 #pragma unroll 1
             for (int e = 0; e < E; ++e) {
                 const uint32_t key = keys[i * E + e];
-                if (key >= bound && key) {
+                if (key >= bound) {
                     const uint32_t at = C > 1 ? remote_add(&s.collected, 0, 1) : atomicAdd(&s.collected, 1u);
                     if (at < CAP) {
                         const u64 entry = (u64)key << 32 | (0xffffffffu - (uint32_t)(s0 + i * E + e - off));
@@ -461,268 +457,358 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
             }
         }
         join(C);
+        const int nc = (int)(C > 1 ? remote_load32(&s.collected, 0) : s.collected);
+        if (nc > CAP) return false;
         if (rank == 0) {
-            const int nc = (int)min(s.collected, (uint32_t)CAP + 1);
-            int n2 = 64;
-            while (n2 < nc) n2 *= 2;
-            if (nc <= CAP && tid < n2 / 2) {
-                // the first n2 / 2 threads: elements 2t and 2t + 1 of the order
-                const int i0 = 2 * tid, lim = min(nc, k);
-                if (i0 >= nc) s.list[i0] = 0;
-                if (i0 + 1 >= nc) s.list[i0 + 1] = 0;
-                part_sync(n2 / 2);
-                sort_list(s.list, n2, true);
-                const u64 e0 = s.list[i0], e1 = s.list[i0 + 1];
-                u64 w0 = i0 < lim ? mass((uint32_t)(e0 >> 32)) : 0, w1 = i0 + 1 < lim ? mass((uint32_t)(e1 >> 32)) : 0;
-                u64 sum;
-                const u64 before = part_before(w0 + w1, &sum, n2 / 2, s);
-                const u64 tau = max(fraction_of(P, cut_k ? sum : total_k, true), 1ull);
-                const bool done = cut_k || sum >= tau;
-                if (done) {
-                    const bool keep0 = i0 < lim && before < tau && w0 >= least;
-                    const bool keep1 = i0 + 1 < lim && before + w0 < tau && w1 >= least;
-                    u64 kept;              // the first `kept` of the order
-                    part_before((u64)keep0 + keep1, &kept, n2 / 2, s);
-                    s.list[i0] = keep0 ? (u64)(0xffffffffu - (uint32_t)e0) << 32 | e0 >> 32 : ~0ull;
-                    s.list[i0 + 1] = keep1 ? (u64)(0xffffffffu - (uint32_t)e1) << 32 | e1 >> 32 : ~0ull;
+            auto answer = [&](u64 entry, u64 w, u64 total) {
+                p.token[row] = (int64_t)(0xffffffffu - (uint32_t)entry);
+                if (p.logprob) p.logprob[row] = logf(__fdiv_rn((float)w, (float)total));
+            };
+            const int lim = min(nc, k);
+            if (nc <= RANKED) {
+                // `part` threads share a token; each compares it with every part-th of the list
+                int part = 2;
+                while (part < 32 && part * 2 * nc <= ST) part *= 2;
+                const int c = tid / part, q = tid % part;
+                const u64 mine = c < nc ? s.list[c] : 0;
+                const u64 w = c < nc ? mass((uint32_t)(mine >> 32)) : 0;
+                if (q == 0 && c < nc) s.masses[c] = w;
+                __syncthreads();
+                uint32_t rank_ = 0;
+                u64 before = 0, sum = 0;
+#pragma unroll 4
+                for (int i = q; i < nc; i += part) {
+                    const u64 e = s.list[i], we = s.masses[i];
+                    if (e > mine) ++rank_, before += we;
+                }
+                for (int o = 1; o < part; o <<= 1) {
+                    rank_ += __shfl_xor_sync(DG_FULL_MASK, rank_, o);
+                    before += __shfl_xor_sync(DG_FULL_MASK, before, o);
+                }
+                const bool in_k = c < nc && rank_ < (uint32_t)lim;
+                const u64 k_mass = block_sum(in_k && q == 0 ? w : 0, s);     // (masses[] have been read)
+                if (cut_k) total_k = k_mass;
+                const u64 tau = max(fraction_of(P, total_k, true), 1ull);
+                const bool keep = in_k && before < tau && w >= least;
+                if (q == 0 && c < nc && !keep) s.masses[c] = 0;
+                sum = block_sum(keep && q == 0 ? w : 0, s);      // its barriers also order masses[]
+                u64 run = 0;               // kept mass of smaller indexes: larger complements
+#pragma unroll 4
+                for (int i = q; i < nc; i += part)
+                    if ((uint32_t)s.list[i] > (uint32_t)mine) run += s.masses[i];
+                for (int o = 1; o < part; o <<= 1) run += __shfl_xor_sync(DG_FULL_MASK, run, o);
+                const u64 at = fraction_of(U, sum, false);
+                if (keep && q == 0 && run <= at && at < run + w) answer(mine, w, sum);
+            } else {
+                int n2 = 2 * RANKED;
+                while (n2 < nc) n2 *= 2;
+                if (tid < n2 / 2) {
+                    // the first n2 / 2 threads: elements 2t and 2t + 1 of the order
+                    const int i0 = 2 * tid;
+                    if (i0 >= nc) s.list[i0] = 0;
+                    if (i0 + 1 >= nc) s.list[i0 + 1] = 0;
                     part_sync(n2 / 2);
-                    n2 = 64;
-                    while (n2 < (int)kept) n2 *= 2;
-                    if (tid < n2 / 2) {
-                        sort_list(s.list, n2, false);
-                        const u64 d0 = s.list[i0], d1 = s.list[i0 + 1];
-                        w0 = i0 < (int)kept ? mass((uint32_t)d0) : 0;
-                        w1 = i0 + 1 < (int)kept ? mass((uint32_t)d1) : 0;
-                        u64 total;
-                        const u64 run = part_before(w0 + w1, &total, n2 / 2, s), at = fraction_of(U, total, false);
-                        if (run <= at && at < run + w0 + w1) {
-                            const bool second = at >= run + w0;
-                            p.token[row] = (int64_t)((second ? d1 : d0) >> 32);
-                            if (p.logprob) p.logprob[row] = logf(__fdiv_rn((float)(second ? w1 : w0), (float)total));
-                        }
+                    sort_list(s.list, n2, true);
+                    const u64 e0 = s.list[i0], e1 = s.list[i0 + 1];
+                    u64 w0 = i0 < lim ? mass((uint32_t)(e0 >> 32)) : 0, w1 = i0 + 1 < lim ? mass((uint32_t)(e1 >> 32)) : 0;
+                    u64 sum;
+                    const u64 before = part_before(w0 + w1, &sum, n2 / 2, s);
+                    const u64 tau = max(fraction_of(P, cut_k ? sum : total_k, true), 1ull);
+                    // the kept ones by index, the others behind them
+                    if (before + w0 >= tau || w1 < least) w1 = 0;
+                    if (before >= tau || w0 < least) w0 = 0;
+                    s.list[i0] = w0 ? (u64)(0xffffffffu - (uint32_t)e0) << 32 | e0 >> 32 : ~0ull;
+                    s.list[i0 + 1] = w1 ? (u64)(0xffffffffu - (uint32_t)e1) << 32 | e1 >> 32 : ~0ull;
+                    part_sync(n2 / 2);
+                    sort_list(s.list, n2, false);
+                    const u64 d0 = s.list[i0], d1 = s.list[i0 + 1];
+                    w0 = ~d0 ? mass((uint32_t)d0) : 0;
+                    w1 = ~d1 ? mass((uint32_t)d1) : 0;
+                    u64 total;
+                    const u64 run = part_before(w0 + w1, &total, n2 / 2, s), at = fraction_of(U, total, false);
+                    if (run <= at && at < run + w0 + w1) {
+                        const bool second = at >= run + w0;
+                        answer(0xffffffffu - ((second ? d1 : d0) >> 32), second ? w1 : w0, total);
                     }
                 }
-                if (tid == 0) s.flag = done;
-            } else if (nc > CAP && tid == 0) {
-                s.flag = 0;
             }
         }
-        join(C);
-        const bool done = C > 1 ? remote_load32(&s.flag, 0) != 0 : s.flag != 0;
-        if (C > 1) join(C);
-        if (done) return;
-    }
+        if (C > 1) join(C);                // rank 0's counter has been read
+        return true;
+    };
 
-    // ---- the cut by counting
-    // the largest key K with measure(key >= K) >= target, and *above = measure(key > K).  The counters are
-    // zero before and after a call.
-    int buf = 0;
-    auto find_cut = [&](bool by_mass, u64 target, u64* above_out) {
-        u64 above = 0;
-        uint32_t lo = 1, hi = (uint32_t)mx;
+    if (collect && collect_and_draw(max(bound, 1u), 0)) return;
+
+    uint32_t cut = 0;                      // kept: key > cut, and the first `ties` with key == cut
+    u64 ties = 0;
+    if (cut_k || cut_p) {
+        // ---- the cut by counting.  Each pass leaves counts and masses of 256 bins in s.all_*.
         const float scale = 255.f / fminf(28.f * tdiv, 3.0e38f);
         auto far = [&](uint32_t key) {     // bins of the distance below the maximum; monotone in the key
             const float dist = (m - K::value(key)) * scale;
             return dist < 255.f ? (int)dist : dist == dist ? 255 : 0;
         };
-        int far_bin = -1, shift = 0;
-        while (true) {
-            each([&](uint32_t key, int) {
+        int buf = 0;
+        auto count = [&](uint32_t lo, uint32_t hi, auto&& bin_of) {
+            each([&](uint32_t key) {
                 if (key < lo || key > hi) return;
-                int b;
-                if (far_bin < 0) b = far(key);
-                else if (far(key) != far_bin) return;
-                else b = (int)((hi - key) >> shift);
+                const int b = bin_of(key);
+                if (b < 0) return;
                 atomicAdd(&s.hist[0][b], 1u);
-                if (by_mass) {
-                    const u64 w = mass(key);
-                    if (w) {
-                        atomicAdd(&s.hist[1][b], (uint32_t)w & 0x1fffu);
-                        atomicAdd(&s.hist[2][b], (uint32_t)(w >> 13) & 0x1fffu);
-                        atomicAdd(&s.hist[3][b], (uint32_t)(w >> 26));
-                    }
+                const u64 w = mass(key);
+                if (w) {
+                    atomicAdd(&s.hist[1][b], (uint32_t)w & 0x1fffu);
+                    atomicAdd(&s.hist[2][b], (uint32_t)(w >> 13) & 0x1fffu);
+                    atomicAdd(&s.hist[3][b], (uint32_t)(w >> 26));
                 }
             });
             __syncthreads();
             if (tid < 256) {
-                s.bins[buf][tid] = by_mass ? (u64)s.hist[1][tid] + ((u64)s.hist[2][tid] << 13) + ((u64)s.hist[3][tid] << 26)
-                                           : (u64)s.hist[0][tid];
+                const u64 w = (u64)s.hist[1][tid] + ((u64)s.hist[2][tid] << 13) + ((u64)s.hist[3][tid] << 26);
+                if (C > 1) {
+                    s.bin_mass[buf][tid] = w;
+                    s.bin_count[buf][tid] = s.hist[0][tid];
+                } else {
+                    s.all_mass[tid] = w;
+                    s.all_count[tid] = s.hist[0][tid];
+                }
 #pragma unroll
                 for (int q = 0; q < 4; ++q) s.hist[q][tid] = 0;
             }
             join(C);
-            // every warp finds the bin for itself; lane l: bins 8 l to 8 l + 7
-            u64 v[8], sum = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = C > 1 ? 0 : s.bins[buf][8 * lane + i];
-            if (C > 1) {                   // the cluster's sums, a part of the bins to each warp
-                const int b = tid >> 1;
-                u64 x = 0;
-                for (int r = tid & 1; r < C; r += 2) x += remote_load64(&s.bins[buf][b], r);
-                x += __shfl_xor_sync(DG_FULL_MASK, x, 1);
-                if (!(tid & 1)) s.list[b] = x;
+            if (C > 1) {
+                const int b = tid >> 1;    // two threads to a bin
+                u64 w = 0;
+                uint32_t c = 0;
+                for (int r = tid & 1; r < C; r += 2) {
+                    w += remote_load64(&s.bin_mass[buf][b], r);
+                    c += remote_load32(&s.bin_count[buf][b], r);
+                }
+                w += __shfl_xor_sync(DG_FULL_MASK, w, 1);
+                c += __shfl_xor_sync(DG_FULL_MASK, c, 1);
+                if (!(tid & 1)) s.all_mass[b] = w, s.all_count[b] = c;
                 __syncthreads();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = s.list[8 * lane + i];
             }
             buf ^= 1;
+        };
+        // the bin in which the running count or mass (from `count0`, `mass0`) reaches the target, and the
+        // running values before it; every warp for itself, lane l: bins 8 l to 8 l + 7
+        auto crossing = [&](bool by_mass, u64 target, u64& count0, u64& mass0) {
+            u64 sc = 0, sw = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += v[i];
-            const u64 inc = warp_scan(sum, lane) + above;
-            const unsigned hit = __ballot_sync(DG_FULL_MASK, inc >= target);
-            const int at = hit ? __ffs(hit) - 1 : 31;
-            u64 run = inc - sum;
+            for (int i = 0; i < 8; ++i) sc += s.all_count[8 * lane + i], sw += s.all_mass[8 * lane + i];
+            const u64 ic = warp_scan(sc, lane) + count0, iw = warp_scan(sw, lane) + mass0;
+            const unsigned hit = __ballot_sync(DG_FULL_MASK, (by_mass ? iw : ic) >= target);
+            u64 c = ic - sc, w = iw - sw;
             int bin = 8 * lane;
-#pragma unroll
-            for (int i = 0; i < 7; ++i)
-                if (run + v[i] < target && bin == 8 * lane + i) run += v[i], ++bin;
-            bin = __shfl_sync(DG_FULL_MASK, bin, at);
-            above = __shfl_sync(DG_FULL_MASK, run, at);
-            if (far_bin < 0) {
-                // keys that surely hold the bin's, rounding errors of m and the distance included; the
-                // digits below only count those in it
-                far_bin = bin;
-                const float edge = (float)(bin + 1) / scale, fuzz = 1e-6f * (edge + fabsf(m));
-                const uint32_t a = K::near(m - edge - fuzz), b = K::near(m - (float)bin / scale + fuzz);
-                lo = bin == 255 || a <= 2 ? 1 : a - 2;
-                hi = bin == 0 ? (uint32_t)mx : min((uint32_t)mx, b + 2);
-            } else {
+            for (int i = 0; i < 7; ++i) {
+                const u64 nc = c + s.all_count[8 * lane + i], nw_ = w + s.all_mass[8 * lane + i];
+                if ((by_mass ? nw_ : nc) >= target) break;
+                c = nc, w = nw_, ++bin;
+            }
+            const int at = hit ? __ffs(hit) - 1 : 31;
+            count0 = __shfl_sync(DG_FULL_MASK, c, at);
+            mass0 = __shfl_sync(DG_FULL_MASK, w, at);
+            return __shfl_sync(DG_FULL_MASK, bin, at);
+        };
+        // within bin `first` of the distance: the one key in which the target is reached, the running values
+        // before it, and how many tokens have it
+        auto narrow = [&](bool by_mass, u64 target, int first, u64& count0, u64& mass0, uint32_t& here) {
+            // keys that surely hold the bin's, rounding errors of m and the distance included; only those
+            // in the bin are counted
+            const float edge = (float)(first + 1) / scale, fuzz = 1e-6f * (edge + fabsf(m));
+            const uint32_t a = K::near(m - edge - fuzz), b = K::near(m - (float)first / scale + fuzz);
+            uint32_t lo = first == 255 || a <= 2 ? 1 : a - 2;
+            uint32_t hi = first == 0 ? (uint32_t)mx : min((uint32_t)mx, b + 2);
+            while (true) {
+                int shift = 0;
+                while (((hi - lo) >> shift) > 255) ++shift;
+                __syncthreads();           // s.all_* have been read
+                count(lo, hi, [&](uint32_t key) { return far(key) == first ? (int)((hi - key) >> shift) : -1; });
+                const int bin = crossing(by_mass, target, count0, mass0);
+                here = s.all_count[bin];
                 const uint32_t top = hi - ((uint32_t)bin << shift), bottom = top - ((1u << shift) - 1);
                 lo = bottom > lo && bottom <= top ? bottom : lo;
                 hi = top;
+                if (shift == 0 || lo >= hi) return hi;
             }
-            if (lo >= hi) break;
-            shift = 0;
-            while (((hi - lo) >> shift) > 255) ++shift;
-            if (C > 1) __syncthreads();    // list[] has been read
+        };
+        count(1, (uint32_t)mx, far);
+        u64 total_k = 0, kc = 0, kw = 0, pc = 0, pw = 0;
+        uint32_t here = 0;
+        int kbin = 0, pbin = -1;
+        if (cut_k) {
+            kbin = crossing(false, (u64)k, kc, kw);
+        } else {
+            u64 sw = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sw += s.all_mass[8 * lane + i];
+            total_k = warp_sum(sw);
+            const u64 tau = max(fraction_of(P, total_k, true), 1ull);
+            pbin = crossing(true, tau, pc, pw);
+            const u64 reached = pc + s.all_count[pbin];
+            if (reached <= CAP && tau < total_k) {
+                // few tokens down to the cut: draw from them (a key below the bin's lowest does no harm)
+                const float edge = (float)(pbin + 1) / scale, fuzz = 1e-6f * (edge + fabsf(m));
+                const uint32_t a = K::near(m - edge - fuzz);
+                if (pbin < 255 && collect_and_draw(a <= 2 ? 1 : a - 2, total_k)) return;
+            }
         }
-        __syncthreads();
-        *above_out = above;
-        return hi;
-    };
-    auto mass_above = [&](uint32_t key, int slot) {
-        u64 w = 0;
-        each([&](uint32_t kk, int) { if (kk > key) w += mass(kk); });
-        return over_cluster(block_sum(w, s), slot, C, s, add);
-    };
-    uint32_t cut = 0;                      // kept: key > cut, and the first `ties` with key == cut
-    u64 ties = 0;
-    if (cut_k) {
-        u64 above;
-        cut = find_cut(false, (u64)k, &above);
-        ties = (u64)k - above;
-        if (cut_p) total_k = mass_above(cut, 3) + ties * mass(cut);
-    }
-    if (cut_p) {
-        const u64 tau = max(fraction_of(P, total_k, true), 1ull);
-        if (tau < total_k) {
-            u64 above;
-            cut = find_cut(true, tau, &above);
-            const u64 w = mass(cut);
-            ties = (tau - above + w - 1) / w;
+        if (cut_k) {
+            // top_p's share is known once the k-th key is: keep the first pass's bins for it
+            if (cut_p) {
+                __syncthreads();
+                if (tid < 256) s.list[tid] = s.all_mass[tid], s.list[256 + tid] = s.all_count[tid];
+                __syncthreads();
+            }
+            cut = narrow(false, (u64)k, kbin, kc, kw, here);
+            ties = (u64)k - kc;
+            total_k = kw + ties * mass(cut);
+            if (ties == here) --cut, ties = 0;         // all of them: simply the keys above
+            if (cut_p) {
+                const u64 tau = max(fraction_of(P, total_k, true), 1ull);
+                if (tau < total_k) {
+                    __syncthreads();
+                    if (tid < 256) s.all_mass[tid] = s.list[tid], s.all_count[tid] = (uint32_t)s.list[256 + tid];
+                    __syncthreads();
+                    pbin = crossing(true, tau, pc, pw);
+                    cut = narrow(true, tau, pbin, pc, pw, here);
+                    const u64 w = mass(cut);
+                    ties = (tau - pw + w - 1) / w;
+                    if (ties == here) --cut, ties = 0;
+                }
+            }
+        } else {
+            const u64 tau = max(fraction_of(P, total_k, true), 1ull);
+            if (tau < total_k) {
+                cut = narrow(true, tau, pbin, pc, pw, here);
+                const u64 w = mass(cut);
+                ties = (tau - pw + w - 1) / w;
+                if (ties == here) --cut, ties = 0;
+            }
         }
     }
 
     // ---- the draw in index order: each warp walks a contiguous piece of the words
-    const int piece = (nw + WARPS - 1) / WARPS, i0 = min(warp * piece, nw), i1 = min(i0 + piece, nw);
-    uint32_t seen0 = 0;                    // tokens with the cut key before this warp's piece
-    if (cut) {
+    const int piece = (nw + WARPS - 1) / WARPS;
+    // tokens with the cut key in words [a, b), by one warp
+    auto ties_in = [&](int a, int b) {
         uint32_t c = 0;
-        for (int i = i0 + lane; i < i1; i += 32) {
+        for (int i = a + lane; i < b; i += 32) {
             const uint32_t w = words[i];
 #pragma unroll
             for (int e = 0; e < W; ++e) c += K::at(w, e) == cut;
         }
-        c = __reduce_add_sync(DG_FULL_MASK, c);
-        u64 all;
-        const u64 before = block_before(lane == 0 ? c : 0, &all, s);
-        seen0 = (uint32_t)__shfl_sync(DG_FULL_MASK, before, 0);
-        if (C > 1) {
-            if (tid == 0) s.post[4] = all;
-            join(C);
-            for (int r = 0; r < rank; ++r) seen0 += (uint32_t)remote_load64(&s.post[4], r);
-        }
-    }
-    // f(word index, the masses of this lane's keys in it) in index order; returns when f says so
-    auto walk = [&](auto&& f) {
-        uint32_t seen = seen0;
-        for (int b = i0; b < i1; b += 32) {
-            const int i = b + lane;
-            const uint32_t word = i < i1 ? words[i] : 0;
+        return __reduce_add_sync(DG_FULL_MASK, c);
+    };
+    // f(word index, the masses of this lane's keys in it) over words [a, b) in index order, `seen` tokens with
+    // the cut key before them
+    auto walk = [&](int a, int b, uint32_t seen, auto&& f) {
+#pragma unroll 2
+        for (int base = a; base < b; base += 32) {
+            const int i = base + lane;
+            const uint32_t word = i < b ? words[i] : 0;
             u64 w[W];
             uint32_t t = seen;
-            if (cut) {
-                unsigned is[W];
+            if (ties) {
 #pragma unroll
                 for (int e = 0; e < W; ++e) {
-                    is[e] = __ballot_sync(DG_FULL_MASK, K::at(word, e) == cut);
-                    t += __popc(is[e] & ((1u << lane) - 1));
-                    seen += __popc(is[e]);
+                    const unsigned is = __ballot_sync(DG_FULL_MASK, K::at(word, e) == cut);
+                    t += __popc(is & ((1u << lane) - 1));
+                    seen += __popc(is);
                 }
             }
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 const uint32_t key = K::at(word, e);
-                w[e] = key > cut || (cut && key == cut && t < ties) ? mass(key) : 0;
+                w[e] = key > cut || (key == cut && t < ties) ? mass(key) : 0;
                 t += key == cut;
                 if (w[e] < least) w[e] = 0;
             }
-            if (f(i, w)) return;
+            f(i, w);
         }
     };
-    u64 mine = 0;
-    walk([&](int, const u64 (&w)[W]) {
+    auto sum_of = [&](int a, int b, uint32_t seen) {
+        u64 v = 0;
+        walk(a, b, seen, [&](int, const u64 (&w)[W]) {
 #pragma unroll
-        for (int e = 0; e < W; ++e) mine += w[e];
-        return false;
-    });
-    mine = warp_sum(mine);
-    u64 total;
+            for (int e = 0; e < W; ++e) v += w[e];
+        });
+        return warp_sum(v);
+    };
+    int a0 = min(warp * piece, nw), a1 = min(a0 + piece, nw);
+    uint32_t seen = 0;
+    if (ties) {
+        const uint32_t c = ties_in(a0, a1);
+        u64 all;
+        const u64 before = block_before(lane == 0 ? c : 0, &all, s);
+        seen = (uint32_t)__shfl_sync(DG_FULL_MASK, before, 0);
+        if (C > 1) {
+            if (tid == 0) s.post[4] = all;
+            join(C);
+            for (int r = 0; r < rank; ++r) seen += (uint32_t)remote_load64(&s.post[4], r);
+        }
+    }
+    u64 mine = sum_of(a0, a1, seen), total;
     u64 start = block_before(lane == 0 ? mine : 0, &total, s);
     start = __shfl_sync(DG_FULL_MASK, start, 0);
+    u64 cta_start = 0;
+    const u64 cta_mass = total;
     if (C > 1) {
         if (tid == 0) s.post[5] = total;
         join(C);
         total = 0;
         for (int r = 0; r < C; ++r) {
             const u64 v = remote_load64(&s.post[5], r);
-            if (r < rank) start += v;
+            if (r < rank) cta_start += v;
             total += v;
         }
+        start += cta_start;
         join(C);                           // all slots have been read: any CTA may end
     }
     const u64 at = fraction_of(U, total, false);
+    if (at < cta_start || at >= cta_start + cta_mass) return;
+    // the CTA whose keys hold the draw: all its warps share the piece that does
+    if (lane == 0 && start <= at && at < start + mine) s.flag = (uint32_t)warp, s.post[6] = start, s.post[7] = seen;
+    __syncthreads();
+    const int base = min((int)s.flag * piece, nw), last = min(base + piece, nw), part = ((last - base + WARPS - 1) / WARPS + 31) / 32 * 32;
+    start = s.post[6];
+    seen = (uint32_t)s.post[7];
+    a0 = min(base + warp * part, last), a1 = min(a0 + part, last);
+    if (ties) {
+        const uint32_t c = ties_in(a0, a1);
+        u64 all;
+        const u64 before = block_before(lane == 0 ? c : 0, &all, s);
+        seen += (uint32_t)__shfl_sync(DG_FULL_MASK, before, 0);
+    }
+    mine = sum_of(a0, a1, seen);
+    u64 all;
+    const u64 before = block_before(lane == 0 ? mine : 0, &all, s);
+    start += __shfl_sync(DG_FULL_MASK, before, 0);
     if (start <= at && at < start + mine) {
         u64 run = start;
-        walk([&](int i, const u64 (&w)[W]) {
+        walk(a0, a1, seen, [&](int i, const u64 (&w)[W]) {
             u64 sum = 0;
 #pragma unroll
             for (int e = 0; e < W; ++e) sum += w[e];
-            const u64 inc = warp_scan(sum, lane);
-            const unsigned hit = __ballot_sync(DG_FULL_MASK, run + inc > at);
-            if (hit) {
-                if (lane == __ffs(hit) - 1) {
-                    const u64 r = run + inc - sum;
-                    const int e = W > 1 && at >= r + w[0] ? 1 : 0;
-                    const u64 we = w[e ? W - 1 : 0];
-                    p.token[row] = (int64_t)s0 + i * W + e - off;
-                    if (p.logprob) p.logprob[row] = logf(__fdiv_rn((float)we, (float)total));
-                }
-                return true;
+            const u64 inc = warp_scan(sum, lane), r = run + inc - sum;
+            if (r <= at && at < r + sum) {
+                const int e = W > 1 && at >= r + w[0] ? 1 : 0;
+                p.token[row] = (int64_t)s0 + i * W + e - off;
+                if (p.logprob) p.logprob[row] = logf(__fdiv_rn((float)w[e ? W - 1 : 0], (float)total));
             }
             run += __shfl_sync(DG_FULL_MASK, inc, 31);
-            return false;
         });
     }
 }
 
 // CTAs per row: as many (up to 16) as give each SM one, with at least 2048 logits each; and as many as a
-// slice of at most 92 KB (two CTAs to an SM) asks for.  A CTA's work beyond its logits is the same
+// slice of at most 88 KB (two CTAs to an SM) asks for.  A CTA's work beyond its logits is the same
 // whatever it holds, so more CTAs than SMs cost more than they save.
 int cluster_of(int B, int V, size_t elem) {
     int c = 1;
     while (c < 16 && ((int64_t)B * c * 2 <= 148 && V / (2 * c) >= 2048)) c *= 2;
-    while (c < 16 && ((size_t)V + c - 1) / c * elem > 92 * 1024) c *= 2;
+    while (c < 16 && ((size_t)V + c - 1) / c * elem > 88 * 1024) c *= 2;
     return c;
 }
 
