@@ -158,12 +158,12 @@ __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
 }
 __device__ __forceinline__ u64 remote_load64(const u64* p, uint32_t rank) {
     u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote(p, rank)) : "memory");
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote(p, rank)));
     return v;
 }
 __device__ __forceinline__ uint32_t remote_load32(const uint32_t* p, uint32_t rank) {
     uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote(p, rank)) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote(p, rank)));
     return v;
 }
 __device__ __forceinline__ void remote_store64(u64* p, uint32_t rank, u64 v) {
@@ -185,7 +185,8 @@ struct Shared {
     uint32_t all_count[256];
     u64 warp[WARPS];
     u64 post[8];                           // values that the cluster's other CTAs read
-    uint32_t collected;
+    uint32_t queue[CAP];                   // vectors that hold a token to collect
+    uint32_t vectors, collected;
     uint32_t flag;
 };
 
@@ -263,15 +264,13 @@ __device__ __forceinline__ u64 block_before(u64 v, u64* total, Shared& s) {
     *total = t;
     return before + inc - v;
 }
-// sum, or largest or smallest, of one value per CTA over the cluster; slots of s.post alternate, so that
-// a slot is written again only after a barrier that follows its last reading
-template <typename F> __device__ __forceinline__ u64 over_cluster(u64 v, int slot, int cluster, Shared& s, F&& f) {
-    if (cluster == 1) return v;
+// One value per CTA of the cluster, in lane r the value of CTA r (0 beyond): one remote load each, side by
+// side.  A slot is written again only after a barrier that follows its last reading.
+__device__ __forceinline__ u64 over_cluster(u64 v, int slot, int cluster, Shared& s) {
     if (threadIdx.x == 0) s.post[slot] = v;
     join(cluster);
-    u64 r = remote_load64(&s.post[slot], 0);
-    for (int k = 1; k < cluster; ++k) r = f(r, remote_load64(&s.post[slot], k));
-    return r;
+    const int lane = threadIdx.x & 31;
+    return lane < cluster ? remote_load64(&s.post[slot], lane) : 0;
 }
 
 // sorts list[0, n2) (n2 a power of two, 64 to 1024) by the first n2 / 2 threads, one exchange per thread
@@ -322,7 +321,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     const int nw = nv * 4;                 // words
     uint32_t top0 = K::NONE, top1 = K::NONE;       // largest values of this thread's even and odd vectors
     if (tid < 4 * 256) (&s.hist[0][0])[tid] = (&s.hist[0][0])[tid + ST] = 0;
-    if (tid == 0) s.collected = 0;
+    if (tid == 0) s.collected = s.vectors = 0;
     if (tid < off) keys[tid] = 0;
     if (tid < nv * E - off - n) keys[off + n + tid] = 0;
     uint32_t most0 = 0, most1 = 0;
@@ -411,11 +410,9 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     }
     if (C > 1) {
         // j tokens of each CTA reach its bound, so C j reach the smallest
-        const u64 both = over_cluster(mx << 32 | (0xffffffffu - bound), 0, C, s, [](u64 a, u64 b) {
-            return max(a >> 32, b >> 32) << 32 | max(a & 0xffffffffu, b & 0xffffffffu);
-        });
-        mx = both >> 32;
-        bound = 0xffffffffu - (uint32_t)both;
+        const u64 v = over_cluster(mx << 32 | (0xffffffffu - bound), 0, C, s);
+        mx = __reduce_max_sync(DG_FULL_MASK, (uint32_t)(v >> 32));
+        bound = 0xffffffffu - __reduce_max_sync(DG_FULL_MASK, (uint32_t)v);
     }
     const float m = K::value((uint32_t)mx);
     if (m == -INFINITY) {                  // nothing can be drawn
@@ -439,17 +436,35 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     };
 
     // ---- collect the tokens that reach `bound`, and draw from them: thread t of the CTA that holds the
-    // list.  Returns whether they were few enough; uniform over the cluster.
+    // list.  total_k: what top_p takes its share of, or 0 where that is the mass of the first k of them.
+    // Returns whether they were few enough; uniform over the cluster.
     auto collect_and_draw = [&](uint32_t bound, u64 total_k) {
-        for (int i = tid; i < nv; i += ST) {
-            if (!K::reaches(vecs[i], bound)) continue;
-#pragma unroll 1
-            for (int e = 0; e < E; ++e) {
-                const uint32_t key = keys[i * E + e];
+        // the vectors with such a token first, then one thread for each of their elements
+        for (int i0 = tid; i0 < nv; i0 += 4 * ST) {
+            uint4 v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = i0 + q * ST < nv ? vecs[i0 + q * ST] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (K::reaches(v[q], bound)) {
+                    const uint32_t at = atomicAdd(&s.vectors, 1u);
+                    if (at < CAP) s.queue[at] = (uint32_t)(i0 + q * ST);
+                }
+        }
+        __syncthreads();
+        const uint32_t nq = s.vectors;
+        if (nq > CAP) {
+            if (tid == 0) {                // more tokens than vectors
+                if (C > 1) remote_add(&s.collected, 0, nq);
+                else s.collected = nq;
+            }
+        } else {
+            for (uint32_t i = tid; i < nq * E; i += ST) {
+                const uint32_t place = s.queue[i / E] * E + i % E, key = keys[place];
                 if (key >= bound) {
                     const uint32_t at = C > 1 ? remote_add(&s.collected, 0, 1) : atomicAdd(&s.collected, 1u);
                     if (at < CAP) {
-                        const u64 entry = (u64)key << 32 | (0xffffffffu - (uint32_t)(s0 + i * E + e - off));
+                        const u64 entry = (u64)key << 32 | (0xffffffffu - (uint32_t)(s0 + (int)place - off));
                         if (C > 1) remote_store64(&s.list[at], 0, entry);
                         else s.list[at] = entry;
                     }
@@ -487,7 +502,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
                 }
                 const bool in_k = c < nc && rank_ < (uint32_t)lim;
                 const u64 k_mass = block_sum(in_k && q == 0 ? w : 0, s);     // (masses[] have been read)
-                if (cut_k) total_k = k_mass;
+                if (total_k == 0) total_k = k_mass;
                 const u64 tau = max(fraction_of(P, total_k, true), 1ull);
                 const bool keep = in_k && before < tau && w >= least;
                 if (q == 0 && c < nc && !keep) s.masses[c] = 0;
@@ -513,7 +528,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
                     u64 w0 = i0 < lim ? mass((uint32_t)(e0 >> 32)) : 0, w1 = i0 + 1 < lim ? mass((uint32_t)(e1 >> 32)) : 0;
                     u64 sum;
                     const u64 before = part_before(w0 + w1, &sum, n2 / 2, s);
-                    const u64 tau = max(fraction_of(P, cut_k ? sum : total_k, true), 1ull);
+                    const u64 tau = max(fraction_of(P, total_k ? total_k : sum, true), 1ull);
                     // the kept ones by index, the others behind them
                     if (before + w0 >= tau || w1 < least) w1 = 0;
                     if (before >= tau || w0 < least) w0 = 0;
@@ -542,7 +557,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     uint32_t cut = 0;                      // kept: key > cut, and the first `ties` with key == cut
     u64 ties = 0;
     if (cut_k || cut_p) {
-        // ---- the cut by counting.  Each pass leaves counts and masses of 256 bins in s.all_*.
+        // ---- the cut by counting.  Each pass leaves counts and masses of 256 bins in s.all_*.  Tokens
+        // without mass are left out: they cannot be drawn, so a cut among them is as good as none.
         const float scale = 255.f / fminf(28.f * tdiv, 3.0e38f);
         auto far = [&](uint32_t key) {     // bins of the distance below the maximum; monotone in the key
             const float dist = (m - K::value(key)) * scale;
@@ -553,14 +569,12 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
             each([&](uint32_t key) {
                 if (key < lo || key > hi) return;
                 const int b = bin_of(key);
-                if (b < 0) return;
+                const u64 w = b < 0 ? 0 : mass(key);
+                if (w == 0) return;
                 atomicAdd(&s.hist[0][b], 1u);
-                const u64 w = mass(key);
-                if (w) {
-                    atomicAdd(&s.hist[1][b], (uint32_t)w & 0x1fffu);
-                    atomicAdd(&s.hist[2][b], (uint32_t)(w >> 13) & 0x1fffu);
-                    atomicAdd(&s.hist[3][b], (uint32_t)(w >> 26));
-                }
+                atomicAdd(&s.hist[1][b], (uint32_t)w & 0x1fffu);
+                atomicAdd(&s.hist[2][b], (uint32_t)(w >> 13) & 0x1fffu);
+                atomicAdd(&s.hist[3][b], (uint32_t)(w >> 26));
             });
             __syncthreads();
             if (tid < 256) {
@@ -580,10 +594,16 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
                 const int b = tid >> 1;    // two threads to a bin
                 u64 w = 0;
                 uint32_t c = 0;
-                for (int r = tid & 1; r < C; r += 2) {
-                    w += remote_load64(&s.bin_mass[buf][b], r);
-                    c += remote_load32(&s.bin_count[buf][b], r);
+                u64 rw[8];
+                uint32_t rc[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const int from = 2 * r + (tid & 1);
+                    rw[r] = from < C ? remote_load64(&s.bin_mass[buf][b], from) : 0;
+                    rc[r] = from < C ? remote_load32(&s.bin_count[buf][b], from) : 0;
                 }
+#pragma unroll
+                for (int r = 0; r < 8; ++r) w += rw[r], c += rc[r];
                 w += __shfl_xor_sync(DG_FULL_MASK, w, 1);
                 c += __shfl_xor_sync(DG_FULL_MASK, c, 1);
                 if (!(tid & 1)) s.all_mass[b] = w, s.all_count[b] = c;
@@ -634,27 +654,28 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
             }
         };
         count(1, (uint32_t)mx, far);
-        u64 total_k = 0, kc = 0, kw = 0, pc = 0, pw = 0;
-        uint32_t here = 0;
-        int kbin = 0, pbin = -1;
-        if (cut_k) {
-            kbin = crossing(false, (u64)k, kc, kw);
-        } else {
-            u64 sw = 0;
+        u64 total_k = 0, tokens = 0, kc = 0, kw = 0, pc = 0, pw = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sw += s.all_mass[8 * lane + i];
-            total_k = warp_sum(sw);
+        for (int i = 0; i < 8; ++i) total_k += s.all_mass[8 * lane + i], tokens += s.all_count[8 * lane + i];
+        total_k = warp_sum(total_k);
+        tokens = warp_sum(tokens);
+        const bool by_k = cut_k && (u64)k < tokens;
+        uint32_t here = 0;
+        int kbin = 0, pbin = 0;
+        if (by_k) {
+            kbin = crossing(false, (u64)k, kc, kw);
+        } else if (cut_p) {
             const u64 tau = max(fraction_of(P, total_k, true), 1ull);
             pbin = crossing(true, tau, pc, pw);
             const u64 reached = pc + s.all_count[pbin];
-            if (reached <= CAP && tau < total_k) {
+            if (reached <= CAP && tau < total_k && !collect) {
                 // few tokens down to the cut: draw from them (a key below the bin's lowest does no harm)
                 const float edge = (float)(pbin + 1) / scale, fuzz = 1e-6f * (edge + fabsf(m));
                 const uint32_t a = K::near(m - edge - fuzz);
                 if (pbin < 255 && collect_and_draw(a <= 2 ? 1 : a - 2, total_k)) return;
             }
         }
-        if (cut_k) {
+        if (by_k) {
             // top_p's share is known once the k-th key is: keep the first pass's bins for it
             if (cut_p) {
                 __syncthreads();
@@ -678,7 +699,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
                     if (ties == here) --cut, ties = 0;
                 }
             }
-        } else {
+        } else if (cut_p) {
             const u64 tau = max(fraction_of(P, total_k, true), 1ull);
             if (tau < total_k) {
                 cut = narrow(true, tau, pbin, pc, pw, here);
@@ -744,9 +765,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
         const u64 before = block_before(lane == 0 ? c : 0, &all, s);
         seen = (uint32_t)__shfl_sync(DG_FULL_MASK, before, 0);
         if (C > 1) {
-            if (tid == 0) s.post[4] = all;
-            join(C);
-            for (int r = 0; r < rank; ++r) seen += (uint32_t)remote_load64(&s.post[4], r);
+            const u64 v = over_cluster(all, 4, C, s);
+            seen += __reduce_add_sync(DG_FULL_MASK, lane < rank ? (uint32_t)v : 0u);
         }
     }
     u64 mine = sum_of(a0, a1, seen), total;
@@ -755,14 +775,9 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     u64 cta_start = 0;
     const u64 cta_mass = total;
     if (C > 1) {
-        if (tid == 0) s.post[5] = total;
-        join(C);
-        total = 0;
-        for (int r = 0; r < C; ++r) {
-            const u64 v = remote_load64(&s.post[5], r);
-            if (r < rank) cta_start += v;
-            total += v;
-        }
+        const u64 v = over_cluster(total, 5, C, s);
+        cta_start = warp_sum(lane < rank ? v : 0);
+        total = warp_sum(v);
         start += cta_start;
         join(C);                           // all slots have been read: any CTA may end
     }
@@ -803,12 +818,12 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
 }
 
 // CTAs per row: as many (up to 16) as give each SM one, with at least 2048 logits each; and as many as a
-// slice of at most 88 KB (two CTAs to an SM) asks for.  A CTA's work beyond its logits is the same
+// slice of at most 84 KB (two CTAs to an SM) asks for.  A CTA's work beyond its logits is the same
 // whatever it holds, so more CTAs than SMs cost more than they save.
 int cluster_of(int B, int V, size_t elem) {
     int c = 1;
     while (c < 16 && ((int64_t)B * c * 2 <= 148 && V / (2 * c) >= 2048)) c *= 2;
-    while (c < 16 && ((size_t)V + c - 1) / c * elem > 88 * 1024) c *= 2;
+    while (c < 16 && ((size_t)V + c - 1) / c * elem > 84 * 1024) c *= 2;
     return c;
 }
 
