@@ -2,13 +2,16 @@
 // backward pass on CUDA cores: 64 x 64 output tiles, 16 of the contracted axis at a time
 // through shared memory, 4 x 4 outputs per thread.  These kernels take any storage type, size
 // and alignment; 16-bit calls with D and F multiples of 8 and 16-byte aligned rows go to the
-// tcgen05 kernel of gated_ffn_tc.cu.
+// tcgen05 kernel of gated_ffn_tc.cu or, with few tokens, to gated_ffn_few.cu.
 #include "lm_common.cuh"
 
 namespace dg_host {
 bool ffn_tc_supports(int dtype, int64_t M, int D, int F);
 bool ffn_tc_aligned(const void* a, int64_t lda, const void* b, const void* c, const void* d, int64_t ldd,
                     const void* e, const void* f);
+bool ffn_few_supports(int64_t M, int D, int F);
+int ffn_few_forward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
+                    const void* bias, void* h, cudaStream_t s);
 int ffn_tc_forward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
                    const void* bias, void* h, int32_t* status, cudaStream_t s);
 size_t ffn_tc_workspace(int64_t M, int D, int F);
@@ -160,8 +163,11 @@ int dg_gated_ffn_forward(int dtype, int64_t M, int D, int F, int activation, con
     if (M == 0) return DG_OK;
     if (!x || !weight || !h || ldx < D) return DG_ERR_INVALID_ARGUMENT;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dg_host::ffn_tc_supports(dtype, M, D, F) && dg_host::ffn_tc_aligned(x, ldx, weight, bias, h, 0, h, h))
+    if (dg_host::ffn_tc_supports(dtype, M, D, F) && dg_host::ffn_tc_aligned(x, ldx, weight, bias, h, 0, h, h)) {
+        if (dg_host::ffn_few_supports(M, D, F))
+            return dg_host::ffn_few_forward(dtype, M, D, F, activation, x, ldx, weight, bias, h, s);
         return dg_host::ffn_tc_forward(dtype, M, D, F, activation, x, ldx, weight, bias, h, dev_status, s);
+    }
     const dim3 grid((F + TN - 1) / TN, (unsigned)((M + TM - 1) / TM));
     DG_DISPATCH_LM(dtype, S, {
         auto k = activation == DG_ACT_SILU ? ffn_gate_kernel<S, DG_ACT_SILU> : ffn_gate_kernel<S, DG_ACT_GELU>;
