@@ -42,7 +42,8 @@ template <int ROLE> struct Cfg {
     static constexpr uint32_t DH = STAGES * 2 * TILE;              // DGATE: dh, then dG (one slice per group)
     static constexpr uint32_t OUT = DH + (ROLE == DGATE ? 2 * TILE : 0);
     static constexpr uint32_t BAR = OUT + 2 * TILE;
-    static constexpr uint32_t BYTES = BAR + 256;
+    static constexpr uint32_t BIAS = BAR + 256;                    // fp32: per group 64 gate and 64 value biases
+    static constexpr uint32_t BYTES = BIAS + 1024;
 };
 
 struct FfnParams {
@@ -118,29 +119,24 @@ __device__ __forceinline__ Work work_of(const FfnParams& p, int64_t i) {
     return {g * GROUP_M + r % rows, r / rows, s};
 }
 
-__device__ __forceinline__ void load_bias8(const void* bias, int64_t at, bool bf16, float (&b)[8]) {
-    const uint4 v = dg::ldg16(static_cast<const uint16_t*>(bias) + at);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = bf16 ? dgc::Io<__nv_bfloat16>::unpack2(u[i]) : dgc::Io<__half>::unpack2(u[i]);
-        b[2 * i] = f.x;
-        b[2 * i + 1] = f.y;
-    }
+// nothing that uses these registers moves above this point (the wait for the loads that fill them)
+__device__ __forceinline__ void loaded(uint32_t (&r)[16]) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
 }
 
-// sums of v[c] over the warp's 32 lanes for c = 0..31: lane c gets column c's
-__device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
+// sums of v[c] over the warp's 32 lanes for c = 0..15: lane l gets column l / 2's
+__device__ __forceinline__ float column_sums(float (&v)[16], int lane) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
+    for (int o = 16; o > 1; o >>= 1) {
         const bool up = lane & o;
 #pragma unroll
-        for (int i = 0; i < o; ++i) {
-            const float send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+        for (int i = 0; i < o / 2; ++i) {
+            const float send = up ? v[i] : v[i + o / 2], keep = up ? v[i + o / 2] : v[i];
             v[i] = keep + __shfl_xor_sync(DG_FULL_MASK, send, o);
         }
     }
-    return v[0];
+    return v[0] + __shfl_xor_sync(DG_FULL_MASK, v[0], 1);
 }
 
 template <typename T, int ROLE, int ACT, bool A_MN, bool B_MN, bool F32_OUT>
@@ -273,6 +269,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const uint32_t trow = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         uint8_t* out = sm + C::OUT + g * TILE;
         uint8_t* dh = sm + C::DH + g * TILE;
+        float* bias = reinterpret_cast<float*>(sm + C::BIAS) + 128 * g;
         int acc = 0;
         uint32_t acc_ph = 0, dh_ph = 0;
         // the buffer's last TMA store has read it
@@ -288,52 +285,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         for (int64_t it = first; it < items; it += stride) {
             const Work w = work_of(p, it);
             const int row0 = w.mt * 2 * BM + (int)rank * BM;
+            const int f0 = w.nt * BM + 64 * g;                 // GATE, DGATE: this group's 64 features
+            if (ROLE != PLAIN) {                               // (read last before the store's barrier)
+                const int f = f0 + (t & 63);
+                bias[t] = p.bias && f < p.N
+                              ? dg::to_f(static_cast<const T*>(p.bias)[(int64_t)(t >> 6) * p.N + f]) : 0.f;
+            }
             bad = !tc::mbar_wait(acc_full + acc, acc_ph, p.wait_limit);
             if (ROLE == DGATE && !bad) bad = !tc::mbar_wait(dh_full + g, dh_ph, p.wait_limit);
             if (tc::group_sync_or(bar_id, bad)) { bad = true; break; }
             tc::tc_fence_after();
             const uint32_t d = trow + acc * BN;
             if (ROLE != PLAIN) {
-                const int f0 = w.nt * BM + 64 * g;             // this group's 64 features
-                buffer_free();
-                float sums[4];
+                // 16 columns of gate and value at a time, the next ones on their way from TMEM
+                uint32_t gr[2][16], ur[2][16];
+                tc::tmem_ld16(d + 64 * g, gr[0]);
+                tc::tmem_ld16(d + BM + 64 * g, ur[0]);
+                float sum_g[4], sum_u[4];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t gr[32], ur[32];
-                    tc::tmem_ld32(d + 64 * g + 32 * half, gr);
-                    tc::tmem_ld32(d + BM + 64 * g + 32 * half, ur);
+                for (int q = 0; q < 4; ++q) {
                     tc::tmem_wait_ld();
-                    if (half == 1 && ROLE == GATE) release_acc();
-                    float zg[32], zu[32];
+                    loaded(gr[q & 1]);
+                    loaded(ur[q & 1]);
+                    if (q < 3) {
+                        tc::tmem_ld16(d + 64 * g + 16 * (q + 1), gr[(q + 1) & 1]);
+                        tc::tmem_ld16(d + BM + 64 * g + 16 * (q + 1), ur[(q + 1) & 1]);
+                    } else {
+                        release_acc();
+                    }
+                    if (q == 0) buffer_free();
+                    float zg[16], zu[16];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float bg[8] = {}, bu[8] = {};
-                        const int f = f0 + 32 * half + 8 * c;
-                        if (p.bias && f < p.N) {
-                            load_bias8(p.bias, f, BF16, bg);
-                            load_bias8(p.bias, (int64_t)p.N + f, BF16, bu);
-                        }
-                        const uint32_t at = tc::sw128((uint32_t)t, (uint32_t)(4 * half + c));
-                        uint32_t o[4], o2[4], q[4];
-                        if (ROLE == DGATE) *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(dh + at);
+                    for (int c = 0; c < 2; ++c) {
+                        const uint32_t at = tc::sw128((uint32_t)t, (uint32_t)(2 * q + c));
+                        uint32_t o[4], o2[4], dv[4];
+                        if (ROLE == DGATE) *reinterpret_cast<uint4*>(dv) = *reinterpret_cast<const uint4*>(dh + at);
 #pragma unroll
                         for (int e = 0; e < 8; e += 2) {
                             const int i = 8 * c + e;
-                            const float g0 = __uint_as_float(gr[i]) + bg[e], g1 = __uint_as_float(gr[i + 1]) + bg[e + 1];
-                            const float u0 = __uint_as_float(ur[i]) + bu[e], u1 = __uint_as_float(ur[i + 1]) + bu[e + 1];
+                            const dg::F2 bg = *reinterpret_cast<const dg::F2*>(bias + 16 * q + i);
+                            const dg::F2 bu = *reinterpret_cast<const dg::F2*>(bias + 64 + 16 * q + i);
+                            const dg::F2 gv = dg::add2({__uint_as_float(gr[q & 1][i]), __uint_as_float(gr[q & 1][i + 1])}, bg);
+                            const dg::F2 uv = dg::add2({__uint_as_float(ur[q & 1][i]), __uint_as_float(ur[q & 1][i + 1])}, bu);
                             if (ROLE == GATE) {
-                                o[e / 2] = dgc::Io<T>::pack2(dg::act_fn<ACT>(g0) * u0, dg::act_fn<ACT>(g1) * u1);
+                                const dg::F2 h = dg::mul2(dg::act_fn2<ACT>(gv), uv);
+                                o[e / 2] = dgc::Io<T>::pack2(h.x, h.y);
                             } else {
-                                const float2 dv = dgc::Io<T>::unpack2(q[e / 2]);
-                                float a0, a1, s0, s1;
-                                dg::act_grad<ACT>(g0, a0, s0);
-                                dg::act_grad<ACT>(g1, a1, s1);
-                                zg[i] = dv.x * u0 * s0;
-                                zg[i + 1] = dv.y * u1 * s1;
-                                zu[i] = dv.x * a0;
-                                zu[i + 1] = dv.y * a1;
-                                o[e / 2] = dgc::Io<T>::pack2(zg[i], zg[i + 1]);
-                                o2[e / 2] = dgc::Io<T>::pack2(zu[i], zu[i + 1]);
+                                const float2 dhv = dgc::Io<T>::unpack2(dv[e / 2]);
+                                const dg::F2 dd{dhv.x, dhv.y};
+                                dg::F2 a, s;
+                                dg::act_grad2<ACT>(gv, a, s);
+                                const dg::F2 xg = dg::mul2(dg::mul2(dd, uv), s), xu = dg::mul2(dd, a);
+                                zg[i] = xg.x, zg[i + 1] = xg.y;
+                                zu[i] = xu.x, zu[i + 1] = xu.y;
+                                o[e / 2] = dgc::Io<T>::pack2(xg.x, xg.y);
+                                o2[e / 2] = dgc::Io<T>::pack2(xu.x, xu.y);
                             }
                         }
                         if (ROLE == GATE) {
@@ -344,22 +350,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         }
                     }
                     if (ROLE == DGATE && p.colsum) {
-                        sums[2 * half] = column_sums(zg, lane);
-                        sums[2 * half + 1] = column_sums(zu, lane);
+                        sum_g[q] = column_sums(zg, lane);
+                        sum_u[q] = column_sums(zu, lane);
                     }
                 }
-                if (ROLE == DGATE) {
-                    release_acc();
-                    if (p.colsum) {
-                        float* dst = p.colsum + ((int64_t)(w.mt * 2 + (int)rank) * 4 + (warp & 3)) * 2 * p.N;
+                if (ROLE == DGATE && p.colsum) {
+                    float* dst = p.colsum + ((int64_t)(w.mt * 2 + (int)rank) * 4 + (warp & 3)) * 2 * p.N;
+                    // even lanes write the gate's sums, odd ones the value's
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const int f = f0 + 32 * half + lane;
-                            if (f < p.N) {
-                                dst[f] = sums[2 * half];
-                                dst[p.N + f] = sums[2 * half + 1];
-                            }
-                        }
+                    for (int q = 0; q < 4; ++q) {
+                        const int f = f0 + 16 * q + (lane >> 1);
+                        if (f < p.N) dst[(lane & 1 ? p.N : 0) + f] = lane & 1 ? sum_u[q] : sum_g[q];
                     }
                 }
                 tc::fence_proxy_async();
@@ -438,22 +439,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
 }
 
-// dbias[c] = sum over the 32-row sums, in a fixed order: warp w of the block takes rows w, w + 8, ...
+// dbias[c] = sum over the 32-row sums, in a fixed order: warp w of the block takes rows w, w + 32, ...
 template <typename T>
-__global__ void __launch_bounds__(256) colsum_kernel(int rows, int cols, const float* part, T* out) {
-    __shared__ float s[8][32];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) colsum_kernel(int rows, int cols, const float* part, T* out) {
+    __shared__ float s[32][33];
+    const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, w = threadIdx.x >> 5;
     float a = 0.f;
     if (c < cols)
-        for (int r = w; r < rows; r += 8) a += part[(int64_t)r * cols + c];
-    s[w][threadIdx.x & 31] = a;
+        for (int r = w; r < rows; r += 32) a += part[(int64_t)r * cols + c];
+    s[w][lane] = a;
     __syncthreads();
-    if (w == 0 && c < cols) {
-        float v = 0.f;
+    float v = s[lane][w];                  // column w of the block, partial sum `lane`
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v += s[i][threadIdx.x];
-        out[c] = dg::from_f<T>(v);
-    }
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(DG_FULL_MASK, v, o);
+    if (lane == 0 && blockIdx.x * 32 + w < cols) out[blockIdx.x * 32 + w] = dg::from_f<T>(v);
 }
 
 // out = sum of the fp32 partial products, in order of the splits
@@ -670,7 +669,7 @@ static int backward_t(int64_t M, int D, int F, int act, const void* x, int64_t l
     if (rc == DG_OK && dw)
         rc = product<T, true, true>(2 * (int64_t)F, D, M, dz, 2 * (int64_t)F, x, ldx, dw, part, sp.splits_dw, status, s);
     if (rc == DG_OK && db) {
-        colsum_kernel<T><<<(2 * F + 31) / 32, 256, 0, s>>>(p.m_tiles * 8, 2 * F, colsum, static_cast<T*>(db));
+        colsum_kernel<T><<<(2 * F + 31) / 32, 1024, 0, s>>>(p.m_tiles * 8, 2 * F, colsum, static_cast<T*>(db));
         rc = check_launch();
     }
     return rc;

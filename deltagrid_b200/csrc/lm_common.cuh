@@ -38,6 +38,47 @@ __device__ __forceinline__ float sigmoid(float z) {
     return rcp_ftz(1.f + exp2_ftz(fminf(z * -1.4426950408889634f, 115.f)));
 }
 
+// two fp32 values at a time (the two-wide instructions of sm_100)
+struct F2 {
+    float x, y;
+};
+__device__ __forceinline__ uint64_t f2_bits(F2 a) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+__device__ __forceinline__ F2 f2_from(uint64_t a) {
+    F2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+    return f2_from(r);
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+    return f2_from(r);
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+    return f2_from(r);
+}
+__device__ __forceinline__ F2 both(float a) { return {a, a}; }
+
+// sigmoid_pair of two values
+__device__ __forceinline__ void sigmoid_pair2(F2 z, F2& a, F2& one_minus_a) {
+    F2 e = mul2(z, both(-1.4426950408889634f));
+    e.x = exp2_ftz(fminf(e.x, 115.f));
+    e.y = exp2_ftz(fminf(e.y, 115.f));
+    a = add2(e, both(1.f));
+    a.x = rcp_ftz(a.x);
+    a.y = rcp_ftz(a.y);
+    one_minus_a = mul2(e, a);
+}
 // activations of the feed-forward block and their derivatives
 template <int ACT>
 __device__ __forceinline__ float act_fn(float z) {
@@ -58,6 +99,30 @@ __device__ __forceinline__ void act_grad(float z, float& f, float& df) {
         f = z * s;
         df = s * fmaf(z * n, 1.5957691216057308f * fmaf(0.134145f, z2, 1.f), 1.f);
     }
+}
+
+template <int ACT> __device__ __forceinline__ F2 act_fn2(F2 z) {
+    F2 s, n;
+    if (ACT == DG_ACT_SILU) {
+        sigmoid_pair2(z, s, n);
+    } else {
+        const F2 z2 = mul2(z, z);
+        sigmoid_pair2(mul2(both(1.5957691216057308f), fma2(mul2(both(0.044715f), z2), z, z)), s, n);
+    }
+    return mul2(z, s);
+}
+template <int ACT> __device__ __forceinline__ void act_grad2(F2 z, F2& f, F2& df) {
+    F2 s, n;
+    if (ACT == DG_ACT_SILU) {
+        sigmoid_pair2(z, s, n);
+        df = mul2(s, fma2(z, n, both(1.f)));
+    } else {
+        const F2 z2 = mul2(z, z);
+        sigmoid_pair2(mul2(both(1.5957691216057308f), fma2(mul2(both(0.044715f), z2), z, z)), s, n);
+        const F2 slope = mul2(both(1.5957691216057308f), fma2(both(0.134145f), z2, both(1.f)));
+        df = mul2(s, fma2(mul2(z, n), slope, both(1.f)));
+    }
+    f = mul2(z, s);
 }
 
 }  // namespace dg
