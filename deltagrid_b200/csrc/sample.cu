@@ -12,10 +12,11 @@
 //      each with all (512 threads share that), more are sorted.  Ranks and the mass before
 //      each give the kept ones, the same comparison by index gives the token.  Only collected
 //      tokens need an exponential.
-//   2. Where that does not do (no top_k, a large one, many equal logits): counts and masses in
-//      256 bins of the distance below the maximum.  If the bins down to the one that holds
-//      the cut have few tokens, these are collected as in 1.  Otherwise the cut's bin is
-//      counted again by keys, until one key is left, and two walks over the keys in index
+//   2. Where that does not do (no top_k, a large one, many equal logits): counts in 255 bins of
+//      the distance below the maximum.  For top_p they say nearly where the cut lies: counts
+//      times the mass at a bin's middle.  Then only keys near the cut are counted again,
+//      finer, with their exact masses, beside the exact mass of all above them; the few tokens
+//      of the bin that holds the cut are ranked in one CTA.  Two walks over the keys in index
 //      order draw the token.  Without a cut (no top_k, no top_p) only the walks are needed.
 //
 // What bounds it: not the 64 KB of a bf16 row of 32000 (2.5 us for 256 rows) but the latency
@@ -125,19 +126,33 @@ template <> struct Key<float> {
     __device__ static __forceinline__ uint32_t near(float l) { return one(l); }
 };
 
-// The mass of a token; the row's maximum m is above -inf.  Below -28 (2^40 e^-28 < 1) it is 0, as it
-// is for -inf and for the undefined quotients of infinite operands.  Dividing by a power of two is
-// the same as multiplying by its inverse.
+// The masses of N tokens; the row's maximum m is above -inf.  Below -28 (2^40 e^-28 < 1) a mass is 0, as it
+// is for -inf and for the undefined quotients of infinite operands.  (l - m) / T is rounded to 32 bits
+// once: times an inverse that is exact (T a power of two), or times the 64-bit inverse, whose error of
+// 2^-52 cannot move the rounding, as a quotient of 24-bit numbers stays 2^-49 away from every midpoint.
+// Side by side and without branches, for the chain of one is long.
 struct Mass {
-    float m, T, inverse;
-    bool exact;
-    __device__ __forceinline__ Mass(float m_, float T_) : m(m_), T(T_), inverse(1.f / T_) {
-        exact = (__float_as_uint(T_) & 0x7fffffu) == 0 && T_ > 1e-18f && T_ < 1e18f;
+    float m, inverse;                      // inverse: of a power of two, else 0
+    double inverse64;
+    __device__ __forceinline__ Mass(float m_, float T) : m(m_), inverse64(1.0 / (double)T) {
+        inverse = (__float_as_uint(T) & 0x7fffffu) == 0 && T > 1e-18f && T < 1e18f ? 1.f / T : 0.f;
     }
-    __device__ __forceinline__ u64 operator()(float l) const {
-        if (l == m) return 1ull << 40;
-        const float d = l - m, z = exact ? d * inverse : __fdiv_rn(d, T);
-        return z > -28.f ? (u64)__float2ll_rz(expf(z) * 1099511627776.f) : 0ull;
+    template <int N> __device__ __forceinline__ void of(const float (&l)[N], u64 (&w)[N]) const {
+        float z[N];
+        if (inverse != 0.f) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) z[i] = (l[i] - m) * inverse;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) z[i] = (float)((double)(l[i] - m) * inverse64);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            // floor(2^40 e) from the bits of e = f 2^(E - 150), f of 24 bits, E <= 127
+            const uint32_t b = __float_as_uint(expf(fmaxf(z[i], -28.f))), f = (b & 0x7fffffu) | 0x800000u;
+            const u64 v = ((u64)f << 17) >> (127 - (b >> 23));
+            w[i] = l[i] == m ? 1ull << 40 : z[i] > -28.f ? v : 0;
+        }
     }
 };
 // floor (up = 0) or ceiling of n f / 2^24, f <= 2^24, n < 2^58
@@ -182,11 +197,12 @@ struct Shared {
     u64 bin_mass[2][256];                  // what they amount to: this CTA's, read by the cluster
     uint32_t bin_count[2][256];
     u64 all_mass[256];                     // the cluster's
-    uint32_t all_count[256];
+    uint32_t all_count[256], far_count[256];
     u64 warp[WARPS];
-    u64 post[8];                           // values that the cluster's other CTAs read
+    u64 post[16];                          // values that the cluster's other CTAs read
+    u64 cross[3];                          // a crossing: its bin, and the running values before it
     uint32_t queue[CAP];                   // vectors that hold a token to collect
-    uint32_t vectors, collected;
+    uint32_t vectors, collected[3];
     uint32_t flag;
 };
 
@@ -293,8 +309,11 @@ __device__ __forceinline__ void sort_list(u64* list, int n2, bool descending) {
         }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
+// MANY: a row has a CTA of its own and two share an SM; else a cluster's CTAs have an SM each, and twice the
+// registers for independent chains.
+template <typename T, bool MANY>
+__global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p) {
+    constexpr int GROUP = (MANY ? 4 : 8) / Key<T>::PER;
     typedef Key<T> K;
     typedef typename K::type key_t;
     constexpr int E = 16 / sizeof(T);
@@ -321,7 +340,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     const int nw = nv * 4;                 // words
     uint32_t top0 = K::NONE, top1 = K::NONE;       // largest values of this thread's even and odd vectors
     if (tid < 4 * 256) (&s.hist[0][0])[tid] = (&s.hist[0][0])[tid + ST] = 0;
-    if (tid == 0) s.collected = s.vectors = 0;
+    if (tid == 0) s.vectors = s.collected[0] = s.collected[1] = s.collected[2] = 0;
     if (tid < off) keys[tid] = 0;
     if (tid < nv * E - off - n) keys[off + n + tid] = 0;
     uint32_t most0 = 0, most1 = 0;
@@ -334,13 +353,14 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
         keys[off + head + body * E + tid] = (key_t)most1;
     }
     const uint4* vsrc = reinterpret_cast<const uint4*>(src + head);
-    for (int i = tid; i < body; i += 8 * ST) {
-        uint4 v[8];
+#pragma unroll 1
+    for (int i = tid; i < body; i += 4 * ST) {
+        uint4 v[4];
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
+        for (int q = 0; q < 4; ++q)
             if (i + q * ST < body) v[q] = dg::ldg16(vsrc + i + q * ST);
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
+        for (int q = 0; q < 4; ++q)
             if (i + q * ST < body) {
                 v[q] = make_uint4(K::clean(v[q].x), K::clean(v[q].y), K::clean(v[q].z), K::clean(v[q].w));
                 const uint32_t t = K::larger(K::larger(v[q].x, v[q].y), K::larger(v[q].z, v[q].w));
@@ -424,55 +444,69 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
         return;
     }
     const Mass mass_of(m, tdiv);
-    auto mass = [&](uint32_t key) { return mass_of(K::value(key)); };
-    // f(key) for the keys of this CTA's words, any order
-    auto each = [&](auto&& f) {
-#pragma unroll 4
-        for (int i = tid; i < nw; i += ST) {
-            const uint32_t w = words[i];
+    auto mass = [&](uint32_t key) {
+        const float l[1] = {K::value(key)};
+        u64 w[1];
+        mass_of.of(l, w);
+        return w[0];
+    };
+    // f(key, mass or 0) for the keys of this CTA's words, any order, GROUP words of a thread at a time
+    auto each = [&](bool with_mass, auto&& f) {
+#pragma unroll 1
+        for (int i = tid; i < nw; i += GROUP * ST) {
+            uint32_t key[GROUP * W];
+            u64 w[GROUP * W] = {};
 #pragma unroll
-            for (int e = 0; e < W; ++e) f(K::at(w, e));
+            for (int q = 0; q < GROUP; ++q) {
+                const uint32_t word = i + q * ST < nw ? words[i + q * ST] : 0;
+#pragma unroll
+                for (int e = 0; e < W; ++e) key[q * W + e] = K::at(word, e);
+            }
+            if (with_mass) {
+                float l[GROUP * W];
+#pragma unroll
+                for (int q = 0; q < GROUP * W; ++q) l[q] = K::value(key[q]);
+                mass_of.of(l, w);
+            }
+#pragma unroll
+            for (int q = 0; q < GROUP * W; ++q) f(key[q], w[q]);
         }
     };
 
     // ---- collect the tokens that reach `bound`, and draw from them: thread t of the CTA that holds the
     // list.  total_k: what top_p takes its share of, or 0 where that is the mass of the first k of them.
-    // Returns whether they were few enough; uniform over the cluster.
+    // Returns whether they were few enough, and enough; uniform over the cluster.
+    auto push = [&](int counter, uint32_t key, uint32_t place) {
+        const uint32_t at = C > 1 ? remote_add(&s.collected[counter], 0, 1) : atomicAdd(&s.collected[counter], 1u);
+        if (at < CAP) {
+            const u64 entry = (u64)key << 32 | (0xffffffffu - (uint32_t)(s0 + (int)place - off));
+            if (C > 1) remote_store64(&s.list[at], 0, entry);
+            else s.list[at] = entry;
+        }
+    };
     auto collect_and_draw = [&](uint32_t bound, u64 total_k) {
         // the vectors with such a token first, then one thread for each of their elements
-        for (int i0 = tid; i0 < nv; i0 += 4 * ST) {
-            uint4 v[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = i0 + q * ST < nv ? vecs[i0 + q * ST] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (K::reaches(v[q], bound)) {
-                    const uint32_t at = atomicAdd(&s.vectors, 1u);
-                    if (at < CAP) s.queue[at] = (uint32_t)(i0 + q * ST);
-                }
-        }
+#pragma unroll 2
+        for (int i = tid; i < nv; i += ST)
+            if (K::reaches(vecs[i], bound)) {
+                const uint32_t at = atomicAdd(&s.vectors, 1u);
+                if (at < CAP) s.queue[at] = (uint32_t)i;
+            }
         __syncthreads();
         const uint32_t nq = s.vectors;
         if (nq > CAP) {
             if (tid == 0) {                // more tokens than vectors
-                if (C > 1) remote_add(&s.collected, 0, nq);
-                else s.collected = nq;
+                if (C > 1) remote_add(&s.collected[0], 0, nq);
+                else s.collected[0] = nq;
             }
         } else {
             for (uint32_t i = tid; i < nq * E; i += ST) {
                 const uint32_t place = s.queue[i / E] * E + i % E, key = keys[place];
-                if (key >= bound) {
-                    const uint32_t at = C > 1 ? remote_add(&s.collected, 0, 1) : atomicAdd(&s.collected, 1u);
-                    if (at < CAP) {
-                        const u64 entry = (u64)key << 32 | (0xffffffffu - (uint32_t)(s0 + (int)place - off));
-                        if (C > 1) remote_store64(&s.list[at], 0, entry);
-                        else s.list[at] = entry;
-                    }
-                }
+                if (key >= bound) push(0, key, place);
             }
         }
         join(C);
-        const int nc = (int)(C > 1 ? remote_load32(&s.collected, 0) : s.collected);
+        const int nc = (int)(C > 1 ? remote_load32(&s.collected[0], 0) : s.collected[0]);
         if (nc > CAP) return false;
         if (rank == 0) {
             auto answer = [&](u64 entry, u64 w, u64 total) {
@@ -504,6 +538,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
                 const u64 k_mass = block_sum(in_k && q == 0 ? w : 0, s);     // (masses[] have been read)
                 if (total_k == 0) total_k = k_mass;
                 const u64 tau = max(fraction_of(P, total_k, true), 1ull);
+                const bool enough = k_mass >= tau;
+                if (tid == 0) s.flag = enough;
                 const bool keep = in_k && before < tau && w >= least;
                 if (q == 0 && c < nc && !keep) s.masses[c] = 0;
                 sum = block_sum(keep && q == 0 ? w : 0, s);      // its barriers also order masses[]
@@ -513,7 +549,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
                     if ((uint32_t)s.list[i] > (uint32_t)mine) run += s.masses[i];
                 for (int o = 1; o < part; o <<= 1) run += __shfl_xor_sync(DG_FULL_MASK, run, o);
                 const u64 at = fraction_of(U, sum, false);
-                if (keep && q == 0 && run <= at && at < run + w) answer(mine, w, sum);
+                if (enough && keep && q == 0 && run <= at && at < run + w) answer(mine, w, sum);
             } else {
                 int n2 = 2 * RANKED;
                 while (n2 < nc) n2 *= 2;
@@ -529,6 +565,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
                     u64 sum;
                     const u64 before = part_before(w0 + w1, &sum, n2 / 2, s);
                     const u64 tau = max(fraction_of(P, total_k ? total_k : sum, true), 1ull);
+                    const bool enough = sum >= tau;
+                    if (tid == 0) s.flag = enough;
                     // the kept ones by index, the others behind them
                     if (before + w0 >= tau || w1 < least) w1 = 0;
                     if (before >= tau || w0 < least) w0 = 0;
@@ -541,53 +579,43 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
                     w1 = ~d1 ? mass((uint32_t)d1) : 0;
                     u64 total;
                     const u64 run = part_before(w0 + w1, &total, n2 / 2, s), at = fraction_of(U, total, false);
-                    if (run <= at && at < run + w0 + w1) {
+                    if (enough && run <= at && at < run + w0 + w1) {
                         const bool second = at >= run + w0;
                         answer(0xffffffffu - ((second ? d1 : d0) >> 32), second ? w1 : w0, total);
                     }
                 }
             }
         }
-        if (C > 1) join(C);                // rank 0's counter has been read
-        return true;
+        join(C);                           // rank 0's counter has been read, its verdict is there
+        const bool done = (C > 1 ? remote_load32(&s.flag, 0) : s.flag) != 0;
+        if (C > 1) join(C);
+        return done;
     };
-
-    if (collect && collect_and_draw(max(bound, 1u), 0)) return;
 
     uint32_t cut = 0;                      // kept: key > cut, and the first `ties` with key == cut
     u64 ties = 0;
     if (cut_k || cut_p) {
-        // ---- the cut by counting.  Each pass leaves counts and masses of 256 bins in s.all_*.  Tokens
-        // without mass are left out: they cannot be drawn, so a cut among them is as good as none.
-        const float scale = 255.f / fminf(28.f * tdiv, 3.0e38f);
+        // ---- the cut by counting.  Tokens 28 T or more below the maximum have no mass: they cannot be drawn,
+        // so a cut among them is as good as none, and they are left out.
+        const float span = fminf(28.f * tdiv, 3.0e38f), scale = 255.f / span;
         auto far = [&](uint32_t key) {     // bins of the distance below the maximum; monotone in the key
             const float dist = (m - K::value(key)) * scale;
             return dist < 255.f ? (int)dist : dist == dist ? 255 : 0;
         };
         int buf = 0;
-        auto count = [&](uint32_t lo, uint32_t hi, auto&& bin_of) {
-            each([&](uint32_t key) {
-                if (key < lo || key > hi) return;
-                const int b = bin_of(key);
-                const u64 w = b < 0 ? 0 : mass(key);
-                if (w == 0) return;
-                atomicAdd(&s.hist[0][b], 1u);
-                atomicAdd(&s.hist[1][b], (uint32_t)w & 0x1fffu);
-                atomicAdd(&s.hist[2][b], (uint32_t)(w >> 13) & 0x1fffu);
-                atomicAdd(&s.hist[3][b], (uint32_t)(w >> 26));
-            });
+        // s.hist, counted by each CTA, becomes s.all_* over the cluster
+        auto gather = [&](bool by_mass) {
             __syncthreads();
             if (tid < 256) {
-                const u64 w = (u64)s.hist[1][tid] + ((u64)s.hist[2][tid] << 13) + ((u64)s.hist[3][tid] << 26);
-                if (C > 1) {
-                    s.bin_mass[buf][tid] = w;
-                    s.bin_count[buf][tid] = s.hist[0][tid];
-                } else {
-                    s.all_mass[tid] = w;
-                    s.all_count[tid] = s.hist[0][tid];
+                const uint32_t c = s.hist[0][tid];
+                u64 w = 0;
+                s.hist[0][tid] = 0;
+                if (by_mass) {
+                    w = (u64)s.hist[1][tid] + ((u64)s.hist[2][tid] << 13) + ((u64)s.hist[3][tid] << 26);
+                    s.hist[1][tid] = s.hist[2][tid] = s.hist[3][tid] = 0;
                 }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) s.hist[q][tid] = 0;
+                if (C > 1) s.bin_mass[buf][tid] = w, s.bin_count[buf][tid] = c;
+                else s.all_mass[tid] = w, s.all_count[tid] = c;
             }
             join(C);
             if (C > 1) {
@@ -599,7 +627,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
                     const int from = 2 * r + (tid & 1);
-                    rw[r] = from < C ? remote_load64(&s.bin_mass[buf][b], from) : 0;
+                    rw[r] = by_mass && from < C ? remote_load64(&s.bin_mass[buf][b], from) : 0;
                     rc[r] = from < C ? remote_load32(&s.bin_count[buf][b], from) : 0;
                 }
 #pragma unroll
@@ -612,100 +640,244 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
             buf ^= 1;
         };
         // the bin in which the running count or mass (from `count0`, `mass0`) reaches the target, and the
-        // running values before it; every warp for itself, lane l: bins 8 l to 8 l + 7
-        auto crossing = [&](bool by_mass, u64 target, u64& count0, u64& mass0) {
-            u64 sc = 0, sw = 0;
+        // running values before it; false where it does not.  One warp looks, lane l at bins 8 l to 8 l + 7.
+        auto crossing = [&](bool by_mass, u64 target, u64& count0, u64& mass0, int& bin_out) {
+            if (warp == 0) {
+                uint32_t c[8], sc = 0;
+                u64 w[8], sw = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sc += s.all_count[8 * lane + i], sw += s.all_mass[8 * lane + i];
-            const u64 ic = warp_scan(sc, lane) + count0, iw = warp_scan(sw, lane) + mass0;
-            const unsigned hit = __ballot_sync(DG_FULL_MASK, (by_mass ? iw : ic) >= target);
-            u64 c = ic - sc, w = iw - sw;
-            int bin = 8 * lane;
-            for (int i = 0; i < 7; ++i) {
-                const u64 nc = c + s.all_count[8 * lane + i], nw_ = w + s.all_mass[8 * lane + i];
-                if ((by_mass ? nw_ : nc) >= target) break;
-                c = nc, w = nw_, ++bin;
+                for (int i = 0; i < 8; ++i) {
+                    c[i] = s.all_count[8 * lane + i], sc += c[i];
+                    w[i] = by_mass ? s.all_mass[8 * lane + i] : 0, sw += w[i];
+                }
+                u64 rc = warp_scan(sc, lane) + count0, rw = warp_scan(sw, lane) + mass0;
+                const unsigned hit = __ballot_sync(DG_FULL_MASK, (by_mass ? rw : rc) >= target);
+                if (hit && lane == __ffs(hit) - 1) {
+                    rc -= sc;
+                    rw -= sw;
+                    int bin = 8 * lane;
+#pragma unroll
+                    for (int i = 0; i < 7; ++i)
+                        if (bin == 8 * lane + i && (by_mass ? rw + w[i] : rc + c[i]) < target) rc += c[i], rw += w[i], ++bin;
+                    s.cross[0] = (u64)bin, s.cross[1] = rc, s.cross[2] = rw;
+                }
+                if (!hit && lane == 0) s.cross[0] = ~0ull;
             }
-            const int at = hit ? __ffs(hit) - 1 : 31;
-            count0 = __shfl_sync(DG_FULL_MASK, c, at);
-            mass0 = __shfl_sync(DG_FULL_MASK, w, at);
-            return __shfl_sync(DG_FULL_MASK, bin, at);
+            __syncthreads();
+            const u64 b = s.cross[0];
+            if (b == ~0ull) return false;
+            bin_out = (int)b;
+            count0 = s.cross[1];
+            mass0 = s.cross[2];
+            return true;
         };
-        // within bin `first` of the distance: the one key in which the target is reached, the running values
-        // before it, and how many tokens have it
-        auto narrow = [&](bool by_mass, u64 target, int first, u64& count0, u64& mass0, uint32_t& here) {
-            // keys that surely hold the bin's, rounding errors of m and the distance included; only those
-            // in the bin are counted
-            const float edge = (float)(first + 1) / scale, fuzz = 1e-6f * (edge + fabsf(m));
-            const uint32_t a = K::near(m - edge - fuzz), b = K::near(m - (float)first / scale + fuzz);
-            uint32_t lo = first == 255 || a <= 2 ? 1 : a - 2;
-            uint32_t hi = first == 0 ? (uint32_t)mx : min((uint32_t)mx, b + 2);
-            while (true) {
-                int shift = 0;
+        // keys that surely hold bins [blo, bhi], rounding errors of m and the distance included
+        auto lowest = [&](int b) {
+            const float edge = (float)(b + 1) / scale, fuzz = 1e-6f * (edge + fabsf(m));
+            const uint32_t a = K::near(m - edge - fuzz);
+            return a <= 2 ? 1u : a - 2;
+        };
+        auto highest = [&](int b) {
+            const float edge = (float)b / scale, fuzz = 1e-6f * (edge + fabsf(m));
+            return b == 0 ? (uint32_t)mx : min((uint32_t)mx, K::near(m - edge + fuzz) + 2);
+        };
+
+        // The cut: the token at which the count or mass reaches the target, expected in bins [blo, bhi] with
+        // `count0` tokens before them.  Leaves cut and ties, and returns false where the target is not in
+        // those bins.
+        int uses = 0, sums = 0;
+        auto resolve = [&](bool by_mass, u64 target, int blo, int bhi, u64 count0) {
+            uint32_t lo = lowest(bhi), hi = highest(blo);
+            u64 mass0 = 0;
+            for (int level = 0;; ++level) {
+                int shift = 0, bin;
                 while (((hi - lo) >> shift) > 255) ++shift;
-                __syncthreads();           // s.all_* have been read
-                count(lo, hi, [&](uint32_t key) { return far(key) == first ? (int)((hi - key) >> shift) : -1; });
-                const int bin = crossing(by_mass, target, count0, mass0);
-                here = s.all_count[bin];
+                u64 above = 0;
+                const uint32_t to = by_mass && level == 0 ? 0xffffffffu : hi;      // above the range: exact mass, once
+                each(by_mass, [&](uint32_t key, u64 w) {
+                    if (key < lo || key > to) return;
+                    const int b = key > hi ? -1 : far(key);
+                    if (b < blo) above += w;
+                    if (b < blo || b > bhi) return;
+                    const int at = (int)((hi - key) >> shift);
+                    atomicAdd(&s.hist[0][at], 1u);
+                    if (by_mass) {
+                        atomicAdd(&s.hist[1][at], (uint32_t)w & 0x1fffu);
+                        atomicAdd(&s.hist[2][at], (uint32_t)(w >> 13) & 0x1fffu);
+                        atomicAdd(&s.hist[3][at], (uint32_t)(w >> 26));
+                    }
+                });
+                if (by_mass && level == 0) {
+                    above = block_sum(above, s);
+                    if (tid == 0) s.post[8 + sums] = above;        // read after the barrier in gather
+                }
+                gather(by_mass);
+                if (by_mass && level == 0) {
+                    if (C > 1) above = warp_sum(lane < C ? remote_load64(&s.post[8 + sums], lane) : 0);
+                    ++sums;
+                    mass0 = above;
+                    if (mass0 >= target) return false;
+                }
+                if (!crossing(by_mass, target, count0, mass0, bin)) return false;
+                const uint32_t here = s.all_count[bin];
                 const uint32_t top = hi - ((uint32_t)bin << shift), bottom = top - ((1u << shift) - 1);
                 lo = bottom > lo && bottom <= top ? bottom : lo;
                 hi = top;
-                if (shift == 0 || lo >= hi) return hi;
+                if (shift == 0 || lo == hi) {
+                    // one key: as many of its tokens as the target asks for
+                    const u64 w = mass(hi);
+                    cut = hi;
+                    ties = by_mass ? (target - mass0 + w - 1) / w : target - count0;
+                    if (ties == here) --cut, ties = 0;             // all of them: simply the keys above
+                    return true;
+                }
+                if (here <= RANKED) break;
+                __syncthreads();           // s.all_* have been read
             }
-        };
-        count(1, (uint32_t)mx, far);
-        u64 total_k = 0, tokens = 0, kc = 0, kw = 0, pc = 0, pw = 0;
+            // few tokens: ranked in one CTA
+            const int counter = 1 + uses++;
+            for (int i = tid; i < nw; i += ST) {
+                const uint32_t w = words[i];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) total_k += s.all_mass[8 * lane + i], tokens += s.all_count[8 * lane + i];
-        total_k = warp_sum(total_k);
-        tokens = warp_sum(tokens);
-        const bool by_k = cut_k && (u64)k < tokens;
-        uint32_t here = 0;
-        int kbin = 0, pbin = 0;
-        if (by_k) {
-            kbin = crossing(false, (u64)k, kc, kw);
-        } else if (cut_p) {
-            const u64 tau = max(fraction_of(P, total_k, true), 1ull);
-            pbin = crossing(true, tau, pc, pw);
-            const u64 reached = pc + s.all_count[pbin];
-            if (reached <= CAP && tau < total_k && !collect) {
-                // few tokens down to the cut: draw from them (a key below the bin's lowest does no harm)
-                const float edge = (float)(pbin + 1) / scale, fuzz = 1e-6f * (edge + fabsf(m));
-                const uint32_t a = K::near(m - edge - fuzz);
-                if (pbin < 255 && collect_and_draw(a <= 2 ? 1 : a - 2, total_k)) return;
-            }
-        }
-        if (by_k) {
-            // top_p's share is known once the k-th key is: keep the first pass's bins for it
-            if (cut_p) {
-                __syncthreads();
-                if (tid < 256) s.list[tid] = s.all_mass[tid], s.list[256 + tid] = s.all_count[tid];
-                __syncthreads();
-            }
-            cut = narrow(false, (u64)k, kbin, kc, kw, here);
-            ties = (u64)k - kc;
-            total_k = kw + ties * mass(cut);
-            if (ties == here) --cut, ties = 0;         // all of them: simply the keys above
-            if (cut_p) {
-                const u64 tau = max(fraction_of(P, total_k, true), 1ull);
-                if (tau < total_k) {
-                    __syncthreads();
-                    if (tid < 256) s.all_mass[tid] = s.list[tid], s.all_count[tid] = (uint32_t)s.list[256 + tid];
-                    __syncthreads();
-                    pbin = crossing(true, tau, pc, pw);
-                    cut = narrow(true, tau, pbin, pc, pw, here);
-                    const u64 w = mass(cut);
-                    ties = (tau - pw + w - 1) / w;
-                    if (ties == here) --cut, ties = 0;
+                for (int e = 0; e < W; ++e) {
+                    const uint32_t key = K::at(w, e);
+                    if (key < lo || key > hi) continue;
+                    const int b = far(key);
+                    if (b >= blo && b <= bhi) push(counter, key, (uint32_t)(i * W + e));
                 }
             }
-        } else if (cut_p) {
-            const u64 tau = max(fraction_of(P, total_k, true), 1ull);
-            if (tau < total_k) {
-                cut = narrow(true, tau, pbin, pc, pw, here);
-                const u64 w = mass(cut);
-                ties = (tau - pw + w - 1) / w;
-                if (ties == here) --cut, ties = 0;
+            join(C);
+            if (rank == 0) {
+                const int nc = (int)s.collected[counter];
+                const int c = tid >> 1, q = tid & 1;               // two threads to a token
+                const u64 mine = c < nc ? s.list[c] : 0;
+                const u64 w = c < nc ? mass((uint32_t)(mine >> 32)) : 0;
+                if (q == 0 && c < nc) s.masses[c] = w;
+                __syncthreads();
+                uint32_t rank_ = 0, over = 0, same = 0;
+                u64 before = 0;
+#pragma unroll 4
+                for (int i = q; i < nc; i += 2) {
+                    const u64 e = s.list[i], we = s.masses[i];
+                    if (e > mine) ++rank_, before += we;
+                    over += e >> 32 > mine >> 32;
+                    same += e >> 32 == mine >> 32;
+                }
+                rank_ += __shfl_xor_sync(DG_FULL_MASK, rank_, 1);
+                over += __shfl_xor_sync(DG_FULL_MASK, over, 1);
+                same += __shfl_xor_sync(DG_FULL_MASK, same, 1);
+                before += __shfl_xor_sync(DG_FULL_MASK, before, 1);
+                const bool it = by_mass ? mass0 + before < target && mass0 + before + w >= target
+                                        : count0 + rank_ + 1 == target;
+                if (c < nc && q == 0 && it) {
+                    const uint32_t n = rank_ - over + 1;           // of its key, this many
+                    s.post[12] = (u64)(n == same ? (uint32_t)(mine >> 32) - 1 : (uint32_t)(mine >> 32)) << 32 | (n == same ? 0 : n);
+                }
+            }
+            join(C);
+            const u64 answer = C > 1 ? remote_load64(&s.post[12], 0) : s.post[12];
+            cut = (uint32_t)(answer >> 32);
+            ties = answer & 0xffffffffu;
+            join(C);                       // the slots have been read, the list too
+            return true;
+        };
+
+        // The steps, each of whose pieces stands here once: draw from collected tokens (`from`: the key they
+        // reach, or 0), count, cut by top_k, cut by top_p in the bins near a guess, cut by top_p anywhere.
+        uint32_t from = collect ? max(bound, 1u) : 0;
+        u64 total_k = 0, tau = 0, c0 = 0;
+        int blo = 0, bhi = 0;
+        enum { COUNT, TOP_K, GUESS, TOP_P, ANYWHERE, DONE };
+#pragma unroll 1
+        for (int step = COUNT; step != DONE;) {
+            if (from) {
+                if (collect_and_draw(from, total_k)) return;
+                from = 0;
+            }
+            if (step == COUNT) {
+                // counts of all tokens, and the mass where top_k does not limit it
+                u64 all = 0;
+                each(!cut_k, [&](uint32_t key, u64 w) {
+                    const int b = far(key);
+                    if (key == 0 || b == 255) return;
+                    atomicAdd(&s.hist[0][b], 1u);
+                    all += w;
+                });
+                all = block_sum(all, s);
+                if (tid == 0) s.post[6] = all;
+                gather(false);
+                total_k = C > 1 ? warp_sum(lane < C ? remote_load64(&s.post[6], lane) : 0) : all;
+                if (tid < 256) s.far_count[tid] = s.all_count[tid];
+                step = cut_k ? TOP_K : GUESS;
+                if (cut_k) {
+                    u64 w0 = 0;
+                    if (!crossing(false, (u64)k, c0, w0, blo)) step = GUESS;
+                    bhi = blo;
+                }
+            }
+            if (step == GUESS) {
+                if (!cut_p) break;
+                if (cut_k) {               // (the cut has not summed what lies above its bin)
+                    u64 w = 0;
+                    each(true, [&](uint32_t key, u64 v) { w += key > cut ? v : 0; });
+                    w = block_sum(w, s);
+                    if (C > 1) w = warp_sum(over_cluster(w, 7, C, s));
+                    total_k = w + (ties ? ties * mass(cut) : 0);
+                }
+                tau = max(fraction_of(P, total_k, true), 1ull);
+                if (tau >= total_k) break;
+                __syncthreads();
+                // nearly where the mass reaches tau: counts times the mass at the middle of each bin
+                if (warp == 0) {
+                    float v[8], sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int b = 8 * lane + i;
+                        v[i] = b < 255 ? (float)s.far_count[b] * __expf(-((float)b + 0.5f) * (28.f / 255.f)) : 0.f;
+                        sum += v[i];
+                    }
+                    float run = sum;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const float x = __shfl_up_sync(DG_FULL_MASK, run, o);
+                        if (lane >= o) run += x;
+                    }
+                    const float want = (float)tau * (1.f / 1099511627776.f);
+                    const unsigned hit = __ballot_sync(DG_FULL_MASK, run >= want);
+                    if (lane == (hit ? __ffs(hit) - 1 : 31)) {
+                        run -= sum;
+                        int b = 8 * lane;
+#pragma unroll
+                        for (int i = 0; i < 7; ++i)
+                            if (b == 8 * lane + i && run + v[i] < want) run += v[i], ++b;
+                        s.cross[0] = (u64)min(b, 254);
+                    }
+                }
+                __syncthreads();
+                const int guess = (int)s.cross[0];
+                blo = max(guess - 1, 0);
+                bhi = min(guess + 1, 254);
+                uint32_t upto = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (8 * lane + i <= bhi) upto += s.far_count[8 * lane + i];
+                upto = __reduce_add_sync(DG_FULL_MASK, upto);
+                step = TOP_P;
+                // few tokens down to there: draw from them (a key below the bin's lowest does no harm)
+                if (!cut_k && upto <= RANKED) {
+                    from = lowest(bhi);
+                    continue;
+                }
+            }
+            const bool by_mass = step != TOP_K;
+            const bool found = resolve(by_mass, by_mass ? tau : (u64)k, blo, bhi, c0);
+            if (step == TOP_K) {
+                step = GUESS;
+            } else if (step == TOP_P && !found) {
+                step = ANYWHERE;
+                blo = 0, bhi = 254;
+            } else {
+                step = DONE;
             }
         }
     }
@@ -725,28 +897,40 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(SampleParams p) {
     // f(word index, the masses of this lane's keys in it) over words [a, b) in index order, `seen` tokens with
     // the cut key before them
     auto walk = [&](int a, int b, uint32_t seen, auto&& f) {
-#pragma unroll 2
-        for (int base = a; base < b; base += 32) {
-            const int i = base + lane;
-            const uint32_t word = i < b ? words[i] : 0;
-            u64 w[W];
-            uint32_t t = seen;
-            if (ties) {
+#pragma unroll 1
+        for (int base = a; base < b; base += 32 * GROUP) {
+            uint32_t word[GROUP];
+            float l[GROUP * W];
+            u64 w[GROUP * W];
+#pragma unroll
+            for (int q = 0; q < GROUP; ++q) {
+                const int i = base + 32 * q + lane;
+                word[q] = i < b ? words[i] : 0;
+#pragma unroll
+                for (int e = 0; e < W; ++e) l[q * W + e] = K::value(K::at(word[q], e));
+            }
+            mass_of.of(l, w);
+#pragma unroll
+            for (int q = 0; q < GROUP; ++q) {
+                uint32_t t = seen;
+                if (ties) {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const unsigned is = __ballot_sync(DG_FULL_MASK, K::at(word[q], e) == cut);
+                        t += __popc(is & ((1u << lane) - 1));
+                        seen += __popc(is);
+                    }
+                }
+                u64 v[W];
 #pragma unroll
                 for (int e = 0; e < W; ++e) {
-                    const unsigned is = __ballot_sync(DG_FULL_MASK, K::at(word, e) == cut);
-                    t += __popc(is & ((1u << lane) - 1));
-                    seen += __popc(is);
+                    const uint32_t key = K::at(word[q], e);
+                    v[e] = key > cut || (key && key == cut && t < ties) ? w[q * W + e] : 0;
+                    t += key == cut;
+                    if (v[e] < least) v[e] = 0;
                 }
+                f(base + 32 * q + lane, v);
             }
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                const uint32_t key = K::at(word, e);
-                w[e] = key > cut || (key == cut && t < ties) ? mass(key) : 0;
-                t += key == cut;
-                if (w[e] < least) w[e] = 0;
-            }
-            f(i, w);
         }
     };
     auto sum_of = [&](int a, int b, uint32_t seen) {
@@ -832,7 +1016,7 @@ template <typename T> int run(SampleParams p, int B, cudaStream_t stream) {
     p.slice = ((p.V + p.cluster - 1) / p.cluster + 7) / 8 * 8;
     if ((int64_t)B * p.cluster > 0x7fffffff) return DG_ERR_UNSUPPORTED;
     const size_t smem = (size_t)(p.slice + 16) * sizeof(T) + 16;
-    auto kern = sample_kernel<T>;
+    auto kern = p.cluster == 1 ? sample_kernel<T, true> : sample_kernel<T, false>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return dg_host::record_cuda_error(e);
     if (p.cluster == 1) {
