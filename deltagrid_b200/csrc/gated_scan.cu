@@ -686,10 +686,11 @@ int width_of(int D, size_t elem, std::initializer_list<Row> rows) {
     return units % (int64_t)(16 / elem) || bytes % 16 ? 1 : 2;
 }
 
-// Channels per CTA (lpr x vec) and cluster size: the least work of the busiest SM, CTAs on it x
-// walked steps x channels.  Clusters fill some SMs before others, so the busiest has `occ` of their
-// CTAs.  An SM with a single CTA waits at its barriers (1.5 x its work here); larger clusters and
-// narrower rows cost a little more, which also decides ties.
+// Channels per CTA (lpr x vec) and cluster size, by the work of the busiest SM: CTAs on it x walked steps x
+// lanes, a half of 2048 more for each tile walked and almost two for each wave of CTAs.  Clusters fill some
+// SMs before others, so their SMs count as full; an SM with a single CTA waits at its barriers (1.5 x its
+// work).  Larger clusters and narrower rows cost a little more.  Measured, forward: 2 x 300 x 512 lpr 32
+// cluster 5 4.3 us, none 8.2; 8 x 4096 x 768 cluster 4 55 us, 2 77; 32 x 2048 x 1024 cluster 2 112 us, 8 152.
 struct Shape {
     int lpr, cluster;
 };
@@ -706,10 +707,12 @@ Shape shape_of(int B, int T, int D, int vec, int steps_per_thread, int occ, bool
         const int64_t units = (int64_t)B * ((D + lpr * vec - 1) / (lpr * vec));
         const int steps = THREADS / lpr * steps_per_thread, tiles = (T + steps - 1) / steps;
         for (int s = 1; s <= 16 && (s == 1 || s <= tiles); ++s) {
-            const int64_t waves = (units + kClusters[occ - 1][s - 1] - 1) / kClusters[occ - 1][s - 1];
-            const int64_t per_sm = (units * s + 147) / 148;
-            double cost = waves > 1 || (s > 1 && units * s > 148) ? (double)waves * occ : per_sm > 1 ? (double)per_sm : 1.5;
-            cost *= (double)((tiles + s - 1) / s) * steps * lpr * (1.0 + 0.01 * s + (lpr < 32 ? 0.04 : 0.0));
+            const int64_t slots = kClusters[occ - 1][s - 1], n = units * s, per_sm = (n + 147) / 148;
+            const double waves = units <= slots ? 1.0 : (double)units / slots + 0.35;
+            const double share = waves > 1.0 || (s > 1 && n > 148) ? waves * occ : per_sm > 1 ? (double)per_sm : 1.5;
+            const double walked = (double)((tiles + s - 1) / s);
+            const double cost = share * walked * steps * lpr * (1.0 + 0.01 * s + (lpr < 32 ? 0.04 : 0.0)) +
+                                waves * (1000.0 * walked + 3600.0);
             if (least < 0 || cost < least) {
                 least = cost;
                 best = {lpr, s};
