@@ -17,7 +17,9 @@
 //      times the mass at a bin's middle.  Then only keys near the cut are counted again,
 //      finer, with their exact masses, beside the exact mass of all above them; the few tokens
 //      of the bin that holds the cut are ranked in one CTA.  Two walks over the keys in index
-//      order draw the token.  Without a cut (no top_k, no top_p) only the walks are needed.
+//      order draw the token.  Where a row has a cluster, what a cut leaves is copied together
+//      first, in index order, for the steps after it.  Without a cut (no top_k, no top_p) only
+//      the walks are needed.
 //
 // What bounds it: not the 64 KB of a bf16 row of 32000 (2.5 us for 256 rows) but the latency
 // of the steps after it, some fifteen barriers of up to 512 threads; two CTAs share an SM.
@@ -34,7 +36,7 @@ typedef unsigned long long u64;
 struct SampleParams {
     const void* logits;
     int64_t row_stride;
-    int V, slice, cluster;
+    int V, slice, cluster, room;           // room: tokens that can be copied together
     const float* u;
     const float *temperature, *top_p, *min_p;
     const int32_t* top_k;
@@ -49,7 +51,7 @@ struct SampleParams {
 // marks places outside the row.
 template <typename T> struct Key {         // 16-bit logits, two to a word
     typedef uint16_t type;
-    static constexpr int BITS = 16, PER = 2;
+    static constexpr int BITS = 16;
     static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     // NaN -> -inf (the larger of the two that is a number), -0 -> +0
     __device__ static __forceinline__ uint32_t clean(uint32_t x) {
@@ -87,8 +89,7 @@ template <typename T> struct Key {         // 16-bit logits, two to a word
         const uint16_t h = (uint16_t)b;
         return __half2float(*reinterpret_cast<const __half*>(&h));
     }
-    // key `e` of a word, and the larger of its two
-    __device__ static __forceinline__ uint32_t at(uint32_t w, int e) { return e ? w >> 16 : w & 0xffffu; }
+    // the larger key of a word
     __device__ static __forceinline__ uint32_t most(uint32_t w) { return max(w >> 16, w & 0xffffu); }
     __device__ static __forceinline__ uint32_t larger_key(uint32_t a, uint32_t b) {       // of both halves
         uint32_t r;
@@ -105,7 +106,7 @@ template <typename T> struct Key {         // 16-bit logits, two to a word
 };
 template <> struct Key<float> {
     typedef uint32_t type;
-    static constexpr int BITS = 32, PER = 1;
+    static constexpr int BITS = 32;
     static constexpr uint32_t NONE = 0xff800000u;
     __device__ static __forceinline__ uint32_t clean(uint32_t x) {
         return __float_as_uint(fmaxf(__uint_as_float(x), -INFINITY) + 0.f);
@@ -118,7 +119,6 @@ template <> struct Key<float> {
     __device__ static __forceinline__ float value(uint32_t k) {
         return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
     }
-    __device__ static __forceinline__ uint32_t at(uint32_t w, int) { return w; }
     __device__ static __forceinline__ uint32_t most(uint32_t w) { return w; }
     __device__ static __forceinline__ bool reaches(const uint4& v, uint32_t bound) {
         return max(max(v.x, v.y), max(v.z, v.w)) >= bound;
@@ -313,15 +313,13 @@ __device__ __forceinline__ void sort_list(u64* list, int n2, bool descending) {
 // registers for independent chains.
 template <typename T, bool MANY>
 __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p) {
-    constexpr int GROUP = (MANY ? 4 : 8) / Key<T>::PER;
+    constexpr int GROUP = MANY ? 4 : 8;
     typedef Key<T> K;
     typedef typename K::type key_t;
     constexpr int E = 16 / sizeof(T);
-    constexpr int W = K::PER;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Shared s;
     uint4* vecs = reinterpret_cast<uint4*>(smem);
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(smem);
     key_t* keys = reinterpret_cast<key_t*>(smem);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int C = p.cluster, rank = C > 1 ? (int)cluster_rank() : 0, row = blockIdx.x / C;
@@ -337,7 +335,6 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
     // vectors of the table, zeros around the slice
     const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / (int)sizeof(T), n);
     const int off = (E - head % E) % E, nv = (off + n + E - 1) / E, body = (n - head) / E, v0 = (off + head) / E;
-    const int nw = nv * 4;                 // words
     uint32_t top0 = K::NONE, top1 = K::NONE;       // largest values of this thread's even and odd vectors
     if (tid < 4 * 256) (&s.hist[0][0])[tid] = (&s.hist[0][0])[tid + ST] = 0;
     if (tid == 0) s.vectors = s.collected[0] = s.collected[1] = s.collected[2] = 0;
@@ -450,27 +447,56 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
         mass_of.of(l, w);
         return w[0];
     };
-    // f(key, mass or 0) for the keys of this CTA's words, any order, GROUP words of a thread at a time
+    // The tokens that the steps look at: the whole table or, once `dense`, those copied together behind it
+    uint32_t* copied_key = reinterpret_cast<uint32_t*>(vecs + nv);
+    uint32_t* copied_place = copied_key + p.room;
+    bool dense = false;
+    int count_of = nv * E;
+    auto key_at = [&](int i) { return dense ? copied_key[i] : (uint32_t)keys[i]; };
+    auto place_at = [&](int i) { return dense ? copied_place[i] : (uint32_t)i; };
+    // f(key, mass or 0) for all of them, any order, GROUP of a thread at a time
     auto each = [&](bool with_mass, auto&& f) {
 #pragma unroll 1
-        for (int i = tid; i < nw; i += GROUP * ST) {
-            uint32_t key[GROUP * W];
-            u64 w[GROUP * W] = {};
+        for (int i = tid; i < count_of; i += GROUP * ST) {
+            uint32_t key[GROUP];
+            u64 w[GROUP] = {};
 #pragma unroll
-            for (int q = 0; q < GROUP; ++q) {
-                const uint32_t word = i + q * ST < nw ? words[i + q * ST] : 0;
-#pragma unroll
-                for (int e = 0; e < W; ++e) key[q * W + e] = K::at(word, e);
-            }
+            for (int q = 0; q < GROUP; ++q) key[q] = i + q * ST < count_of ? key_at(i + q * ST) : 0;
             if (with_mass) {
-                float l[GROUP * W];
+                float l[GROUP];
 #pragma unroll
-                for (int q = 0; q < GROUP * W; ++q) l[q] = K::value(key[q]);
+                for (int q = 0; q < GROUP; ++q) l[q] = K::value(key[q]);
                 mass_of.of(l, w);
             }
 #pragma unroll
-            for (int q = 0; q < GROUP * W; ++q) f(key[q], w[q]);
+            for (int q = 0; q < GROUP; ++q) f(key[q], w[q]);
         }
+    };
+    // copies the tokens whose keys reach `lo` together, in index order, where there is room for them
+    auto copy_together = [&](uint32_t lo) {
+        if (p.room == 0 || dense) return;
+        const int piece = (count_of + WARPS - 1) / WARPS, a = min(warp * piece, count_of), b = min(a + piece, count_of);
+        uint32_t c = 0;
+        for (int i = a + lane; i < b; i += 32) c += keys[i] >= lo;
+        c = __reduce_add_sync(DG_FULL_MASK, c);
+        u64 n;
+        uint32_t at = (uint32_t)block_before(lane == 0 ? c : 0, &n, s);
+        if (n > (u64)p.room) return;
+        at = __shfl_sync(DG_FULL_MASK, at, 0);
+        for (int base = a; base < b; base += 32) {
+            const int i = base + lane;
+            const uint32_t key = i < b ? (uint32_t)keys[i] : 0;
+            const unsigned is = __ballot_sync(DG_FULL_MASK, key >= lo);
+            if (key >= lo) {
+                const uint32_t to = at + __popc(is & ((1u << lane) - 1));
+                copied_key[to] = key;
+                copied_place[to] = (uint32_t)i;
+            }
+            at += __popc(is);
+        }
+        __syncthreads();
+        dense = true;
+        count_of = (int)n;
     };
 
     // ---- collect the tokens that reach `bound`, and draw from them: thread t of the CTA that holds the
@@ -736,15 +762,11 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
             }
             // few tokens: ranked in one CTA
             const int counter = 1 + uses++;
-            for (int i = tid; i < nw; i += ST) {
-                const uint32_t w = words[i];
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    const uint32_t key = K::at(w, e);
-                    if (key < lo || key > hi) continue;
-                    const int b = far(key);
-                    if (b >= blo && b <= bhi) push(counter, key, (uint32_t)(i * W + e));
-                }
+            for (int i = tid; i < count_of; i += ST) {
+                const uint32_t key = key_at(i);
+                if (key < lo || key > hi) continue;
+                const int b = far(key);
+                if (b >= blo && b <= bhi) push(counter, key, place_at(i));
             }
             join(C);
             if (rank == 0) {
@@ -863,6 +885,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                     if (8 * lane + i <= bhi) upto += s.far_count[8 * lane + i];
                 upto = __reduce_add_sync(DG_FULL_MASK, upto);
                 step = TOP_P;
+                if (!cut_k && upto > RANKED && bhi < 254) copy_together(lowest(bhi));
                 // few tokens down to there: draw from them (a key below the bin's lowest does no harm)
                 if (!cut_k && upto <= RANKED) {
                     from = lowest(bhi);
@@ -873,75 +896,58 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
             const bool found = resolve(by_mass, by_mass ? tau : (u64)k, blo, bhi, c0);
             if (step == TOP_K) {
                 step = GUESS;
+                copy_together(ties ? cut : cut + 1);
             } else if (step == TOP_P && !found) {
                 step = ANYWHERE;
                 blo = 0, bhi = 254;
+                if (!cut_k) dense = false, count_of = nv * E;
             } else {
                 step = DONE;
             }
         }
     }
 
-    // ---- the draw in index order: each warp walks a contiguous piece of the words
-    const int piece = (nw + WARPS - 1) / WARPS;
-    // tokens with the cut key in words [a, b), by one warp
+    // ---- the draw in index order: each warp walks a contiguous piece of the tokens
+    const int piece = (count_of + WARPS - 1) / WARPS;
+    // tokens with the cut key in [a, b), by one warp
     auto ties_in = [&](int a, int b) {
         uint32_t c = 0;
-        for (int i = a + lane; i < b; i += 32) {
-            const uint32_t w = words[i];
-#pragma unroll
-            for (int e = 0; e < W; ++e) c += K::at(w, e) == cut;
-        }
+        for (int i = a + lane; i < b; i += 32) c += key_at(i) == cut;
         return __reduce_add_sync(DG_FULL_MASK, c);
     };
-    // f(word index, the masses of this lane's keys in it) over words [a, b) in index order, `seen` tokens with
-    // the cut key before them
+    // f(token, its mass or 0) over [a, b) in index order, a token to a lane, `seen` tokens with the cut key
+    // before them
     auto walk = [&](int a, int b, uint32_t seen, auto&& f) {
 #pragma unroll 1
         for (int base = a; base < b; base += 32 * GROUP) {
-            uint32_t word[GROUP];
-            float l[GROUP * W];
-            u64 w[GROUP * W];
+            uint32_t key[GROUP];
+            float l[GROUP];
+            u64 w[GROUP];
 #pragma unroll
             for (int q = 0; q < GROUP; ++q) {
                 const int i = base + 32 * q + lane;
-                word[q] = i < b ? words[i] : 0;
-#pragma unroll
-                for (int e = 0; e < W; ++e) l[q * W + e] = K::value(K::at(word[q], e));
+                key[q] = i < b ? key_at(i) : 0;
+                l[q] = K::value(key[q]);
             }
             mass_of.of(l, w);
 #pragma unroll
             for (int q = 0; q < GROUP; ++q) {
-                uint32_t t = seen;
+                bool in = key[q] > cut;
                 if (ties) {
-#pragma unroll
-                    for (int e = 0; e < W; ++e) {
-                        const unsigned is = __ballot_sync(DG_FULL_MASK, K::at(word[q], e) == cut);
-                        t += __popc(is & ((1u << lane) - 1));
-                        seen += __popc(is);
-                    }
+                    const unsigned is = __ballot_sync(DG_FULL_MASK, key[q] == cut);
+                    in |= key[q] == cut && seen + __popc(is & ((1u << lane) - 1)) < ties;
+                    seen += __popc(is);
                 }
-                u64 v[W];
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    const uint32_t key = K::at(word[q], e);
-                    v[e] = key > cut || (key && key == cut && t < ties) ? w[q * W + e] : 0;
-                    t += key == cut;
-                    if (v[e] < least) v[e] = 0;
-                }
-                f(base + 32 * q + lane, v);
+                f(base + 32 * q + lane, in && w[q] >= least ? w[q] : 0);
             }
         }
     };
     auto sum_of = [&](int a, int b, uint32_t seen) {
         u64 v = 0;
-        walk(a, b, seen, [&](int, const u64 (&w)[W]) {
-#pragma unroll
-            for (int e = 0; e < W; ++e) v += w[e];
-        });
+        walk(a, b, seen, [&](int, u64 w) { v += w; });
         return warp_sum(v);
     };
-    int a0 = min(warp * piece, nw), a1 = min(a0 + piece, nw);
+    int a0 = min(warp * piece, count_of), a1 = min(a0 + piece, count_of);
     uint32_t seen = 0;
     if (ties) {
         const uint32_t c = ties_in(a0, a1);
@@ -970,7 +976,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
     // the CTA whose keys hold the draw: all its warps share the piece that does
     if (lane == 0 && start <= at && at < start + mine) s.flag = (uint32_t)warp, s.post[6] = start, s.post[7] = seen;
     __syncthreads();
-    const int base = min((int)s.flag * piece, nw), last = min(base + piece, nw), part = ((last - base + WARPS - 1) / WARPS + 31) / 32 * 32;
+    const int base = min((int)s.flag * piece, count_of), last = min(base + piece, count_of), part = ((last - base + WARPS - 1) / WARPS + 31) / 32 * 32;
     start = s.post[6];
     seen = (uint32_t)s.post[7];
     a0 = min(base + warp * part, last), a1 = min(a0 + part, last);
@@ -986,15 +992,11 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
     start += __shfl_sync(DG_FULL_MASK, before, 0);
     if (start <= at && at < start + mine) {
         u64 run = start;
-        walk(a0, a1, seen, [&](int i, const u64 (&w)[W]) {
-            u64 sum = 0;
-#pragma unroll
-            for (int e = 0; e < W; ++e) sum += w[e];
-            const u64 inc = warp_scan(sum, lane), r = run + inc - sum;
-            if (r <= at && at < r + sum) {
-                const int e = W > 1 && at >= r + w[0] ? 1 : 0;
-                p.token[row] = (int64_t)s0 + i * W + e - off;
-                if (p.logprob) p.logprob[row] = logf(__fdiv_rn((float)w[e ? W - 1 : 0], (float)total));
+        walk(a0, a1, seen, [&](int i, u64 w) {
+            const u64 inc = warp_scan(w, lane), r = run + inc - w;
+            if (r <= at && at < r + w) {
+                p.token[row] = (int64_t)s0 + (int)place_at(i) - off;
+                if (p.logprob) p.logprob[row] = logf(__fdiv_rn((float)w, (float)total));
             }
             run += __shfl_sync(DG_FULL_MASK, inc, 31);
         });
@@ -1015,7 +1017,13 @@ template <typename T> int run(SampleParams p, int B, cudaStream_t stream) {
     p.cluster = cluster_of(B, p.V, sizeof(T));
     p.slice = ((p.V + p.cluster - 1) / p.cluster + 7) / 8 * 8;
     if ((int64_t)B * p.cluster > 0x7fffffff) return DG_ERR_UNSUPPORTED;
-    const size_t smem = (size_t)(p.slice + 16) * sizeof(T) + 16;
+    // the table and, beside a cluster's slice, room for half of its tokens (8 bytes each) as far as it goes
+    size_t smem = (size_t)(p.slice + 16) * sizeof(T) + 16;
+    if (p.cluster > 1) {
+        const size_t left = (180 * 1024 - smem) / 8;
+        p.room = (int)(left < (size_t)p.slice / 2 ? left : (size_t)p.slice / 2);
+        smem += (size_t)p.room * 8;
+    }
     auto kern = p.cluster == 1 ? sample_kernel<T, true> : sample_kernel<T, false>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return dg_host::record_cuda_error(e);
@@ -1054,7 +1062,7 @@ extern "C" int dg_sample(int dtype, int B, int V, const void* logits, int64_t ro
     if (B == 0) return DG_OK;
     if (!logits || !u || !token) return DG_ERR_INVALID_ARGUMENT;
     if (V > (1 << 18)) return DG_ERR_UNSUPPORTED;              // masses of 2^40 and their sums in 58 bits
-    SampleParams p{logits, row_stride, V, 0, 1, u, temperature, top_p, min_p, top_k, temperature_value, top_p_value,
+    SampleParams p{logits, row_stride, V, 0, 1, 0, u, temperature, top_p, min_p, top_k, temperature_value, top_p_value,
                    min_p_value, top_k_value, token, logprob};
     DG_DISPATCH_LM(dtype, S, { return run<S>(p, B, static_cast<cudaStream_t>(stream)); });
     return DG_OK;
