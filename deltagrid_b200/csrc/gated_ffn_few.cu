@@ -48,6 +48,8 @@ __global__ void __launch_bounds__(THREADS)
     const int f0 = blockIdx.x * 8 * G, chunks = (D + CHUNK - 1) / CHUNK;
     const uint4 zero = make_uint4(0, 0, 0, 0);
     float c[G][NT][4] = {};
+    dg::let_next_start();
+    dg::wait_for_previous();
     const T* wg[G];
 #pragma unroll
     for (int i = 0; i < G; ++i) wg[i] = w + (int64_t)min(f0 + 8 * i + row, F - 1) * D + k8;       // (beyond F: not written)
@@ -100,8 +102,8 @@ __global__ void __launch_bounds__(THREADS)
 template <typename T, int NT, int G, int U>
 int run(int act, int M, int D, int F, const void* x, int64_t ldx, const void* w, const void* bias, void* h, cudaStream_t s) {
     auto k = act == DG_ACT_SILU ? ffn_few_kernel<T, DG_ACT_SILU, NT, G, U> : ffn_few_kernel<T, DG_ACT_GELU, NT, G, U>;
-    k<<<(unsigned)((F / 8 + G - 1) / G), THREADS, 0, s>>>(M, D, F, (const T*)x, ldx, (const T*)w, (const T*)bias, (T*)h);
-    return dg_host::check_launch();
+    return dg_host::launch_lm(k, dim3((unsigned)((F / 8 + G - 1) / G)), dim3(THREADS), 0, 0, s, M, D, F, (const T*)x, ldx,
+                              (const T*)w, (const T*)bias, (T*)h);
 }
 
 template <typename T>

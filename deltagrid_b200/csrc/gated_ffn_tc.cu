@@ -177,17 +177,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         *aborted = 0;
         tc::fence_barrier_init();
     }
+    if (tid == 0) {
+        tc::prefetch_tmap(&tma);
+        tc::prefetch_tmap(&tmb);
+        tc::prefetch_tmap(&tmo);
+    }
     tc::tc_fence_before();
     __syncthreads();
     cluster_sync();
     tc::tc_fence_after();
+    dg::let_next_start();
+    dg::wait_for_previous();
     const uint32_t tmem = *tmem_holder;
     bool bad = false;
 
     if (warp == 0 && (tid & 31) == 0) {
         // ============================ operand loads ============================
-        tc::prefetch_tmap(&tma);
-        tc::prefetch_tmap(&tmb);
         int s = 0;
         uint32_t ph = 1;                       // the empty barriers' first phase counts as passed
         for (int64_t it = first; it < items && !bad; it += stride) {
@@ -443,6 +448,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 template <typename T>
 __global__ void __launch_bounds__(1024) colsum_kernel(int rows, int cols, const float* part, T* out) {
     __shared__ float s[32][33];
+    dg::let_next_start();
+    dg::wait_for_previous();
     const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, w = threadIdx.x >> 5;
     float a = 0.f;
     if (c < cols)
@@ -459,6 +466,8 @@ __global__ void __launch_bounds__(1024) colsum_kernel(int rows, int cols, const 
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(int64_t n8, int splits, const float4* part, uint4* out) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    dg::let_next_start();
+    dg::wait_for_previous();
     if (i >= n8) return;
     float4 a = part[2 * i], b = part[2 * i + 1];
     for (int s = 1; s < splits; ++s) {
@@ -520,10 +529,8 @@ int launch(K kern, uint32_t smem, int64_t items, const CUtensorMap& a, const CUt
     int np = 0;
     const int rc = pairs(&np);
     if (rc != DG_OK) return rc;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem + 1024);
-    if (e != cudaSuccess) return record_cuda_error(e);
-    kern<<<(unsigned)(2 * (items < np ? items : np)), THREADS, smem + 1024, s>>>(a, b, d, o, p);
-    return check_launch();
+    // (the cluster size stands at the kernel)
+    return launch_lm(kern, dim3((unsigned)(2 * (items < np ? items : np))), dim3(THREADS), smem + 1024, 0, s, a, b, d, o, p);
 }
 
 FfnParams tiles_of(int64_t M, int N, int K, int tile_n, int32_t* status) {
@@ -573,9 +580,8 @@ int product(int64_t M, int N, int64_t K, const void* a, int64_t lda, const void*
     const int rc = launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, true>, Cfg<PLAIN>::BYTES, items, ma, mb, ma, mo, p, s);
     if (rc != DG_OK) return rc;
     const int64_t n8 = M * N / 8;
-    join_kernel<T><<<(unsigned)((n8 + 255) / 256), 256, 0, s>>>(n8, splits, reinterpret_cast<const float4*>(part),
-                                                               static_cast<uint4*>(c));
-    return check_launch();
+    return launch_lm(join_kernel<T>, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, 0, s, n8, splits,
+                     reinterpret_cast<const float4*>(part), static_cast<uint4*>(c));
 }
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -669,8 +675,8 @@ static int backward_t(int64_t M, int D, int F, int act, const void* x, int64_t l
     if (rc == DG_OK && dw)
         rc = product<T, true, true>(2 * (int64_t)F, D, M, dz, 2 * (int64_t)F, x, ldx, dw, part, sp.splits_dw, status, s);
     if (rc == DG_OK && db) {
-        colsum_kernel<T><<<(2 * F + 31) / 32, 1024, 0, s>>>(p.m_tiles * 8, 2 * F, colsum, static_cast<T*>(db));
-        rc = check_launch();
+        rc = launch_lm(colsum_kernel<T>, dim3((2 * F + 31) / 32), dim3(1024), 0, 0, s, p.m_tiles * 8, 2 * F, colsum,
+                       static_cast<T*>(db));
     }
     return rc;
 }

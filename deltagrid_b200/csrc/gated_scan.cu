@@ -279,7 +279,7 @@ __device__ __forceinline__ void warp_maps(Fv<VEC> P, Fv<VEC> H, Fv<VEC>& Pb, Fv<
 
 // where a thread stands: shared by both passes
 template <int LPR, int VEC, int R> struct Place {
-    int warp, lane, lc, rank, b, d0, d, len, span, ntiles;
+    int warp, lane, lc, rank, b, d0, d, span, ntiles;
     bool on;
     __device__ __forceinline__ Place(const ScanIn& in) {
         constexpr int CH = LPR * VEC, STEPS = THREADS / LPR * R;
@@ -290,7 +290,6 @@ template <int LPR, int VEC, int R> struct Place {
         d0 = unit % blocks * CH;
         d = d0 + lc * VEC;
         on = d < in.D;
-        len = in.lengths ? min(max(in.lengths[b], 0), in.T) : in.T;
         span = in.cluster * STEPS;
         ntiles = (in.T + span - 1) / span;
     }
@@ -401,7 +400,7 @@ __global__ void __launch_bounds__(THREADS, 3)
     float2* cta_maps = reinterpret_cast<float2*>(smem + STAGES * Tl::STAGE);
     __shared__ Maps<Tl::CH> maps;
     const Place<LPR, VEC, R> at(in);
-    const int tid = threadIdx.x, S = in.cluster, d = at.d, len = at.len;
+    const int tid = threadIdx.x, S = in.cluster, d = at.d;
     const T* x = (const T*)in.x + at.b * in.x_sb;
     const T* g = (const T*)in.g + at.b * in.g_sb;
     const T* o = OG ? (const T*)in.o + at.b * in.o_sb : nullptr;
@@ -412,6 +411,8 @@ __global__ void __launch_bounds__(THREADS, 3)
     const int own = at.lane / LPR * (R * LPR + kPad<LPR>) + at.lc;              // this thread's first pack in it
     bool bad = false;
     open_exchange(maps.received, S);
+    dg::wait_for_previous();
+    const int len = in.lengths ? min(max(in.lengths[at.b], 0), in.T) : in.T;
 
     uint8_t next_reset = 0;
     auto prefetch = [&](int it) {
@@ -479,6 +480,7 @@ __global__ void __launch_bounds__(THREADS, 3)
             else forward_apply<false, T, VEC, LPR, OG, R>(h, c, u, st + 2 * ARR, yp, in.D, len - t, in.T - t);
         }
     }
+    dg::let_next_start();                  // not before: its CTAs would fill the SMs unevenly (8 us of 162)
     if (h_last && at.rank == 0 && tid < Tl::CH && at.d0 + tid < in.D)
         h_last[(int64_t)at.b * in.D + at.d0 + tid] = state;
     close_exchange(S, bad, in.status);
@@ -526,7 +528,7 @@ __global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, Sc
     float2* cta_maps = reinterpret_cast<float2*>(smem + STAGES * Tl::STAGE);
     __shared__ MapsBack<Tl::CH> maps;
     const Place<LPR, VEC, R> at(in);
-    const int tid = threadIdx.x, S = in.cluster, d = at.d, len = at.len;
+    const int tid = threadIdx.x, S = in.cluster, d = at.d;
     const T* x = (const T*)in.x + at.b * in.x_sb;
     const T* g = (const T*)in.g + at.b * in.g_sb;
     const T* o = OG ? (const T*)in.o + at.b * in.o_sb : nullptr;
@@ -539,6 +541,8 @@ __global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, Sc
     const bool carries = tid < Tl::CH && at.d0 + tid < in.D;      // thread c carries channel d0 + c
     bool bad = false;
     open_exchange(maps.received, S);
+    dg::wait_for_previous();
+    const int len = in.lengths ? min(max(in.lengths[at.b], 0), in.T) : in.T;
 
     uint8_t next_reset = 0;
     float next_mark = 0.f;                 // the state before the CTA's tile
@@ -642,6 +646,7 @@ __global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, Sc
             }
         }
     }
+    dg::let_next_start();
     if (q.dh0 && at.rank == 0 && carries) q.dh0[(int64_t)at.b * in.D + at.d0 + tid] = state;
     close_exchange(S, bad, in.status);
 }
@@ -651,6 +656,8 @@ __global__ void scan_step_kernel(int D, const T* x, int64_t x_sb, const T* g, in
                                  float* h, T* y) {
     const int d = blockIdx.x * blockDim.x + threadIdx.x;
     const int64_t b = blockIdx.y;
+    dg::let_next_start();
+    dg::wait_for_previous();
     if (d >= D) return;
     float a, na;
     dg::sigmoid_pair(dg::to_f(g[b * g_sb + d]), a, na);
@@ -722,44 +729,21 @@ Shape shape_of(int B, int T, int D, int vec, int steps_per_thread, int occ, bool
     return best;
 }
 
-template <typename K, typename... A>
-int launch(K kern, unsigned grid, int cluster, size_t smem, cudaStream_t stream, A... args) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return dg_host::record_cuda_error(e);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cluster > 8) {
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return dg_host::record_cuda_error(e);
-    }
-    e = cudaLaunchKernelEx(&cfg, kern, args...);
-    if (e != cudaSuccess) return dg_host::record_cuda_error(e);
-    return dg_host::check_launch();
-}
-
 template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 int run_forward(const ScanIn& in, const float* h0, void* y, float* h_last, float* marks, cudaStream_t s) {
     typedef Tile<T, VEC, LPR, kForwardSteps, OG ? 3 : 2> Tl;
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
-    return launch(scan_forward_kernel<T, VEC, LPR, WIDE, OG>, (unsigned)grid, in.cluster, Tl::bytes(in.cluster), s, in, h0,
-                  (T*)y, h_last, marks);
+    return dg_host::launch_lm(scan_forward_kernel<T, VEC, LPR, WIDE, OG>, dim3((unsigned)grid), dim3(THREADS),
+                              Tl::bytes(in.cluster), in.cluster, s, in, h0, (T*)y, h_last, marks);
 }
 template <typename T, int VEC, int LPR, bool WIDE, bool OG>
 int run_backward(const ScanIn& in, const ScanGrad& q, cudaStream_t s) {
     typedef Tile<T, VEC, LPR, kBackwardSteps, OG ? 4 : 3> Tl;
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
-    return launch(scan_backward_kernel<T, VEC, LPR, WIDE, OG>, (unsigned)grid, in.cluster, Tl::bytes(in.cluster), s, in, q);
+    return dg_host::launch_lm(scan_backward_kernel<T, VEC, LPR, WIDE, OG>, dim3((unsigned)grid), dim3(THREADS),
+                              Tl::bytes(in.cluster), in.cluster, s, in, q);
 }
 
 // calls F<T, VEC, LPR, WIDE, OG>(...) for the shape at hand
@@ -841,11 +825,12 @@ int dg_gated_scan_step(int dtype, int B, int D, const void* x, int64_t x_sb, con
     if (!x || !gate || !h || !y) return DG_ERR_INVALID_ARGUMENT;
     if (B > 65535) return DG_ERR_UNSUPPORTED;
     DG_DISPATCH_LM(dtype, S, {
-        scan_step_kernel<S><<<dim3((D + 127) / 128, B), 128, 0, static_cast<cudaStream_t>(stream)>>>(
-            D, static_cast<const S*>(x), x_sb, static_cast<const S*>(gate), gate_sb, static_cast<const S*>(out_gate),
-            out_gate_sb, h, static_cast<S*>(y));
+        return dg_host::launch_lm(scan_step_kernel<S>, dim3((D + 127) / 128, B), dim3(128), 0, 0,
+                                  static_cast<cudaStream_t>(stream), D, static_cast<const S*>(x), x_sb,
+                                  static_cast<const S*>(gate), gate_sb, static_cast<const S*>(out_gate), out_gate_sb, h,
+                                  static_cast<S*>(y));
     });
-    return dg_host::check_launch();
+    return DG_OK;
 }
 
 }  // extern "C"

@@ -15,6 +15,12 @@
 
 namespace dg {
 
+// Programmatic dependent launch: a kernel lets the next one of its stream start as soon as its own blocks
+// leave room, and touches no memory before the kernel in front of it has completed, so that launch
+// latency and set-up run under the end of the work before (about 2 us a kernel back to back).
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // one special-function operation each, results below the normal range flushed to 0
 __device__ __forceinline__ float exp2_ftz(float x) {
     float r;
@@ -126,3 +132,35 @@ template <int ACT> __device__ __forceinline__ void act_grad2(F2 z, F2& f, F2& df
 }
 
 }  // namespace dg
+
+namespace dg_host {
+// launches with programmatic dependent launch and, with cluster > 0, that cluster size
+template <typename... P, typename... A>
+int launch_lm(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, A... args) {
+    cudaError_t e;
+    if (smem > 16 * 1024) {                    // (static shared memory counts against the 48 KB too)
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return record_cuda_error(e);
+    }
+    if (cluster > 8) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return record_cuda_error(e);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    return check_launch();
+}
+}  // namespace dg_host

@@ -326,6 +326,8 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
     const int V = p.V, s0 = min(rank * p.slice, V), n = min(p.slice, V - s0);
     const T* src = static_cast<const T*>(p.logits) + (int64_t)row * p.row_stride + s0;
 
+    dg::let_next_start();
+    dg::wait_for_previous();
     // ---- parameters
     const float temp = p.temperature ? p.temperature[row] : p.temperature_v;
     int k = p.top_k ? p.top_k[row] : p.top_k_v;
@@ -1025,30 +1027,7 @@ template <typename T> int run(SampleParams p, int B, cudaStream_t stream) {
         smem += (size_t)p.room * 8;
     }
     auto kern = p.cluster == 1 ? sample_kernel<T, true> : sample_kernel<T, false>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return dg_host::record_cuda_error(e);
-    if (p.cluster == 1) {
-        kern<<<(unsigned)B, ST, smem, stream>>>(p);
-        return dg_host::check_launch();
-    }
-    if (p.cluster > 8) {
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return dg_host::record_cuda_error(e);
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(B * p.cluster));
-    cfg.blockDim = dim3(ST);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, p);
-    if (e != cudaSuccess) return dg_host::record_cuda_error(e);
-    return dg_host::check_launch();
+    return dg_host::launch_lm(kern, dim3((unsigned)(B * p.cluster)), dim3(ST), smem, p.cluster > 1 ? p.cluster : 0, stream, p);
 }
 
 }  // namespace
