@@ -18,6 +18,9 @@
 // (even CTA only), warp 2 loads DGATE's dh tiles, warps 4-7 and 8-11 are two epilogue groups
 // (thread = TMEM lane = row) that take alternate slices of 64 columns.
 //
+// GATE and DGATE take 128 features a tile, or 64 where there are few tiles: then a tile's
+// accumulator has 128 columns, four of them fit, and the epilogue groups take alternate tiles.
+//
 // Every wait is bounded by the library's wait limit; a role that gives up flags
 // DG_DEVCHK_TIMEOUT, the others run into their own limits, and the CTA lets what it has in
 // flight land before it frees its TMEM.
@@ -37,9 +40,13 @@ constexpr int THREADS = 384;
 constexpr uint32_t TILE = BM * BK * 2;     // 16 KB: one operand tile, one staging buffer
 constexpr int GROUP_M = 8;                 // tile rows walked together, for L2
 
-template <int ROLE> struct Cfg {
-    static constexpr int STAGES = ROLE == DGATE ? 5 : 6;
-    static constexpr uint32_t DH = STAGES * 2 * TILE;              // DGATE: dh, then dG (one slice per group)
+// FT: features of a tile (GATE, DGATE; PLAIN tiles have the shape of 128)
+template <int ROLE, int FT> struct Cfg {
+    static constexpr int STAGES = FT == 64 ? (ROLE == DGATE ? 6 : 8) : (ROLE == DGATE ? 5 : 6);
+    static constexpr uint32_t BTILE = FT * BK * 2;                 // this CTA's half of B
+    static constexpr uint32_t STAGE = TILE + BTILE;
+    static constexpr int ACC = FT == 64 ? 4 : 2, ACCW = 2 * FT;    // accumulators and their columns
+    static constexpr uint32_t DH = STAGES * STAGE;                 // DGATE: dh, then dG (one slice per group)
     static constexpr uint32_t OUT = DH + (ROLE == DGATE ? 2 * TILE : 0);
     static constexpr uint32_t BAR = OUT + 2 * TILE;
     static constexpr uint32_t BIAS = BAR + 256;                    // fp32: per group 64 gate and 64 value biases
@@ -139,20 +146,20 @@ __device__ __forceinline__ float column_sums(float (&v)[16], int lane) {
     return v[0] + __shfl_xor_sync(DG_FULL_MASK, v[0], 1);
 }
 
-template <typename T, int ROLE, int ACT, bool A_MN, bool B_MN, bool F32_OUT>
+template <typename T, int ROLE, int ACT, bool A_MN, bool B_MN, bool F32_OUT, int FT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     ffn_tc_kernel(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmb,
                   const __grid_constant__ CUtensorMap tmd, const __grid_constant__ CUtensorMap tmo, FfnParams p) {
-    using C = Cfg<ROLE>;
+    using C = Cfg<ROLE, FT>;
     constexpr bool BF16 = !std::is_same<T, __half>::value;
     constexpr int ST = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::BAR);      // [ST], counted in the even CTA
     uint64_t* empty = full + ST;                                    // [ST]
-    uint64_t* acc_full = empty + ST;                                // [2]
-    uint64_t* acc_empty = acc_full + 2;                             // [2], counted in the even CTA
-    uint64_t* dh_full = acc_empty + 2;                              // [2] one per epilogue group
+    uint64_t* acc_full = empty + ST;                                // [ACC]
+    uint64_t* acc_empty = acc_full + C::ACC;                        // [ACC], counted in the even CTA
+    uint64_t* dh_full = acc_empty + C::ACC;                         // [2] one per epilogue group
     uint64_t* dh_empty = dh_full + 2;                               // [2]
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dh_empty + 2);
     int* aborted = reinterpret_cast<int*>(tmem_holder + 1);
@@ -168,9 +175,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             tc::mbar_init(full + i, 1);
             tc::mbar_init(empty + i, 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < C::ACC; ++i) {
             tc::mbar_init(acc_full + i, 1);
-            tc::mbar_init(acc_empty + i, 4);
+            tc::mbar_init(acc_empty + i, FT == 64 ? 2 : 4);        // epilogue groups of both CTAs that read it
+        }
+        for (int i = 0; i < 2; ++i) {
             tc::mbar_init(dh_full + i, 1);
             tc::mbar_init(dh_empty + i, 1);
         }
@@ -199,13 +208,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const Work w = work_of(p, it);
             const int row = w.mt * 2 * BM + (int)rank * BM;
             // B's half of this CTA: GATE / DGATE the gate or the value rows, PLAIN columns
-            const int col = ROLE == PLAIN ? w.nt * BN + (int)rank * BM : (int)rank * p.N + w.nt * BM;
+            const int col = ROLE == PLAIN ? w.nt * BN + (int)rank * BM : (int)rank * p.N + w.nt * FT;
             const int kb0 = w.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, nkb_all);
             for (int kb = kb0; kb < kb1; ++kb) {
                 if (!tc::mbar_wait(empty + s, ph, p.wait_limit)) { bad = true; break; }
-                if (rank == 0) tc::mbar_expect_tx(full + s, 4 * TILE);
+                if (rank == 0) tc::mbar_expect_tx(full + s, 2 * C::STAGE);
                 const uint32_t bar = in_leader(full + s);
-                uint8_t* a = sm + s * 2 * TILE;
+                uint8_t* a = sm + s * C::STAGE;
                 uint8_t* b = a + TILE;
                 const int k = kb * BK;
                 if (A_MN) {
@@ -225,19 +234,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
     } else if (warp == 1 && rank == 0 && (tid & 31) == 0) {
         // ================================= MMAs =================================
-        constexpr uint32_t idesc = tc::make_idesc(2 * BM, BN, BF16 ? 1 : 0, A_MN ? 1 : 0, B_MN ? 1 : 0);
-        int s = 0, acc = 0;
-        uint32_t ph = 0, acc_ph = 1;
-        for (int64_t it = first; it < items && !bad; it += stride) {
+        constexpr uint32_t idesc = tc::make_idesc(2 * BM, C::ACCW, BF16 ? 1 : 0, A_MN ? 1 : 0, B_MN ? 1 : 0);
+        int s = 0;
+        uint32_t ph = 0, n = 0;
+        for (int64_t it = first; it < items && !bad; it += stride, ++n) {
+            const uint32_t acc = n % C::ACC;
             const Work w = work_of(p, it);
             const int kb0 = w.split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, nkb_all);
-            if (!tc::mbar_wait(acc_empty + acc, acc_ph, p.wait_limit)) { bad = true; break; }
+            if (!tc::mbar_wait(acc_empty + acc, (n / C::ACC & 1) ^ 1, p.wait_limit)) { bad = true; break; }
             tc::tc_fence_after();
-            const uint32_t d = tmem + acc * BN;
+            const uint32_t d = tmem + acc * C::ACCW;
             for (int kb = kb0; kb < kb1; ++kb) {
                 if (!tc::mbar_wait(full + s, ph, p.wait_limit)) { bad = true; break; }
                 tc::tc_fence_after();
-                const uint32_t a = tc::smem_u32(sm + s * 2 * TILE), b = a + TILE;
+                const uint32_t a = tc::smem_u32(sm + s * C::STAGE), b = a + TILE;
 #pragma unroll
                 for (int kk = 0; kk < BK / 16; ++kk) {
                     // K-major: 16 elements are 32 bytes of each 128-byte row, 8 rows 1024 bytes apart.
@@ -253,17 +263,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             }
             if (bad) break;
             commit_pair(acc_full + acc);
-            if (++acc == 2) { acc = 0; acc_ph ^= 1; }
         }
     } else if (ROLE == DGATE && warp == 2 && (tid & 31) == 0) {
         // ============================ dh tiles ============================
-        uint32_t ph = 1;
-        for (int64_t it = first; it < items && !bad; it += stride, ph ^= 1) {
+        uint32_t n = 0;
+        for (int64_t it = first; it < items && !bad; it += stride, ++n) {
             const Work w = work_of(p, it);
             for (int g = 0; g < 2; ++g) {
-                if (!tc::mbar_wait(dh_empty + g, ph, p.wait_limit)) { bad = true; break; }
+                if (FT == 64 && (int)(n & 1) != g) continue;
+                const uint32_t use = FT == 64 ? n >> 1 : n;
+                if (!tc::mbar_wait(dh_empty + g, (use & 1) ^ 1, p.wait_limit)) { bad = true; break; }
                 tc::mbar_expect_tx(dh_full + g, TILE);
-                tc::tma_load_2d(sm + C::DH + g * TILE, &tmd, dh_full + g, w.nt * BM + 64 * g,
+                tc::tma_load_2d(sm + C::DH + g * TILE, &tmd, dh_full + g, w.nt * FT + (FT == 64 ? 0 : 64 * g),
                                 w.mt * 2 * BM + (int)rank * BM);
             }
         }
@@ -275,8 +286,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         uint8_t* out = sm + C::OUT + g * TILE;
         uint8_t* dh = sm + C::DH + g * TILE;
         float* bias = reinterpret_cast<float*>(sm + C::BIAS) + 128 * g;
-        int acc = 0;
-        uint32_t acc_ph = 0, dh_ph = 0;
+        uint32_t n = 0, acc = 0;
         // the buffer's last TMA store has read it
         auto buffer_free = [&]() {
             if (t == 0) tc::bulk_wait_read0();
@@ -287,25 +297,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             tc::group_sync(bar_id);
             if (t == 0) arrive_at(in_leader(acc_empty + acc));
         };
-        for (int64_t it = first; it < items; it += stride) {
+        for (int64_t it = first; it < items; it += stride, ++n) {
+            if (FT == 64 && (int)(n & 1) != g) continue;
             const Work w = work_of(p, it);
+            acc = n % C::ACC;
             const int row0 = w.mt * 2 * BM + (int)rank * BM;
-            const int f0 = w.nt * BM + 64 * g;                 // GATE, DGATE: this group's 64 features
+            const int c0 = FT == 64 ? 0 : 64 * g;              // this group's columns of the gate
+            const int f0 = w.nt * FT + c0;                 // GATE, DGATE: this group's 64 features
             if (ROLE != PLAIN) {                               // (read last before the store's barrier)
                 const int f = f0 + (t & 63);
                 bias[t] = p.bias && f < p.N
                               ? dg::to_f(static_cast<const T*>(p.bias)[(int64_t)(t >> 6) * p.N + f]) : 0.f;
             }
-            bad = !tc::mbar_wait(acc_full + acc, acc_ph, p.wait_limit);
-            if (ROLE == DGATE && !bad) bad = !tc::mbar_wait(dh_full + g, dh_ph, p.wait_limit);
+            bad = !tc::mbar_wait(acc_full + acc, n / C::ACC & 1, p.wait_limit);
+            if (ROLE == DGATE && !bad) bad = !tc::mbar_wait(dh_full + g, (FT == 64 ? n >> 1 : n) & 1, p.wait_limit);
             if (tc::group_sync_or(bar_id, bad)) { bad = true; break; }
             tc::tc_fence_after();
-            const uint32_t d = trow + acc * BN;
+            const uint32_t d = trow + acc * C::ACCW;
             if (ROLE != PLAIN) {
                 // 16 columns of gate and value at a time, the next ones on their way from TMEM
                 uint32_t gr[2][16], ur[2][16];
-                tc::tmem_ld16(d + 64 * g, gr[0]);
-                tc::tmem_ld16(d + BM + 64 * g, ur[0]);
+                tc::tmem_ld16(d + c0, gr[0]);
+                tc::tmem_ld16(d + FT + c0, ur[0]);
                 float sum_g[4], sum_u[4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -313,8 +326,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     loaded(gr[q & 1]);
                     loaded(ur[q & 1]);
                     if (q < 3) {
-                        tc::tmem_ld16(d + 64 * g + 16 * (q + 1), gr[(q + 1) & 1]);
-                        tc::tmem_ld16(d + BM + 64 * g + 16 * (q + 1), ur[(q + 1) & 1]);
+                        tc::tmem_ld16(d + c0 + 16 * (q + 1), gr[(q + 1) & 1]);
+                        tc::tmem_ld16(d + FT + c0 + 16 * (q + 1), ur[(q + 1) & 1]);
                     } else {
                         release_acc();
                     }
@@ -420,8 +433,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     }
                 }
             }
-            if (++acc == 2) { acc = 0; acc_ph ^= 1; }
-            dh_ph ^= 1;
         }
         if (t == 0) tc::bulk_wait0();
     }
@@ -576,8 +587,8 @@ int product(int64_t M, int N, int64_t K, const void* a, int64_t lda, const void*
     if (!ok) return DG_ERR_UNSUPPORTED;
     const int64_t items = (int64_t)p.m_tiles * p.n_tiles * p.splits;
     if (splits == 1)
-        return launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, false>, Cfg<PLAIN>::BYTES, items, ma, mb, ma, mo, p, s);
-    const int rc = launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, true>, Cfg<PLAIN>::BYTES, items, ma, mb, ma, mo, p, s);
+        return launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, false, 128>, (Cfg<PLAIN, 128>::BYTES), items, ma, mb, ma, mo, p, s);
+    const int rc = launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, true, 128>, (Cfg<PLAIN, 128>::BYTES), items, ma, mb, ma, mo, p, s);
     if (rc != DG_OK) return rc;
     const int64_t n8 = M * N / 8;
     return launch_lm(join_kernel<T>, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, 0, s, n8, splits,
@@ -618,22 +629,49 @@ bool ffn_tc_aligned(const void* a, int64_t lda, const void* b, const void* c, co
            ldd % 8 == 0;
 }
 
+// Features per tile.  A tile of 64 takes not half but four fifths of one of 128: its MMAs read A from shared
+// memory twice as often (16384 x 768 x 768: 49 us in 11 waves of 64, 37 us in 6 of 128).  So it is taken
+// where its tiles need no more waves (33 to 256 x 768 x 768: 7.4 us against 9.8).
+static int tile_features(int64_t M, int F, int np) {
+    const int64_t rows = (M + 2 * BM - 1) / (2 * BM);
+    const int64_t waves128 = (rows * ((F + 127) / 128) + np - 1) / np, waves64 = (rows * ((F + 63) / 64) + np - 1) / np;
+    return waves64 * 4 < waves128 * 5 ? 64 : 128;
+}
+
+template <typename T, int ROLE, int FT>
+static int gate_t(int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w, const CUtensorMap& md,
+                  const CUtensorMap& mo, FfnParams p, cudaStream_t s) {
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    CUtensorMap mx, mw;
+    if (!map_matrix(&mx, x, M, D, ldx, BM, bf16) || !map_matrix(&mw, w, 2 * (int64_t)F, D, D, FT, bf16))
+        return DG_ERR_UNSUPPORTED;
+    p.n_tiles = (F + FT - 1) / FT;
+    const int64_t items = (int64_t)p.m_tiles * p.n_tiles;
+    return act == DG_ACT_SILU
+               ? launch(ffn_tc_kernel<T, ROLE, DG_ACT_SILU, false, false, false, FT>, Cfg<ROLE, FT>::BYTES, items, mx, mw,
+                        md, mo, p, s)
+               : launch(ffn_tc_kernel<T, ROLE, DG_ACT_GELU, false, false, false, FT>, Cfg<ROLE, FT>::BYTES, items, mx, mw,
+                        md, mo, p, s);
+}
+template <typename T, int ROLE>
+static int gate(int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w, const CUtensorMap& md,
+                const CUtensorMap& mo, const FfnParams& p, cudaStream_t s) {
+    int np = 0;
+    const int rc = pairs(&np);
+    if (rc != DG_OK) return rc;
+    return tile_features(M, F, np) == 64 ? gate_t<T, ROLE, 64>(M, D, F, act, x, ldx, w, md, mo, p, s)
+                                         : gate_t<T, ROLE, 128>(M, D, F, act, x, ldx, w, md, mo, p, s);
+}
+
 template <typename T>
 static int forward_t(int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w, const void* bias,
                      void* h, int32_t* status, cudaStream_t s) {
     constexpr bool bf16 = !std::is_same<T, __half>::value;
     FfnParams p = tiles_of(M, F, D, BM, status);
     p.bias = bias;
-    CUtensorMap mx, mw, mh;
-    if (!map_matrix(&mx, x, M, D, ldx, BM, bf16) || !map_matrix(&mw, w, 2 * (int64_t)F, D, D, BM, bf16) ||
-        !map_matrix(&mh, h, M, F, F, BM, bf16))
-        return DG_ERR_UNSUPPORTED;
-    const int64_t items = (int64_t)p.m_tiles * p.n_tiles;
-    return act == DG_ACT_SILU
-               ? launch(ffn_tc_kernel<T, GATE, DG_ACT_SILU, false, false, false>, Cfg<GATE>::BYTES, items, mx, mw, mx,
-                        mh, p, s)
-               : launch(ffn_tc_kernel<T, GATE, DG_ACT_GELU, false, false, false>, Cfg<GATE>::BYTES, items, mx, mw, mx,
-                        mh, p, s);
+    CUtensorMap mh;
+    if (!map_matrix(&mh, h, M, F, F, BM, bf16)) return DG_ERR_UNSUPPORTED;
+    return gate<T, GATE>(M, D, F, act, x, ldx, w, mh, mh, p, s);
 }
 
 int ffn_tc_forward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
@@ -657,19 +695,13 @@ static int backward_t(int64_t M, int D, int F, int act, const void* x, int64_t l
     FfnParams p = tiles_of(M, F, D, BM, status);
     p.bias = bias;
     p.colsum = db ? colsum : nullptr;
-    CUtensorMap mx, mw, md, mz;
+    CUtensorMap md, mz;
     cuuint64_t dims[3] = {(cuuint64_t)F, 2, (cuuint64_t)M};
     cuuint64_t strides[2] = {(cuuint64_t)F * 2, (cuuint64_t)F * 4};
     cuuint32_t box[3] = {64, 1, BM};
-    if (!map_matrix(&mx, x, M, D, ldx, BM, bf16) || !map_matrix(&mw, w, 2 * (int64_t)F, D, D, BM, bf16) ||
-        !map_matrix(&md, dh, M, F, ld_dh, BM, bf16) || !make_tmap(&mz, map_type(bf16), dz, 3, dims, strides, box))
+    if (!map_matrix(&md, dh, M, F, ld_dh, BM, bf16) || !make_tmap(&mz, map_type(bf16), dz, 3, dims, strides, box))
         return DG_ERR_UNSUPPORTED;
-    const int64_t items = (int64_t)p.m_tiles * p.n_tiles;
-    int rc = act == DG_ACT_SILU
-                 ? launch(ffn_tc_kernel<T, DGATE, DG_ACT_SILU, false, false, false>, Cfg<DGATE>::BYTES, items, mx, mw,
-                          md, mz, p, s)
-                 : launch(ffn_tc_kernel<T, DGATE, DG_ACT_GELU, false, false, false>, Cfg<DGATE>::BYTES, items, mx, mw,
-                          md, mz, p, s);
+    int rc = gate<T, DGATE>(M, D, F, act, x, ldx, w, md, mz, p, s);
     if (rc == DG_OK && dx)
         rc = product<T, false, true>(M, D, 2 * (int64_t)F, dz, 2 * (int64_t)F, w, D, dx, part, sp.splits_dx, status, s);
     if (rc == DG_OK && dw)

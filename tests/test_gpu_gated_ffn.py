@@ -75,6 +75,14 @@ def test_forward_and_backward(M, D, F, dtype):
     _check(*_inputs(M, D, F, dtype, seed=M + D + F), "silu")
 
 
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("M,D,F", [(2600, 136, 760), (2560, 768, 768), (9000, 72, 1104), (300, 192, 4096)])
+def test_many_tiles(M, D, F, bias):
+    """Tiles of 128 features and of 64, several to a CTA, the last ones ragged."""
+    x, w, b, dh = _inputs(M, D, F, torch.bfloat16, seed=M, bias=bias)
+    _check(x, w, b, dh, "silu")
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("M", [3, 130, 700])
 def test_gelu_without_bias(M, dtype):
