@@ -235,10 +235,10 @@ __device__ __forceinline__ u64 block_sum(u64 v, Shared& s) {
     __syncthreads();
     if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5] = v;
     __syncthreads();
-    u64 t = 0;
+    v = s.warp[threadIdx.x % WARPS];
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) t += s.warp[i];
-    return t;
+    for (int o = WARPS / 2; o; o >>= 1) v += __shfl_xor_sync(DG_FULL_MASK, v, o);
+    return v;
 }
 // barrier of the first `threads` threads (whole warps)
 __device__ __forceinline__ void part_sync(int threads) {
@@ -271,13 +271,10 @@ __device__ __forceinline__ u64 block_before(u64 v, u64* total, Shared& s) {
     __syncthreads();
     if (lane == 31) s.warp[warp] = inc;
     __syncthreads();
-    u64 before = 0, t = 0;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) {
-        if (i == warp) before = t;
-        t += s.warp[i];
-    }
-    *total = t;
+    const u64 all = warp_scan(lane < WARPS ? s.warp[lane] : 0, lane);
+    *total = __shfl_sync(DG_FULL_MASK, all, 31);
+    u64 before = __shfl_sync(DG_FULL_MASK, all, (warp - 1) & 31);
+    if (warp == 0) before = 0;
     return before + inc - v;
 }
 // One value per CTA of the cluster, in lane r the value of CTA r (0 beyond): one remote load each, side by
@@ -388,8 +385,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
     u64 mx = __reduce_max_sync(DG_FULL_MASK, max(most0, most1));
     if (lane == 0) s.warp[warp] = mx;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) mx = max(mx, s.warp[i]);
+    mx = __reduce_max_sync(DG_FULL_MASK, (uint32_t)s.warp[lane % WARPS]);
     if (collect) {
         // counts of the partial maxima by their keys' distance below the largest (bf16's resolution
         // for 32-bit keys); the bound is the first key of the bin in which the j-th lies
@@ -398,22 +394,30 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
         if (most0) atomicAdd(&s.hist[0][bin_of(most0)], 1u);
         if (most1) atomicAdd(&s.hist[0][bin_of(most1)], 1u);
         __syncthreads();
-        uint32_t v[8], sum = 0;
+        if (warp == 0) {
+            uint32_t v[8], sum = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = s.hist[0][8 * lane + i], sum += v[i];
-        uint32_t run = sum;
+            for (int i = 0; i < 8; ++i) v[i] = s.hist[0][8 * lane + i], sum += v[i];
+            uint32_t run = sum;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t x = __shfl_up_sync(DG_FULL_MASK, run, o);
-            if (lane >= o) run += x;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t x = __shfl_up_sync(DG_FULL_MASK, run, o);
+                if (lane >= o) run += x;
+            }
+            const unsigned hit = __ballot_sync(DG_FULL_MASK, run >= (uint32_t)j);
+            if (lane == (hit ? __ffs(hit) - 1 : 31)) {
+                run -= sum;
+                uint32_t b = 8 * lane;
+#pragma unroll
+                for (int i = 0; i < 7; ++i)
+                    if (run + v[i] < (uint32_t)j && b == 8 * lane + i) run += v[i], ++b;
+                s.cross[0] = b;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s.hist[0][8 * lane + i] = 0;
         }
-        const unsigned hit = __ballot_sync(DG_FULL_MASK, run >= (uint32_t)j);
-        run -= sum;
-        uint32_t bin = 8 * lane;
-#pragma unroll
-        for (int i = 0; i < 7; ++i)
-            if (run + v[i] < (uint32_t)j && bin == 8 * lane + i) run += v[i], ++bin;
-        bin = __shfl_sync(DG_FULL_MASK, bin, hit ? __ffs(hit) - 1 : 31);
+        __syncthreads();
+        const uint32_t bin = (uint32_t)s.cross[0];
         if (bin < 255 && (uint64_t)mx >= ((uint64_t)(bin + 1) << low)) {
             bound = (uint32_t)mx - (((bin + 1) << low) - 1);
         } else {
@@ -424,8 +428,6 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                 if (reach >= j) bound = c;
             }
         }
-        __syncthreads();
-        if (tid < 256) s.hist[0][tid] = 0;
     }
     if (C > 1) {
         // j tokens of each CTA reach its bound, so C j reach the smallest
