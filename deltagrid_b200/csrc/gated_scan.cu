@@ -694,10 +694,12 @@ int width_of(int D, size_t elem, std::initializer_list<Row> rows) {
 }
 
 // Channels per CTA (lpr x vec) and cluster size, by the work of the busiest SM: CTAs on it x walked steps x
-// lanes, a half of 2048 more for each tile walked and almost two for each wave of CTAs.  Clusters fill some
-// SMs before others, so their SMs count as full; an SM with a single CTA waits at its barriers (1.5 x its
-// work).  Larger clusters and narrower rows cost a little more.  Measured, forward: 2 x 300 x 512 lpr 32
-// cluster 5 4.3 us, none 8.2; 8 x 4096 x 768 cluster 4 55 us, 2 77; 32 x 2048 x 1024 cluster 2 112 us, 8 152.
+// channels, 1100 more for each tile walked and 24000 for each wave of CTAs.  Clusters fill some SMs before
+// others, so their SMs count as full, and 0.3 of a wave more is counted where there are several; an SM with a
+// single CTA waits at its barriers (1.6 x its work).  Rows of 32 and 64 bytes cost HBM 38% and 15% more than
+// rows of 128.  Fitted to 48 shapes, whose choice takes 1% longer than the best on average and 13% at worst.
+// Forward: 2 x 300 x 512 lpr 32 cluster 5 3.4 us, none 7.5; 8 x 4096 x 768 cluster 4 50 us, 2 70, lpr 8 66;
+// 32 x 2048 x 1024 cluster 2 109 us, none 114, lpr 8 146.
 struct Shape {
     int lpr, cluster;
 };
@@ -715,11 +717,11 @@ Shape shape_of(int B, int T, int D, int vec, int steps_per_thread, int occ, bool
         const int steps = THREADS / lpr * steps_per_thread, tiles = (T + steps - 1) / steps;
         for (int s = 1; s <= 16 && (s == 1 || s <= tiles); ++s) {
             const int64_t slots = kClusters[occ - 1][s - 1], n = units * s, per_sm = (n + 147) / 148;
-            const double waves = units <= slots ? 1.0 : (double)units / slots + 0.35;
-            const double share = waves > 1.0 || (s > 1 && n > 148) ? waves * occ : per_sm > 1 ? (double)per_sm : 1.5;
+            const double waves = units <= slots ? 1.0 : (double)units / slots + 0.3;
+            const double share = waves > 1.0 || (s > 1 && n > 148) ? waves * occ : per_sm > 1 ? (double)per_sm : 1.6;
             const double walked = (double)((tiles + s - 1) / s);
-            const double cost = share * walked * steps * lpr * (1.0 + 0.01 * s + (lpr < 32 ? 0.04 : 0.0)) +
-                                waves * (1000.0 * walked + 3600.0);
+            const double cost = share * walked * steps * lpr * vec * (lpr == 8 ? 1.38 : lpr == 16 ? 1.15 : 1.0) +
+                                waves * (1100.0 * walked + 24000.0);
             if (least < 0 || cost < least) {
                 least = cost;
                 best = {lpr, s};
