@@ -2,7 +2,8 @@
 // backward pass on CUDA cores: 64 x 64 output tiles, 16 of the contracted axis at a time
 // through shared memory, 4 x 4 outputs per thread.  These kernels take any storage type, size
 // and alignment; 16-bit calls with D and F multiples of 8 and 16-byte aligned rows go to the
-// tcgen05 kernel of gated_ffn_tc.cu or, with few tokens, to gated_ffn_few.cu.
+// tcgen05 kernel of gated_ffn_tc.cu or, forward with up to 256 tokens, to gated_ffn_few.cu and
+// gated_ffn_split.cu.
 #include "lm_common.cuh"
 
 namespace dg_host {
@@ -14,6 +15,9 @@ int ffn_few_forward(int dtype, int64_t M, int D, int F, int act, const void* x, 
                     const void* bias, void* h, cudaStream_t s);
 int ffn_tc_forward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
                    const void* bias, void* h, int32_t* status, cudaStream_t s);
+bool ffn_split_supports(int64_t M, int D, int F);
+int ffn_split_forward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
+                      const void* bias, void* h, int32_t* status, cudaStream_t s);
 size_t ffn_tc_workspace(int64_t M, int D, int F);
 int ffn_tc_backward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
                     const void* bias, const void* dh, int64_t ld_dh, void* dx, void* dw, void* db, void* workspace,
@@ -166,6 +170,8 @@ int dg_gated_ffn_forward(int dtype, int64_t M, int D, int F, int activation, con
     if (dg_host::ffn_tc_supports(dtype, M, D, F) && dg_host::ffn_tc_aligned(x, ldx, weight, bias, h, 0, h, h)) {
         if (dg_host::ffn_few_supports(M, D, F))
             return dg_host::ffn_few_forward(dtype, M, D, F, activation, x, ldx, weight, bias, h, s);
+        if (dg_host::ffn_split_supports(M, D, F))
+            return dg_host::ffn_split_forward(dtype, M, D, F, activation, x, ldx, weight, bias, h, dev_status, s);
         return dg_host::ffn_tc_forward(dtype, M, D, F, activation, x, ldx, weight, bias, h, dev_status, s);
     }
     const dim3 grid((F + TN - 1) / TN, (unsigned)((M + TM - 1) / TM));

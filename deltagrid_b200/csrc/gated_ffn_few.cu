@@ -1,5 +1,6 @@
-// gated_ffn_few.cu -- the gated feed-forward block for few tokens (f16 / bf16): the serving
-// form, bound by reading the 2 F D weights once.
+// gated_ffn_few.cu -- the gated feed-forward block for a few tokens (f16 / bf16), up to 32: bound
+// by reading the 2 F D weights once and, where they are small, by latency (one token of 768 x 768
+// 2.2 us; 8 of 2048 x 5504, 45 MB, 11 us, 0.64 of what HBM allows).
 //
 // The weights go from global memory straight into matrix fragments (mma.sync m16n8k16): rows
 // 0-7 of a fragment are eight gate rows, rows 8-15 the value rows of the same features, and
@@ -120,11 +121,16 @@ int by_tokens(int act, int M, int D, int F, const void* x, int64_t ldx, const vo
 
 namespace dg_host {
 
-// Whether this form is taken (16-bit types, D and F multiples of 8, aligned rows).  Up to 16 tokens it
-// always wins (2048 x 5504: 11 us against the tile kernel's 17).  With 17 to 32 every weight byte meets
-// two bytes of x from L2: it wins below 16 MB of weights (768 x 768: 3.8 us against 9.8) and loses
-// above (2048 x 5504: 21 us against 17).
-bool ffn_few_supports(int64_t M, int D, int F) { return M <= 16 || (M <= 32 && (int64_t)4 * F * D <= (16 << 20)); }
+// Whether this form is taken rather than the split one (16-bit types, D and F multiples of 8, aligned rows).
+// It starts faster, but every weight byte meets 1/8 byte of x for each token, from L2, and a CTA's eight
+// features take all of D.  Up to 8 tokens it wins below 64 MB of weights (768 x 768: 2.2 us against 4.8;
+// 2048 x 5504, 45 MB: 10.6 against 10.9; 4096 x 11008, 180 MB: 36 against 33), up to 16 below 12 MB and up to
+// 32 below 8 MB (32 x 768 x 768: 4.0 us against 5.2; 32 x 1536 x 2048: 9.0 against 7.6), D not long (16 x 4096
+// x 400: 10.8 against 6.9).
+bool ffn_few_supports(int64_t M, int D, int F) {
+    const int64_t bytes = (int64_t)4 * F * D;
+    return M <= 8 ? bytes <= 64 << 20 : D <= 2048 && ((M <= 16 && bytes <= 12 << 20) || (M <= 32 && bytes <= 8 << 20));
+}
 
 int ffn_few_forward(int dtype, int64_t M, int D, int F, int act, const void* x, int64_t ldx, const void* w,
                     const void* bias, void* h, cudaStream_t s) {

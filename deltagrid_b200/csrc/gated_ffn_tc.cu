@@ -631,7 +631,7 @@ bool ffn_tc_aligned(const void* a, int64_t lda, const void* b, const void* c, co
 
 // Features per tile.  A tile of 64 takes not half but four fifths of one of 128: its MMAs read A from shared
 // memory twice as often (16384 x 768 x 768: 49 us in 11 waves of 64, 37 us in 6 of 128).  So it is taken
-// where its tiles need no more waves (33 to 256 x 768 x 768: 7.4 us against 9.8).
+// where its tiles need no more waves (129 to 256 x 768 x 768: 8.1 us against 9.8).
 static int tile_features(int64_t M, int F, int np) {
     const int64_t rows = (M + 2 * BM - 1) / (2 * BM);
     const int64_t waves128 = (rows * ((F + 127) / 128) + np - 1) / np, waves64 = (rows * ((F + 63) / 64) + np - 1) / np;

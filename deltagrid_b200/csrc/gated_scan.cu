@@ -703,11 +703,6 @@ int width_of(int D, size_t elem, std::initializer_list<Row> rows) {
 struct Shape {
     int lpr, cluster;
 };
-// Clusters of 1..16 CTAs that are resident at once on a whole B200 with 1, 2 or 3 such CTAs to an SM
-// (cudaOccupancyMaxActiveClusters; a cluster stays inside one group of SMs)
-constexpr int kClusters[3][16] = {{148, 74, 45, 33, 26, 22, 15, 15, 15, 11, 7, 7, 7, 7, 7, 7},
-                                  {296, 148, 93, 71, 56, 45, 37, 33, 30, 26, 21, 21, 17, 14, 14, 14},
-                                  {444, 222, 142, 104, 82, 71, 56, 48, 45, 41, 31, 31, 28, 24, 24, 21}};
 Shape shape_of(int B, int T, int D, int vec, int steps_per_thread, int occ, bool narrow) {
     Shape best{32, 1};
     double least = -1.0;
@@ -716,7 +711,7 @@ Shape shape_of(int B, int T, int D, int vec, int steps_per_thread, int occ, bool
         const int64_t units = (int64_t)B * ((D + lpr * vec - 1) / (lpr * vec));
         const int steps = THREADS / lpr * steps_per_thread, tiles = (T + steps - 1) / steps;
         for (int s = 1; s <= 16 && (s == 1 || s <= tiles); ++s) {
-            const int64_t slots = kClusters[occ - 1][s - 1], n = units * s, per_sm = (n + 147) / 148;
+            const int64_t slots = dg_host::kClusters[occ - 1][s - 1], n = units * s, per_sm = (n + 147) / 148;
             const double waves = units <= slots ? 1.0 : (double)units / slots + 0.3;
             const double share = waves > 1.0 || (s > 1 && n > 148) ? waves * occ : per_sm > 1 ? (double)per_sm : 1.6;
             const double walked = (double)((tiles + s - 1) / s);

@@ -134,6 +134,11 @@ template <int ACT> __device__ __forceinline__ void act_grad2(F2 z, F2& f, F2& df
 }  // namespace dg
 
 namespace dg_host {
+// Clusters of 1..16 CTAs that are resident at once on a whole B200 with 1, 2 or 3 such CTAs to an SM
+// (cudaOccupancyMaxActiveClusters; a cluster stays inside one group of SMs)
+constexpr int kClusters[3][16] = {{148, 74, 45, 33, 26, 22, 15, 15, 15, 11, 7, 7, 7, 7, 7, 7},
+                                  {296, 148, 93, 71, 56, 45, 37, 33, 30, 26, 21, 21, 17, 14, 14, 14},
+                                  {444, 222, 142, 104, 82, 71, 56, 48, 45, 41, 31, 31, 28, 24, 24, 21}};
 // launches with programmatic dependent launch and, with cluster > 0, that cluster size
 template <typename... P, typename... A>
 int launch_lm(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, A... args) {

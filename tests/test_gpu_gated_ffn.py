@@ -100,6 +100,22 @@ def test_few_tokens(M, D, F, dtype):
     assert ext.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,D,F", [(9, 4096, 128), (16, 2056, 1000), (33, 64, 40), (47, 200, 4000), (64, 8, 8),
+                                   (97, 4096, 136), (128, 512, 9480), (129, 1536, 72), (200, 4104, 1000),
+                                   (255, 1544, 4096), (256, 1536, 520), (256, 1528, 520), (257, 2048, 64),
+                                   (7, 4096, 4104)])
+def test_tokens_against_a_split_axis(M, D, F, act, dtype):
+    """Up to 256 tokens: parts of D on several CTAs, tails of D, F and the tokens, one part and eight."""
+    x, w, b, _ = _inputs(M, D, F, dtype, seed=M + F)
+    h = gated_ffn(x, w, b, act)
+    torch.cuda.synchronize()
+    assert rel_err(h.float().cpu(), _ref(x, w, b, act).cpu()) < TOL[dtype]
+    assert torch.equal(h, gated_ffn(x, w, b, act))
+    assert ext.device_status() == 0
+
+
 @pytest.mark.parametrize("M", [5, 200])
 @pytest.mark.parametrize("D,F,off", [(64, 64, 0), (64, 64, 1), (72, 40, 4), (72, 40, 8), (65, 33, 3)])
 def test_row_strides_and_offsets(M, D, F, off):
