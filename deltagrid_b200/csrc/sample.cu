@@ -23,6 +23,8 @@
 //
 // What bounds it: not the 64 KB of a bf16 row of 32000 (2.5 us for 256 rows) but the latency
 // of the steps after it, some fifteen barriers of up to 512 threads; two CTAs share an SM.
+#include <type_traits>
+
 #include "lm_common.cuh"
 
 namespace {
@@ -184,6 +186,9 @@ __device__ __forceinline__ uint32_t remote_load32(const uint32_t* p, uint32_t ra
 __device__ __forceinline__ void remote_store64(u64* p, uint32_t rank, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(p, rank)), "l"(v) : "memory");
 }
+__device__ __forceinline__ void remote_store32(uint32_t* p, uint32_t rank, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote(p, rank)), "r"(v) : "memory");
+}
 __device__ __forceinline__ uint32_t remote_add(uint32_t* p, uint32_t rank, uint32_t v) {
     uint32_t o;
     asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(o) : "r"(remote(p, rank)), "r"(v) : "memory");
@@ -194,13 +199,13 @@ struct Shared {
     u64 list[CAP];                         // collected tokens: key << 32 | ~index
     u64 masses[RANKED];                    // theirs
     uint32_t hist[4][256];                 // counts, and the masses' 13 + 13 + 14 bits
-    u64 bin_mass[2][256];                  // what they amount to: this CTA's, read by the cluster
-    uint32_t bin_count[2][256];
+    u64 bin_mass[256];                     // what they amount to: this CTA's, read by the cluster
+    uint32_t bin_count[256];
     u64 all_mass[256];                     // the cluster's
     uint32_t all_count[256], far_count[256];
     u64 warp[WARPS];
     u64 post[16];                          // values that the cluster's other CTAs read
-    u64 cross[3];                          // a crossing: its bin, and the running values before it
+    u64 cross[2];                          // a crossing: its bin, and the running value before it
     uint32_t queue[CAP];                   // vectors that hold a token to collect
     uint32_t vectors, collected[3];
     uint32_t flag;
@@ -451,56 +456,106 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
         mass_of.of(l, w);
         return w[0];
     };
-    // The tokens that the steps look at: the whole table or, once `dense`, those copied together behind it
-    uint32_t* copied_key = reinterpret_cast<uint32_t*>(vecs + nv);
+    // The tokens that the steps look at: the whole table or, once `dense`, those copied together behind it with
+    // their masses
+    u64* copied_mass = reinterpret_cast<u64*>(vecs + nv);
+    uint32_t* copied_key = reinterpret_cast<uint32_t*>(copied_mass + p.room);
     uint32_t* copied_place = copied_key + p.room;
     bool dense = false;
     int count_of = nv * E;
     auto key_at = [&](int i) { return dense ? copied_key[i] : (uint32_t)keys[i]; };
     auto place_at = [&](int i) { return dense ? copied_place[i] : (uint32_t)i; };
+    auto vector_keys = [&](const uint4& v, uint32_t* key) {
+        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < E; ++e) key[e] = E == 4 ? x[e & 3] : x[e / 2 & 3] >> 16 * (e & 1) & 0xffffu;
+    };
     // f(key, mass or 0) for all of them, any order, GROUP of a thread at a time
     auto each = [&](bool with_mass, auto&& f) {
+        if (dense) {
+#pragma unroll 2
+            for (int i = tid; i < count_of; i += ST) f(copied_key[i], with_mass ? copied_mass[i] : 0);
+            return;
+        }
+        constexpr int VECS = GROUP >= E ? GROUP / E : 1, N = VECS * E;
 #pragma unroll 1
-        for (int i = tid; i < count_of; i += GROUP * ST) {
-            uint32_t key[GROUP];
-            u64 w[GROUP] = {};
+        for (int i = tid; i < nv; i += VECS * ST) {
+            uint32_t key[N];
 #pragma unroll
-            for (int q = 0; q < GROUP; ++q) key[q] = i + q * ST < count_of ? key_at(i + q * ST) : 0;
+            for (int q = 0; q < VECS; ++q)
+                vector_keys(i + q * ST < nv ? vecs[i + q * ST] : make_uint4(0, 0, 0, 0), key + q * E);
+            u64 w[N] = {};
             if (with_mass) {
-                float l[GROUP];
+                float l[N];
 #pragma unroll
-                for (int q = 0; q < GROUP; ++q) l[q] = K::value(key[q]);
+                for (int q = 0; q < N; ++q) l[q] = K::value(key[q]);
                 mass_of.of(l, w);
             }
 #pragma unroll
-            for (int q = 0; q < GROUP; ++q) f(key[q], w[q]);
+            for (int q = 0; q < N; ++q) f(key[q], w[q]);
         }
     };
-    // copies the tokens whose keys reach `lo` together, in index order, where there is room for them
+    // copies the tokens whose keys reach `lo` together, in index order, where there is room for them: four
+    // consecutive keys to a lane
     auto copy_together = [&](uint32_t lo) {
-        if (p.room == 0 || dense) return;
-        const int piece = (count_of + WARPS - 1) / WARPS, a = min(warp * piece, count_of), b = min(a + piece, count_of);
+        if (MANY || p.room == 0 || dense) return;
+        auto four = [&](int i, uint32_t (&key)[4]) {
+            if constexpr (sizeof(key_t) == 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(keys + i);
+                key[0] = v.x, key[1] = v.y, key[2] = v.z, key[3] = v.w;
+            } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(keys + i);
+                key[0] = v.x & 0xffffu, key[1] = v.x >> 16, key[2] = v.y & 0xffffu, key[3] = v.y >> 16;
+            }
+        };
+        const int piece = ((count_of + WARPS - 1) / WARPS + 3) / 4 * 4, a = min(warp * piece, count_of), b = min(a + piece, count_of);
         uint32_t c = 0;
-        for (int i = a + lane; i < b; i += 32) c += keys[i] >= lo;
+#pragma unroll 2
+        for (int i = a + 4 * lane; i < b; i += 128) {
+            uint32_t key[4];
+            four(i, key);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c += key[e] >= lo;
+        }
         c = __reduce_add_sync(DG_FULL_MASK, c);
         u64 n;
         uint32_t at = (uint32_t)block_before(lane == 0 ? c : 0, &n, s);
         if (n > (u64)p.room) return;
         at = __shfl_sync(DG_FULL_MASK, at, 0);
-        for (int base = a; base < b; base += 32) {
-            const int i = base + lane;
-            const uint32_t key = i < b ? (uint32_t)keys[i] : 0;
-            const unsigned is = __ballot_sync(DG_FULL_MASK, key >= lo);
-            if (key >= lo) {
-                const uint32_t to = at + __popc(is & ((1u << lane) - 1));
-                copied_key[to] = key;
-                copied_place[to] = (uint32_t)i;
+#pragma unroll 2
+        for (int base = a; base < b; base += 128) {
+            const int i = base + 4 * lane;
+            uint32_t key[4] = {0, 0, 0, 0}, to = at;
+            if (i < b) four(i, key);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned is = __ballot_sync(DG_FULL_MASK, key[e] >= lo);
+                to += __popc(is & ((1u << lane) - 1));
+                at += __popc(is);
             }
-            at += __popc(is);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (key[e] >= lo) {
+                    copied_key[to] = key[e];
+                    copied_place[to++] = (uint32_t)(i + e);
+                }
         }
         __syncthreads();
         dense = true;
         count_of = (int)n;
+        // their masses, once for all the steps to come
+#pragma unroll 1
+        for (int i = tid; i < count_of; i += 4 * ST) {
+            float l[4];
+            u64 w[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) l[q] = K::value(i + q * ST < count_of ? copied_key[i + q * ST] : 1);
+            mass_of.of(l, w);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (i + q * ST < count_of) copied_mass[i + q * ST] = w[q];
+        }
+        __syncthreads();
     };
 
     // ---- collect the tokens that reach `bound`, and draw from them: thread t of the CTA that holds the
@@ -632,8 +687,8 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
             const float dist = (m - K::value(key)) * scale;
             return dist < 255.f ? (int)dist : dist == dist ? 255 : 0;
         };
-        int buf = 0;
-        // s.hist, counted by each CTA, becomes s.all_* over the cluster
+        // s.hist, counted by each CTA, becomes s.all_* over the cluster: each CTA adds up its part of the bins
+        // and sends it to all
         auto gather = [&](bool by_mass) {
             __syncthreads();
             if (tid < 256) {
@@ -644,61 +699,56 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                     w = (u64)s.hist[1][tid] + ((u64)s.hist[2][tid] << 13) + ((u64)s.hist[3][tid] << 26);
                     s.hist[1][tid] = s.hist[2][tid] = s.hist[3][tid] = 0;
                 }
-                if (C > 1) s.bin_mass[buf][tid] = w, s.bin_count[buf][tid] = c;
+                if (C > 1) s.bin_mass[tid] = w, s.bin_count[tid] = c;
                 else s.all_mass[tid] = w, s.all_count[tid] = c;
             }
             join(C);
             if (C > 1) {
-                const int b = tid >> 1;    // two threads to a bin
-                u64 w = 0;
-                uint32_t c = 0;
-                u64 rw[8];
-                uint32_t rc[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const int from = 2 * r + (tid & 1);
-                    rw[r] = by_mass && from < C ? remote_load64(&s.bin_mass[buf][b], from) : 0;
-                    rc[r] = from < C ? remote_load32(&s.bin_count[buf][b], from) : 0;
+                if (tid < 256) {           // thread: a bin of this CTA's and a CTA that it reads, then sends to
+                    const int with = tid & (C - 1), b = (rank * 256 + tid) / C;
+                    u64 w = by_mass ? remote_load64(&s.bin_mass[b], with) : 0;
+                    uint32_t c = remote_load32(&s.bin_count[b], with);
+                    for (int o = 1; o < C; o <<= 1) {
+                        if (by_mass) w += __shfl_xor_sync(DG_FULL_MASK, w, o);
+                        c += __shfl_xor_sync(DG_FULL_MASK, c, o);
+                    }
+                    if (by_mass) remote_store64(&s.all_mass[b], with, w);
+                    remote_store32(&s.all_count[b], with, c);
                 }
-#pragma unroll
-                for (int r = 0; r < 8; ++r) w += rw[r], c += rc[r];
-                w += __shfl_xor_sync(DG_FULL_MASK, w, 1);
-                c += __shfl_xor_sync(DG_FULL_MASK, c, 1);
-                if (!(tid & 1)) s.all_mass[b] = w, s.all_count[b] = c;
-                __syncthreads();
+                join(C);
             }
-            buf ^= 1;
         };
-        // the bin in which the running count or mass (from `count0`, `mass0`) reaches the target, and the
-        // running values before it; false where it does not.  One warp looks, lane l at bins 8 l to 8 l + 7.
-        auto crossing = [&](bool by_mass, u64 target, u64& count0, u64& mass0, int& bin_out) {
+        // the bin in which the running count or mass (from `run0`) reaches the target, and the running value
+        // before it; false where it does not.  One warp looks, lane l at bins 8 l to 8 l + 7, then eight lanes at
+        // those of the one that holds it.
+        auto crossing = [&](bool by_mass, u64 target, u64& run0, int& bin_out) {
             if (warp == 0) {
-                uint32_t c[8], sc = 0;
-                u64 w[8], sw = 0;
+                u64 v = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    c[i] = s.all_count[8 * lane + i], sc += c[i];
-                    w[i] = by_mass ? s.all_mass[8 * lane + i] : 0, sw += w[i];
-                }
-                u64 rc = warp_scan(sc, lane) + count0, rw = warp_scan(sw, lane) + mass0;
-                const unsigned hit = __ballot_sync(DG_FULL_MASK, (by_mass ? rw : rc) >= target);
-                if (hit && lane == __ffs(hit) - 1) {
-                    rc -= sc;
-                    rw -= sw;
-                    int bin = 8 * lane;
+                for (int i = 0; i < 8; ++i) v += by_mass ? s.all_mass[8 * lane + i] : s.all_count[8 * lane + i];
+                u64 run = warp_scan(v, lane) + run0;
+                const unsigned hit = __ballot_sync(DG_FULL_MASK, run >= target);
+                if (hit) {
+                    const int h = __ffs(hit) - 1, b = 8 * h + (lane & 7);
+                    run = __shfl_sync(DG_FULL_MASK, run - v, h);
+                    v = by_mass ? s.all_mass[b] : s.all_count[b];
+                    u64 to = v;
 #pragma unroll
-                    for (int i = 0; i < 7; ++i)
-                        if (bin == 8 * lane + i && (by_mass ? rw + w[i] : rc + c[i]) < target) rc += c[i], rw += w[i], ++bin;
-                    s.cross[0] = (u64)bin, s.cross[1] = rc, s.cross[2] = rw;
+                    for (int o = 1; o < 8; o <<= 1) {
+                        const u64 x = __shfl_up_sync(DG_FULL_MASK, to, o, 8);
+                        if ((lane & 7) >= o) to += x;
+                    }
+                    const unsigned in = __ballot_sync(DG_FULL_MASK, run + to >= target);
+                    if (lane == __ffs(in) - 1) s.cross[0] = (u64)b, s.cross[1] = run + to - v;
+                } else if (lane == 0) {
+                    s.cross[0] = ~0ull;
                 }
-                if (!hit && lane == 0) s.cross[0] = ~0ull;
             }
             __syncthreads();
             const u64 b = s.cross[0];
             if (b == ~0ull) return false;
             bin_out = (int)b;
-            count0 = s.cross[1];
-            mass0 = s.cross[2];
+            run0 = s.cross[1];
             return true;
         };
         // keys that surely hold bins [blo, bhi], rounding errors of m and the distance included
@@ -713,12 +763,12 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
         };
 
         // The cut: the token at which the count or mass reaches the target, expected in bins [blo, bhi] with
-        // `count0` tokens before them.  Leaves cut and ties, and returns false where the target is not in
+        // `before_bins` tokens before them.  Leaves cut and ties, and returns false where the target is not in
         // those bins.
         int uses = 0, sums = 0;
-        auto resolve = [&](bool by_mass, u64 target, int blo, int bhi, u64 count0) {
+        auto resolve = [&](bool by_mass, u64 target, int blo, int bhi, u64 before_bins) {
             uint32_t lo = lowest(bhi), hi = highest(blo);
-            u64 mass0 = 0;
+            u64 run0 = before_bins;        // count or mass above the range
             for (int level = 0;; ++level) {
                 int shift = 0, bin;
                 while (((hi - lo) >> shift) > 255) ++shift;
@@ -745,10 +795,10 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                 if (by_mass && level == 0) {
                     if (C > 1) above = warp_sum(lane < C ? remote_load64(&s.post[8 + sums], lane) : 0);
                     ++sums;
-                    mass0 = above;
-                    if (mass0 >= target) return false;
+                    run0 = above;
+                    if (run0 >= target) return false;
                 }
-                if (!crossing(by_mass, target, count0, mass0, bin)) return false;
+                if (!crossing(by_mass, target, run0, bin)) return false;
                 const uint32_t here = s.all_count[bin];
                 const uint32_t top = hi - ((uint32_t)bin << shift), bottom = top - ((1u << shift) - 1);
                 lo = bottom > lo && bottom <= top ? bottom : lo;
@@ -757,7 +807,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                     // one key: as many of its tokens as the target asks for
                     const u64 w = mass(hi);
                     cut = hi;
-                    ties = by_mass ? (target - mass0 + w - 1) / w : target - count0;
+                    ties = by_mass ? (target - run0 + w - 1) / w : target - run0;
                     if (ties == here) --cut, ties = 0;             // all of them: simply the keys above
                     return true;
                 }
@@ -793,8 +843,8 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                 over += __shfl_xor_sync(DG_FULL_MASK, over, 1);
                 same += __shfl_xor_sync(DG_FULL_MASK, same, 1);
                 before += __shfl_xor_sync(DG_FULL_MASK, before, 1);
-                const bool it = by_mass ? mass0 + before < target && mass0 + before + w >= target
-                                        : count0 + rank_ + 1 == target;
+                const bool it = by_mass ? run0 + before < target && run0 + before + w >= target
+                                        : run0 + rank_ + 1 == target;
                 if (c < nc && q == 0 && it) {
                     const uint32_t n = rank_ - over + 1;           // of its key, this many
                     s.post[12] = (u64)(n == same ? (uint32_t)(mine >> 32) - 1 : (uint32_t)(mine >> 32)) << 32 | (n == same ? 0 : n);
@@ -836,8 +886,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                 if (tid < 256) s.far_count[tid] = s.all_count[tid];
                 step = cut_k ? TOP_K : GUESS;
                 if (cut_k) {
-                    u64 w0 = 0;
-                    if (!crossing(false, (u64)k, c0, w0, blo)) step = GUESS;
+                    if (!crossing(false, (u64)k, c0, blo)) step = GUESS;
                     bhi = blo;
                 }
             }
@@ -921,21 +970,26 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
     };
     // f(token, its mass or 0) over [a, b) in index order, a token to a lane, `seen` tokens with the cut key
     // before them
-    auto walk = [&](int a, int b, uint32_t seen, auto&& f) {
+    auto walk = [&](auto group, int a, int b, uint32_t seen, auto&& f) {
+        constexpr int N = decltype(group)::value;
 #pragma unroll 1
-        for (int base = a; base < b; base += 32 * GROUP) {
-            uint32_t key[GROUP];
-            float l[GROUP];
-            u64 w[GROUP];
+        for (int base = a; base < b; base += 32 * N) {
+            uint32_t key[N];
+            u64 w[N];
 #pragma unroll
-            for (int q = 0; q < GROUP; ++q) {
+            for (int q = 0; q < N; ++q) {
                 const int i = base + 32 * q + lane;
                 key[q] = i < b ? key_at(i) : 0;
-                l[q] = K::value(key[q]);
+                if (dense) w[q] = i < b ? copied_mass[i] : 0;
             }
-            mass_of.of(l, w);
+            if (!dense) {
+                float l[N];
 #pragma unroll
-            for (int q = 0; q < GROUP; ++q) {
+                for (int q = 0; q < N; ++q) l[q] = K::value(key[q]);
+                mass_of.of(l, w);
+            }
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
                 bool in = key[q] > cut;
                 if (ties) {
                     const unsigned is = __ballot_sync(DG_FULL_MASK, key[q] == cut);
@@ -946,9 +1000,9 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
             }
         }
     };
-    auto sum_of = [&](int a, int b, uint32_t seen) {
+    auto sum_of = [&](auto group, int a, int b, uint32_t seen) {
         u64 v = 0;
-        walk(a, b, seen, [&](int, u64 w) { v += w; });
+        walk(group, a, b, seen, [&](int, u64 w) { v += w; });
         return warp_sum(v);
     };
     int a0 = min(warp * piece, count_of), a1 = min(a0 + piece, count_of);
@@ -963,7 +1017,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
             seen += __reduce_add_sync(DG_FULL_MASK, lane < rank ? (uint32_t)v : 0u);
         }
     }
-    u64 mine = sum_of(a0, a1, seen), total;
+    u64 mine = sum_of(std::integral_constant<int, GROUP>(), a0, a1, seen), total;
     u64 start = block_before(lane == 0 ? mine : 0, &total, s);
     start = __shfl_sync(DG_FULL_MASK, start, 0);
     u64 cta_start = 0;
@@ -990,13 +1044,14 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
         const u64 before = block_before(lane == 0 ? c : 0, &all, s);
         seen += (uint32_t)__shfl_sync(DG_FULL_MASK, before, 0);
     }
-    mine = sum_of(a0, a1, seen);
+    const std::integral_constant<int, 1> one_each;             // few tokens to a warp now
+    mine = sum_of(one_each, a0, a1, seen);
     u64 all;
     const u64 before = block_before(lane == 0 ? mine : 0, &all, s);
     start += __shfl_sync(DG_FULL_MASK, before, 0);
     if (start <= at && at < start + mine) {
         u64 run = start;
-        walk(a0, a1, seen, [&](int i, u64 w) {
+        walk(one_each, a0, a1, seen, [&](int i, u64 w) {
             const u64 inc = warp_scan(w, lane), r = run + inc - w;
             if (r <= at && at < r + w) {
                 p.token[row] = (int64_t)s0 + (int)place_at(i) - off;
@@ -1021,12 +1076,12 @@ template <typename T> int run(SampleParams p, int B, cudaStream_t stream) {
     p.cluster = cluster_of(B, p.V, sizeof(T));
     p.slice = ((p.V + p.cluster - 1) / p.cluster + 7) / 8 * 8;
     if ((int64_t)B * p.cluster > 0x7fffffff) return DG_ERR_UNSUPPORTED;
-    // the table and, beside a cluster's slice, room for half of its tokens (8 bytes each) as far as it goes
+    // the table and, beside a cluster's slice, room for half of its tokens (16 bytes each) as far as it goes
     size_t smem = (size_t)(p.slice + 16) * sizeof(T) + 16;
     if (p.cluster > 1) {
-        const size_t left = (180 * 1024 - smem) / 8;
+        const size_t left = (180 * 1024 - smem) / 16;
         p.room = (int)(left < (size_t)p.slice / 2 ? left : (size_t)p.slice / 2);
-        smem += (size_t)p.room * 8;
+        smem += (size_t)p.room * 16;
     }
     auto kern = p.cluster == 1 ? sample_kernel<T, true> : sample_kernel<T, false>;
     return dg_host::launch_lm(kern, dim3((unsigned)(B * p.cluster)), dim3(ST), smem, p.cluster > 1 ? p.cluster : 0, stream, p);
