@@ -173,11 +173,6 @@ __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
     return a;
 }
-__device__ __forceinline__ u64 remote_load64(const u64* p, uint32_t rank) {
-    u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote(p, rank)));
-    return v;
-}
 __device__ __forceinline__ uint32_t remote_load32(const uint32_t* p, uint32_t rank) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote(p, rank)));
@@ -185,6 +180,9 @@ __device__ __forceinline__ uint32_t remote_load32(const uint32_t* p, uint32_t ra
 }
 __device__ __forceinline__ void remote_store64(u64* p, uint32_t rank, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(p, rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ void remote_store128(void* p, uint32_t rank, uint4 v) {
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(remote(p, rank)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ void remote_store32(uint32_t* p, uint32_t rank, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote(p, rank)), "r"(v) : "memory");
@@ -195,16 +193,17 @@ __device__ __forceinline__ uint32_t remote_add(uint32_t* p, uint32_t rank, uint3
     return o;
 }
 
-struct Shared {
+struct alignas(16) Shared {
     u64 list[CAP];                         // collected tokens: key << 32 | ~index
     u64 masses[RANKED];                    // theirs
     uint32_t hist[4][256];                 // counts, and the masses' 13 + 13 + 14 bits
-    u64 bin_mass[256];                     // what they amount to: this CTA's, read by the cluster
+    u64 bin_mass[256];                     // what they amount to: every CTA's, this one's part of the bins
     uint32_t bin_count[256];
     u64 all_mass[256];                     // the cluster's
     uint32_t all_count[256], far_count[256];
     u64 warp[WARPS];
-    u64 post[16];                          // values that the cluster's other CTAs read
+    u64 sent[4][16], extra[16];            // values from the cluster's CTAs
+    u64 found[2];                          // where a cut lies; the piece that holds the draw
     u64 cross[2];                          // a crossing: its bin, and the running value before it
     uint32_t queue[CAP];                   // vectors that hold a token to collect
     uint32_t vectors, collected[3];
@@ -282,13 +281,13 @@ __device__ __forceinline__ u64 block_before(u64 v, u64* total, Shared& s) {
     if (warp == 0) before = 0;
     return before + inc - v;
 }
-// One value per CTA of the cluster, in lane r the value of CTA r (0 beyond): one remote load each, side by
-// side.  A slot is written again only after a barrier that follows its last reading.
-__device__ __forceinline__ u64 over_cluster(u64 v, int slot, int cluster, Shared& s) {
-    if (threadIdx.x == 0) s.post[slot] = v;
+// One value per CTA of the cluster, in lane r the value of CTA r (0 beyond).  Values are sent, not fetched: after
+// the barrier they are here, and no CTA's memory is read from outside.  Each slot is used once.
+__device__ __forceinline__ u64 over_cluster(u64 v, int slot, int cluster, int rank, Shared& s) {
+    if (threadIdx.x < cluster) remote_store64(&s.sent[slot][rank], threadIdx.x, v);
     join(cluster);
     const int lane = threadIdx.x & 31;
-    return lane < cluster ? remote_load64(&s.post[slot], lane) : 0;
+    return lane < cluster ? s.sent[slot][lane] : 0;
 }
 
 // sorts list[0, n2) (n2 a power of two, 64 to 1024) by the first n2 / 2 threads, one exchange per thread
@@ -328,6 +327,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
     const int V = p.V, s0 = min(rank * p.slice, V), n = min(p.slice, V - s0);
     const T* src = static_cast<const T*>(p.logits) + (int64_t)row * p.row_stride + s0;
 
+    if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");       // (waited for before the first sending)
     dg::let_next_start();
     dg::wait_for_previous();
     // ---- parameters
@@ -436,7 +436,9 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
     }
     if (C > 1) {
         // j tokens of each CTA reach its bound, so C j reach the smallest
-        const u64 v = over_cluster(mx << 32 | (0xffffffffu - bound), 0, C, s);
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");        // all CTAs have started
+        const u64 v = over_cluster(mx << 32 | (0xffffffffu - bound), 0, C, rank, s);
         mx = __reduce_max_sync(DG_FULL_MASK, (uint32_t)(v >> 32));
         bound = 0xffffffffu - __reduce_max_sync(DG_FULL_MASK, (uint32_t)v);
     }
@@ -446,7 +448,6 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
             p.token[row] = -1;
             if (p.logprob) p.logprob[row] = -INFINITY;
         }
-        if (C > 1) join(C);                // the others may still read this CTA's slot
         return;
     }
     const Mass mass_of(m, tdiv);
@@ -598,6 +599,10 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                 p.token[row] = (int64_t)(0xffffffffu - (uint32_t)entry);
                 if (p.logprob) p.logprob[row] = logf(__fdiv_rn((float)w, (float)total));
             };
+            auto say = [&](bool enough) {  // rank 0's verdict, to all
+                if (C == 1) s.flag = enough;
+                else if (tid < C) remote_store32(&s.flag, tid, enough);
+            };
             const int lim = min(nc, k);
             if (nc <= RANKED) {
                 // `part` threads share a token; each compares it with every part-th of the list
@@ -624,7 +629,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                 if (total_k == 0) total_k = k_mass;
                 const u64 tau = max(fraction_of(P, total_k, true), 1ull);
                 const bool enough = k_mass >= tau;
-                if (tid == 0) s.flag = enough;
+                say(enough);
                 const bool keep = in_k && before < tau && w >= least;
                 if (q == 0 && c < nc && !keep) s.masses[c] = 0;
                 sum = block_sum(keep && q == 0 ? w : 0, s);      // its barriers also order masses[]
@@ -651,7 +656,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                     const u64 before = part_before(w0 + w1, &sum, n2 / 2, s);
                     const u64 tau = max(fraction_of(P, total_k ? total_k : sum, true), 1ull);
                     const bool enough = sum >= tau;
-                    if (tid == 0) s.flag = enough;
+                    say(enough);
                     // the kept ones by index, the others behind them
                     if (before + w0 >= tau || w1 < least) w1 = 0;
                     if (before >= tau || w0 < least) w0 = 0;
@@ -672,9 +677,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
             }
         }
         join(C);                           // rank 0's counter has been read, its verdict is there
-        const bool done = (C > 1 ? remote_load32(&s.flag, 0) : s.flag) != 0;
-        if (C > 1) join(C);
-        return done;
+        return s.flag != 0;
     };
 
     uint32_t cut = 0;                      // kept: key > cut, and the first `ties` with key == cut
@@ -687,36 +690,61 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
             const float dist = (m - K::value(key)) * scale;
             return dist < 255.f ? (int)dist : dist == dist ? 255 : 0;
         };
-        // s.hist, counted by each CTA, becomes s.all_* over the cluster: each CTA adds up its part of the bins
-        // and sends it to all
-        auto gather = [&](bool by_mass) {
+        // s.hist, counted by each CTA, becomes s.all_* over the cluster: each CTA gets all counts of its part of
+        // the bins, adds them up and sends the sums to all, 16 bytes at a time (a warp's remote store takes some
+        // 5 cycles a lane, whatever its width).  Returns the sum of `extra`.
+        auto bin_masses = [&](int b) {
+            const u64 w = (u64)s.hist[1][b] + ((u64)s.hist[2][b] << 13) + ((u64)s.hist[3][b] << 26);
+            s.hist[1][b] = s.hist[2][b] = s.hist[3][b] = 0;
+            return w;
+        };
+        auto gather = [&](bool by_mass, u64 extra) {
             __syncthreads();
-            if (tid < 256) {
-                const uint32_t c = s.hist[0][tid];
-                u64 w = 0;
-                s.hist[0][tid] = 0;
-                if (by_mass) {
-                    w = (u64)s.hist[1][tid] + ((u64)s.hist[2][tid] << 13) + ((u64)s.hist[3][tid] << 26);
-                    s.hist[1][tid] = s.hist[2][tid] = s.hist[3][tid] = 0;
+            if (C == 1) {
+                if (tid < 256) {
+                    s.all_count[tid] = s.hist[0][tid];
+                    s.hist[0][tid] = 0;
+                    if (by_mass) s.all_mass[tid] = bin_masses(tid);
                 }
-                if (C > 1) s.bin_mass[tid] = w, s.bin_count[tid] = c;
-                else s.all_mass[tid] = w, s.all_count[tid] = c;
+                __syncthreads();
+                return extra;
+            }
+            const int part = 256 / C;
+            const int b4 = 4 * tid, b2 = 2 * (tid - 64);
+            const bool counts = tid < 64, masses = by_mass && tid >= 64 && tid < 192;
+            if (counts) {
+                uint4* at = reinterpret_cast<uint4*>(&s.hist[0][b4]);
+                remote_store128(&s.bin_count[rank * part + (b4 & (part - 1))], b4 / part, *at);
+                *at = make_uint4(0, 0, 0, 0);
+            } else if (masses) {
+                const u64 w0 = bin_masses(b2), w1 = bin_masses(b2 + 1);
+                remote_store128(&s.bin_mass[rank * part + (b2 & (part - 1))], b2 / part,
+                                make_uint4((uint32_t)w0, (uint32_t)(w0 >> 32), (uint32_t)w1, (uint32_t)(w1 >> 32)));
+            } else if (tid >= 192 && tid - 192 < C) {
+                remote_store64(&s.extra[rank], tid - 192, extra);
             }
             join(C);
-            if (C > 1) {
-                if (tid < 256) {           // thread: a bin of this CTA's and a CTA that it reads, then sends to
-                    const int with = tid & (C - 1), b = (rank * 256 + tid) / C;
-                    u64 w = by_mass ? remote_load64(&s.bin_mass[b], with) : 0;
-                    uint32_t c = remote_load32(&s.bin_count[b], with);
-                    for (int o = 1; o < C; o <<= 1) {
-                        if (by_mass) w += __shfl_xor_sync(DG_FULL_MASK, w, o);
-                        c += __shfl_xor_sync(DG_FULL_MASK, c, o);
-                    }
-                    if (by_mass) remote_store64(&s.all_mass[b], with, w);
-                    remote_store32(&s.all_count[b], with, c);
+            extra = warp_sum(lane < C ? s.extra[lane] : 0);
+            if (counts) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+                for (int r = 0; r < C; ++r) {
+                    const uint4 c = *reinterpret_cast<const uint4*>(&s.bin_count[r * part + (b4 & (part - 1))]);
+                    v.x += c.x, v.y += c.y, v.z += c.z, v.w += c.w;
                 }
-                join(C);
+                remote_store128(&s.all_count[rank * part + (b4 & (part - 1))], b4 / part, v);
+            } else if (masses) {
+                u64 w0 = 0, w1 = 0;
+#pragma unroll 4
+                for (int r = 0; r < C; ++r) {
+                    const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&s.bin_mass[r * part + (b2 & (part - 1))]);
+                    w0 += w.x, w1 += w.y;
+                }
+                remote_store128(&s.all_mass[rank * part + (b2 & (part - 1))], b2 / part,
+                                make_uint4((uint32_t)w0, (uint32_t)(w0 >> 32), (uint32_t)w1, (uint32_t)(w1 >> 32)));
             }
+            join(C);
+            return extra;
         };
         // the bin in which the running count or mass (from `run0`) reaches the target, and the running value
         // before it; false where it does not.  One warp looks, lane l at bins 8 l to 8 l + 7, then eight lanes at
@@ -765,7 +793,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
         // The cut: the token at which the count or mass reaches the target, expected in bins [blo, bhi] with
         // `before_bins` tokens before them.  Leaves cut and ties, and returns false where the target is not in
         // those bins.
-        int uses = 0, sums = 0;
+        int uses = 0;
         auto resolve = [&](bool by_mass, u64 target, int blo, int bhi, u64 before_bins) {
             uint32_t lo = lowest(bhi), hi = highest(blo);
             u64 run0 = before_bins;        // count or mass above the range
@@ -787,14 +815,9 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                         atomicAdd(&s.hist[3][at], (uint32_t)(w >> 26));
                     }
                 });
+                if (by_mass && level == 0) above = block_sum(above, s);
+                above = gather(by_mass, above);
                 if (by_mass && level == 0) {
-                    above = block_sum(above, s);
-                    if (tid == 0) s.post[8 + sums] = above;        // read after the barrier in gather
-                }
-                gather(by_mass);
-                if (by_mass && level == 0) {
-                    if (C > 1) above = warp_sum(lane < C ? remote_load64(&s.post[8 + sums], lane) : 0);
-                    ++sums;
                     run0 = above;
                     if (run0 >= target) return false;
                 }
@@ -847,14 +870,16 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                                         : run0 + rank_ + 1 == target;
                 if (c < nc && q == 0 && it) {
                     const uint32_t n = rank_ - over + 1;           // of its key, this many
-                    s.post[12] = (u64)(n == same ? (uint32_t)(mine >> 32) - 1 : (uint32_t)(mine >> 32)) << 32 | (n == same ? 0 : n);
+                    const u64 where = (u64)((uint32_t)(mine >> 32) - (n == same)) << 32 | (n == same ? 0 : n);
+                    if (C == 1) s.found[0] = where;
+                    else
+                        for (int r = 0; r < C; ++r) remote_store64(&s.found[0], r, where);
                 }
             }
             join(C);
-            const u64 answer = C > 1 ? remote_load64(&s.post[12], 0) : s.post[12];
+            const u64 answer = s.found[0];
             cut = (uint32_t)(answer >> 32);
             ties = answer & 0xffffffffu;
-            join(C);                       // the slots have been read, the list too
             return true;
         };
 
@@ -880,9 +905,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                     all += w;
                 });
                 all = block_sum(all, s);
-                if (tid == 0) s.post[6] = all;
-                gather(false);
-                total_k = C > 1 ? warp_sum(lane < C ? remote_load64(&s.post[6], lane) : 0) : all;
+                total_k = gather(false, all);
                 if (tid < 256) s.far_count[tid] = s.all_count[tid];
                 step = cut_k ? TOP_K : GUESS;
                 if (cut_k) {
@@ -896,7 +919,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
                     u64 w = 0;
                     each(true, [&](uint32_t key, u64 v) { w += key > cut ? v : 0; });
                     w = block_sum(w, s);
-                    if (C > 1) w = warp_sum(over_cluster(w, 7, C, s));
+                    if (C > 1) w = warp_sum(over_cluster(w, 1, C, rank, s));
                     total_k = w + (ties ? ties * mass(cut) : 0);
                 }
                 tau = max(fraction_of(P, total_k, true), 1ull);
@@ -1013,7 +1036,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
         const u64 before = block_before(lane == 0 ? c : 0, &all, s);
         seen = (uint32_t)__shfl_sync(DG_FULL_MASK, before, 0);
         if (C > 1) {
-            const u64 v = over_cluster(all, 4, C, s);
+            const u64 v = over_cluster(all, 2, C, rank, s);
             seen += __reduce_add_sync(DG_FULL_MASK, lane < rank ? (uint32_t)v : 0u);
         }
     }
@@ -1023,20 +1046,19 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
     u64 cta_start = 0;
     const u64 cta_mass = total;
     if (C > 1) {
-        const u64 v = over_cluster(total, 5, C, s);
+        const u64 v = over_cluster(total, 3, C, rank, s);
         cta_start = warp_sum(lane < rank ? v : 0);
         total = warp_sum(v);
         start += cta_start;
-        join(C);                           // all slots have been read: any CTA may end
     }
     const u64 at = fraction_of(U, total, false);
     if (at < cta_start || at >= cta_start + cta_mass) return;
     // the CTA whose keys hold the draw: all its warps share the piece that does
-    if (lane == 0 && start <= at && at < start + mine) s.flag = (uint32_t)warp, s.post[6] = start, s.post[7] = seen;
+    if (lane == 0 && start <= at && at < start + mine) s.flag = (uint32_t)warp, s.found[0] = start, s.found[1] = seen;
     __syncthreads();
     const int base = min((int)s.flag * piece, count_of), last = min(base + piece, count_of), part = ((last - base + WARPS - 1) / WARPS + 31) / 32 * 32;
-    start = s.post[6];
-    seen = (uint32_t)s.post[7];
+    start = s.found[0];
+    seen = (uint32_t)s.found[1];
     a0 = min(base + warp * part, last), a1 = min(a0 + part, last);
     if (ties) {
         const uint32_t c = ties_in(a0, a1);
