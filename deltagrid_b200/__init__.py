@@ -5,7 +5,10 @@
 * ``deltagrid_b200.install()`` -- registers it under that name in sys.modules so
   the reference loader (src/ops/_backend.py) finds it;
 * ``deltagrid_b200._lib`` -- the ctypes binding of the C ABI
-  (include/deltagrid_b200.h) that both sit on.
+  (include/deltagrid_b200.h) that both sit on;
+* ``deltagrid_b200.recurrence``, ``.ffn``, ``.sampling`` -- a gated linear recurrence, a
+  gated feed-forward block and token sampling for models built on the memory layer, and
+  ``deltagrid_b200.hybrid`` -- a small language model of them.
 """
 from __future__ import annotations
 
