@@ -460,43 +460,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
 }
 
-// dbias[c] = sum over the 32-row sums, in a fixed order: warp w of the block takes rows w, w + 32, ...
+// What a backward pass still has to add up, in one launch after its products: the fp32 partial products of a
+// split dx or dW, in order of the splits (8 values a thread), and dbias from its sums over 32
+// rows, in a fixed order (32 columns a block, warp w takes rows w, w + 32, ...).
+struct Join {
+    const float4* part;
+    uint4* out;
+    int64_t n8;                            // outputs / 8
+    int splits, blocks;
+};
+constexpr int kFinish = 1024;
 template <typename T>
-__global__ void __launch_bounds__(1024) colsum_kernel(int rows, int cols, const float* part, T* out) {
+__global__ void __launch_bounds__(kFinish) finish_kernel(Join dx, Join dw, const float* sums, int rows, int cols, T* dbias) {
     __shared__ float s[32][33];
     dg::let_next_start();
     dg::wait_for_previous();
-    const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, w = threadIdx.x >> 5;
+    int block = (int)blockIdx.x - (dbias ? (cols + 31) / 32 : 0);      // dbias first: its chains are the longest
+    if (block >= 0) {
+        const Join& q = block < dx.blocks ? dx : dw;
+        if (block >= dx.blocks) block -= dx.blocks;
+        const int64_t i = (int64_t)block * kFinish + threadIdx.x;
+        if (i >= q.n8) return;
+        float4 a = q.part[2 * i], b = q.part[2 * i + 1];
+#pragma unroll 4
+        for (int k = 1; k < q.splits; ++k) {
+            const float4 c = q.part[2 * (q.n8 * k + i)], d = q.part[2 * (q.n8 * k + i) + 1];
+            a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+            b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
+        }
+        uint4 v;
+        v.x = dgc::Io<T>::pack2(a.x, a.y);
+        v.y = dgc::Io<T>::pack2(a.z, a.w);
+        v.z = dgc::Io<T>::pack2(b.x, b.y);
+        v.w = dgc::Io<T>::pack2(b.z, b.w);
+        q.out[i] = v;
+        return;
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float a = 0.f;
     if (c < cols)
-        for (int r = w; r < rows; r += 32) a += part[(int64_t)r * cols + c];
-    s[w][lane] = a;
+        for (int r = warp; r < rows; r += 32) a += sums[(int64_t)r * cols + c];
+    s[warp][lane] = a;
     __syncthreads();
-    float v = s[lane][w];                  // column w of the block, partial sum `lane`
+    a = s[lane][warp];                     // column `warp` of the block, partial sum `lane`
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(DG_FULL_MASK, v, o);
-    if (lane == 0 && blockIdx.x * 32 + w < cols) out[blockIdx.x * 32 + w] = dg::from_f<T>(v);
-}
-
-// out = sum of the fp32 partial products, in order of the splits
-template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(int64_t n8, int splits, const float4* part, uint4* out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    dg::let_next_start();
-    dg::wait_for_previous();
-    if (i >= n8) return;
-    float4 a = part[2 * i], b = part[2 * i + 1];
-    for (int s = 1; s < splits; ++s) {
-        const float4 c = part[2 * (n8 * s + i)], d = part[2 * (n8 * s + i) + 1];
-        a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
-        b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
-    }
-    uint4 v;
-    v.x = dgc::Io<T>::pack2(a.x, a.y);
-    v.y = dgc::Io<T>::pack2(a.z, a.w);
-    v.z = dgc::Io<T>::pack2(b.x, b.y);
-    v.w = dgc::Io<T>::pack2(b.z, b.w);
-    out[i] = v;
+    for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(DG_FULL_MASK, a, o);
+    if (lane == 0 && blockIdx.x * 32 + warp < cols) dbias[blockIdx.x * 32 + warp] = dg::from_f<T>(a);
 }
 
 CUtensorMapDataType map_type(bool bf16) {
@@ -571,10 +580,11 @@ int splits_of(int64_t M, int N, int64_t K, int np) {
     return (int)(s < 1 ? 1 : s);
 }
 
-// C [M,N] = A B, contracted length K; A as [M,K] (a_mn: [K,M]), B as [N,K] (b_mn: [K,N])
+// C [M,N] = A B, contracted length K; A as [M,K] (a_mn: [K,M]), B as [N,K] (b_mn: [K,N]).  Where it is split,
+// `join` gets what remains to be added up.
 template <typename T, bool A_MN, bool B_MN>
 int product(int64_t M, int N, int64_t K, const void* a, int64_t lda, const void* b, int64_t ldb, void* c, float* part,
-            int splits, int32_t* status, cudaStream_t s) {
+            int splits, Join* join, int32_t* status, cudaStream_t s) {
     constexpr bool bf16 = !std::is_same<T, __half>::value;
     FfnParams p = tiles_of(M, N, (int)K, BN, status);
     const int nkb = p.kb_per_split;
@@ -591,20 +601,20 @@ int product(int64_t M, int N, int64_t K, const void* a, int64_t lda, const void*
                          splits > 1 ? static_cast<void*>(part) : c, 3, dims, strides, box);
     if (!ok) return DG_ERR_UNSUPPORTED;
     const int64_t items = (int64_t)p.m_tiles * p.n_tiles * p.splits;
-    if (splits == 1)
-        return launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, false, 128>, (Cfg<PLAIN, 128>::BYTES), items, ma, mb, ma, mo, p, s);
-    const int rc = launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, true, 128>, (Cfg<PLAIN, 128>::BYTES), items, ma, mb, ma, mo, p, s);
-    if (rc != DG_OK) return rc;
-    const int64_t n8 = M * N / 8;
-    return launch_lm(join_kernel<T>, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, 0, s, n8, splits,
-                     reinterpret_cast<const float4*>(part), static_cast<uint4*>(c));
+    if (splits > 1) {
+        const int64_t n8 = M * N / 8;
+        *join = {reinterpret_cast<const float4*>(part), static_cast<uint4*>(c), n8, splits, (int)((n8 + kFinish - 1) / kFinish)};
+    }
+    return splits == 1
+               ? launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, false, 128>, (Cfg<PLAIN, 128>::BYTES), items, ma, mb, ma, mo, p, s)
+               : launch(ffn_tc_kernel<T, PLAIN, 0, A_MN, B_MN, true, 128>, (Cfg<PLAIN, 128>::BYTES), items, ma, mb, ma, mo, p, s);
 }
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
 struct Spaces {
-    size_t dz, colsum, part, total;
+    size_t dz, colsum, part_dx, part_dw, total;
     int splits_dx, splits_dw;
 };
 Spaces spaces(int64_t M, int D, int F) {
@@ -615,10 +625,9 @@ Spaces spaces(int64_t M, int D, int F) {
     w.splits_dw = splits_of(2 * (int64_t)F, D, M, np);
     w.dz = round256((size_t)M * 2 * F * 2);
     w.colsum = round256((size_t)((M + 2 * BM - 1) / (2 * BM)) * 8 * 2 * F * 4);
-    const size_t dx = w.splits_dx > 1 ? (size_t)w.splits_dx * M * D * 4 : 0;
-    const size_t dw = w.splits_dw > 1 ? (size_t)w.splits_dw * 2 * F * D * 4 : 0;
-    w.part = round256(dx > dw ? dx : dw);
-    w.total = w.dz + w.colsum + w.part;
+    w.part_dx = round256(w.splits_dx > 1 ? (size_t)w.splits_dx * M * D * 4 : 0);
+    w.part_dw = round256(w.splits_dw > 1 ? (size_t)w.splits_dw * 2 * F * D * 4 : 0);
+    w.total = w.dz + w.colsum + w.part_dx + w.part_dw;
     return w;
 }
 
@@ -696,7 +705,8 @@ static int backward_t(int64_t M, int D, int F, int act, const void* x, int64_t l
     char* ws = static_cast<char*>(workspace);
     void* dz = ws;
     float* colsum = reinterpret_cast<float*>(ws + sp.dz);
-    float* part = reinterpret_cast<float*>(ws + sp.dz + sp.colsum);
+    float* part_dx = reinterpret_cast<float*>(ws + sp.dz + sp.colsum);
+    float* part_dw = reinterpret_cast<float*>(ws + sp.dz + sp.colsum + sp.part_dx);
     FfnParams p = tiles_of(M, F, D, BM, status);
     p.bias = bias;
     p.colsum = db ? colsum : nullptr;
@@ -707,14 +717,15 @@ static int backward_t(int64_t M, int D, int F, int act, const void* x, int64_t l
     if (!map_matrix(&md, dh, M, F, ld_dh, BM, bf16) || !make_tmap(&mz, map_type(bf16), dz, 3, dims, strides, box))
         return DG_ERR_UNSUPPORTED;
     int rc = gate<T, DGATE>(M, D, F, act, x, ldx, w, md, mz, p, s);
+    Join join_dx{}, join_dw{};
     if (rc == DG_OK && dx)
-        rc = product<T, false, true>(M, D, 2 * (int64_t)F, dz, 2 * (int64_t)F, w, D, dx, part, sp.splits_dx, status, s);
+        rc = product<T, false, true>(M, D, 2 * (int64_t)F, dz, 2 * (int64_t)F, w, D, dx, part_dx, sp.splits_dx, &join_dx, status, s);
     if (rc == DG_OK && dw)
-        rc = product<T, true, true>(2 * (int64_t)F, D, M, dz, 2 * (int64_t)F, x, ldx, dw, part, sp.splits_dw, status, s);
-    if (rc == DG_OK && db) {
-        rc = launch_lm(colsum_kernel<T>, dim3((2 * F + 31) / 32), dim3(1024), 0, 0, s, p.m_tiles * 8, 2 * F, colsum,
-                       static_cast<T*>(db));
-    }
+        rc = product<T, true, true>(2 * (int64_t)F, D, M, dz, 2 * (int64_t)F, x, ldx, dw, part_dw, sp.splits_dw, &join_dw, status, s);
+    const int blocks = join_dx.blocks + join_dw.blocks + (db ? (2 * F + 31) / 32 : 0);
+    if (rc == DG_OK && blocks > 0)
+        rc = launch_lm(finish_kernel<T>, dim3((unsigned)blocks), dim3(kFinish), 0, 0, s, join_dx, join_dw, (const float*)colsum,
+                       p.m_tiles * 8, 2 * F, static_cast<T*>(db));
     return rc;
 }
 
