@@ -105,6 +105,29 @@ def test_forward_and_backward(B, T, D, dtype):
     _check(*_inputs(B, T, D, dtype, seed=T + D), dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,T,D", [(1, 1, 1), (2, 5, 1), (3, 70, 7), (2, 300, 65), (1, 2100, 33), (2, 131, 64)])
+@pytest.mark.parametrize("start,gap", [(0, 0), (1, 0), (0, 1), (1, 1), (3, 4)])
+def test_single_elements_beside_junk(B, T, D, start, gap, dtype):
+    """Rows that start at odd and even elements with odd and even strides, NaN before and behind each."""
+    (x, g, o), h0, _, r, dy, dh = _inputs(B, T, D, dtype, seed=D + start, resets=True)
+    def beside_junk(p):
+        wide = torch.full((start + B * T * (D + gap) + 1,), float("nan"), dtype=dtype, device="cuda")
+        v = wide[start:start + B * T * (D + gap)].view(B, T, D + gap)[..., :D]
+        v.copy_(p)
+        return v
+    plain = [p.clone().requires_grad_(True) for p in (x, g, o)]
+    leaves = [beside_junk(p).requires_grad_(True) for p in (x, g, o)]
+    want = gated_scan(*plain, h0, None, r)
+    got = gated_scan(*leaves, h0, None, r)
+    for a, b in zip(got, _ref(x, g, o, h0, None, r)):
+        assert rel_err(a.detach().float().cpu(), b.float().cpu()) < (TOL[dtype] if a.dtype == dtype else STATE)
+    want = torch.autograd.grad(want, plain, (dy, dh))
+    got = torch.autograd.grad(got, leaves, (beside_junk(dy), dh))
+    for a, b in zip(got, want):
+        assert rel_err(a.float().cpu(), b.float().cpu()) < TOL[dtype]
+
+
 @pytest.mark.parametrize("layout", ["packed", "time_first", "offset"])
 @pytest.mark.parametrize("D", [64, 65, 96])
 def test_strides(layout, D):
