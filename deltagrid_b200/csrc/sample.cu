@@ -693,8 +693,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
             return dist < 255.f ? (int)dist : dist == dist ? 255 : 0;
         };
         // s.hist, counted by each CTA, becomes s.all_* over the cluster: each CTA gets all counts of its part of
-        // the bins, adds them up and sends the sums to all, 16 bytes at a time (a warp's remote store takes some
-        // 5 cycles a lane, whatever its width).  Returns the sum of `extra`.
+        // the bins, adds them up and sends the sums to all, 16 bytes at a time.  Returns the sum of `extra`.
         auto bin_masses = [&](int b) {
             const u64 w = (u64)s.hist[1][b] + ((u64)s.hist[2][b] << 13) + ((u64)s.hist[3][b] << 26);
             s.hist[1][b] = s.hist[2][b] = s.hist[3][b] = 0;
