@@ -24,6 +24,7 @@ extern PyObject* g_error;      // deltagrid_b200._lib.DeltaGridError, set at imp
     std::string msg = std::string(what) + " failed: " + dg_status_string(st);
     if (st == DG_ERR_CUDA) msg += " (cudaError " + std::to_string(dg_last_cuda_error()) + ")";
     msg += " [status " + std::to_string(st) + "]";
+    const py::gil_scoped_acquire lock;         // autograd runs C++ backward nodes on threads that do not hold it
     PyErr_SetString(g_error ? g_error : PyExc_RuntimeError, msg.c_str());
     throw py::error_already_set();
 }

@@ -1,0 +1,46 @@
+"""How the language-model operators are called: errors inside a backward pass, calls of several
+host threads and from threads that have not used the device before."""
+import os
+import subprocess
+import sys
+import textwrap
+
+import pytest
+import torch
+
+from conftest import REPO
+
+pytestmark = pytest.mark.gpu
+
+
+def _child(code, **env):
+    r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], cwd=REPO, env=dict(os.environ, **env),
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, (r.returncode, r.stdout, r.stderr)
+
+
+@pytest.mark.parametrize("call", ["gated_scan(a, a)[0]", "gated_ffn(a, w)"])
+def test_an_error_in_a_backward_pass_raises(call, tmp_path):
+    """The C call refuses (a library loaded in front of the package's own): autograd's thread, which does
+    not hold Python's lock, hands the error on."""
+    src, refuse = tmp_path / "refuse.c", tmp_path / "librefuse.so"
+    src.write_text("int dg_gated_scan_backward(void) { return -2; }\nint dg_gated_ffn_backward(void) { return -2; }\n")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(refuse), str(src)], check=True)
+    _child(f"""
+        import torch
+        from deltagrid_b200._lib import DeltaGridError
+        from deltagrid_b200.ffn import gated_ffn
+        from deltagrid_b200.recurrence import gated_scan
+        a = torch.ones(2, 4, 8, device="cuda", requires_grad=True)
+        w = torch.ones(16, 8, device="cuda")
+        y = {call}
+        torch.cuda.synchronize()
+        for _ in range(3):
+            try:
+                y.sum().backward(retain_graph=True)
+            except DeltaGridError as e:
+                assert "backward failed: unsupported" in str(e), e
+            else:
+                raise SystemExit("no error")
+        print("done")
+        """, LD_PRELOAD=str(refuse))
