@@ -23,6 +23,24 @@ int sm_count(int device, int* out) {
     return DG_OK;
 }
 
+void bind_context() {
+    typedef int (*GetCurrent)(void**);          // cuCtxGetCurrent
+    static GetCurrent fn = nullptr;
+    GetCurrent get = __atomic_load_n(&fn, __ATOMIC_RELAXED);
+    if (!get) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return;
+        get = reinterpret_cast<GetCurrent>(p);
+        __atomic_store_n(&fn, get, __ATOMIC_RELAXED);
+    }
+    void* context = nullptr;
+    int dev = 0;
+    if (get(&context) == 0 && !context && cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
+}
+
 int record_cuda_error(cudaError_t e) {
     g_last_cuda_error = (int)e;
     return DG_ERR_CUDA;

@@ -242,6 +242,7 @@ inline EncodeTiledFn encode_fn() {
             q == cudaDriverEntryPointSuccess)
             fn = reinterpret_cast<EncodeTiledFn>(p);
     }
+    dg_host::bind_context();
     return fn;
 }
 

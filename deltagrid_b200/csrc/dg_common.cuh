@@ -62,6 +62,9 @@ inline int check_launch() {
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? DG_OK : record_cuda_error(e);
 }
+// Makes the device's context current on a host thread that has none yet, as the driver's own calls
+// (cuTensorMapEncodeTiled) need one: autograd's threads and a host's new ones may come here first.
+void bind_context();
 // multiprocessor count of a device, queried once per device and cached
 int sm_count(int device, int* out);
 inline size_t dtype_size(int dtype) {

@@ -635,6 +635,7 @@ EncodeTiledFn encode_fn() {
             q == cudaDriverEntryPointSuccess)
             fn = reinterpret_cast<EncodeTiledFn>(ptr);
     }
+    dg_host::bind_context();
     return fn;
 }
 

@@ -44,3 +44,27 @@ def test_an_error_in_a_backward_pass_raises(call, tmp_path):
                 raise SystemExit("no error")
         print("done")
         """, LD_PRELOAD=str(refuse))
+
+
+def test_the_first_work_of_a_thread():
+    """Tensor-core calls on threads that have made no CUDA call before: autograd's, in a backward pass, and a
+    new one of the host's."""
+    _child("""
+        import threading
+        import torch
+        from deltagrid_b200.ffn import gated_ffn
+        x = torch.randn(200, 64, device="cuda").bfloat16().requires_grad_(True)
+        w = torch.randn(128, 64, device="cuda").bfloat16()
+        dh = torch.randn(200, 64, device="cuda").bfloat16()
+        h = gated_ffn(x, w)
+        spare = [torch.empty(1 << 20, device="cuda") for _ in range(4)]      # memory the backward pass finds cached
+        torch.cuda.synchronize()
+        del spare
+        torch.autograd.grad(h, [x], dh)
+        got = []
+        t = threading.Thread(target=lambda: got.append(gated_ffn(x.detach(), w)))
+        t.start()
+        t.join()
+        assert len(got) == 1 and torch.equal(got[0], h)
+        print("done")
+        """)
