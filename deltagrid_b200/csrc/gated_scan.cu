@@ -167,7 +167,7 @@ template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> narrow(Fv
     return p;
 }
 
-// a = sigmoid(z) and na = 1 - a = exp(-z) a, each to fp32's relative precision for z > -80
+// a = sigmoid(z) and na = 1 - a = exp(-z) a of the recurrence's gate
 template <int VEC> __device__ __forceinline__ void gates(Fv<VEC> z, Fv<VEC>& a, Fv<VEC>& na) {
     Fv<VEC> e = vmul(z, all<VEC>(-1.4426950408889634f));
 #pragma unroll
@@ -177,10 +177,24 @@ template <int VEC> __device__ __forceinline__ void gates(Fv<VEC> z, Fv<VEC>& a, 
     for (int i = 0; i < VEC; ++i) a.v[i] = dg::rcp_ftz(a.v[i]);
     na = vmul(e, a);
 }
+// z sigmoid(z) (dg::sigmoid), and dg::slope_pair
 template <int VEC> __device__ __forceinline__ Fv<VEC> silu(Fv<VEC> z) {
-    Fv<VEC> a, na;
-    gates(z, a, na);
-    return vmul(z, a);
+    Fv<VEC> e = vmul(z, all<VEC>(-1.4426950408889634f));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e.v[i] = dg::exp2_ftz(e.v[i]);
+    e = vadd(e, all<VEC>(1.f));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e.v[i] = dg::rcp_ftz(e.v[i]);
+    return vmul(z, e);
+}
+template <int VEC> __device__ __forceinline__ void slope_pair(Fv<VEC> z, Fv<VEC>& s, Fv<VEC>& n) {
+    Fv<VEC> e = vmul(z, all<VEC>(-1.4426950408889634f));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e.v[i] = fminf(dg::exp2_ftz(e.v[i]), 3.4e38f);
+    s = vadd(e, all<VEC>(1.f));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s.v[i] = dg::rcp_ftz(s.v[i]);
+    n = vmul(e, s);
 }
 
 // What a CTA keeps of its tile, per channel; the maps of the cluster's CTAs (two tiles' worth of
@@ -506,7 +520,7 @@ __device__ __forceinline__ void backward_apply(Fv<VEC> rr, const Fv<VEC> (&c)[R]
         if (OG) {
             const Fv<VEC> z = widen(os[r * LPR]);
             Fv<VEC> sg_, sn;
-            gates(z, sg_, sn);
+            slope_pair(z, sg_, sn);
             const Fv<VEC> ht = vfma(a, u[r], vmul(n, xt));
             go = vmul(vmul(widen(dys[r * LPR]), ht), vmul(sg_, vfma(z, sn, all<VEC>(1.f))));
         }

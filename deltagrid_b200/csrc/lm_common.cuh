@@ -33,15 +33,33 @@ __device__ __forceinline__ float rcp_ftz(float x) {
     return r;
 }
 
-// a = sigmoid(z) and 1 - a, each to fp32's relative precision: with e = exp(-z),
-// a = 1 / (1 + e) and 1 - a = e a.  z is held above -80, where a is 2e-35 (and e finite).
+// the smaller and the larger of two; a NaN stays one
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The recurrence's gate: a = sigmoid(z) and 1 - a, with e = exp(-z): a = 1 / (1 + e) and 1 - a = e a.
+// z is held above -80, where a is 2e-35 (and e finite).  z log2(e) is rounded once, so e and the smaller
+// of the two carry |z| 2^-24 relative.
 __device__ __forceinline__ void sigmoid_pair(float z, float& a, float& one_minus_a) {
     const float e = exp2_ftz(fminf(z * -1.4426950408889634f, 115.f));
     a = rcp_ftz(1.f + e);
     one_minus_a = e * a;
 }
-__device__ __forceinline__ float sigmoid(float z) {
-    return rcp_ftz(1.f + exp2_ftz(fminf(z * -1.4426950408889634f, 115.f)));
+// sigmoid(z) for z sigmoid(z): 0 for z below -88, where 1 + exp(-z) has no normal inverse, and so the product
+__device__ __forceinline__ float sigmoid(float z) { return rcp_ftz(1.f + exp2_ftz(z * -1.4426950408889634f)); }
+// s = sigmoid(z) and n = 1 - s for a slope s (1 + z n ...): both are 0 for z below -88, and so the slope
+__device__ __forceinline__ void slope_pair(float z, float& s, float& n) {
+    const float e = fminf(exp2_ftz(z * -1.4426950408889634f), 3.4e38f);
+    s = rcp_ftz(1.f + e);
+    n = e * s;
 }
 
 // two fp32 values at a time (the two-wide instructions of sm_100)
@@ -75,58 +93,61 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 }
 __device__ __forceinline__ F2 both(float a) { return {a, a}; }
 
-// sigmoid_pair of two values
-__device__ __forceinline__ void sigmoid_pair2(F2 z, F2& a, F2& one_minus_a) {
+// slope_pair of two values
+__device__ __forceinline__ void slope_pair2(F2 z, F2& s, F2& n) {
     F2 e = mul2(z, both(-1.4426950408889634f));
-    e.x = exp2_ftz(fminf(e.x, 115.f));
-    e.y = exp2_ftz(fminf(e.y, 115.f));
-    a = add2(e, both(1.f));
-    a.x = rcp_ftz(a.x);
-    a.y = rcp_ftz(a.y);
-    one_minus_a = mul2(e, a);
+    e.x = fminf(exp2_ftz(e.x), 3.4e38f);
+    e.y = fminf(exp2_ftz(e.y), 3.4e38f);
+    s = add2(e, both(1.f));
+    s.x = rcp_ftz(s.x);
+    s.y = rcp_ftz(s.y);
+    n = mul2(e, s);
 }
-// activations of the feed-forward block and their derivatives
+__device__ __forceinline__ F2 sigmoid2(F2 z) {
+    F2 e = mul2(z, both(-1.4426950408889634f));
+    e.x = exp2_ftz(e.x);
+    e.y = exp2_ftz(e.y);
+    e = add2(e, both(1.f));
+    return {rcp_ftz(e.x), rcp_ftz(e.y)};
+}
+// Activations of the feed-forward block and their derivatives.  GELU's tanh form is z sigmoid(2 s), s =
+// sqrt(2 / pi) (z + 0.044715 z^3); its slope is formed at z held to +-12, beyond which it is 0 or 1 to
+// fp32 (2 s is 142 there) and z^2 may leave fp32.
+__device__ __forceinline__ float held(float z) { return min_nan(max_nan(z, -12.f), 12.f); }
 template <int ACT>
 __device__ __forceinline__ float act_fn(float z) {
     if (ACT == DG_ACT_SILU) return z * sigmoid(z);
-    // z/2 (1 + tanh s) = z sigmoid(2 s)
     return z * sigmoid(1.5957691216057308f * fmaf(0.044715f * z * z, z, z));
 }
 template <int ACT>
 __device__ __forceinline__ void act_grad(float z, float& f, float& df) {
     float s, n;
     if (ACT == DG_ACT_SILU) {
-        sigmoid_pair(z, s, n);
-        f = z * s;
+        slope_pair(z, s, n);
         df = s * fmaf(z, n, 1.f);
     } else {
-        const float z2 = z * z;
-        sigmoid_pair(1.5957691216057308f * fmaf(0.044715f * z2, z, z), s, n);
-        f = z * s;
-        df = s * fmaf(z * n, 1.5957691216057308f * fmaf(0.134145f, z2, 1.f), 1.f);
+        const float h = held(z), h2 = h * h;
+        slope_pair(1.5957691216057308f * fmaf(0.044715f * h2, h, h), s, n);
+        df = s * fmaf(h * n, 1.5957691216057308f * fmaf(0.134145f, h2, 1.f), 1.f);
     }
+    f = z * s;
 }
 
 template <int ACT> __device__ __forceinline__ F2 act_fn2(F2 z) {
-    F2 s, n;
-    if (ACT == DG_ACT_SILU) {
-        sigmoid_pair2(z, s, n);
-    } else {
-        const F2 z2 = mul2(z, z);
-        sigmoid_pair2(mul2(both(1.5957691216057308f), fma2(mul2(both(0.044715f), z2), z, z)), s, n);
-    }
-    return mul2(z, s);
+    if (ACT == DG_ACT_SILU) return mul2(z, sigmoid2(z));
+    const F2 z2 = mul2(z, z);
+    return mul2(z, sigmoid2(mul2(both(1.5957691216057308f), fma2(mul2(both(0.044715f), z2), z, z))));
 }
 template <int ACT> __device__ __forceinline__ void act_grad2(F2 z, F2& f, F2& df) {
     F2 s, n;
     if (ACT == DG_ACT_SILU) {
-        sigmoid_pair2(z, s, n);
+        slope_pair2(z, s, n);
         df = mul2(s, fma2(z, n, both(1.f)));
     } else {
-        const F2 z2 = mul2(z, z);
-        sigmoid_pair2(mul2(both(1.5957691216057308f), fma2(mul2(both(0.044715f), z2), z, z)), s, n);
-        const F2 slope = mul2(both(1.5957691216057308f), fma2(both(0.134145f), z2, both(1.f)));
-        df = mul2(s, fma2(mul2(z, n), slope, both(1.f)));
+        const F2 h{held(z.x), held(z.y)}, h2 = mul2(h, h);
+        slope_pair2(mul2(both(1.5957691216057308f), fma2(mul2(both(0.044715f), h2), h, h)), s, n);
+        const F2 slope = mul2(both(1.5957691216057308f), fma2(both(0.134145f), h2, both(1.f)));
+        df = mul2(s, fma2(mul2(h, n), slope, both(1.f)));
     }
     f = mul2(z, s);
 }

@@ -253,3 +253,40 @@ def test_wait_timeout_flags_status():
     again = gated_ffn(x, w, b)
     torch.cuda.synchronize()
     assert ext.device_status() == 0 and torch.equal(want, again)
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+@pytest.mark.parametrize("M,D,dtype", [(4, 16, torch.bfloat16), (100, 16, torch.bfloat16), (600, 16, torch.bfloat16),
+                                       (70, 15, torch.bfloat16), (70, 16, torch.float32)])
+def test_very_negative_gates(M, D, dtype, kind):
+    """Both activations and their slopes vanish down to the type's lowest value."""
+    x = torch.zeros(M, D, device="cuda", dtype=dtype)
+    x[:, 0] = 1.0
+    low = torch.finfo(dtype).min
+    z = torch.tensor([low, low / 2, -1e38, -1e30, -1e20, -1e12, -1e5, -120.0, -90.0, -88.0, -60.0, -13.0, -5.0, -0.5,
+                      0.0, 0.5, 5.0, 13.0, 60.0], device="cuda")
+    w = torch.zeros(64, D, device="cuda", dtype=dtype)
+    w[:32, 0] = z[torch.arange(32) % 19].to(dtype)
+    w[32:, 0] = 1.0
+    dh = torch.randn(M, 32, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    h = gated_ffn(*leaves, None, kind)
+    grads = torch.autograd.grad(h, leaves, dh)
+    for i, (got, ref) in enumerate(zip((h, *grads), _ref(x.detach(), w.detach(), None, kind, dh))):
+        assert rel_err(got.detach().float().cpu(), ref.cpu()) < TOL[dtype] * (1 if i == 0 else 2)
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+def test_very_positive_gates(kind):
+    """Slopes of 1 up to the largest values; f(z) = z."""
+    z = torch.tensor([13.0, 100.0, 1e4, 1e12, 1e20, 1e30, 3e38, 2.0], device="cuda")
+    w = torch.zeros(16, 8, device="cuda")
+    w[:8, 0], w[8:, 0] = z, 1.0
+    x = torch.zeros(1, 8, device="cuda")
+    x[:, 0] = 1.0
+    w.requires_grad_(True)
+    h = gated_ffn(x, w, None, kind)
+    (g,) = torch.autograd.grad(h, [w], torch.ones_like(h))
+    rh, _, rw, _ = _ref(x, w.detach(), None, kind, torch.ones_like(h))
+    for got, ref in ((h, rh), (g, rw)):
+        assert float(((got.detach().double() - ref).abs() / ref.abs().clamp(min=1e-30)).max()) < 1e-5

@@ -324,3 +324,17 @@ def test_wait_timeout_flags_status():
     torch.cuda.synchronize()
     assert ext.device_status() == 0
     assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_output_gates_down_to_the_lowest_value(dtype):
+    """z sigmoid(z) and its slope vanish for very negative z, masks of the type's lowest value among them."""
+    parts, h, _, _, dy, dh = _inputs(2, 300, 40, dtype, seed=31)
+    low = torch.finfo(dtype).min
+    closed = torch.tensor([low, low / 2, -1e30, -1e20, -1e5, -120.0, -90.0, -88.0, -60.0], device="cuda").to(dtype)
+    parts[2][:, ::3] = closed[torch.arange(100 * 40, device="cuda") % 9].view(100, 40)
+    _check(parts, h, None, None, dy, dh, dtype)
+    s = h.clone()
+    y = gated_scan_step(parts[0][:, 0], parts[1][:, 0], s, parts[2][:, 0])
+    want = _ref(*[p[:, :1] for p in parts], h, None, None)[0][:, 0]
+    assert rel_err(y.float().cpu(), want.cpu()) < TOL[dtype]
