@@ -167,15 +167,17 @@ template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> narrow(Fv
     return p;
 }
 
-// a = sigmoid(z) and na = 1 - a = exp(-z) a of the recurrence's gate
+// dg::sigmoid_pair: the recurrence's gate a and na = 1 - a
 template <int VEC> __device__ __forceinline__ void gates(Fv<VEC> z, Fv<VEC>& a, Fv<VEC>& na) {
     Fv<VEC> e = vmul(z, all<VEC>(-1.4426950408889634f));
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) e.v[i] = dg::exp2_ftz(fminf(e.v[i], 115.f));
+    for (int i = 0; i < VEC; ++i) e.v[i] = dg::exp2_ftz(e.v[i]);
     a = vadd(e, all<VEC>(1.f));
 #pragma unroll
     for (int i = 0; i < VEC; ++i) a.v[i] = dg::rcp_ftz(a.v[i]);
-    na = vmul(e, a);
+    const Fv<VEC> small = vmul(e, a), large = vfma(a, all<VEC>(-1.f), all<VEC>(1.f));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) na.v[i] = e.v[i] > 1.f ? large.v[i] : small.v[i];
 }
 // z sigmoid(z) (dg::sigmoid), and dg::slope_pair
 template <int VEC> __device__ __forceinline__ Fv<VEC> silu(Fv<VEC> z) {

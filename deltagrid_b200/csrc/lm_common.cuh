@@ -45,13 +45,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// The recurrence's gate: a = sigmoid(z) and 1 - a, with e = exp(-z): a = 1 / (1 + e) and 1 - a = e a.
-// z is held above -80, where a is 2e-35 (and e finite).  z log2(e) is rounded once, so e and the smaller
-// of the two carry |z| 2^-24 relative.
+// The recurrence's gate: a = sigmoid(z) = 1 / (1 + e) with e = exp(-z), and 1 - a, as e a where e is small
+// and a near 1, else by the difference (e may be infinite: a is 0 there and forgets any state).  A NaN
+// stays one in both.  z log2(e) is rounded once, so e and the smaller of the two carry |z| 2^-24 relative.
 __device__ __forceinline__ void sigmoid_pair(float z, float& a, float& one_minus_a) {
-    const float e = exp2_ftz(fminf(z * -1.4426950408889634f, 115.f));
+    const float e = exp2_ftz(z * -1.4426950408889634f);
     a = rcp_ftz(1.f + e);
-    one_minus_a = e * a;
+    one_minus_a = e > 1.f ? 1.f - a : e * a;
 }
 // sigmoid(z) for z sigmoid(z): 0 for z below -88, where 1 + exp(-z) has no normal inverse, and so the product
 __device__ __forceinline__ float sigmoid(float z) { return rcp_ftz(1.f + exp2_ftz(z * -1.4426950408889634f)); }

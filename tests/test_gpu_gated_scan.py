@@ -338,3 +338,34 @@ def test_output_gates_down_to_the_lowest_value(dtype):
     y = gated_scan_step(parts[0][:, 0], parts[1][:, 0], s, parts[2][:, 0])
     want = _ref(*[p[:, :1] for p in parts], h, None, None)[0][:, 0]
     assert rel_err(y.float().cpu(), want.cpu()) < TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,T,D,t", [(2, 300, 64, 137), (1, 3000, 72, 1700), (2, 40, 33, 0), (3, 700, 130, 699)])
+def test_a_gate_that_is_not_a_number_shows(B, T, D, t, dtype):
+    """The outputs and gradients that the formulas make NaN, and no others."""
+    parts, h, _, r, dy, dh = _inputs(B, T, D, dtype, seed=t)
+    parts[1][0, t, 5] = float("nan")
+    leaves = [p.detach().requires_grad_(True) for p in parts] + [h.clone().requires_grad_(True)]
+    y, last = gated_scan(*leaves, None, r)
+    grads = torch.autograd.grad((y, last), leaves, (dy, dh))
+    for got, ref in zip((y, last, *grads), _ref(*parts, h, None, r, dy, dh)):
+        bad = torch.isnan(ref)
+        assert torch.equal(torch.isnan(got), bad)
+        tol = STATE if got.dtype == torch.float32 else TOL[dtype]
+        assert rel_err(got.detach().float().masked_fill(bad, 0.0).cpu(), ref.masked_fill(bad, 0.0).cpu()) < tol
+    s = h.clone()
+    y = gated_scan_step(parts[0][:, t], parts[1][:, t], s, parts[2][:, t])
+    assert torch.isnan(y[0, 5]) and torch.isnan(s[0, 5]) and int(torch.isnan(y).sum() + torch.isnan(s).sum()) == 2
+
+
+def test_closed_gates_forget_any_state():
+    """sigmoid of a very negative gate is 0 to a state of any finite size."""
+    h = torch.full((2, 40), 3e38, device="cuda")
+    x = torch.randn(2, 3, 40, generator=torch.Generator().manual_seed(1)).cuda()
+    gate = torch.full_like(x, -1e4)
+    gate[0, :, ::2], gate[1, :, ::2] = torch.finfo(torch.float32).min, float("-inf")
+    y, last = gated_scan(x, gate, None, h)
+    assert rel_err(y.cpu(), x.cpu()) < STATE and rel_err(last.cpu(), x[:, -1].cpu()) < STATE
+    s = h.clone()
+    assert rel_err(gated_scan_step(x[:, 0], gate[:, 0], s).cpu(), x[:, 0].cpu()) < STATE
