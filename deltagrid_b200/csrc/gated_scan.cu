@@ -12,6 +12,8 @@
 //   - where rows and channels give too few CTAs, a cluster of up to 16 takes consecutive
 //     tiles and exchanges their maps through distributed shared memory: asynchronous stores
 //     that count on the receiver's mbarrier, so that no fence waits for a warp's other stores.
+// A reset (c = 0) is a product of -0, which no product of gates is: there a map gives H whatever the
+// state before it, infinite or NaN, where 0 h + H would not.
 // Each input is read and each output written once.  The order of every composition is fixed
 // by the sizes alone, so results repeat bit for bit.
 //
@@ -199,6 +201,41 @@ template <int VEC> __device__ __forceinline__ void slope_pair(Fv<VEC> z, Fv<VEC>
     n = vmul(e, s);
 }
 
+// The marked product of a map that holds a reset, whether a product is one, and the state after a map.
+// The chains over warps and CTAs compute P s + H and look at their end alone: a state that is not finite
+// does not become so again, and then, in calls with resets, the chain is taken once more by after().
+// (after() at each link cost up to 18% of a call, 1 x 65536 x 768 backward 299 to 353 us; the look at the
+// end 2%, 306 us.  Calls without resets, RS = false, have neither.)
+constexpr float kReset = -0.f;
+__device__ __forceinline__ bool is_reset(float P) { return __float_as_uint(P) == 0x80000000u; }
+__device__ __forceinline__ bool finite(float s) { return fabsf(s) < INFINITY; }
+__device__ __forceinline__ float after(float P, float H, float s) { return is_reset(P) ? H : fmaf(P, s, H); }
+template <int VEC> __device__ __forceinline__ Fv<VEC> after(Fv<VEC> P, Fv<VEC> H, Fv<VEC> s) {
+    s = vfma(P, s, H);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s.v[i] = is_reset(P.v[i]) ? H.v[i] : s.v[i];
+    return s;
+}
+
+// p, marked where one of the products in `marks` is
+__device__ __forceinline__ float marked(float p, uint32_t marks) {
+    return __uint_as_float(__float_as_uint(p) | (marks & 0x80000000u));
+}
+// A thread's chain over its warps' maps (P of `maps`, H of `maps` or `back`) by after(), first to last or last to
+// first, from the state s: the states between them into carry (or null), the last returned.
+template <bool FORWARD, int CH>
+__device__ __forceinline__ float chain_again(const float2 (*maps)[CH], const float (*back)[CH], int tid, float s,
+                                             float (*carry)[CH]) {
+#pragma unroll 1
+    for (int i = 0; i < WARPS; ++i) {
+        const int w = FORWARD ? i : WARPS - 1 - i;
+        if (carry) carry[w][tid] = s;
+        const float2 m = maps[w][tid];
+        s = after(m.x, back ? back[w][tid] : m.y, s);
+    }
+    return s;
+}
+
 // What a CTA keeps of its tile, per channel; the maps of the cluster's CTAs (two tiles' worth of
 // [cluster][CH]) lie behind the input stages
 template <int CH> struct Maps {
@@ -266,7 +303,8 @@ __device__ __forceinline__ void fetch(Pack<T, VEC>* warp_part, const T* row, int
 
 // composes (P, H) maps over the row groups of a warp.  In: the thread's own map; out: the map of
 // the groups before it (FORWARD) or after it, and the whole warp's, which the last (first) group has
-template <int LPR, int VEC, bool FORWARD>
+// (MARKED: some group's map holds a reset)
+template <int LPR, int VEC, bool FORWARD, bool MARKED>
 __device__ __forceinline__ void warp_maps(Fv<VEC> P, Fv<VEC> H, Fv<VEC>& Pb, Fv<VEC>& Hb, Fv<VEC>& Pw, Fv<VEC>& Hw,
                                           int lane) {
     auto from = [&](float x, int o) {
@@ -277,7 +315,7 @@ __device__ __forceinline__ void warp_maps(Fv<VEC> P, Fv<VEC> H, Fv<VEC>& Pb, Fv<
 #pragma unroll
         for (int o = LPR; o < 32; o <<= 1) {
             const float p = from(P.v[v], o), h = from(H.v[v], o);
-            if (FORWARD ? lane >= o : lane + o < 32) {
+            if ((FORWARD ? lane >= o : lane + o < 32) && !(MARKED && is_reset(P.v[v]))) {
                 H.v[v] = fmaf(P.v[v], h, H.v[v]);
                 P.v[v] *= p;
             }
@@ -319,14 +357,14 @@ template <int LPR, int VEC, int R> struct Place {
     __device__ __forceinline__ int step(int it) const { return warp_step(it) + lane / LPR * R; }
 };
 
-// bit r: a document starts at step r of this thread.  The load was made a tile earlier: lane r of
-// a group holds step r.
+// Where documents start in a warp's steps.  The load was made a tile earlier: lane r of a group holds step
+// r, so the group's bits of the vote are its thread's: bit r for step r.
 template <int LPR, int R> __device__ __forceinline__ uint8_t load_reset(const uint8_t* rs, int t, int lc, int len) {
     return lc < R && t + lc < len ? rs[t + lc] : 0;
 }
-template <int LPR, int R> __device__ __forceinline__ unsigned reset_bits(uint8_t mine, int lane) {
+template <int LPR, int R> __device__ __forceinline__ unsigned reset_bits(unsigned vote, int lane) {
     static_assert(LPR >= R, "one lane per step");
-    return __ballot_sync(DG_FULL_MASK, mine != 0) >> (lane & ~(LPR - 1)) & ((1u << R) - 1);
+    return vote >> (lane & ~(LPR - 1)) & ((1u << R) - 1);
 }
 
 // the forward map of a thread's steps: c, u and their composition (P, H).  WHOLE: every step is
@@ -339,12 +377,11 @@ __device__ __forceinline__ void forward_map(const Pack<T, VEC>* xs, const Pack<T
         Fv<VEC> na;
         gates(widen(gs[r * LPR]), c[r], na);
         u[r] = vmul(na, widen(xs[r * LPR]));
-        if (!WHOLE) {
-            if (r >= left) c[r] = all<VEC>(1.f), u[r] = all<VEC>(0.f);
-            else if ((resets >> r) & 1) c[r] = all<VEC>(0.f);
-        }
-        H = r == 0 ? u[0] : vfma(c[r], H, u[r]);
-        P = r == 0 ? c[0] : vmul(P, c[r]);
+        const bool reset = !WHOLE && r < left && (resets >> r) & 1;
+        if (!WHOLE && r >= left) c[r] = all<VEC>(1.f), u[r] = all<VEC>(0.f);
+        if (reset) c[r] = all<VEC>(kReset);
+        H = r == 0 || reset ? u[r] : vfma(c[r], H, u[r]);
+        P = r == 0 || reset ? c[r] : vmul(P, c[r]);
         if (nas) nas[r] = na;
     }
 }
@@ -355,7 +392,7 @@ __device__ __forceinline__ void forward_apply(Fv<VEC> h, const Fv<VEC> (&c)[R], 
                                               const Pack<T, VEC>* os, T* y, int D, int left, int room) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        h = vfma(c[r], h, u[r]);
+        h = WHOLE ? vfma(c[r], h, u[r]) : after(c[r], u[r], h);
         Fv<VEC> w = h;
         if (OG) w = vmul(w, silu(widen(os[r * LPR])));
         if (!WHOLE && r >= left) w = all<VEC>(0.f);
@@ -365,7 +402,7 @@ __device__ __forceinline__ void forward_apply(Fv<VEC> h, const Fv<VEC> (&c)[R], 
 
 // The cluster's part of a tile: this CTA's map to all, then the state before this CTA and (returned
 // in `state`) after the whole span.  Called by the threads that carry a channel.
-template <int CH, bool FORWARD>
+template <int CH, bool FORWARD, bool RS>
 __device__ __forceinline__ float through_cluster(float2* maps, uint64_t* received, float2 own, int tid, int rank, int S,
                                                  int n, float& state, uint32_t limit, bool& bad) {
     const int buf = n & 1;
@@ -379,6 +416,16 @@ __device__ __forceinline__ float through_cluster(float2* maps, uint64_t* receive
         if (k == rank) before = s;
         const float2 a = m[k * CH + tid];
         s = fmaf(a.x, s, a.y);
+    }
+    if (RS && !finite(s)) {
+        s = state;
+#pragma unroll 1
+        for (int i = 0; i < S; ++i) {
+            const int k = FORWARD ? i : S - 1 - i;
+            if (k == rank) before = s;
+            const float2 a = m[k * CH + tid];
+            s = after(a.x, a.y, s);
+        }
     }
     state = s;
     return before;
@@ -407,8 +454,9 @@ __device__ __forceinline__ void close_exchange(int S, bool bad, int32_t* status)
     cluster_barrier();
 }
 
-template <typename T, int VEC, int LPR, bool WIDE, bool OG>
-__global__ void __launch_bounds__(THREADS, 3)
+// RS: the call has resets.  Three CTAs share an SM, two where pairs of fp32 channels fill its shared memory.
+template <typename T, int VEC, int LPR, bool WIDE, bool OG, bool RS>
+__global__ void __launch_bounds__(THREADS, sizeof(T) * VEC == 8 ? 2 : 3)
     scan_forward_kernel(ScanIn in, const float* h0, T* y, float* h_last, float* marks) {
     constexpr int R = kForwardSteps;
     static_assert(DG_SCAN_MARK_STEPS % R == 0, "a mark falls on a thread's first step");
@@ -423,7 +471,7 @@ __global__ void __launch_bounds__(THREADS, 3)
     const T* x = (const T*)in.x + at.b * in.x_sb;
     const T* g = (const T*)in.g + at.b * in.g_sb;
     const T* o = OG ? (const T*)in.o + at.b * in.o_sb : nullptr;
-    const uint8_t* rs = in.resets ? in.resets + (int64_t)at.b * in.T : nullptr;
+    const uint8_t* rs = RS ? in.resets + (int64_t)at.b * in.T : nullptr;
     const int nblk = (in.T + DG_SCAN_MARK_STEPS - 1) / DG_SCAN_MARK_STEPS;
     constexpr int ARR = Tl::ARRAY, STG = (OG ? 3 : 2) * ARR;
     Pk* warp_part = reinterpret_cast<Pk*>(smem) + at.warp * Tl::WARP_PACKS;
@@ -441,7 +489,7 @@ __global__ void __launch_bounds__(THREADS, 3)
         fetch<T, VEC, LPR, R, WIDE>(st + ARR, g, in.g_st, t, len, at.d0, in.D, at.lane);
         if (OG) fetch<T, VEC, LPR, R, WIDE>(st + 2 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
         copy_commit();
-        if (rs) next_reset = load_reset<LPR, R>(rs, at.step(it), at.lc, len);
+        if (RS) next_reset = load_reset<LPR, R>(rs, at.step(it), at.lc, len);
     };
 
     // thread c < CH carries channel d0 + c from tile to tile
@@ -450,7 +498,8 @@ __global__ void __launch_bounds__(THREADS, 3)
     if (at.ntiles > 0) prefetch(0);
     for (int it = 0; it < at.ntiles; ++it) {
         const int t = at.step(it);
-        const unsigned resets = rs ? reset_bits<LPR, R>(next_reset, at.lane) : 0;
+        const unsigned vote = RS ? __ballot_sync(DG_FULL_MASK, next_reset != 0) : 0;
+        const unsigned resets = reset_bits<LPR, R>(vote, at.lane);
         __syncwarp();                      // the other stage has been read
         if (it + 1 < at.ntiles) prefetch(it + 1);
         else copy_commit();
@@ -462,7 +511,8 @@ __global__ void __launch_bounds__(THREADS, 3)
         if (whole) forward_map<true, T, VEC, LPR, R>(st, st + ARR, R, 0, c, u, nullptr, P, H);
         else forward_map<false, T, VEC, LPR, R>(st, st + ARR, len - t, resets, c, u, nullptr, P, H);
         V Pb, Hb, Pw, Hw;
-        warp_maps<LPR, VEC, true>(P, H, Pb, Hb, Pw, Hw, at.lane);
+        if (vote) warp_maps<LPR, VEC, true, true>(P, H, Pb, Hb, Pw, Hw, at.lane);
+        else warp_maps<LPR, VEC, true, false>(P, H, Pb, Hb, Pw, Hw, at.lane);
         if (at.lane >= 32 - LPR)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) maps.warp[at.warp][at.lc * VEC + v] = make_float2(Pw.v[v], Hw.v[v]);
@@ -474,21 +524,29 @@ __global__ void __launch_bounds__(THREADS, 3)
             float s = state;
             if (S > 1) {
                 float2 a = m[0];
+                uint32_t mark = __float_as_uint(a.x);
 #pragma unroll
-                for (int w = 1; w < WARPS; ++w) a = make_float2(a.x * m[w].x, fmaf(m[w].x, a.y, m[w].y));
-                s = through_cluster<Tl::CH, true>(cta_maps, maps.received, a, tid, at.rank, S, it, state, in.wait_limit,
-                                                  bad);
+                for (int w = 1; w < WARPS; ++w) {
+                    a = make_float2(a.x * m[w].x, fmaf(m[w].x, a.y, m[w].y));
+                    mark |= __float_as_uint(m[w].x);
+                }
+                a.x = marked(a.x, mark);
+                if (RS && !finite(a.y)) a.y = chain_again<true, Tl::CH>(maps.warp, nullptr, tid, 0.f, nullptr);
+                s = through_cluster<Tl::CH, true, RS>(cta_maps, maps.received, a, tid, at.rank, S, it, state,
+                                                      in.wait_limit, bad);
             }
+            const float s0 = s;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
                 maps.carry[w][tid] = s;
                 s = fmaf(m[w].x, s, m[w].y);
             }
+            if (RS && !finite(s)) s = chain_again<true, Tl::CH>(maps.warp, nullptr, tid, s0, maps.carry);
             if (S == 1) state = s;
         }
         __syncthreads();
         V h = *reinterpret_cast<const V*>(&maps.carry[at.warp][at.lc * VEC]);
-        if (LPR < 32) h = vfma(Pb, h, Hb);
+        if (LPR < 32) h = vote ? after(Pb, Hb, h) : vfma(Pb, h, Hb);
         if (at.on) {
             if (marks && t < in.T && t % DG_SCAN_MARK_STEPS == 0)
 #pragma unroll
@@ -527,6 +585,7 @@ __device__ __forceinline__ void backward_apply(Fv<VEC> rr, const Fv<VEC> (&c)[R]
             go = vmul(vmul(widen(dys[r * LPR]), ht), vmul(sg_, vfma(z, sn, all<VEC>(1.f))));
         }
         rr = vmul(c[r], et);
+        if (!WHOLE && ((resets >> r) & 1)) rr = all<VEC>(0.f);
         if (!WHOLE && r >= left) gx = gg = go = all<VEC>(0.f);
         if (WHOLE || r < room) {
             *reinterpret_cast<Pack<T, VEC>*>(px + r * sx) = narrow<T>(gx);
@@ -536,8 +595,8 @@ __device__ __forceinline__ void backward_apply(Fv<VEC> rr, const Fv<VEC> (&c)[R]
     }
 }
 
-template <typename T, int VEC, int LPR, bool WIDE, bool OG>
-__global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, ScanGrad q) {
+template <typename T, int VEC, int LPR, bool WIDE, bool OG, bool RS>
+__global__ void __launch_bounds__(THREADS, sizeof(T) * VEC == 8 ? 2 : 3) scan_backward_kernel(ScanIn in, ScanGrad q) {
     constexpr int R = kBackwardSteps;
     typedef Tile<T, VEC, LPR, R, OG ? 4 : 3> Tl;
     static_assert(Tl::STEPS % DG_SCAN_MARK_STEPS == 0, "tiles start at marks");
@@ -552,7 +611,7 @@ __global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, Sc
     const T* g = (const T*)in.g + at.b * in.g_sb;
     const T* o = OG ? (const T*)in.o + at.b * in.o_sb : nullptr;
     const T* dy = (const T*)q.dy + at.b * q.dy_sb;
-    const uint8_t* rs = in.resets ? in.resets + (int64_t)at.b * in.T : nullptr;
+    const uint8_t* rs = RS ? in.resets + (int64_t)at.b * in.T : nullptr;
     const int nblk = (in.T + DG_SCAN_MARK_STEPS - 1) / DG_SCAN_MARK_STEPS;
     constexpr int ARR = Tl::ARRAY, STG = (OG ? 4 : 3) * ARR;
     Pk* warp_part = reinterpret_cast<Pk*>(smem) + at.warp * Tl::WARP_PACKS;
@@ -573,7 +632,7 @@ __global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, Sc
         fetch<T, VEC, LPR, R, WIDE>(st + 2 * ARR, dy, q.dy_st, t, len, at.d0, in.D, at.lane);
         if (OG) fetch<T, VEC, LPR, R, WIDE>(st + 3 * ARR, o, in.o_st, t, len, at.d0, in.D, at.lane);
         copy_commit();
-        if (rs) next_reset = load_reset<LPR, R>(rs, at.step(it), at.lc, len);
+        if (RS) next_reset = load_reset<LPR, R>(rs, at.step(it), at.lc, len);
         if (carries && t0 < in.T)
             next_mark = q.marks[((int64_t)at.b * nblk + t0 / DG_SCAN_MARK_STEPS) * in.D + at.d0 + tid];
     };
@@ -583,7 +642,8 @@ __global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, Sc
     if (at.ntiles > 0) prefetch(at.ntiles - 1);
     for (int it = at.ntiles - 1; it >= 0; --it) {
         const int t = at.step(it);
-        const unsigned resets = rs ? reset_bits<LPR, R>(next_reset, at.lane) : 0;
+        const unsigned vote = RS ? __ballot_sync(DG_FULL_MASK, next_reset != 0) : 0;
+        const unsigned resets = reset_bits<LPR, R>(vote, at.lane);
         const float mark = next_mark;
         __syncwarp();
         if (it > 0) prefetch(it - 1);
@@ -602,9 +662,19 @@ __global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, Sc
             if (OG) e[r] = vmul(e[r], silu(widen(st[3 * ARR + r * LPR])));
             Q = r == R - 1 ? vmul(c[r], e[r]) : vmul(c[r], vadd(Q, e[r]));       // dy is 0 beyond len
         }
+        if (resets) {                      // what comes back stops at a reset, finite or not
+#pragma unroll
+            for (int r = R - 1; r >= 0; --r)
+                Q = (resets >> r) & 1 ? all<VEC>(0.f) : r == R - 1 ? vmul(c[r], e[r]) : vmul(c[r], vadd(Q, e[r]));
+        }
         V Pb, Hb, Pa, Qa, Pw, Hw, Pv, Qw;
-        warp_maps<LPR, VEC, true>(P, H, Pb, Hb, Pw, Hw, at.lane);
-        warp_maps<LPR, VEC, false>(P, Q, Pa, Qa, Pv, Qw, at.lane);
+        if (vote) {
+            warp_maps<LPR, VEC, true, true>(P, H, Pb, Hb, Pw, Hw, at.lane);
+            warp_maps<LPR, VEC, false, true>(P, Q, Pa, Qa, Pv, Qw, at.lane);
+        } else {
+            warp_maps<LPR, VEC, true, false>(P, H, Pb, Hb, Pw, Hw, at.lane);
+            warp_maps<LPR, VEC, false, false>(P, Q, Pa, Qa, Pv, Qw, at.lane);
+        }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             if (at.lane >= 32 - LPR) maps.warp[at.warp][at.lc * VEC + v] = make_float2(Pw.v[v], Hw.v[v]);
@@ -622,26 +692,35 @@ __global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, Sc
                 maps.carry[w][tid] = f;
                 f = fmaf(m[w].x, f, m[w].y);
             }
+            if (RS && !finite(f)) chain_again<true, Tl::CH>(maps.warp, nullptr, tid, mark, maps.carry);
             if (S > 1) {
                 float2 a = make_float2(m[WARPS - 1].x, bk[WARPS - 1]);
+                uint32_t marks = __float_as_uint(a.x);
 #pragma unroll
-                for (int w = WARPS - 2; w >= 0; --w) a = make_float2(a.x * m[w].x, fmaf(m[w].x, a.y, bk[w]));
-                s = through_cluster<Tl::CH, false>(cta_maps, maps.received, a, tid, at.rank, S, at.ntiles - 1 - it, state,
-                                                   in.wait_limit, bad);
+                for (int w = WARPS - 2; w >= 0; --w) {
+                    a = make_float2(a.x * m[w].x, fmaf(m[w].x, a.y, bk[w]));
+                    marks |= __float_as_uint(m[w].x);
+                }
+                a.x = marked(a.x, marks);
+                if (RS && !finite(a.y)) a.y = chain_again<false, Tl::CH>(maps.warp, maps.back, tid, 0.f, nullptr);
+                s = through_cluster<Tl::CH, false, RS>(cta_maps, maps.received, a, tid, at.rank, S, at.ntiles - 1 - it,
+                                                       state, in.wait_limit, bad);
             }
+            const float s0 = s;
 #pragma unroll
             for (int w = WARPS - 1; w >= 0; --w) {
                 maps.carry_back[w][tid] = s;
                 s = fmaf(m[w].x, s, bk[w]);
             }
+            if (RS && !finite(s)) s = chain_again<false, Tl::CH>(maps.warp, maps.back, tid, s0, maps.carry_back);
             if (S == 1) state = s;
         }
         __syncthreads();
         V h = *reinterpret_cast<const V*>(&maps.carry[at.warp][at.lc * VEC]);
         V rr = *reinterpret_cast<const V*>(&maps.carry_back[at.warp][at.lc * VEC]);
         if (LPR < 32) {
-            h = vfma(Pb, h, Hb);
-            rr = vfma(Pa, rr, Qa);
+            h = vote ? after(Pb, Hb, h) : vfma(Pb, h, Hb);
+            rr = vote ? after(Pa, Qa, rr) : vfma(Pa, rr, Qa);
         }
         if (at.on) {
 #pragma unroll
@@ -657,9 +736,17 @@ __global__ void __launch_bounds__(THREADS, 3) scan_backward_kernel(ScanIn in, Sc
                 backward_apply<true, T, VEC, LPR, OG, R>(rr, c, u, na, e, st, st + 2 * ARR, st + 3 * ARR, px, q.dx_st, pg,
                                                       q.dg_st, po, q.do_st, R, R, 0);
             } else {
+                if (resets) {              // 0 at a reset, and what follows it from there on
+                    bool started = false;
 #pragma unroll
-                for (int r = 0; r < R; ++r)
-                    if ((resets >> r) & 1) u[r] = all<VEC>(0.f);
+                    for (int r = 0; r < R; ++r) {
+                        const bool reset = (resets >> r) & 1;
+                        if (reset) u[r] = all<VEC>(0.f);
+                        else if (started) u[r] = h;
+                        started |= reset;
+                        h = vfma(c[r], u[r], vmul(na[r], widen(st[r * LPR])));
+                    }
+                }
                 backward_apply<false, T, VEC, LPR, OG, R>(rr, c, u, na, e, st, st + 2 * ARR, st + 3 * ARR, px, q.dx_st, pg,
                                                        q.dg_st, po, q.do_st, len - t, in.T - t, resets);
             }
@@ -745,34 +832,37 @@ Shape shape_of(int B, int T, int D, int vec, int steps_per_thread, int occ, bool
     return best;
 }
 
-template <typename T, int VEC, int LPR, bool WIDE, bool OG>
+template <typename T, int VEC, int LPR, bool WIDE, bool OG, bool RS>
 int run_forward(const ScanIn& in, const float* h0, void* y, float* h_last, float* marks, cudaStream_t s) {
     typedef Tile<T, VEC, LPR, kForwardSteps, OG ? 3 : 2> Tl;
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
-    return dg_host::launch_lm(scan_forward_kernel<T, VEC, LPR, WIDE, OG>, dim3((unsigned)grid), dim3(THREADS),
+    return dg_host::launch_lm(scan_forward_kernel<T, VEC, LPR, WIDE, OG, RS>, dim3((unsigned)grid), dim3(THREADS),
                               Tl::bytes(in.cluster), in.cluster, s, in, h0, (T*)y, h_last, marks);
 }
-template <typename T, int VEC, int LPR, bool WIDE, bool OG>
+template <typename T, int VEC, int LPR, bool WIDE, bool OG, bool RS>
 int run_backward(const ScanIn& in, const ScanGrad& q, cudaStream_t s) {
     typedef Tile<T, VEC, LPR, kBackwardSteps, OG ? 4 : 3> Tl;
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
-    return dg_host::launch_lm(scan_backward_kernel<T, VEC, LPR, WIDE, OG>, dim3((unsigned)grid), dim3(THREADS),
+    return dg_host::launch_lm(scan_backward_kernel<T, VEC, LPR, WIDE, OG, RS>, dim3((unsigned)grid), dim3(THREADS),
                               Tl::bytes(in.cluster), in.cluster, s, in, q);
 }
 
-// calls F<T, VEC, LPR, WIDE, OG>(...) for the shape at hand
-#define SCAN_OG(F, T, VEC, LPR, WIDE, og, ...) \
-    ((og) ? F<T, VEC, LPR, WIDE, true>(__VA_ARGS__) : F<T, VEC, LPR, WIDE, false>(__VA_ARGS__))
-#define SCAN_RUN(F, T, width, lpr, og, ...)                                  \
-    ((width) == 2   ? (lpr) == 32   ? SCAN_OG(F, T, 2, 32, true, og, __VA_ARGS__)  \
-                      : (lpr) == 16 ? SCAN_OG(F, T, 2, 16, true, og, __VA_ARGS__)  \
-                                    : SCAN_OG(F, T, 2, 8, true, og, __VA_ARGS__)   \
-     : (width) == 1 ? (lpr) == 32 ? SCAN_OG(F, T, 2, 32, false, og, __VA_ARGS__)   \
-                                  : SCAN_OG(F, T, 2, 8, false, og, __VA_ARGS__)    \
-     : (lpr) == 32  ? SCAN_OG(F, T, 1, 32, false, og, __VA_ARGS__)                 \
-                    : SCAN_OG(F, T, 1, 8, false, og, __VA_ARGS__))
+// calls F<T, VEC, LPR, WIDE, OG, RS>(...) for the shape at hand
+#define SCAN_RS(F, T, VEC, LPR, WIDE, OG, rs, ...) \
+    ((rs) ? F<T, VEC, LPR, WIDE, OG, true>(__VA_ARGS__) : F<T, VEC, LPR, WIDE, OG, false>(__VA_ARGS__))
+#define SCAN_OG(F, T, VEC, LPR, WIDE, og, rs, ...)                   \
+    ((og) ? SCAN_RS(F, T, VEC, LPR, WIDE, true, rs, __VA_ARGS__)     \
+          : SCAN_RS(F, T, VEC, LPR, WIDE, false, rs, __VA_ARGS__))
+#define SCAN_RUN(F, T, width, lpr, og, rs, ...)                                  \
+    ((width) == 2   ? (lpr) == 32   ? SCAN_OG(F, T, 2, 32, true, og, rs, __VA_ARGS__)  \
+                      : (lpr) == 16 ? SCAN_OG(F, T, 2, 16, true, og, rs, __VA_ARGS__)  \
+                                    : SCAN_OG(F, T, 2, 8, true, og, rs, __VA_ARGS__)   \
+     : (width) == 1 ? (lpr) == 32 ? SCAN_OG(F, T, 2, 32, false, og, rs, __VA_ARGS__)   \
+                                  : SCAN_OG(F, T, 2, 8, false, og, rs, __VA_ARGS__)    \
+     : (lpr) == 32  ? SCAN_OG(F, T, 1, 32, false, og, rs, __VA_ARGS__)                 \
+                    : SCAN_OG(F, T, 1, 8, false, og, rs, __VA_ARGS__))
 
 // CTAs that share an SM, by shared memory and registers
 constexpr int occupancy(bool backward, size_t elem) { return elem == 4 ? 2 : 3; }
@@ -800,7 +890,8 @@ int dg_gated_scan_forward(int dtype, int B, int T, int D, const void* x, int64_t
                     sh.cluster, dev_status, dg_host::wait_limit()};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     DG_DISPATCH_LM(dtype, S, {
-        return SCAN_RUN(run_forward, S, width, sh.lpr, out_gate != nullptr, in, h0, y, h_last, marks, s);
+        return SCAN_RUN(run_forward, S, width, sh.lpr, out_gate != nullptr, resets != nullptr, in, h0, y, h_last, marks,
+                        s);
     });
     return DG_OK;
 }
@@ -829,7 +920,9 @@ int dg_gated_scan_backward(int dtype, int B, int T, int D, const void* x, int64_
     const ScanGrad q{marks, dy, dy_sb, dy_st, dh_last, dx, dgate, dout_gate, dx_sb, dx_st, dgate_sb, dgate_st,
                      dout_gate_sb, dout_gate_st, dh0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DG_DISPATCH_LM(dtype, S, { return SCAN_RUN(run_backward, S, width, sh.lpr, out_gate != nullptr, in, q, s); });
+    DG_DISPATCH_LM(dtype, S, {
+        return SCAN_RUN(run_backward, S, width, sh.lpr, out_gate != nullptr, resets != nullptr, in, q, s);
+    });
     return DG_OK;
 }
 

@@ -369,3 +369,63 @@ def test_closed_gates_forget_any_state():
     assert rel_err(y.cpu(), x.cpu()) < STATE and rel_err(last.cpu(), x[:, -1].cpu()) < STATE
     s = h.clone()
     assert rel_err(gated_scan_step(x[:, 0], gate[:, 0], s).cpu(), x[:, 0].cpu()) < STATE
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,D,t", [(2, 300, 64, 137), (1, 3000, 72, 1700), (4, 600, 768, 33), (2, 90, 33, 64),
+                                     (8, 2100, 64, 2050), (64, 40, 130, 8)])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf")])
+def test_nothing_crosses_a_reset(B, T, D, t, junk, dtype):
+    """A state that is not finite stays in its document, and so does a gradient."""
+    parts, h, _, _, dy, dh = _inputs(B, T, D, dtype, seed=T + t)
+    r = torch.zeros(B, T, dtype=torch.bool, device="cuda")
+    r[:, t] = True
+    if t > 40:
+        r[:, [5, t - 1]] = True          # several in a thread's steps and in a warp's
+    cut = lambda ts, a, b: [p[:, a:b] for p in ts]  # noqa: E731
+    zero = torch.zeros_like(h)
+    # forward: the document that starts at t
+    sick = [p.clone() for p in parts]
+    sick[0][:, t - 1] = junk
+    sick_h = torch.full_like(h, junk)
+    leaves = [p.requires_grad_(True) for p in sick] + [sick_h.requires_grad_(True)]
+    y, last = gated_scan(*leaves, None, r)
+    ry, rl, rx, rg, ro, _ = _ref(*cut(parts, t, T), zero, None, None, dy[:, t:], dh)
+    grads = torch.autograd.grad((y, last), leaves, (dy, dh))
+    for got, ref in zip((y[:, t:], last, *cut(grads[:3], t, T)), (ry, rl, rx, rg, ro)):
+        tol = STATE if got.dtype == torch.float32 else TOL[dtype]
+        assert rel_err(got.detach().float().cpu(), ref.cpu()) < tol
+    # backward: the documents before it
+    leaves = [p.detach().requires_grad_(True) for p in parts] + [h.clone().requires_grad_(True)]
+    y, last = gated_scan(*leaves, None, r)
+    sick_dy = dy.clone()
+    sick_dy[:, t] = junk
+    grads = torch.autograd.grad((y, last), leaves, (sick_dy, torch.full_like(dh, junk)))
+    refs = _ref(*cut(parts, 0, t), h, None, r[:, :t], dy[:, :t], zero)[2:]
+    for got, ref in zip((*cut(grads[:3], 0, t), grads[3]), refs):
+        tol = STATE if got.dtype == torch.float32 else TOL[dtype]
+        assert rel_err(got.float().cpu(), ref.cpu()) < tol
+
+
+def test_a_reset_at_the_first_step_drops_h0():
+    parts, _, _, _, dy, dh = _inputs(3, 50, 40, torch.float32, seed=4)
+    h = torch.full((3, 40), float("nan"), device="cuda", requires_grad=True)
+    r = torch.zeros(3, 50, dtype=torch.bool, device="cuda")
+    r[:, 0] = True
+    y, last = gated_scan(*parts, h, None, r)
+    want, rl = _ref(*parts, None, None, None)
+    assert rel_err(y.detach().cpu(), want.cpu()) < STATE and rel_err(last.detach().cpu(), rl.cpu()) < STATE
+    (g,) = torch.autograd.grad((y, last), [h], (dy, dh))
+    assert not g.any()
+
+
+def test_an_infinite_state_stays_where_nothing_drops_it():
+    """Products of many small gates vanish in 32 bits; that is not a reset."""
+    x = torch.zeros(2, 600, 64, device="cuda")
+    x[:, 3] = float("inf")
+    gate = torch.full_like(x, -20.0)
+    r = torch.zeros(2, 600, dtype=torch.bool, device="cuda")
+    r[:, 2] = True
+    for resets in (None, r):
+        y, last = gated_scan(x, gate, None, None, None, resets)
+        assert not torch.isfinite(y[:, 3:]).any() and not torch.isfinite(last).any() and torch.isfinite(y[:, :3]).all()
