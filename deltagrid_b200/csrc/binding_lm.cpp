@@ -26,6 +26,12 @@ inline void no_second_order(const char* op) {
     TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the backward pass is not differentiable (create_graph=True)");
 }
 
+// tangents would be dropped without a word
+inline void no_forward_mode(const char* op, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), op, ": forward-mode differentiation is not supported");
+}
+
 inline int to_int(int64_t n, const char* op) {
     TORCH_CHECK(n <= 0x7fffffff, op, ": a size of ", n, " is too large");
     return (int)n;
@@ -194,6 +200,7 @@ inline bool needs_grad(std::initializer_list<const Tensor*> ts) {
 std::vector<Tensor> gated_scan(const Tensor& x, const Tensor& gate, const OptTensor& out_gate, const OptTensor& h0,
                                const OptTensor& lengths, const OptTensor& resets) {
     const Tensor o = value(out_gate), h = value(h0), n = value(lengths), r = value(resets);
+    no_forward_mode("gated_scan", {&x, &gate, &o, &h});
     if (needs_grad({&x, &gate, &o, &h})) return GatedScan::apply(x, OptTensor(gate), out_gate, h0, lengths, resets, false, false);
     const ScanOut out = scan_forward(scan_args(x, gate, o, h, n, r), false);
     return {out.y, out.h_last};
@@ -205,6 +212,7 @@ std::vector<Tensor> gated_scan_packed(const Tensor& packed, const OptTensor& h0,
     TORCH_CHECK(packed.dim() == 3 && packed.size(2) % (out_gate ? 3 : 2) == 0, "gated_scan_packed: expected packed [B,T,",
                 out_gate ? 3 : 2, "D], got ", packed.sizes());
     const Tensor h = value(h0), n = value(lengths), r = value(resets);
+    no_forward_mode("gated_scan_packed", {&packed, &h});
     if (needs_grad({&packed, &h})) return GatedScan::apply(packed, OptTensor(), OptTensor(), h0, lengths, resets, true, out_gate);
     const auto p = parts_of(packed, out_gate);
     const ScanOut out = scan_forward(scan_args(p[0], p[1], p[2], h, n, r), false);
@@ -225,6 +233,7 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& h, con
     same_device(x, op, "h", h);
     TORCH_CHECK(h.scalar_type() == at::kFloat && h.sizes() == x.sizes() && h.is_contiguous(), op,
                 ": expected h to be contiguous float32 with x's shape (it is updated in place)");
+    no_forward_mode(op, {&x, &gate, &o, &h});
     TORCH_CHECK(!needs_grad({&x, &gate, &o, &h}), op, ": has no backward pass (use gated_scan, or torch.no_grad())");
     const Tensor g_c = rows(gate), o_c = o.defined() ? rows(o) : o;
     Tensor y = at::empty(x.sizes(), x.options());
@@ -333,6 +342,7 @@ struct GatedFfn : public torch::autograd::Function<GatedFfn> {
 
 Tensor gated_ffn(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t activation) {
     const Tensor b = value(bias);
+    no_forward_mode("gated_ffn", {&x, &weight, &b});
     if (needs_grad({&x, &weight, &b})) return GatedFfn::apply(x, weight, bias, activation);
     return ffn_forward(ffn_args(x, weight, b, activation), x);
 }

@@ -290,3 +290,14 @@ def test_very_positive_gates(kind):
     rh, _, rw, _ = _ref(x, w.detach(), None, kind, torch.ones_like(h))
     for got, ref in ((h, rh), (g, rw)):
         assert float(((got.detach().double() - ref).abs() / ref.abs().clamp(min=1e-30)).max()) < 1e-5
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    x, w, b, _ = _inputs(4, 16, 8, torch.float16, seed=1)
+    with fwd.dual_level():
+        for i in range(3):
+            a = [x, w, b]
+            a[i] = fwd.make_dual(a[i], torch.ones_like(a[i]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                gated_ffn(*a)

@@ -429,3 +429,21 @@ def test_an_infinite_state_stays_where_nothing_drops_it():
     for resets in (None, r):
         y, last = gated_scan(x, gate, None, None, None, resets)
         assert not torch.isfinite(y[:, 3:]).any() and not torch.isfinite(last).any() and torch.isfinite(y[:, :3]).all()
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(2, 5, 8, device="cuda")
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            gated_scan(d, x)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            gated_scan(x, x, None, fwd.make_dual(x[:, 0].clone(), x[:, 0].clone()))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            gated_scan_packed(fwd.make_dual(torch.zeros(2, 5, 24, device="cuda"), torch.ones(2, 5, 24, device="cuda")))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            gated_scan_step(d[:, 0], x[:, 0], torch.zeros(2, 8, device="cuda"))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            gated_scan(d, x)
+    gated_scan(x, x)
