@@ -242,6 +242,8 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& h, con
                              g_c.data_ptr(), st(g_c, 0), ptr_or_null(o_c), st(o_c, 0), h.data_ptr<float>(),
                              y.data_ptr(), stream_of(x)),
           "dg_gated_scan_step");
+    // as any in-place operation: a backward pass that has saved h finds that it has changed
+    if (!h.is_inference()) h.unsafeGetTensorImpl()->bump_version();
     return y;
 }
 

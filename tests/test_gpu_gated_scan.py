@@ -447,3 +447,18 @@ def test_forward_mode_is_refused():
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             gated_scan(d, x)
     gated_scan(x, x)
+
+
+def test_step_counts_as_a_change_of_the_state():
+    """A state that autograd has saved and a step has advanced since is an error in the backward pass."""
+    w = torch.randn(2, 8, device="cuda", requires_grad=True)
+    state = w * 2.0
+    loss = state.pow(2).sum()
+    with torch.no_grad():
+        gated_scan_step(torch.zeros(2, 8, device="cuda"), torch.zeros(2, 8, device="cuda"), state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        s = torch.ones(2, 8, device="cuda")
+        gated_scan_step(torch.zeros(2, 8, device="cuda"), torch.zeros(2, 8, device="cuda"), s)
+    assert float(s.sum()) == 8.0
