@@ -757,24 +757,26 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) * VEC == 8 ? 2 : 3) scan_ba
     close_exchange(S, bad, in.status);
 }
 
+// grid: channels x rows, the rows walked where there are more than a grid has
 template <typename T>
-__global__ void scan_step_kernel(int D, const T* x, int64_t x_sb, const T* g, int64_t g_sb, const T* o, int64_t o_sb,
+__global__ void scan_step_kernel(int B, int D, const T* x, int64_t x_sb, const T* g, int64_t g_sb, const T* o, int64_t o_sb,
                                  float* h, T* y) {
     const int d = blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t b = blockIdx.y;
     dg::let_next_start();
     dg::wait_for_previous();
     if (d >= D) return;
-    float a, na;
-    dg::sigmoid_pair(dg::to_f(g[b * g_sb + d]), a, na);
-    const float hn = fmaf(a, h[b * D + d], na * dg::to_f(x[b * x_sb + d]));
-    h[b * D + d] = hn;
-    float out = hn;
-    if (o) {
-        const float z = dg::to_f(o[b * o_sb + d]);
-        out = hn * (z * dg::sigmoid(z));
+    for (int64_t b = blockIdx.y; b < B; b += gridDim.y) {
+        float a, na;
+        dg::sigmoid_pair(dg::to_f(g[b * g_sb + d]), a, na);
+        const float hn = fmaf(a, h[b * D + d], na * dg::to_f(x[b * x_sb + d]));
+        h[b * D + d] = hn;
+        float out = hn;
+        if (o) {
+            const float z = dg::to_f(o[b * o_sb + d]);
+            out = hn * (z * dg::sigmoid(z));
+        }
+        y[b * D + d] = dg::from_f<T>(out);
     }
-    y[b * D + d] = dg::from_f<T>(out);
 }
 
 // ---------------------------------------------------------------------------
@@ -932,10 +934,9 @@ int dg_gated_scan_step(int dtype, int B, int D, const void* x, int64_t x_sb, con
     if (dtype < DG_DTYPE_F32 || dtype > DG_DTYPE_BF16 || B < 0 || D < 0) return DG_ERR_INVALID_ARGUMENT;
     if (B == 0 || D == 0) return DG_OK;
     if (!x || !gate || !h || !y) return DG_ERR_INVALID_ARGUMENT;
-    if (B > 65535) return DG_ERR_UNSUPPORTED;
     DG_DISPATCH_LM(dtype, S, {
-        return dg_host::launch_lm(scan_step_kernel<S>, dim3((D + 127) / 128, B), dim3(128), 0, 0,
-                                  static_cast<cudaStream_t>(stream), D, static_cast<const S*>(x), x_sb,
+        return dg_host::launch_lm(scan_step_kernel<S>, dim3(D / 128 + (D % 128 != 0), B < 65535 ? B : 65535), dim3(128), 0, 0,
+                                  static_cast<cudaStream_t>(stream), B, D, static_cast<const S*>(x), x_sb,
                                   static_cast<const S*>(gate), gate_sb, static_cast<const S*>(out_gate), out_gate_sb, h,
                                   static_cast<S*>(y));
     });

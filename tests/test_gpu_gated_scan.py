@@ -462,3 +462,12 @@ def test_step_counts_as_a_change_of_the_state():
         s = torch.ones(2, 8, device="cuda")
         gated_scan_step(torch.zeros(2, 8, device="cuda"), torch.zeros(2, 8, device="cuda"), s)
     assert float(s.sum()) == 8.0
+
+
+def test_step_of_very_many_rows():
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x, gate = (torch.randn(70001, 3, generator=g, device="cuda").half() for _ in range(2))
+    h = torch.randn(70001, 3, generator=g, device="cuda")
+    want = _ref(x[:, None], gate[:, None], None, h, None, None)[1]
+    y = gated_scan_step(x, gate, h)
+    assert rel_err(h.cpu(), want.cpu()) < STATE and rel_err(y.float().cpu(), want.cpu()) < TOL[torch.float16]
