@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(THREADS)
 template <typename T, int NT, int G, int U>
 int run(int act, int M, int D, int F, const void* x, int64_t ldx, const void* w, const void* bias, void* h, cudaStream_t s) {
     auto k = act == DG_ACT_SILU ? ffn_few_kernel<T, DG_ACT_SILU, NT, G, U> : ffn_few_kernel<T, DG_ACT_GELU, NT, G, U>;
-    return dg_host::launch_lm(k, dim3((unsigned)((F / 8 + G - 1) / G)), dim3(THREADS), 0, 0, s, M, D, F, (const T*)x, ldx,
+    return dg_host::launch_lm(k, dim3((unsigned)((F / 8 + G - 1) / G)), dim3(THREADS), 0, 0, 0, s, M, D, F, (const T*)x, ldx,
                               (const T*)w, (const T*)bias, (T*)h);
 }
 

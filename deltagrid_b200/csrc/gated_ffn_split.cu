@@ -33,6 +33,7 @@ constexpr int FEATURES = 64;               // of a CTA
 constexpr int BK = 64;                     // contracted elements per stage: 128 bytes
 constexpr uint32_t W_TILE = 2 * FEATURES * BK * 2;
 constexpr int MAX_STAGES = 8;
+constexpr uint32_t MOST_ROOM = 216 * 1024;  // for stages, of one CTA on an SM
 
 struct SplitParams {
     int M, N, F;                           // N: tokens rounded up to 16
@@ -230,7 +231,7 @@ int ffn_split_forward(int dtype, int64_t M, int D, int F, int act, const void* x
         ++splits;
     p.per_split = (p.blocks + splits - 1) / splits;
     p.splits = (p.blocks + p.per_split - 1) / p.per_split;             // none empty
-    const uint32_t stage = W_TILE + (uint32_t)p.N * BK * 2, room = per_sm == 2 ? 108 * 1024 : 216 * 1024;
+    const uint32_t stage = W_TILE + (uint32_t)p.N * BK * 2, room = per_sm == 2 ? MOST_ROOM / 2 : MOST_ROOM;
     p.stages = (int)(room / stage);
     if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
     uint32_t smem = (uint32_t)p.stages * stage;
@@ -242,8 +243,8 @@ int ffn_split_forward(int dtype, int64_t M, int D, int F, int act, const void* x
         return DG_ERR_UNSUPPORTED;
     auto kern = bf16 ? (act == DG_ACT_SILU ? ffn_split_kernel<__nv_bfloat16, DG_ACT_SILU> : ffn_split_kernel<__nv_bfloat16, DG_ACT_GELU>)
                      : (act == DG_ACT_SILU ? ffn_split_kernel<__half, DG_ACT_SILU> : ffn_split_kernel<__half, DG_ACT_GELU>);
-    return launch_lm(kern, dim3((unsigned)(tiles * p.splits)), dim3(THREADS), smem + 1024, p.splits > 1 ? p.splits : 0, s,
-                     mw, mx, p);
+    return launch_lm(kern, dim3((unsigned)(tiles * p.splits)), dim3(THREADS), smem + 1024, MOST_ROOM + 1024,
+                     p.splits > 1 ? p.splits : 0, s, mw, mx, p);
 }
 
 }  // namespace dg_host

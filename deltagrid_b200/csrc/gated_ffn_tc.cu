@@ -555,7 +555,8 @@ int launch(K kern, uint32_t smem, int64_t items, const CUtensorMap& a, const CUt
     const int rc = pairs(&np);
     if (rc != DG_OK) return rc;
     // (the cluster size stands at the kernel)
-    return launch_lm(kern, dim3((unsigned)(2 * (items < np ? items : np))), dim3(THREADS), smem + 1024, 0, s, a, b, d, o, p);
+    return launch_lm(kern, dim3((unsigned)(2 * (items < np ? items : np))), dim3(THREADS), smem + 1024, smem + 1024, 0, s, a, b, d,
+                     o, p);
 }
 
 FfnParams tiles_of(int64_t M, int N, int K, int tile_n, int32_t* status) {
@@ -724,7 +725,7 @@ static int backward_t(int64_t M, int D, int F, int act, const void* x, int64_t l
         rc = product<T, true, true>(2 * (int64_t)F, D, M, dz, 2 * (int64_t)F, x, ldx, dw, part_dw, sp.splits_dw, &join_dw, status, s);
     const int blocks = join_dx.blocks + join_dw.blocks + (db ? (2 * F + 31) / 32 : 0);
     if (rc == DG_OK && blocks > 0)
-        rc = launch_lm(finish_kernel<T>, dim3((unsigned)blocks), dim3(kFinish), 0, 0, s, join_dx, join_dw, (const float*)colsum,
+        rc = launch_lm(finish_kernel<T>, dim3((unsigned)blocks), dim3(kFinish), 0, 0, 0, s, join_dx, join_dw, (const float*)colsum,
                        p.m_tiles * 8, 2 * F, static_cast<T*>(db));
     return rc;
 }

@@ -840,7 +840,7 @@ int run_forward(const ScanIn& in, const float* h0, void* y, float* h_last, float
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
     return dg_host::launch_lm(scan_forward_kernel<T, VEC, LPR, WIDE, OG, RS>, dim3((unsigned)grid), dim3(THREADS),
-                              Tl::bytes(in.cluster), in.cluster, s, in, h0, (T*)y, h_last, marks);
+                              Tl::bytes(in.cluster), Tl::bytes(16), in.cluster, s, in, h0, (T*)y, h_last, marks);
 }
 template <typename T, int VEC, int LPR, bool WIDE, bool OG, bool RS>
 int run_backward(const ScanIn& in, const ScanGrad& q, cudaStream_t s) {
@@ -848,7 +848,7 @@ int run_backward(const ScanIn& in, const ScanGrad& q, cudaStream_t s) {
     const int64_t grid = (int64_t)in.B * ((in.D + Tl::CH - 1) / Tl::CH) * in.cluster;
     if (grid > 0x7fffffff) return DG_ERR_UNSUPPORTED;
     return dg_host::launch_lm(scan_backward_kernel<T, VEC, LPR, WIDE, OG, RS>, dim3((unsigned)grid), dim3(THREADS),
-                              Tl::bytes(in.cluster), in.cluster, s, in, q);
+                              Tl::bytes(in.cluster), Tl::bytes(16), in.cluster, s, in, q);
 }
 
 // calls F<T, VEC, LPR, WIDE, OG, RS>(...) for the shape at hand
@@ -935,7 +935,7 @@ int dg_gated_scan_step(int dtype, int B, int D, const void* x, int64_t x_sb, con
     if (B == 0 || D == 0) return DG_OK;
     if (!x || !gate || !h || !y) return DG_ERR_INVALID_ARGUMENT;
     DG_DISPATCH_LM(dtype, S, {
-        return dg_host::launch_lm(scan_step_kernel<S>, dim3(D / 128 + (D % 128 != 0), B < 65535 ? B : 65535), dim3(128), 0, 0,
+        return dg_host::launch_lm(scan_step_kernel<S>, dim3(D / 128 + (D % 128 != 0), B < 65535 ? B : 65535), dim3(128), 0, 0, 0,
                                   static_cast<cudaStream_t>(stream), B, D, static_cast<const S*>(x), x_sb,
                                   static_cast<const S*>(gate), gate_sb, static_cast<const S*>(out_gate), out_gate_sb, h,
                                   static_cast<S*>(y));

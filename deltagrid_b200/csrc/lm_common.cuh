@@ -160,12 +160,16 @@ namespace dg_host {
 constexpr int kClusters[3][16] = {{148, 74, 45, 33, 26, 22, 15, 15, 15, 11, 7, 7, 7, 7, 7, 7},
                                   {296, 148, 93, 71, 56, 45, 37, 33, 30, 26, 21, 21, 17, 14, 14, 14},
                                   {444, 222, 142, 104, 82, 71, 56, 48, 45, 41, 31, 31, 28, 24, 24, 21}};
-// launches with programmatic dependent launch and, with cluster > 0, that cluster size
+// Launches with programmatic dependent launch and, with cluster > 0, that cluster size.  most_smem: the dynamic
+// shared memory of the kernel's largest launch; its limit is always set to that, so that another host
+// thread's smaller launch does not lower it between this one's setting and launch.
 template <typename... P, typename... A>
-int launch_lm(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, A... args) {
+int launch_lm(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, size_t most_smem, int cluster, cudaStream_t stream,
+              A... args) {
     cudaError_t e;
-    if (smem > 16 * 1024) {                    // (static shared memory counts against the 48 KB too)
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (smem > most_smem) return DG_ERR_UNSUPPORTED;
+    if (most_smem > 16 * 1024) {               // (static shared memory counts against the 48 KB too)
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem);
         if (e != cudaSuccess) return record_cuda_error(e);
     }
     if (cluster > 8) {

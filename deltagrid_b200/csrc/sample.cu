@@ -33,6 +33,7 @@ namespace {
 
 constexpr int ST = 512;                    // threads per CTA
 constexpr int WARPS = ST / 32;
+constexpr size_t MOST_SMEM = 180 * 1024;   // dynamic, of a cluster's CTA
 constexpr int CAP = 1024;                  // tokens collected at most
 constexpr int RANKED = 256;                // up to here ranked by comparing all, beyond sorted
 typedef unsigned long long u64;
@@ -1102,12 +1103,13 @@ template <typename T> int run(SampleParams p, int B, cudaStream_t stream) {
     // the table and, beside a cluster's slice, room for half of its tokens (16 bytes each) as far as it goes
     size_t smem = (size_t)(p.slice + 16) * sizeof(T) + 16;
     if (p.cluster > 1) {
-        const size_t left = (180 * 1024 - smem) / 16;
+        const size_t left = (MOST_SMEM - smem) / 16;
         p.room = (int)(left < (size_t)p.slice / 2 ? left : (size_t)p.slice / 2);
         smem += (size_t)p.room * 16;
     }
     auto kern = p.cluster == 1 ? sample_kernel<T, true> : sample_kernel<T, false>;
-    return dg_host::launch_lm(kern, dim3((unsigned)(B * p.cluster)), dim3(ST), smem, p.cluster > 1 ? p.cluster : 0, stream, p);
+    return dg_host::launch_lm(kern, dim3((unsigned)(B * p.cluster)), dim3(ST), smem, MOST_SMEM, p.cluster > 1 ? p.cluster : 0, stream,
+                              p);
 }
 
 }  // namespace

@@ -1,9 +1,11 @@
 """How the language-model operators are called: errors inside a backward pass, calls of several
 host threads and from threads that have not used the device before."""
+import ctypes
 import os
 import subprocess
 import sys
 import textwrap
+import threading
 
 import pytest
 import torch
@@ -68,3 +70,30 @@ def test_the_first_work_of_a_thread():
         assert len(got) == 1 and torch.equal(got[0], h)
         print("done")
         """)
+
+
+def test_calls_of_two_host_threads():
+    """Launches of one kernel that take little and much shared memory, from two threads through the C ABI."""
+    from deltagrid_b200 import _lib
+    L, F, bad = _lib.lib(), ctypes.c_float, []
+
+    def worker(V, n):
+        torch.cuda.set_device(0)
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            logits, u = torch.zeros(1, V, device="cuda"), torch.zeros(1, device="cuda")
+            token = torch.zeros(1, device="cuda", dtype=torch.int64)
+            s.synchronize()
+            for _ in range(n):
+                rc = L.dg_sample(0, 1, V, logits.data_ptr(), V, u.data_ptr(), None, F(1.0), None, 0, None, F(1.0), None,
+                                 F(0.0), token.data_ptr(), None, s.cuda_stream)
+                if rc:
+                    bad.append((V, rc, L.dg_last_cuda_error()))
+            s.synchronize()
+
+    ts = [threading.Thread(target=worker, args=(v, 4000)) for v in (8192, 200000)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad, (len(bad), bad[0])
