@@ -12,6 +12,8 @@
 // non-zero dg_status raises deltagrid_b200._lib.DeltaGridError (a RuntimeError).
 #include "binding_util.h"
 
+#include <mutex>
+
 using namespace dgb;
 
 namespace dgb {
@@ -19,11 +21,18 @@ namespace dgb {
 PyObject* g_error = nullptr;
 
 Tensor& status_word(const at::Device& dev) {
+    // autograd's threads come here without Python's lock.  A word is made outside of ours, as torch may want
+    // Python's for it; its place stays while others are added.
     static auto* words = new std::unordered_map<int, Tensor>();
-    auto it = words->find(dev.index());
-    if (it == words->end())
-        it = words->emplace(dev.index(), at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(dev))).first;
-    return it->second;
+    static auto* lock = new std::mutex();
+    {
+        const std::lock_guard<std::mutex> held(*lock);
+        const auto it = words->find(dev.index());
+        if (it != words->end()) return it->second;
+    }
+    const Tensor word = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(dev));
+    const std::lock_guard<std::mutex> held(*lock);
+    return words->emplace(dev.index(), word).first->second;
 }
 
 }  // namespace dgb

@@ -97,3 +97,35 @@ def test_calls_of_two_host_threads():
     for t in ts:
         t.join()
     assert not bad, (len(bad), bad[0])
+
+
+def test_first_calls_of_many_threads():
+    """Forward and backward passes of several threads at once, none of which has called the package before."""
+    _child("""
+        import threading
+        import torch
+        from deltagrid_b200.ffn import gated_ffn
+        from deltagrid_b200.recurrence import gated_scan
+        from deltagrid_b200 import hsru_delta_cuda as ext
+        torch.zeros(1, device="cuda")
+        gate, got = threading.Barrier(8), []
+
+        def worker():
+            torch.manual_seed(0)
+            a = torch.randn(2, 40, 16, device="cuda", requires_grad=True)
+            w = torch.randn(32, 16, device="cuda", requires_grad=True)
+            torch.cuda.synchronize()
+            gate.wait()
+            for _ in range(20):
+                g = torch.autograd.grad(gated_ffn(gated_scan(a, a)[0], w).sum(), [a, w])
+            torch.cuda.synchronize()
+            got.append([t.cpu() for t in g])
+
+        ts = [threading.Thread(target=worker) for _ in range(8)]
+        for t in ts:
+            t.start()
+        for t in ts:
+            t.join()
+        assert len(got) == 8 and ext.device_status() == 0
+        print("done")
+        """)
