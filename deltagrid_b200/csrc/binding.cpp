@@ -30,6 +30,7 @@ Tensor& status_word(const at::Device& dev) {
         const auto it = words->find(dev.index());
         if (it != words->end()) return it->second;
     }
+    const c10::InferenceMode ordinary(false);  // device_status() clears it outside of inference mode
     const Tensor word = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(dev));
     const std::lock_guard<std::mutex> held(*lock);
     return words->emplace(dev.index(), word).first->second;

@@ -129,3 +129,16 @@ def test_first_calls_of_many_threads():
         assert len(got) == 8 and ext.device_status() == 0
         print("done")
         """)
+
+
+def test_a_first_call_in_inference_mode():
+    """The status word of a device is an ordinary tensor, whatever mode its first call was made in."""
+    _child("""
+        import torch
+        from deltagrid_b200.ffn import gated_ffn
+        from deltagrid_b200 import hsru_delta_cuda as ext
+        with torch.inference_mode():
+            gated_ffn(torch.ones(4, 8, device="cuda"), torch.ones(16, 8, device="cuda"))
+        assert ext.device_status() == 0
+        print("done")
+        """)
