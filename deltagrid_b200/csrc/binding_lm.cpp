@@ -360,7 +360,9 @@ Tensor per_row(const Tensor& logits, const char* name, const OptTensor& t, at::S
     same_device(logits, "sample", name, v);
     TORCH_CHECK(v.dim() == 1 && v.size(0) == logits.size(0), "sample: expected ", name, " to be a number or [B], got ",
                 v.sizes());
-    return contig(v.scalar_type() == type ? v : v.to(type));
+    if (v.scalar_type() == type) return contig(v);
+    // a number beyond 32 bits must not wrap around (top_k: any above V keeps all)
+    return contig(type == at::kInt ? v.clamp(-1, 1 << 30).to(type) : v.to(type));
 }
 
 std::vector<Tensor> sample(const Tensor& logits, const Tensor& u, const OptTensor& temperature, double temperature_v,

@@ -197,3 +197,11 @@ def test_empty_batch_and_refusals():
         sample(l.double(), u)
     with pytest.raises(RuntimeError, match="unsupported"):
         sample(torch.zeros(1, (1 << 18) + 1, device="cuda"), u[:1])
+
+
+def test_top_k_beyond_32_bits_keeps_all():
+    logits, u = _logits(3, 400, torch.float32, seed=2)
+    k = torch.tensor([2 ** 32 + 5, 2 ** 31, -2 ** 33 + 7], device="cuda")
+    token, logprob = sample(logits, u, top_k=k)
+    want, lp = sample(logits, u)
+    assert torch.equal(token, want) and torch.equal(logprob, lp)
