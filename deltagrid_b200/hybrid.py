@@ -90,7 +90,9 @@ class HybridLM(nn.Module):
         [B,N] under the filtered distributions).
 
         u [B,N] float32 in [0, 1): the uniform numbers to draw with; without it they are taken
-        from ``generator``.  The other arguments are sampling.sample's.
+        from ``generator``.  The other arguments are sampling.sample's.  Where nothing can be drawn (all
+        of a row's logits NaN or -inf) the token is -1, its log-probability -inf, and the row goes on
+        from token 0.
         """
         if ids.dim() != 2 or ids.shape[1] == 0:
             raise ValueError(f"generate: expected prompts [B,T] with at least one token, got {tuple(ids.shape)}")
@@ -108,7 +110,7 @@ class HybridLM(nn.Module):
         for i in range(max_new_tokens):
             tokens[:, i], logprobs[:, i] = sample(logits, u[:, i], temperature, top_k, top_p, min_p)
             if i + 1 < max_new_tokens:
-                logits, states = self.step(tokens[:, i], states)
+                logits, states = self.step(tokens[:, i].clamp(min=0), states)      # (-1 is no row of the embedding)
         return tokens, logprobs
 
 

@@ -81,3 +81,13 @@ def test_refusals():
         HybridBlock("attention", 64, 2, None, None)
     t, lp = m.generate(torch.zeros(2, 1, dtype=torch.int64, device="cuda"), 0)
     assert t.shape == (2, 0) and lp.shape == (2, 0)
+
+
+def test_generate_where_nothing_can_be_drawn():
+    m = _model().eval()
+    ids = torch.randint(0, 97, (3, 4), generator=torch.Generator().manual_seed(5)).cuda()
+    with torch.no_grad():
+        m.head.weight.fill_(float("nan"))
+    tokens, logprobs = m.generate(ids, 3)
+    torch.cuda.synchronize()
+    assert (tokens == -1).all() and torch.isneginf(logprobs).all()
