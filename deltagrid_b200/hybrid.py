@@ -23,7 +23,8 @@ from .sampling import sample
 
 
 class HybridBlock(nn.Module):
-    """kind "recurrence" or "delta"; forward and step return (x, state)."""
+    """kind "recurrence" or "delta"; forward and step return (x, state).  resets (where documents start) are
+    for the recurrence: the memory layer's state cannot be dropped inside a sequence."""
 
     def __init__(self, kind: str, d_model: int, num_heads: int, num_slots: Optional[int], d_hidden: Optional[int],
                  activation: str = "silu"):
@@ -39,6 +40,8 @@ class HybridBlock(nn.Module):
 
     def forward(self, x: torch.Tensor, state: Optional[torch.Tensor] = None,
                 resets: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        if resets is not None and self.kind == "delta":
+            raise ValueError("HybridBlock: resets are not supported by 'delta' blocks")
         h = self.norm_mixer(x)
         y, state = self.mixer(h, state, resets=resets) if self.kind == "recurrence" else self.mixer(h, state)
         x = x + y

@@ -91,3 +91,15 @@ def test_generate_where_nothing_can_be_drawn():
     tokens, logprobs = m.generate(ids, 3)
     torch.cuda.synchronize()
     assert (tokens == -1).all() and torch.isneginf(logprobs).all()
+
+
+def test_resets_are_refused_by_delta_blocks():
+    """The memory layer has no resets: its state would flow from document to document."""
+    from deltagrid_b200.hybrid import HybridBlock
+    x = torch.zeros(2, 5, 64, device="cuda")
+    r = torch.zeros(2, 5, dtype=torch.bool, device="cuda")
+    HybridBlock("recurrence", 64, 2, None, None).cuda()(x, resets=r)
+    b = HybridBlock("delta", 64, 2, None, None).cuda()
+    b(x)
+    with pytest.raises(ValueError, match="resets"):
+        b(x, resets=r)
