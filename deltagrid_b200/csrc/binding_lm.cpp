@@ -4,6 +4,7 @@
 // allocator and calls the C ABI on torch's current stream of the input's device.
 #include "binding_util.h"
 
+#include <ATen/autocast_mode.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 using namespace dgb;
@@ -342,10 +343,14 @@ struct GatedFfn : public torch::autograd::Function<GatedFfn> {
     }
 };
 
-Tensor gated_ffn(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t activation) {
-    const Tensor b = value(bias);
+Tensor gated_ffn(const Tensor& x_, const Tensor& weight_, const OptTensor& bias, int64_t activation) {
+    Tensor x = x_, weight = weight_, b = value(bias);
+    if (at::autocast::is_autocast_enabled(at::kCUDA))
+        for (Tensor* t : {&x, &weight, &b})    // as a product of torch's own; f64 is left alone there too
+            if (t->defined() && t->is_cuda() && t->is_floating_point() && t->scalar_type() != at::kDouble)
+                *t = t->to(at::autocast::get_autocast_dtype(at::kCUDA));
     no_forward_mode("gated_ffn", {&x, &weight, &b});
-    if (needs_grad({&x, &weight, &b})) return GatedFfn::apply(x, weight, bias, activation);
+    if (needs_grad({&x, &weight, &b})) return GatedFfn::apply(x, weight, OptTensor(b), activation);
     return ffn_forward(ffn_args(x, weight, b, activation), x);
 }
 

@@ -301,3 +301,23 @@ def test_forward_mode_is_refused():
             a[i] = fwd.make_dual(a[i], torch.ones_like(a[i]))
             with pytest.raises(RuntimeError, match="forward-mode"):
                 gated_ffn(*a)
+
+
+def test_autocast_runs_in_its_type():
+    x, w, b, dh = _inputs(40, 64, 48, torch.float32, seed=3)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        h = gated_ffn(*leaves)
+        mixed = gated_ffn(x.bfloat16(), w, b)
+    assert h.dtype == torch.bfloat16 and torch.equal(h, mixed)
+    grads = torch.autograd.grad(h, leaves, dh.bfloat16())
+    low = [t.bfloat16() for t in (x, w, b)]
+    assert torch.equal(h, gated_ffn(*low))
+    for got, ref in zip((h, *grads), _ref(*low, "silu", dh.bfloat16())):
+        assert rel_err(got.detach().float().cpu(), ref.cpu()) < 2 * TOL[torch.bfloat16]
+    assert all(g.dtype == torch.float32 for g in grads)
+    m = GatedFFN(64, 48).cuda()
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert m(torch.nn.functional.layer_norm(x, (64,))).dtype == torch.float16
+        with torch.autocast("cuda", enabled=False):
+            assert gated_ffn(x, w).dtype == torch.float32
