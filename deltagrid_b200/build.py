@@ -17,10 +17,12 @@ from __future__ import annotations
 import concurrent.futures as cf
 import glob
 import os
+import shlex
 import shutil
 import subprocess
 import sys
 import sysconfig
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -60,6 +62,27 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def host_compiler() -> str:
+    """The C++ compiler of the torch extension: CXX where it is set, else g++ or c++.  One that links its
+    own static libstdc++ is passed over: it gives the module a second set of iostream facets, and
+    printing a number in an error message then crashes."""
+    found = [c for c in (os.environ.get("CXX"), shutil.which("g++"), shutil.which("c++")) if c]
+    with tempfile.TemporaryDirectory() as d:
+        src, out = os.path.join(d, "probe.cpp"), os.path.join(d, "probe.so")
+        with open(src, "w") as f:
+            f.write("#include <iostream>\nextern \"C\" void probe(int n) { std::cout << n; }\n")
+        for c in found:
+            try:
+                r = subprocess.run([*shlex.split(c), "-shared", "-fPIC", "-o", out, src], capture_output=True)
+            except OSError:
+                continue
+            if r.returncode == 0:
+                with open(out, "rb") as f:
+                    if b"libstdc++.so" in f.read():
+                        return c
+    return found[0] if found else "c++"
+
+
 def _build_binding() -> str:
     """The torch extension module `_hsru` (needs torch's headers and libraries, no GPU)."""
     shared = [os.path.join(CSRC, "binding_util.h"), os.path.join(INCLUDE, "deltagrid_b200.h")]
@@ -71,10 +94,7 @@ def _build_binding() -> str:
     tinc = os.path.join(tdir, "include")
     tlib = os.path.join(tdir, "lib")
     cuda_home = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
-    # the system compiler first: one that links its own static libstdc++ (as a CXX outside the
-    # system's may) gives the module a second set of iostream facets, and printing a number in an
-    # error message then crashes
-    cxx = shutil.which("g++") or os.environ.get("CXX") or "c++"
+    cxx = shlex.split(host_compiler())
     flags = ["-O2", "-std=c++17", "-fPIC", f"-I{tinc}", f"-I{os.path.join(tinc, 'torch', 'csrc', 'api', 'include')}",
              f"-I{os.path.join(cuda_home, 'include')}", f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}",
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_hsru",
@@ -84,14 +104,14 @@ def _build_binding() -> str:
         obj = os.path.join(OBJ, os.path.splitext(os.path.basename(src))[0] + ".o")
         if os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in [src, *shared]):
             return obj
-        r = subprocess.run([cxx, *flags, "-c", src, "-o", obj], capture_output=True, text=True)
+        r = subprocess.run([*cxx, *flags, "-c", src, "-o", obj], capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"binding build failed:\n{r.stdout}\n{r.stderr}")
         return obj
 
     with cf.ThreadPoolExecutor(max_workers=len(BINDING_SRCS)) as ex:
         objs = list(ex.map(compile_one, BINDING_SRCS))
-    cmd = [cxx, "-shared", "-o", BINDING, *objs, f"-L{tlib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+    cmd = [*cxx, "-shared", "-o", BINDING, *objs, f"-L{tlib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
            "-ltorch_python", f"-L{HERE}", "-ldeltagrid_b200", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
