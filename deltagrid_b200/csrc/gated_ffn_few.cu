@@ -33,10 +33,11 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// weights are read once: past L1
+// Weights are read once: past L1.  (Not by the read-only path: a kernel in front of this one may write what it
+// reads after this one has started.)
 __device__ __forceinline__ uint4 load_once(const void* p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
     return v;
 }
 
@@ -68,7 +69,7 @@ __global__ void __launch_bounds__(THREADS)
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-                b[u][n] = on && 8 * n + row < M ? dg::ldg16(x + (8 * n + row) * ldx + k + k8) : zero;
+                b[u][n] = on && 8 * n + row < M ? dg::ld16(x + (8 * n + row) * ldx + k + k8) : zero;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)

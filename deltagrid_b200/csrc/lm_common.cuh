@@ -17,7 +17,8 @@ namespace dg {
 
 // Programmatic dependent launch: a kernel lets the next one of its stream start as soon as its own blocks
 // leave room, and touches no memory before the kernel in front of it has completed, so that launch
-// latency and set-up run under the end of the work before (about 2 us a kernel back to back).
+// latency and set-up run under the end of the work before (about 2 us a kernel back to back).  Such a kernel's
+// inputs may still be written after it has started, so it loads none by the read-only path (ld.global.nc).
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(ST, MANY ? 2 : 1) sample_kernel(SampleParams p
         uint4 v[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            if (i + q * ST < body) v[q] = dg::ldg16(vsrc + i + q * ST);
+            if (i + q * ST < body) v[q] = dg::ld16(vsrc + i + q * ST);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             if (i + q * ST < body) {
