@@ -471,3 +471,14 @@ def test_step_of_very_many_rows():
     want = _ref(x[:, None], gate[:, None], None, h, None, None)[1]
     y = gated_scan_step(x, gate, h)
     assert rel_err(h.cpu(), want.cpu()) < STATE and rel_err(y.float().cpu(), want.cpu()) < TOL[torch.float16]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,T,D", [(2, 300, 514), (40, 400, 66), (3, 1100, 1026)])
+def test_pairs_of_channels_without_wide_copies(B, T, D, dtype):
+    _check(*_inputs(B, T, D, dtype, seed=B, resets=True), dtype)
+
+
+@pytest.mark.parametrize("B,T,D", [(100, 600, 512), (33, 1500, 520)])
+def test_more_than_one_wave(B, T, D):
+    _check(*_inputs(B, T, D, torch.bfloat16, seed=B, resets=True), torch.bfloat16)

@@ -205,3 +205,26 @@ def test_top_k_beyond_32_bits_keeps_all():
     token, logprob = sample(logits, u, top_k=k)
     want, lp = sample(logits, u)
     assert torch.equal(token, want) and torch.equal(logprob, lp)
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 32000), (torch.float16, 41999), (torch.float32, 20003)])
+@pytest.mark.parametrize("T,k,p,m", [(0.8, 50, 0.95, 0.02), (1.0, 400, 0.9, 0.0), (1.0, 0, 0.92, 0.0), (1.7, 4000, 0.99, 0.0),
+                                     (1.0, 0, 1.0, 0.0)])
+def test_large_vocabularies_of_many_rows(V, T, k, p, m, dtype):
+    """Rows enough for a CTA each: a few of them against the definition."""
+    logits, u = _logits(80, V, dtype, seed=V + k)
+    logits[1, torch.arange(V) % 10 != 3] = float("-inf")
+    token, logprob = sample(logits, u, T, k, p, m)
+    for i in (0, 1, 79):
+        want, lp = _draw(_kept(logits[i], T, k, p, m), u[i].item())
+        assert token[i].item() == want and abs(logprob[i].item() - lp) < 1e-5 * max(1.0, abs(lp))
+
+
+@pytest.mark.parametrize("T,k,p,m", [(0.8, 50, 0.95, 0.02), (1.0, 0, 0.92, 0.0), (1.7, 4000, 0.99, 0.0), (1.0, 0, 1.0, 0.0)])
+def test_a_row_is_the_same_in_any_number_of_ctas(T, k, p, m):
+    """100 rows have a CTA each, 30 clusters of 2, 12 of 8 and one a cluster of 16."""
+    logits, u = _logits(100, 40000, torch.bfloat16, seed=21)
+    token, logprob = sample(logits, u, T, k, p, m)
+    for n in (30, 12, 1):
+        t, lp = sample(logits[:n], u[:n], T, k, p, m)
+        assert torch.equal(t, token[:n]) and torch.equal(lp, logprob[:n])
