@@ -321,3 +321,19 @@ def test_autocast_runs_in_its_type():
         assert m(torch.nn.functional.layer_norm(x, (64,))).dtype == torch.float16
         with torch.autocast("cuda", enabled=False):
             assert gated_ffn(x, w).dtype == torch.float32
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+@pytest.mark.parametrize("M,D,dtype", [(4, 16, torch.bfloat16), (100, 16, torch.float16), (600, 16, torch.bfloat16),
+                                       (70, 15, torch.bfloat16), (70, 16, torch.float32)])
+def test_what_is_not_a_number_shows(M, D, dtype, kind):
+    """A NaN in a row of x, in its outputs and gradients; no other row's."""
+    x, w, b, dh = _inputs(M, D, 32, dtype, seed=M)
+    x[2, 3] = float("nan")
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    h = gated_ffn(*leaves, kind)
+    gx, gw, gb = torch.autograd.grad(h, leaves, dh)
+    rows = torch.arange(M, device="cuda") == 2
+    assert torch.equal(torch.isnan(h).all(1), rows) and torch.equal(torch.isnan(h).any(1), rows)
+    assert torch.equal(torch.isnan(gx).all(1), rows) and torch.equal(torch.isnan(gx).any(1), rows)
+    assert torch.isnan(gw).all() and torch.isnan(gb).all()
