@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(THREADS)
                 float a, da;
                 dg::act_grad<ACT>(gv, a, da);
                 const float d = dg::to_f(dh[m * ld_dh + f]);
-                const float zg = d * uv * da, zu = d * a;
+                const float zg = d * uv * da, zu = d * a;      // stored in T, as the tensor-core kernels have to
                 dz[m * 2 * F + f] = dg::from_f<T>(zg);
                 dz[m * 2 * F + F + f] = dg::from_f<T>(zu);
                 sum_g += zg;

@@ -358,6 +358,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                 const dg::F2 dd{dhv.x, dhv.y};
                                 dg::F2 a, s;
                                 dg::act_grad2<ACT>(gv, a, s);
+                                // dG and dU go to 16 bits: the tensor cores read no other type for dx and dW,
+                                // and a second half of each would double those products.  dbias is summed before
                                 const dg::F2 xg = dg::mul2(dg::mul2(dd, uv), s), xu = dg::mul2(dd, a);
                                 zg[i] = xg.x, zg[i + 1] = xg.y;
                                 zu[i] = xu.x, zu[i + 1] = xu.y;

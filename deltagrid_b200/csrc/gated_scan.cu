@@ -28,9 +28,9 @@
 // What bounds it: HBM at 8 (forward, 16-bit, with an output gate) to 14 bytes (backward) an
 // element, with issue slots and the special-function unit (two operations for each sigmoid)
 // at about half of their limits too; pairs of channels use the two-wide fp32 instructions to
-// keep issue slots free.  8 x 4096 x 768 in bf16: forward 50 us (4.0 TB/s, 0.63 of the copy
-// bandwidth), backward 108 us (3.3 TB/s, 0.51); 1 x 65536 x 768 forward 138 us (2.9 TB/s), as
-// its clusters of 15 leave a fifth of the SM's places empty.
+// keep issue slots free.  8 x 4096 x 768 in bf16: forward 51 us (3.9 TB/s, 0.61 of the copy
+// bandwidth), backward 102 us (3.5 TB/s, 0.54), with resets 52 and 111 us; 1 x 65536 x 768 forward 140 us
+// (2.9 TB/s), as its clusters of 15 leave a fifth of the SM's places empty.
 #include <type_traits>
 
 #include "lm_common.cuh"

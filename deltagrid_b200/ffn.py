@@ -23,8 +23,10 @@ def gated_ffn(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
     """x [..., D], weight [2F, D], bias [2F] (one dtype: f32 / f16 / bf16) -> h [..., F].
 
     activation "silu" or "gelu" (the tanh form).  Differentiable in x, weight and bias; the
-    backward pass forms both projections again, so nothing of size [..., 2F] is kept.  Under
-    torch.autocast it runs in autocast's type, as nn.Linear does.
+    backward pass forms both projections again, so nothing of size [..., 2F] is kept.  The
+    gradients of the projections are rounded to the tensors' type once, before the products
+    that use them (f16: its range).  Under torch.autocast it runs in autocast's type, as
+    nn.Linear does.
     """
     code = _ACT.get(activation)
     if code is None:

@@ -27,8 +27,9 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, out_gate: Optional[torch.Ten
 
     h0 [B,D] float32 starts the state (zeros without it).  lengths [B]: steps at and
     beyond a row's length leave its state, give y = 0 and are not looked at.  resets
-    [B,T] bool: where true the state before that step is dropped (a document starts).
-    Differentiable in x, gate, out_gate and h0.
+    [B,T] bool: where true the state before that step is dropped (a document starts),
+    an infinite or NaN one as well.  Differentiable in x, gate, out_gate and h0 (reverse
+    mode, once).
     """
     y, h = _hsru.gated_scan(x, gate, out_gate, h0, lengths, resets)
     return y, h
@@ -46,7 +47,8 @@ def gated_scan_packed(packed: torch.Tensor, h0: Optional[torch.Tensor] = None,
 
 def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, h: torch.Tensor,
                     out_gate: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """One token: x, gate, out_gate [B,D], h [B,D] float32 updated in place -> y [B,D]."""
+    """One token: x, gate, out_gate [B,D], h [B,D] float32 updated in place -> y [B,D].
+    No backward pass; h counts as changed for one that has saved it."""
     return _hsru.gated_scan_step(x, gate, h, out_gate)
 
 

@@ -23,7 +23,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Number = 1.0, top
 
     Each parameter is a number or a [B] tensor.  temperature <= 0 takes the largest logit
     (lowest index); top_k <= 0 keeps all.  NaN logits count as -inf; a row of -inf gives
-    token -1 and logprob -inf.
+    token -1 and logprob -inf.  V is 2^18 at most.  Not differentiable: logprob carries no
+    gradient.
     """
     t, tv = (temperature, 0.0) if isinstance(temperature, torch.Tensor) else (None, temperature)
     k, kv = (top_k, 0) if isinstance(top_k, torch.Tensor) else (None, top_k)

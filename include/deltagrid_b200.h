@@ -315,8 +315,9 @@ int dg_pkm_route(int dtype, int B, int H, int T, int dh, int g0, int g1, int top
 /*
  * Gated linear recurrence over a sequence, per batch row b and channel d:
  *   a_t = sigmoid(gate_t)        h_t = c_t h_{t-1} + (1 - a_t) x_t        y_t = h_t silu(out_gate_t)
- * with c_t = a_t, or 0 where resets[b,t] is not 0 (a new document starts there), and
- * y_t = h_t when out_gate is NULL.
+ * with c_t = a_t, or no state at all where resets[b,t] is not 0 (a new document starts there: a state that is
+ * infinite or NaN does not enter it), and y_t = h_t when out_gate is NULL.  Gates may have any value (-inf
+ * forgets the state, NaN gives NaN); an out_gate of -inf gives NaN, as its formula does, the lowest finite one 0.
  *   x, gate, out_gate [B,T,D]: element strides (batch, step) each, last dimension contiguous
  *   h0 [B,D] fp32 or NULL (zeros);  lengths [B] int32 or NULL (all T);  resets [B,T] bytes or NULL
  *   y [B,T,D] contiguous;  h_last [B,D] fp32 or NULL
@@ -376,7 +377,7 @@ size_t dg_gated_ffn_backward_workspace_size(int dtype, int64_t M, int D, int F);
  *   dU = dh act(G)   dG = dh U act'(G)   dx = dG Wg + dU Wu   dweight = [dG^T x; dU^T x]
  *   dbias = column sums of [dG, dU] (summed in fp32 before any rounding)
  *   dh [M,F] (row stride ld_dh)   dx [M,D], dweight [2F,D], dbias [2F] contiguous, NULL where not wanted
- * dG and dU pass through the workspace in the storage dtype.  No atomics.
+ * dG and dU pass through the workspace in the storage dtype (one rounding, and f16's range).  No atomics.
  */
 int dg_gated_ffn_backward(int dtype, int64_t M, int D, int F, int activation, const void* x, int64_t ldx,
                           const void* weight, const void* bias, const void* dh, int64_t ld_dh, void* dx,
@@ -392,7 +393,7 @@ int dg_gated_ffn_backward(int dtype, int64_t M, int D, int F, int activation, co
  * those of them with less than top_p times their mass before them, at least one (steps of 2^-24);
  * min_p keeps those with w_i >= min_p 2^40.  The token is the first kept index whose running mass, in
  * index order, exceeds floor(u * kept mass).  temperature <= 0: the largest logit, lowest index.
- * A NaN logit counts as -inf, an infinite one takes all the mass; a row of -inf gives token -1.
+ * A NaN logit counts as -inf, an infinite one takes all the mass; a row of -inf gives token -1.  V is 2^18 at most.
  * Each parameter is a device array of B values or, where the pointer is NULL, the scalar beside it.
  *   token [B] int64   logprob [B] fp32 or NULL: log(w_token / kept mass), -inf for token -1
  */
